@@ -430,6 +430,76 @@ int si_gated_pool(const void* kv, const void* score, void* out, int dtype, int64
                   void* stream);
 
 /*
+ * Serving over a paged cache (no counterparts in the reference, whose operators
+ * take whole sequences).  A cache is [pages, page_size, width]; a page holds
+ * consecutive entries of one request, block_table[r, i] is the page of request
+ * r's entries i * page_size and on, negative where there is none, and
+ * slot = page * page_size + offset names a row.  Tables are int32 with
+ * contiguous rows table_stride elements apart; lengths are below 2^31 and are
+ * read on the device only.
+ *
+ * si_paged_plan: R requests with ctx_lens[r] tokens get new_lens[r] more (int32,
+ * negative = 0).  Entries are tokens (ratio 1) or completed groups of ratio
+ * tokens.  Rows are the new entries, request by request; at most `rows` of them.
+ *   block_table [R,P], in place: new pages in request order from free_pages
+ *     [F], from position *free_start (NULL: 0) on; -1 past its end.
+ *   cu [R+1] first row of each request; seq_lens [R] entries after the step;
+ *   slots (int64), request, positions [rows]: of each row, -1 behind the last
+ *     one (slots also where there is no page); free_next [1]: the position
+ *     after the last page taken.
+ */
+int si_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int64_t R, int64_t ratio, int32_t* block_table,
+                  int64_t table_stride, int64_t P, const int32_t* free_pages, int64_t F, const int32_t* free_start,
+                  int64_t page_size, int64_t rows, int32_t* cu, int32_t* seq_lens, int64_t* slots, int32_t* request,
+                  int32_t* positions, int32_t* free_next, void* stream);
+
+/*
+ * Row t of rows ([n], row_bytes each, row_stride bytes apart) to slots[t] of the
+ * cache (page_stride and slot_stride in bytes); slots outside [0, pages *
+ * page_size) write nothing.  Slots are distinct.
+ */
+int si_paged_write(const void* rows, int64_t row_stride, const int64_t* slots, int64_t n, int64_t row_bytes,
+                   void* cache, int64_t page_stride, int64_t slot_stride, int64_t pages, int64_t page_size,
+                   void* stream);
+
+/*
+ * si_token_compress over paged streams [pages, page_size, C] (strides of 3
+ * elements each, the last 1): entry positions[e] of request request[e] to
+ * slots[e] of out [out_pages, out_page_size, C]; entries without request or slot
+ * are left out.  dtype 0 = fp32, 1 = bf16, 2 = fp16; b_a, b_b [m, C] fp32; c_b,
+ * z_b, b_b NULL: no overlap.  Tokens without a page count as absent.
+ */
+int si_paged_compress(const void* c_a, const int64_t* ca_strides, const void* z_a, const int64_t* za_strides,
+                      const float* b_a, const void* c_b, const int64_t* cb_strides, const void* z_b,
+                      const int64_t* zb_strides, const float* b_b, int dtype, int64_t pages, int64_t page_size,
+                      int64_t C, int64_t m, const int32_t* block_table, int64_t table_stride, int64_t R, int64_t P,
+                      const int32_t* request, const int32_t* positions, const int64_t* slots, int64_t E, void* out,
+                      const int64_t* out_strides, int64_t out_pages, int64_t out_page_size, void* stream);
+
+/*
+ * MQA attention with sink of N new tokens over their requests' paged caches.
+ * Request r's tokens are rows cu_q[r] .. cu_q[r+1]-1 of q [N,H,D] (strides of 3,
+ * the last 1), the last at position seq_lens[r] - 1.  A token at position p sees
+ * entries k of kv [pages, page_size, D] with p - window < k <= p (window 0: all
+ * k <= p) and, with ratio > 0, entries i of kv2 with ratio (i + 1) - 1 <= p.
+ * Keys without a page in [0, pages) are masked.  o [N,H,D] and lse [N,H]
+ * contiguous; rows of no request are written as rows without a key.  A cache
+ * spans at most 64 GiB, its strides are multiples of 8 elements; N * H < 2^31.
+ * scratch: as for si_sparse_attn_fwd_scratch, at least
+ * si_paged_attn_fwd_scratch_bytes(...) bytes for calls that split their keys
+ * over workgroups (keys, keys2: P * page_size of each cache).
+ */
+int64_t si_paged_attn_fwd_scratch_bytes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys,
+                                        int64_t keys2);
+int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* kv, const int64_t* kv_strides,
+                      int64_t pages, int64_t page_size, const int32_t* block_table, int64_t table_stride, int64_t P,
+                      const void* kv2, const int64_t* kv2_strides, int64_t pages2, int64_t page_size2,
+                      const int32_t* block_table2, int64_t table_stride2, int64_t P2, int64_t window, int64_t ratio,
+                      const int32_t* cu_q, const int32_t* seq_lens, const float* attn_sink, int64_t N, int64_t H,
+                      int64_t D, int64_t R, float softmax_scale, int qkv_dtype, void* o, float* lse, void* scratch,
+                      int64_t scratch_bytes, void* stream);
+
+/*
  * Synthetic inputs for benchmarks and tests (no counterpart in the reference,
  * whose harnesses draw with torch.randn on a CUDA generator,
  * eval/test_v4_indexer_parity.py:89-103): out[i] = N(0,1)[seed, stream, i]

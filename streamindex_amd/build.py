@@ -48,6 +48,7 @@ COMMON_FLAGS = [
 # where the fp32 epilogue reads them.
 EXTRA_FLAGS = {
     "sparse_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     **{f"indexer_inst_{u}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]
        for u in ("d32", "d32_wide", "d64", "d64_wide", "d128", "d128_wide", "d256",
                  "split_d32", "split_d64", "split_d128", "split_d256")},

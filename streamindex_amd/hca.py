@@ -22,9 +22,10 @@ import torch
 
 from . import _lib
 from .csa import _launch_hca, _row_len
+from .paged import PagedPlan, paged_attn_fwd, paged_compress, paged_write
 from .sparse_attn import _aligned, _bwd_workspace, sparse_attn_bwd, sparse_attn_fwd_kv2
 
-__all__ = ["flash_hca_forward", "build_hca_topk_idxs", "hca_row_len"]
+__all__ = ["flash_hca_forward", "flash_hca_paged_forward", "build_hca_topk_idxs", "hca_row_len"]
 
 
 def build_hca_topk_idxs(*, B: int, seq_len: int, n_win: int, n_compressed: int, m_prime: int,
@@ -69,6 +70,50 @@ def flash_hca_forward(
     n_compressed = kv_compressed.shape[1]
     assert q.is_cuda
     return _HcaAttnFunc.apply(q, kv, kv_compressed, attn_sink, softmax_scale, n_win, m_prime)
+
+
+def flash_hca_paged_forward(
+    q: torch.Tensor,
+    rows: torch.Tensor,
+    bias: torch.Tensor,
+    attn_sink: torch.Tensor,
+    row_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    tokens: PagedPlan,
+    entry_cache: torch.Tensor,
+    entry_table: torch.Tensor,
+    entries: PagedPlan,
+    *,
+    n_win: int,
+    softmax_scale: Optional[float] = None,
+) -> torch.Tensor:
+    """One serving step of an HCA layer: :func:`flash_hca_forward` for a ragged batch of new tokens over a paged cache.
+
+    Writes the new tokens' rows into their pages, pools the compressed entries that they complete and attends to the
+    window and to every legal entry.
+
+    Args:
+      q: ``[N, n_h, d]`` bf16 or fp16 RoPE-rotated queries of the new tokens.
+      rows: ``[N, 3 d]`` the tokens' uncompressed KV, compressor content and compressor gate, side by side.
+      bias: ``[m', d]`` the compressor's bias, one entry per m' tokens.  attn_sink: ``[n_h]`` fp32.
+      row_cache: ``[pages, page_size, 3 d]`` of q's type, updated in place; ``block_table [R, P]`` and ``tokens`` its plan
+        (:func:`streamindex_amd.paged.paged_plan`).  A page may be given back, and its table entry set to -1, once its
+        tokens are behind the window and in a complete entry.
+      entry_cache: ``[entry_pages, entry_page_size, d]``, updated in place; ``entry_table`` and ``entries`` its plan, made
+        with ``ratio=m'``.
+      n_win: sliding-window size.  softmax_scale: defaults to ``d ** -0.5``.
+    Returns:
+      ``o: [N, n_h, d]`` in q's type, zero in rows behind the last request.
+    """
+    d = q.shape[2]
+    if row_cache.dim() != 3 or row_cache.shape[2] != 3 * d:
+        raise ValueError(f"row_cache must be [pages, page_size, {3 * d}]")
+    paged_write(rows, row_cache, tokens.slots)
+    kv, c, z = row_cache[..., :d], row_cache[..., d:2 * d], row_cache[..., 2 * d:]
+    paged_compress(c, z, bias, block_table, entries.request, entries.positions, entry_cache, entries.slots)
+    o, _ = paged_attn_fwd(q, kv, block_table, tokens.cu, tokens.seq_lens, attn_sink, softmax_scale, window=n_win,
+                          kv2_cache=entry_cache, block_table2=entry_table, ratio=bias.shape[0])
+    return o
 
 
 def _rows(B: int, S: int, n_win: int, n_compressed: int, m_prime: int, device):
