@@ -158,7 +158,15 @@ def qkv_dtype(t: torch.Tensor) -> int:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
+
+
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# (the handle itself, without a Stream object made around it: 2 us a call less)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 _HERE = contextlib.nullcontext()

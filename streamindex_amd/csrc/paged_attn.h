@@ -18,8 +18,9 @@ struct PagedCache {
   const int32_t* table;  // [R, P]
   int64_t tstride;
   uint32_t pstride, rstride;  // page and row, 16-byte units
-  int P, pages;               // pages == 0: no key has a page
-  uint32_t ps, magic, shift;  // key / ps = mulhi(key, magic) >> shift for keys below 2^31 (magic 0: ps = 1)
+  int pages;                  // 0: no key has a page
+  int keys;                   // that a block table row can name
+  uint32_t ps, magic, shift, one;  // key / ps = (mulhi(key, magic) + (key & one)) >> shift for keys below 2^31
 };
 
 struct PagedAttnArgs {
@@ -34,18 +35,14 @@ struct PagedAttnArgs {
   float* lse;        // [N,H] contiguous
   int N, H, R;
   float scale_log2;
-  int want;          // workgroups to fill the GPU with
+  int want_log2;     // workgroups to fill the GPU with: 2^want_log2
   int least;         // fewest tiles of a share
-  int cap;           // workgroups whose items must all fit (0: no bound)
-  float* part_o;     // [items, 64, D]; null: rows are not split
-  float2* part_ml;   // [items, 64]
+  int behind;        // tokens of a row block before its last one at most
+  float* part_o;     // [items, M, D]; null: rows are not split
+  float2* part_ml;   // [items, M]
   int32_t* rec;      // [0]: split row blocks; then 4 each: first item, shares, first row, rows
 };
 
-constexpr int kPagedRows = 64;       // (token, head) rows of a workgroup
 constexpr int kPagedThreads = 256;
-
-int launch_paged_attn(int D, bool f16, const PagedAttnArgs& a, int64_t blocks, int64_t split_blocks, hipStream_t st);
-int paged_attn_per_cu(int D);  // resident workgroups of a CU
 
 }  // namespace si

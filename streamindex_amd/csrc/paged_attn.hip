@@ -33,39 +33,62 @@ namespace si {
 // be a scalar load in flight among the LDS reads, whose lgkmcnt waits count on completion in order.
 template <typename T>
 __device__ __forceinline__ void scalar_tie(T& x) {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two registers");
+  if constexpr (sizeof(T) == 4) {
+    x = __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+  } else {
+    const uint64_t w = __builtin_bit_cast(uint64_t, x);
+    const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w)));
+    const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w >> 32)));
+    x = __builtin_bit_cast(T, hi << 32 | lo);
+  }
   asm volatile("" : "+s"(x));
 }
 
 // A cache as one workgroup reads it.
 struct CacheView {
-  const uint16_t* base;
   const int32_t* table;  // the request's row
-  uint32_t pstride, rstride, ps, magic, shift;
-  int pages;
-  __device__ __forceinline__ CacheView(const PagedCache& c, int req)
-      : base(c.base), table(c.table + (c.pages > 0 ? req * c.tstride : 0)), pstride(c.pstride), rstride(c.rstride), ps(c.ps),
-        magic(c.magic), shift(c.shift), pages(c.pages) {
-    scalar_tie(base);
-    scalar_tie(table);
-    scalar_tie(pstride);
-    scalar_tie(rstride);
-    scalar_tie(ps);
-    scalar_tie(magic);
-    scalar_tie(shift);
-    scalar_tie(pages);
-  }
+  uint32_t ps, rstride, magic, shift, one;
+  __device__ __forceinline__ uint32_t page_of(uint32_t key) const { return (__umulhi(key, magic) + (key & one)) >> shift; }
 };
-__device__ __forceinline__ uint32_t page_div(uint32_t key, uint32_t magic, uint32_t shift) {
-  return magic ? __umulhi(key, magic) >> shift : key;
+struct CacheBase {
+  const char* base;
+  uint32_t pstride, pages;
+};
+// (by value: a choice between two caches stays one between values at hand, not between addresses in memory)
+__device__ __forceinline__ void view_cache(PagedCache c, int req, CacheView& v, CacheBase& b) {
+  v.table = c.table + req * c.tstride;
+  v.ps = c.ps;
+  v.rstride = c.rstride;
+  v.magic = c.magic;
+  v.shift = c.shift;
+  v.one = c.one;
+  b.base = reinterpret_cast<const char*>(c.base);
+  b.pstride = c.pstride;
+  b.pages = static_cast<uint32_t>(c.pages);
+  scalar_tie(v.table);
+  scalar_tie(v.ps);
+  scalar_tie(v.rstride);
+  scalar_tie(v.magic);
+  scalar_tie(v.shift);
+  scalar_tie(v.one);
+  scalar_tie(b.base);
+  scalar_tie(b.pstride);
+  scalar_tie(b.pages);
+}
+template <typename T>
+__device__ __forceinline__ T pick(bool second, T x, T y) {
+  return second ? y : x;
 }
 
 // ---------------------------------------------------------------------------
 // Schedule
 //
-// Request r has blocks(r) = ceil(n_r H / 64) row blocks of about tiles(r) key tiles each.  With U = sum blocks tiles and
-// `want` workgroups, a row block is cut into ceil(tiles / c) shares; c is the smallest of eight steps from U / want to
-// 2.75 U / want with which all shares run at once.  With more row blocks than that, c = 2 U / want cuts only requests
+// Request r has blocks(r) = ceil(n_r H / M) blocks of M rows of about tiles(r) key tiles each.  With U = sum blocks tiles
+// and `want` workgroups, a row block is cut into ceil(tiles / c) shares; c is the smallest of four steps from U / want to
+// 2 U / want with which all shares run at once.  With more row blocks than that, c = 2 U / want cuts only requests
 // far longer than the average, which would otherwise end last on their own.
+// Every workgroup does these sums itself, with lane-shift scans in 32 bits.
 // ---------------------------------------------------------------------------
 struct PagedReq {
   int first, n, len;  // first row of q, new tokens, entries of the first cache
@@ -74,40 +97,27 @@ struct PagedReq {
 
 __device__ __forceinline__ int ceil_div32(int x) { return static_cast<int>((static_cast<uint32_t>(x) + 31u) >> 5); }
 
-// Keys [lo, hi) of the first cache that a token at position p sees.
-__device__ __forceinline__ int64_t win_lo(const PagedAttnArgs& a, int64_t p) {
-  const int64_t lo = p + 1 - a.window;
-  return lo > 0 ? lo : 0;
-}
-__device__ __forceinline__ int64_t key_cap(const PagedCache& c) {  // keys that a block table row can name
-  const int64_t cap = c.pages > 0 ? static_cast<int64_t>(c.P) * c.ps : 0;
-  return cap < 0x7fffffff ? cap : 0x7fffffff;
-}
-__device__ __forceinline__ int64_t win_hi(const PagedAttnArgs& a, int64_t p) {
-  const int64_t cap = key_cap(a.c1);
-  const int64_t hi = p + 1 < cap ? p + 1 : cap;
-  return hi > 0 ? hi : 0;
-}
-__device__ __forceinline__ int64_t ent_hi(const PagedAttnArgs& a, int64_t p) {  // entries of the second cache
+// Keys [lo, hi) of the first cache that a token at position p sees, and entries of the second.  Lengths are taken from 0 on,
+// so positions run from -N to 2^31 - 2 and nothing here leaves 32 bits.
+__device__ __forceinline__ int win_lo(const PagedAttnArgs& a, int p) { return max(max(p + 1, 0) - a.window, 0); }
+__device__ __forceinline__ int win_hi(const PagedAttnArgs& a, int p) { return max(min(p + 1, a.c1.keys), 0); }
+__device__ __forceinline__ int ent_hi(const PagedAttnArgs& a, int p) {
   if (a.ratio == 0 || p < 0) return 0;
-  const int64_t cap = key_cap(a.c2);
-  const int64_t n = static_cast<uint32_t>(p + 1) / static_cast<uint32_t>(a.ratio);
-  return n < cap ? n : cap;
+  return min(static_cast<int>(static_cast<uint32_t>(p + 1) / static_cast<uint32_t>(a.ratio)), a.c2.keys);
 }
 
+template <int M>
 __device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& a, int r) {
   PagedReq q;
   const int c0 = a.cu[r], c1 = a.cu[r + 1];
-  q.first = c0 < 0 ? 0 : (c0 < a.N ? c0 : a.N);
-  const int end = c1 < q.first ? q.first : (c1 < a.N ? c1 : a.N);
-  q.n = end - q.first;
-  q.len = a.lens[r];
-  q.blocks = static_cast<int>((static_cast<uint32_t>(q.n) * static_cast<uint32_t>(a.H) + (kPagedRows - 1)) / kPagedRows);
+  q.len = max(a.lens[r], 0);
+  q.first = min(max(c0, 0), a.N);
+  q.n = max(min(c1, a.N) - q.first, 0);
+  q.blocks = static_cast<int>((static_cast<uint32_t>(q.n) * static_cast<uint32_t>(a.H) + (M - 1)) / M);
   // tiles of the last row block, which sees the most
-  const int64_t p = static_cast<int64_t>(q.len) - 1;
-  const int64_t span = win_hi(a, p) - win_lo(a, p - (kPagedRows - 1) / a.H);
-  q.tiles = ceil_div32(static_cast<int>(span > 0 ? span : 0)) + ceil_div32(static_cast<int>(ent_hi(a, p)));
-  if (q.tiles < 1) q.tiles = 1;
+  const int p = q.len - 1;
+  const int span = max(win_hi(a, p) - win_lo(a, p - a.behind), 0);
+  q.tiles = max(ceil_div32(span) + ceil_div32(ent_hi(a, p)), 1);
   return q;
 }
 
@@ -118,101 +128,138 @@ struct PagedItem {  // what a workgroup does
   int rec;            // number of its row block among the split ones
 };
 
-// Sum of x over the workgroup and, with PREFIX, the sum over lower threads in *before.
-template <bool PREFIX>
-__device__ __forceinline__ int64_t wg_sum(int64_t x, int64_t* lds, int64_t* before) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t v = x;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int64_t y = __shfl_up(v, d);
-    if (lane >= d) v += y;
-  }
-  if (lane == kWave - 1) lds[wave] = v;
-  __syncthreads();
-  int64_t all = 0, low = 0;
-#pragma unroll
-  for (int w = 0; w < kPagedThreads / kWave; ++w) {
-    if (w < wave) low += lds[w];
-    all += lds[w];
-  }
-  __syncthreads();
-  if (PREFIX) *before = low + v - x;
-  return all;
+// Inclusive prefix sum over the wave: shifts within rows of 16 lanes, then the rows' last lanes to the rows behind.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+  return x;
+}
+
+__device__ __forceinline__ int shares_of(int tiles, uint32_t c) {
+  return tiles <= 1 ? 1 : static_cast<int>((static_cast<uint32_t>(tiles) + c - 1) / c);
+}
+
+constexpr uint32_t kWhole = 0x7fffffffu;  // no row block is cut
+
+// The sum over the wave, in lane 63.
+__device__ __forceinline__ float wave_sum_last(float x) {
+  auto shifted = [](float v, auto CTRL, auto MASK) {
+    return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)),
+                                                                             decltype(CTRL)::value, decltype(MASK)::value, 0xf, false)));
+  };
+  using std::integral_constant;
+  x += shifted(x, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  x += shifted(x, integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  x += shifted(x, integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  x += shifted(x, integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  x += shifted(x, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  x += shifted(x, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return x;
 }
 
 // This workgroup's item, or false.  All threads call it.
-__device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int64_t id, PagedItem& it) {
-  __shared__ int64_t lds[kPagedThreads / kWave];
+template <int M>
+__device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, PagedItem& it) {
+  constexpr int W = kPagedThreads / kWave, STEPS = 4;
+  __shared__ float units_lds[W];
+  __shared__ int blocks_lds[W], fits_lds[W][STEPS], sums_lds[3][W];
   __shared__ PagedItem found;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.R + kPagedThreads - 1) / kPagedThreads;
   const int r0 = min(t * per, a.R), r1 = min(r0 + per, a.R);
-  int64_t units = 0, blocks = 0, before;
   PagedReq mine{};  // kept where a thread has one request
+  float units = 0.f;
+  int blocks = 0;
   for (int r = r0; r < r1; ++r) {
-    mine = paged_req(a, r);
-    units += static_cast<int64_t>(mine.blocks) * mine.tiles;
+    mine = paged_req<M>(a, r);
+    units = __builtin_fmaf(static_cast<float>(mine.blocks), static_cast<float>(mine.tiles), units);
     blocks += mine.blocks;
   }
-  auto req = [&](int r) { return per == 1 ? mine : paged_req(a, r); };
-  int64_t c = 0x7fffffff;  // tiles of a share
+  auto req = [&](int r) { return per == 1 ? mine : paged_req<M>(a, r); };
+  uint32_t c = kWhole;  // tiles of a share
   if (a.part_o) {
-    units = wg_sum<false>(units, lds, nullptr);
-    const int64_t all = wg_sum<false>(blocks, lds, nullptr);
-    auto step = [&](int i) {
-      const int64_t x = (units * (4 + i) + 4 * a.want - 1) / (4 * static_cast<int64_t>(a.want));
-      return x > a.least ? x : static_cast<int64_t>(a.least);
-    };
-    c = step(4);
-    if (all < a.want) {
-      // shares of this thread's requests under each step
-      int64_t pick = -1;
-      for (int i = 0; i < 8 && pick < 0; ++i) {
-        const int64_t ci = step(i);
-        int64_t n = 0;
-        for (int r = r0; r < r1; ++r) {
-          const PagedReq q = req(r);
-          n += static_cast<int64_t>(q.blocks) * ((q.tiles + ci - 1) / ci);
-        }
-        if (wg_sum<false>(n, lds, nullptr) <= a.want) pick = ci;
+    units = wave_sum_last(units);
+    blocks = wave_scan(blocks);
+    if (lane == kWave - 1) {
+      units_lds[wave] = units;
+      blocks_lds[wave] = blocks;
+    }
+    __syncthreads();
+    // (rounded up: fp32 sums of whole numbers, at most 2^-20 too small over the few thousand additions of a call)
+    units = ((units_lds[0] + units_lds[1]) + (units_lds[2] + units_lds[3])) * (1.0f + 0x1p-16f);
+    const int all = (blocks_lds[0] + blocks_lds[1]) + (blocks_lds[2] + blocks_lds[3]);
+    const int want = 1 << a.want_log2;
+    const float least = static_cast<float>(a.least);
+    auto tiles_of = [&](float x) { return static_cast<uint32_t>(__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(x), least), 0x1p30f)); };
+    const float each = units / static_cast<float>(want);
+    const uint32_t steps[STEPS] = {tiles_of(each), tiles_of(1.25f * each), tiles_of(1.5f * each), tiles_of(2.f * each)};
+    c = steps[STEPS - 1];
+    if (all < want) {
+      int n[STEPS] = {};
+      for (int r = r0; r < r1; ++r) {
+        const PagedReq q = req(r);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) n[i] += q.blocks * shares_of(q.tiles, steps[i]);
       }
-      if (pick < 0) {  // (sum of ceil(tiles / c) <= units / c + blocks <= want)
-        pick = (units + (a.want - all) - 1) / (a.want - all);
-        if (pick < a.least) pick = a.least;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        n[i] = wave_scan(n[i]);
+        if (lane == kWave - 1) fits_lds[wave][i] = n[i];
       }
-      c = pick;
+      __syncthreads();
+      // (sum of ceil(tiles / c) <= units / c + blocks <= want)
+      c = tiles_of(units / static_cast<float>(want - all));
+#pragma unroll
+      for (int i = STEPS - 1; i >= 0; --i)
+        if ((fits_lds[0][i] + fits_lds[1][i]) + (fits_lds[2][i] + fits_lds[3][i]) <= want) c = steps[i];
     }
   }
-  int64_t items = 0, parts = 0, recs = 0;
-  auto shares_of = [&](const PagedReq& q) { return static_cast<int>((q.tiles + c - 1) / c); };
+  int items = 0, parts = 0, recs = 0;
   for (int r = r0; r < r1; ++r) {
     const PagedReq q = req(r);
-    const int s = shares_of(q);
-    items += static_cast<int64_t>(q.blocks) * s;
+    const int s = shares_of(q.tiles, c);
+    items += q.blocks * s;
     if (s > 1) {
-      parts += static_cast<int64_t>(q.blocks) * s;
+      parts += q.blocks * s;
       recs += q.blocks;
     }
   }
-  int64_t part0, rec0;
-  const int64_t total = wg_sum<true>(items, lds, &before);
-  wg_sum<true>(parts, lds, &part0);
-  const int64_t all_recs = wg_sum<true>(recs, lds, &rec0);
-  if (a.part_o && id == 0 && t == 0) a.rec[0] = static_cast<int>(all_recs);
-  if (id >= total) return false;
-  if (before <= id && id < before + items) {
-    int64_t at = before;
+  int before[3];
+  const int x3[3] = {items, parts, recs};
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const int v = wave_scan(x3[i]);
+    if (lane == kWave - 1) sums_lds[i][wave] = v;
+    before[i] = v - x3[i];
+  }
+  __syncthreads();
+  int total[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    total[i] = 0;
+#pragma unroll
+    for (int w = 0; w < kPagedThreads / kWave; ++w) {
+      if (w < wave) before[i] += sums_lds[i][w];
+      total[i] += sums_lds[i][w];
+    }
+  }
+  if (a.part_o && id == 0 && t == 0) a.rec[0] = total[2];
+  if (id >= total[0]) return false;
+  if (before[0] <= id && id < before[0] + items) {
+    int at = before[0], part0 = before[1], rec0 = before[2];
     for (int r = r0; r < r1; ++r) {
       const PagedReq q = req(r);
-      const int s = shares_of(q);
-      const int64_t n = static_cast<int64_t>(q.blocks) * s;
+      const int s = shares_of(q.tiles, c);
+      const int n = q.blocks * s;
       if (id < at + n) {
-        const int64_t k = id - at;
+        const int k = id - at;
+        const int block = k / s;
         // (the last row blocks see the most keys: they start first)
-        const int block = static_cast<int>(k / s);
-        found = PagedItem{q.first, q.n, q.len, r, q.blocks - 1 - block, static_cast<int>(k - static_cast<int64_t>(block) * s), s,
-                          static_cast<int>(part0 + k), static_cast<int>(rec0 + block)};
+        found = PagedItem{q.first, q.n, q.len, r, q.blocks - 1 - block, k - block * s, s, part0 + k, rec0 + block};
         break;
       }
       at += n;
@@ -227,10 +274,14 @@ __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int64_t i
   return true;
 }
 
-// Waves of a SIMD, which is resident workgroups of a CU: 216 registers of a wave are Q^T and O^T at D = 576, 96 at D = 256.
-constexpr int per_cu(int D) { return D >= 512 ? 1 : D == 256 ? 2 : 4; }
+// Resident workgroups of a CU: 216 registers of a wave hold Q^T and O^T at D = 576, 96 at D = 256.
+constexpr int per_cu(int D) { return D >= 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
+// Tiles resident in LDS.
+constexpr int ring_slots(int D, int RB) { return D == 576 && RB == 2 ? 3 : 4; }
 
 constexpr float kNever = -__builtin_inff();
+constexpr int kOdd = 1;    // a masked score that is not finite
+constexpr int kMoved = 2;  // a reference maximum of the wave's row block b has moved (kMoved << b): alpha is not one
 
 // x with infinities and NaN replaced by zero.
 template <bool F16>
@@ -247,24 +298,31 @@ __device__ __forceinline__ bf16x8 finite_or_zero(bf16x8 x) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-template <int D, bool F16>
+// RB: blocks of 16 rows of a wave (rows of a workgroup: 64 RB).
+template <int D, bool F16, int RB>
 __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(PagedAttnArgs a) {
   using SH = AttnShape<D>;
   constexpr int KS = SH::KS, MBW = SH::MBW, ROW = SH::ROW;
+  constexpr int M = 64 * RB, NB = 4 * RB;          // rows and row blocks of the workgroup
+  constexpr int NS = ring_slots(D, RB), AHEAD = NS - 1;  // tiles in LDS, and copied ahead of P V
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  __shared__ __attribute__((aligned(16))) char kv_lds[2 * SH::TILE];
-  __shared__ __attribute__((aligned(16))) char p_lds[4 * 64 * 16];
-  __shared__ float alpha_lds[64], scale_lds[64];
-  __shared__ int odd_lds[4];  // a masked non-finite score in this tile, by wave
+  static_assert(NS * SH::TILE >= 64 * ROW, "the output is staged 64 rows at a time");
+  __shared__ __attribute__((aligned(16))) char kv_lds[NS * SH::TILE];
+  __shared__ __attribute__((aligned(16))) char p_lds[2][NB * 64 * 16];
+  __shared__ __attribute__((aligned(16))) float alpha_lds[2][M];
+  __shared__ __attribute__((aligned(16))) int flag_lds[2][4];  // kOdd, kMoved of this tile, by wave
+  __shared__ __attribute__((aligned(16))) int page_lds[kAttnWaves][4][64];  // page numbers of four tiles, by wave
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   __builtin_assume(wave >= 0 && wave < 4);
   const int g = lane >> 4, i16 = lane & 15;
+  const int last = a.R > 0 ? a.cu[a.R] : 0;
 
+  PagedItem item;
+  const bool work = paged_schedule<M>(a, xcd_block_order(), item);
   // Rows of no request: as a row without a key.
   {
-    const int last = a.R > 0 ? a.cu[a.R] : 0;
     const int end = last < 0 ? 0 : (last < a.N ? last : a.N);
     for (int64_t t = end + static_cast<int64_t>(blockIdx.x); t < a.N; t += gridDim.x) {
       u32x4* orow = reinterpret_cast<u32x4*>(a.o + t * a.H * D);
@@ -275,88 +333,130 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
       }
     }
   }
-  PagedItem item;
-  if (!paged_schedule(a, xcd_block_order(), item)) return;
+  if (!work) return;
 
-  const int row0 = __builtin_amdgcn_readfirstlane(item.block) * kPagedRows;  // within the request
-  const int nrows = min(__builtin_amdgcn_readfirstlane(item.n) * a.H - row0, kPagedRows);
-  const int64_t pos0 = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(item.len)) - __builtin_amdgcn_readfirstlane(item.n);
+  const int row0 = __builtin_amdgcn_readfirstlane(item.block) * M;  // within the request
+  const int nrows = min(__builtin_amdgcn_readfirstlane(item.n) * a.H - row0, M);
+  const int pos0 = __builtin_amdgcn_readfirstlane(item.len - item.n);
   const int req = __builtin_amdgcn_readfirstlane(item.req);
   const int shares = __builtin_amdgcn_readfirstlane(item.shares);
-  const int64_t pa = pos0 + row0 / a.H, pb = pos0 + (row0 + nrows - 1) / a.H;  // first and last token
+  const int pa = pos0 + row0 / a.H, pb = pos0 + (row0 + nrows - 1) / a.H;  // first and last token
   // tiles of this row block: the window's, then the second cache's; and this share of them
-  const int k1lo = static_cast<int>(win_lo(a, pa)), k1hi = static_cast<int>(win_hi(a, pb));
-  const int k2hi = static_cast<int>(ent_hi(a, pb));
+  const int k1lo = win_lo(a, pa), k1hi = win_hi(a, pb);
+  const int k2hi = ent_hi(a, pb);
   const int n1 = k1hi > k1lo ? ceil_div32(k1hi - k1lo) : 0;
   const int ntiles = n1 + ceil_div32(k2hi);
   const int share = __builtin_amdgcn_readfirstlane(item.share);
   const int tbeg = static_cast<int>(static_cast<int64_t>(ntiles) * share / shares);
   const int tend = static_cast<int>(static_cast<int64_t>(ntiles) * (share + 1) / shares);
 
-  // this lane's row: its Q^T fragments and the keys it sees
-  const int lrow = wave * 16 + i16;
-  const bool live = lrow < nrows;
-  const int tok = live ? (row0 + lrow) / a.H : 0;
-  const int head = live ? row0 + lrow - tok * a.H : 0;
-  const int64_t pos = pos0 + tok;
-  const int lo1 = live ? static_cast<int>(win_lo(a, pos)) : 0;
-  const int cnt1 = live ? static_cast<int>(max(win_hi(a, pos) - win_lo(a, pos), int64_t{0})) : 0;
-  const int cnt2 = live ? static_cast<int>(ent_hi(a, pos)) : 0;
-  bf16x8 qf[KS];
-  {
-    const uint16_t* qrow = a.q + (static_cast<int64_t>(item.first) + tok) * a.qst + head * a.qsh;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = live ? *reinterpret_cast<const bf16x8*>(qrow + ks * 32 + g * 8) : bf16x8{};
-  }
-
   // ---- copies ----------------------------------------------------------------
   // Lanes l and l + 32 resolve key l of a tile; a key past the tile's last one stands in for by that one (it is masked,
-  // and a tile always has a first key).  A key without a page reads row 0 of the cache and is masked.
-  const CacheView c1(a.c1, req), c2(a.c2, req);
-  struct Tile {
-    int k0, end;
-    bool second;
-  };
-  auto tile_of = [&](int t) {
+  // and a tile always has a first key).  A key without a page reads row 0 of the cache and is masked.  Each wave fetches
+  // the page numbers for its own copies into LDS (as registers they would make the compiler wait for every copy in
+  // flight before their use), a tile ahead of the copies; `within` is what the key's place in its page adds.
+  CacheView view1, view2;
+  CacheBase base1, base2;
+  view_cache(a.c1, req, view1, base1);
+  view_cache(a.c2, req, view2, base2);
+  CacheView view;            // of the next tile to fetch page numbers for
+  CacheBase from, from_next; // of the tile to copy, and of the one after it
+  int fkey = 0, fend = 0, ftile = tbeg;
+  auto enter = [&](int t) {  // moves the view to tile t
     const bool second = t >= n1;
-    return second ? Tile{(t - n1) * 32, k2hi, true} : Tile{k1lo + t * 32, k1hi, false};
+    view = CacheView{pick(second, view1.table, view2.table), pick(second, view1.ps, view2.ps),
+                     pick(second, view1.rstride, view2.rstride), pick(second, view1.magic, view2.magic),
+                     pick(second, view1.shift, view2.shift), pick(second, view1.one, view2.one)};
+    from_next = CacheBase{pick(second, base1.base, base2.base), pick(second, base1.pstride, base2.pstride),
+                          pick(second, base1.pages, base2.pages)};
+    fkey = second ? (t - n1) * 32 : k1lo + t * 32;
+    fend = second ? k2hi : k1hi;
   };
-  auto load_page = [&](int t) {  // page number of this lane's key
-    const Tile x = tile_of(t);
-    const uint32_t key = static_cast<uint32_t>(min(x.k0 + (lane & 31), x.end - 1));
-    const uint32_t magic = x.second ? c2.magic : c1.magic, shift = x.second ? c2.shift : c1.shift;
-    const int32_t* table = x.second ? c2.table : c1.table;
-    return table[page_div(key, magic, shift)];
+  auto fetch_pages = [&] {
+    if (__builtin_expect(ftile == n1, 0) && ntiles > n1) enter(n1);
+    const uint32_t key = static_cast<uint32_t>(min(fkey + (lane & 31), fend - 1));
+    const uint32_t col = view.page_of(key);
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(view.table + col),
+                                     (lds_void_t*)&page_lds[wave][ftile & 3][0], 4, 0, 0);
+    ++ftile;
+    fkey += 32;
+    return (key - col * view.ps) * view.rstride;
   };
-  auto row_off = [&](int t, int page, bool& ok) {  // offset of this lane's key, 16-byte units
-    const Tile x = tile_of(t);
-    const uint32_t key = static_cast<uint32_t>(min(x.k0 + (lane & 31), x.end - 1));
-    const uint32_t magic = x.second ? c2.magic : c1.magic, shift = x.second ? c2.shift : c1.shift;
-    const uint32_t ps = x.second ? c2.ps : c1.ps;
-    const uint32_t pstride = x.second ? c2.pstride : c1.pstride, rstride = x.second ? c2.rstride : c1.rstride;
-    const int pages = x.second ? c2.pages : c1.pages;
-    ok = page >= 0 && page < pages;
-    const uint32_t off = static_cast<uint32_t>(page) * pstride + (key - page_div(key, magic, shift) * ps) * rstride;
-    return ok ? off : 0u;
-  };
-  auto copy_tile = [&](int t, uint32_t off) {
-    const char* base = reinterpret_cast<const char*>(tile_of(t).second ? c2.base : c1.base);
-    char* dst0 = kv_lds + (t & 1) * SH::TILE;
-    int ln = lane;
-    reg_tie(ln);  // (the copies' keys and chunks are worked out anew for each tile: kept, they would take 2 LPT registers)
+  // This lane's key and chunk of copy i, kept where registers allow.
+  constexpr bool KEEP = RB == 1;
+  int src_lane[KEEP ? SH::LPT : 1];
+  uint32_t src_chunk[KEEP ? SH::LPT : 1];
+  if constexpr (KEEP) {
 #pragma unroll
     for (int i = 0; i < SH::LPT; ++i) {
-      const int e0 = i * SH::NT + wave * 64;
-      if (SH::CH % SH::NT == 0 || i + 1 < SH::LPT || e0 < SH::CH) {
-        const int e = e0 + ln;
-        const int key = e / SH::CPR;
-        const uint32_t chunk = static_cast<uint32_t>((e % SH::CPR) ^ kv_swz<D>(key));
-        const uint32_t row = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(key * 4, static_cast<int>(off)));
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(base + (static_cast<uint64_t>(row + chunk) << 4));
-        __builtin_amdgcn_global_load_lds(src, (lds_void_t*)(dst0 + e0 * 16), 16, 0, 0);
-      }
+      const int e = i * SH::NT + static_cast<int>(threadIdx.x), k = e / SH::CPR;
+      src_lane[i] = (k & 31) * 4;
+      src_chunk[i] = static_cast<uint32_t>((e % SH::CPR) ^ kv_swz<D>(k));
+    }
+  }
+  auto copy_lane = [&](int i, int ln) {
+    if constexpr (KEEP) return src_lane[i];
+    else return ((i * SH::NT + wave * 64 + ln) / SH::CPR & 31) * 4;
+  };
+  auto copy_chunk = [&](int i, int ln) {
+    if constexpr (KEEP) return src_chunk[i];
+    const int e = i * SH::NT + wave * 64 + ln;
+    return static_cast<uint32_t>((e % SH::CPR) ^ kv_swz<D>(e / SH::CPR));
+  };
+  // Sources of a tile's copies, in 16-byte units; returns which of its keys have a page.
+  auto address_tile = [&](int page, uint32_t within, uint32_t (&src)[SH::LPT]) {
+    const bool ok = static_cast<uint32_t>(page) < from.pages;
+    const uint32_t off = ok ? static_cast<uint32_t>(page) * from.pstride + within : 0u;
+    int ln = lane;
+    reg_tie(ln);
+#pragma unroll
+    for (int i = 0; i < SH::LPT; ++i)
+      src[i] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(copy_lane(i, ln), static_cast<int>(off)));
+    return static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
+  };
+  auto copy = [&](const uint32_t (&src)[SH::LPT], char* dst, auto IC) {
+    constexpr int i = decltype(IC)::value;
+    if (SH::CH % SH::NT == 0 || i + 1 < SH::LPT || i * SH::NT + wave * 64 < SH::CH) {
+      int ln = lane;
+      reg_tie(ln);
+      const char* at = from.base + (static_cast<uint64_t>(src[i] + copy_chunk(i, ln)) << 4);
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint16_t*>(at), (lds_void_t*)(dst + i * (SH::NT * 16)), 16, 0, 0);
     }
   };
+  auto ring = [&](int slot) { return kv_lds + slot * SH::TILE; };
+  auto page_addr = [&](int t) { return lds_addr(reinterpret_cast<const char*>(&page_lds[wave][t & 3][0])) + lane * 4; };
+  // (the first tiles' page numbers are on their way while Q is addressed; tiles past the share's end are not used)
+  uint32_t within[AHEAD + 1];
+  CacheBase froms[AHEAD + 1];
+  if (tbeg < tend) {
+    enter(tbeg);
+#pragma unroll
+    for (int i = 0; i <= AHEAD; ++i) {
+      if (tbeg + i < tend) within[i] = fetch_pages();
+      froms[i] = from_next;
+    }
+  }
+
+  // ---- this lane's rows: their Q^T fragments and the keys they see ----------------
+  int lo1[RB], cnt1[RB], cnt2[RB];
+  bf16x8 qf[RB][KS];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int lrow = (wave * RB + b) * 16 + i16;
+    const bool live = lrow < nrows;
+    const int tok = live ? (row0 + lrow) / a.H : 0;
+    const int head = live ? row0 + lrow - tok * a.H : 0;
+    const int pos = pos0 + tok;
+    lo1[b] = live ? win_lo(a, pos) : 0;
+    cnt1[b] = live ? max(win_hi(a, pos) - win_lo(a, pos), 0) : 0;
+    cnt2[b] = live ? ent_hi(a, pos) : 0;
+    const uint16_t* qrow = a.q + (static_cast<int64_t>(item.first) + tok) * a.qst + head * a.qsh;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[b][ks] = live && a.scale_log2 != 0.f ? *reinterpret_cast<const bf16x8*>(qrow + ks * 32 + g * 8) : bf16x8{};
+      if (__builtin_expect(a.scale_log2 < 0.f, 0)) qf[b][ks] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, qf[b][ks]) ^ 0x80008000u);
+    }
+  }
 
   // ---- S^T -------------------------------------------------------------------
   // A-fragment addresses: key 16mb + i16, chunk 4ks + g; with f = kv_swz(i16), (4ks + g) ^ f = 4 (ks ^ (f >> 2)) +
@@ -364,9 +464,10 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
   const int qf_swz = kv_swz<D>(i16);
   const int qbase = i16 * ROW + 16 * (g ^ (qf_swz & 3));
   const int qadj = 64 * (qf_swz >> 2);
-  constexpr int QPD = KS < 3 ? KS : 3;
-  auto qk = [&](int t, f32x4 (&st)[2]) {
-    const uint32_t tile = lds_addr(kv_lds + (t & 1) * SH::TILE);
+  constexpr int QPD = KS < 4 ? KS : 4;
+  // start() runs behind the first fragments' reads, beside(ks) among the MFMAs of k-step ks.
+  auto qk = [&](int slot, f32x4 (&st)[RB][2], auto&& start, auto&& beside) {
+    const uint32_t tile = lds_addr(ring(slot));
     const uint32_t qa_e = tile + qbase + qadj, qa_o = tile + qbase - qadj;
     bf16x8 kq[QPD][2];
     auto issue = [&](auto KC) {
@@ -376,140 +477,159 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
       kq[ks % QPD][1] = ld128<64 * ks + 16 * ROW>(base);
     };
     attn_static_for<0, QPD>(issue);
-    st[0] = f32x4{0.f, 0.f, 0.f, 0.f};
-    st[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    start();
+#pragma unroll
+    for (int b = 0; b < RB; ++b) st[b][0] = st[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     attn_static_for<0, KS>([&](auto KC) {
       constexpr int ks = decltype(KC)::value;
       constexpr int later = (KS - 1 - ks) < (QPD - 1) ? (KS - 1 - ks) : (QPD - 1);
       lds_wait<2 * later>(kq[ks % QPD][0], kq[ks % QPD][1]);
-      st[0] = mfma16x16x32<F16>(kq[ks % QPD][0], qf[ks], st[0]);
-      st[1] = mfma16x16x32<F16>(kq[ks % QPD][1], qf[ks], st[1]);
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        st[b][0] = mfma16x16x32<F16>(kq[ks % QPD][0], qf[b][ks], st[b][0]);
+        st[b][1] = mfma16x16x32<F16>(kq[ks % QPD][1], qf[b][ks], st[b][1]);
+      }
       if constexpr (ks + QPD < KS) issue(std::integral_constant<int, ks + QPD>{});
+      beside(KC);
     });
-    mfma_result_fence(st[0], st[1]);
   };
 
   // Keys that every row sees: [all1lo, all1hi) of the first cache, [0, all2hi) of the second; none where rows are missing.
-  int all1lo = static_cast<int>(win_lo(a, pb)), all1hi = nrows == kPagedRows ? static_cast<int>(win_hi(a, pa)) : -1;
-  int all2hi = nrows == kPagedRows ? static_cast<int>(ent_hi(a, pa)) : -1;
-  float scale = a.scale_log2;
+  int all1lo = win_lo(a, pb), all1hi = nrows == M ? win_hi(a, pa) : -1;
+  int all2hi = nrows == M ? ent_hi(a, pa) : -1;
+  float scale = a.scale_log2 == 0.f ? 1.0f : __builtin_fabsf(a.scale_log2);
   scalar_tie(all1lo);
   scalar_tie(all1hi);
   scalar_tie(all2hi);
   scalar_tie(scale);
 
   // ---- softmax -----------------------------------------------------------------
-  float m_ref = kNever, l_run = 0.f;  // reference maximum (log2 domain) and this lane's share of the denominator
-  auto softmax = [&](int t, uint32_t okmask, f32x4 (&st)[2]) {
-    const Tile x = tile_of(t);
-    // every row sees every key of the tile (32-bit sums: k0 is below the end of a range that fits 31 bits)
-    const bool full = okmask == 0xffffffffu && (x.second ? x.k0 <= all2hi - 32 : x.k0 >= all1lo && x.k0 <= all1hi - 32);
-    uint32_t seen = 0xffu;
-    bool odd = false;
+  // In steps that run among the MFMAs of the tile before: scores to log2 units and masks, a new reference maximum where one
+  // is due; the weights one by one; their sum and their place in LDS.
+  // (scale is positive: a negative one has changed the sign of Q, zero has made Q zero)
+  constexpr float kLazy = F16 ? 8.0f : 64.0f;  // 2^8 keeps P in fp16's range, 2^64 in bf16's
+  float m_ref[RB], l_run[RB];  // reference maximum (log2 domain) and this lane's share of the denominator
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    m_ref[b] = kNever;
+    l_run[b] = 0.f;
+  }
+  int skey = 0;  // first key of the next tile to mask
+  const uint32_t pdst = lds_addr(&p_lds[0][(wave * RB * 64 + lane) * 16]);
+  auto softmax_begin = [&](int t, uint32_t okmask, f32x4 (&st)[RB][2], float (&ref)[RB], int pbuf) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) mfma_result_fence(st[b][0], st[b][1]);
+    if (t == n1) skey = 0;
+    const bool second = t >= n1;
+    // every row sees every key of the tile (32-bit sums: skey is below the end of a range that fits 31 bits)
+    const bool full = okmask == 0xffffffffu && (second ? skey <= all2hi - 32 : skey >= all1lo && skey <= all1hi - 32);
+    int flags = 0;
     if (!full) {
-      seen = 0;
-      const int lo = x.second ? 0 : lo1, cnt = x.second ? cnt2 : cnt1;
+      bool odd = false;
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
+      for (int b = 0; b < RB; ++b) {
+        const int lo = skey - (second ? 0 : lo1[b]), cnt = second ? cnt2[b] : cnt1[b];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int kk = 16 * mb + 4 * g + r;
-          const bool ok = static_cast<uint32_t>(x.k0 + kk - lo) < static_cast<uint32_t>(cnt) && ((okmask >> kk) & 1);
-          if (ok) seen |= 1u << (4 * mb + r);
-          const bool fin = __builtin_fabsf(st[mb][r]) < __builtin_inff();
-          odd = odd || (!ok && !fin);
-          st[mb][r] = ok ? (fin ? st[mb][r] : __builtin_nanf("")) : kNever;
-        }
-    }
-    float y[8];
+        for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = st[i >> 2][i & 3] * scale;
-    if (!full) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = (seen >> i) & 1 ? y[i] : kNever;  // (a negative scale)
-    }
-    const float lmax = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(y[0], y[1]), __builtin_fmaxf(y[2], y[3])),
-                                       __builtin_fmaxf(__builtin_fmaxf(y[4], y[5]), __builtin_fmaxf(y[6], y[7])));
-    constexpr float kLazy = F16 ? 8.0f : 64.0f;  // 2^8 keeps P in fp16's range, 2^64 in bf16's
-    const bool first = m_ref == kNever;
-    float alpha = 1.0f;
-    if (__builtin_amdgcn_ballot_w64(first ? lmax > kNever : lmax > m_ref + kLazy) != 0) {
-      const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
-      float tmax = __builtin_fmaxf(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
-      const SwapPair r32 = permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax));
-      tmax = __builtin_fmaxf(__uint_as_float(r32.x), __uint_as_float(r32.y));
-      if (first ? tmax > kNever : tmax > m_ref + kLazy) {
-        alpha = first ? 1.0f : __builtin_amdgcn_exp2f(m_ref - tmax);
-        m_ref = tmax;
+          for (int r = 0; r < 4; ++r) {
+            const int kk = 16 * mb + 4 * g + r;
+            const bool ok = static_cast<uint32_t>(kk + lo) < static_cast<uint32_t>(cnt) && ((okmask >> kk) & 1);
+            const bool fin = __builtin_fabsf(st[b][mb][r]) < __builtin_inff();
+            odd = odd || (!ok && !fin);
+            st[b][mb][r] = ok ? (fin ? st[b][mb][r] : __builtin_nanf("")) : kNever;
+          }
       }
+      flags = __builtin_amdgcn_ballot_w64(odd) ? kOdd : 0;
     }
-    const float ref = m_ref == kNever ? 0.f : m_ref;
-    float p[8];
+    skey += 32;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(y[i] - ref);
-    l_run = l_run * alpha + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
-    // P^T B-fragment: k-slots 8g+0..3 <-> keys 4g+0..3, 8g+4..7 <-> keys 16+4g+0..3
-    u32x4 w;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) w[c] = pack2<F16>(p[2 * c], p[2 * c + 1]);
-    const uint32_t pdst = lds_addr(&p_lds[(wave * 64 + lane) * 16]);
-    asm volatile("ds_write_b128 %0, %1" ::"v"(pdst), "v"(w) : "memory");
-    if (g == 0) {
-      const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[lrow]));
-      asm volatile("ds_write_b32 %0, %1" ::"v"(adst), "v"(alpha) : "memory");
+    for (int b = 0; b < RB; ++b) {
+      const f32x4 y0 = st[b][0], y1 = st[b][1];
+      float lmax = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(y0[0], y0[1]), __builtin_fmaxf(y0[2], y0[3])),
+                                   __builtin_fmaxf(__builtin_fmaxf(y1[0], y1[1]), __builtin_fmaxf(y1[2], y1[3])));
+      lmax *= scale;
+      // no lane's keys lift its row's maximum: the tile's maximum over the lanes of a row is not needed
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(lmax > m_ref[b] + kLazy) != 0, 0)) {
+        const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
+        float tmax = __builtin_fmaxf(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
+        const SwapPair r32 = permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax));
+        tmax = __builtin_fmaxf(__uint_as_float(r32.x), __uint_as_float(r32.y));
+        const bool raise = tmax > m_ref[b] + kLazy, first = m_ref[b] == kNever;
+        const float alpha = raise && !first ? __builtin_amdgcn_exp2f(m_ref[b] - tmax) : 1.0f;
+        if (raise) m_ref[b] = tmax;
+        l_run[b] *= alpha;
+        const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][(wave * RB + b) * 16 + i16]));
+        asm volatile("ds_write_b32 %0, %1" ::"v"(adst), "v"(alpha) : "memory");  // (the four lanes of a row write the same)
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) flags |= kMoved << b;
+      }
+      ref[b] = m_ref[b] == kNever ? 0.f : m_ref[b];
     }
-    const int any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-    if (lane == 0) {
-      const uint32_t odst = lds_addr(reinterpret_cast<const char*>(&odd_lds[wave]));
-      asm volatile("ds_write_b32 %0, %1" ::"v"(odst), "v"(any_odd) : "memory");
+    const uint32_t fdst = lds_addr(reinterpret_cast<const char*>(&flag_lds[pbuf][wave]));
+    asm volatile("ds_write_b32 %0, %1" ::"v"(fdst), "v"(flags) : "memory");
+  };
+  auto softmax_exp = [&](int i, f32x4 (&st)[RB][2], const float (&ref)[RB]) {  // i of 8 RB weights
+    const int b = i >> 3, mb = (i >> 2) & 1, r = i & 3;
+    st[b][mb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][mb][r], scale, -ref[b]));
+  };
+  auto softmax_end = [&](const f32x4 (&p)[RB][2], int pbuf) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      l_run[b] += ((p[b][0][0] + p[b][0][1]) + (p[b][0][2] + p[b][0][3])) + ((p[b][1][0] + p[b][1][1]) + (p[b][1][2] + p[b][1][3]));
+      // P^T B-fragment: k-slots 8g+0..3 <-> keys 4g+0..3, 8g+4..7 <-> keys 16+4g+0..3
+      const u32x4 w = u32x4{pack2<F16>(p[b][0][0], p[b][0][1]), pack2<F16>(p[b][0][2], p[b][0][3]),
+                            pack2<F16>(p[b][1][0], p[b][1][1]), pack2<F16>(p[b][1][2], p[b][1][3])};
+      asm volatile("ds_write_b128 %0, %1" ::"v"(pdst + pbuf * (NB * 1024) + b * 1024), "v"(w) : "memory");
     }
   };
 
   // ---- O^T += V^T P^T -------------------------------------------------------------
-  f32x4 oacc[MBW][4];
+  f32x4 oacc[MBW][NB];
 #pragma unroll
   for (int j = 0; j < MBW; ++j)
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) oacc[j][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int nb = 0; nb < NB; ++nb) oacc[j][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   // V^T transposing reads: source lane (g, i16) points at key 4g + (i16 >> 2) (+16 for k-slots 4..7), dims d0 + 4 (i16 & 3)
   // with d0 = 16 (4j + wave); chunk 8j + x, x = 2 wave + ((i16 & 3) >> 1) < 8, swizzles to 8j + (x ^ f): a fixed base + 128 j.
   const int tkey = 4 * g + (i16 >> 2);
   const int tx = 2 * wave + ((i16 & 3) >> 1);
   const int tbase = tkey * ROW + 16 * ((tx ^ kv_swz<D>(tkey)) & (SH::CPR - 1)) + 8 * (i16 & 1);
-  auto pv = [&](int t) {
-    const uint32_t pa_ = lds_addr(&p_lds[0]) + lane * 16;
-    bf16x8 pb_[4];
-    pb_[0] = ld128<0>(pa_);
-    pb_[1] = ld128<1024>(pa_);
-    pb_[2] = ld128<2048>(pa_);
-    pb_[3] = ld128<3072>(pa_);
-    const uint32_t ta = lds_addr(kv_lds + (t & 1) * SH::TILE) + tbase;
-    v4i16 lo[2], hi[2];
-    lo[0] = tr_read<0>(ta);
-    hi[0] = tr_read<16 * ROW>(ta);
-    if constexpr (MBW > 1) {
-      lo[1] = tr_read<128>(ta);
-      hi[1] = tr_read<16 * ROW + 128>(ta);
-    }
+  // V^T blocks go through a queue VQ deep; between(j) runs among the MFMAs of output block j.
+  constexpr int VQ = MBW < 3 ? MBW : (RB == 1 ? 4 : 3) < MBW ? (RB == 1 ? 4 : 3) : MBW;
+  auto pv = [&](int slot, int pbuf, auto&& between) {
+    const uint32_t psrc = lds_addr(&p_lds[0][0]) + pbuf * (NB * 1024) + lane * 16;
+    bf16x8 pf[NB];
+    attn_static_for<0, NB>([&](auto NC) {
+      constexpr int nb = decltype(NC)::value;
+      pf[nb] = ld128<1024 * nb>(psrc);
+    });
+    const uint32_t ta = lds_addr(ring(slot)) + tbase;
+    v4i16 lo[VQ], hi[VQ];
+    auto issue = [&](auto JC) {
+      constexpr int j = decltype(JC)::value;
+      lo[j % VQ] = tr_read<128 * j>(ta);
+      hi[j % VQ] = tr_read<16 * ROW + 128 * j>(ta);
+    };
+    attn_static_for<0, VQ>(issue);
     attn_static_for<0, MBW>([&](auto JC) {
       constexpr int j = decltype(JC)::value;
-      if constexpr (j + 1 < MBW) lds_wait<2>(lo[j & 1], hi[j & 1]); else lds_wait<0>(lo[j & 1], hi[j & 1]);
+      constexpr int later = (MBW - 1 - j) < (VQ - 1) ? (MBW - 1 - j) : (VQ - 1);
+      lds_wait<2 * later>(lo[j % VQ], hi[j % VQ]);
       if constexpr (j == 0) {
 #pragma unroll
-        for (int nb = 0; nb < 4; ++nb) reg_tie(pb_[nb]);
+        for (int nb = 0; nb < NB; ++nb) reg_tie(pf[nb]);
       }
-      const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo[j & 1], hi[j & 1], 0, 1, 2, 3, 4, 5, 6, 7));
+      const bf16x8 vf =
+          __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo[j % VQ], hi[j % VQ], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-      for (int nb = 0; nb < 4; ++nb) oacc[j][nb] = mfma16x16x32<F16>(vf, pb_[nb], oacc[j][nb]);
-      if constexpr (j + 2 < MBW) {
-        lo[j & 1] = tr_read<128 * (j + 2)>(ta);
-        hi[j & 1] = tr_read<16 * ROW + 128 * (j + 2)>(ta);
-      }
+      for (int nb = 0; nb < NB; ++nb) oacc[j][nb] = mfma16x16x32<F16>(vf, pf[nb], oacc[j][nb]);
+      if constexpr (j + VQ < MBW) issue(std::integral_constant<int, j + VQ>{});
+      between(JC);
     });
   };
-  // Values of tile t that are not finite become zero, in its LDS (every wave has done with its scores).
-  auto clean_tile = [&](int t) {
-    const uint32_t tile = lds_addr(kv_lds + (t & 1) * SH::TILE);
+  // Values of a tile that are not finite become zero, in its LDS (every wave has done with its scores).
+  auto clean_tile = [&](int slot) {
+    const uint32_t tile = lds_addr(ring(slot));
     for (int e = threadIdx.x; e < SH::CH; e += kPagedThreads) {
       bf16x8 x;
       asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(x) : "v"(tile + e * 16));
@@ -519,80 +639,150 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
   };
 
   // ---- the tiles -------------------------------------------------------------
+  // Iteration t: P V of tile t beside S^T and softmax of tile t + 1, one barrier.  Tile t lives in slot t - tbeg mod NS,
+  // its P in p_lds[t & 1].  The copies of tile t + AHEAD go out at the start, into the slot of tile t - 1, which every
+  // wave has left; they land by the start of iteration t + AHEAD - 1.
   if (tbeg < tend) {
-    int page = load_page(tbeg);
-    bool ok;
-    uint32_t off = row_off(tbeg, page, ok);
-    uint32_t okmask = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
-    copy_tile(tbeg, off);
-    if (tbeg + 1 < tend) page = load_page(tbeg + 1);
-    for (int t = tbeg; t < tend; ++t) {
-      // this wave's copies of tile t (and the page numbers of t + 1) have landed; behind the barrier every wave's have, and
-      // every wave has left tile t - 1 and its P
-      __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
-      attn_tile_barrier();
-      uint32_t ok_next = 0;
-      if (t + 1 < tend) {
-        bool ok1;
-        const uint32_t off1 = row_off(t + 1, page, ok1);
-        ok_next = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok1));
-        copy_tile(t + 1, off1);
-        if (t + 2 < tend) page = load_page(t + 2);
-      }
-      f32x4 st[2];
-      qk(t, st);
-      softmax(t, okmask, st);
-      attn_tile_barrier();  // P, alpha published
-      float al[4];
-      int odd[4];
-      {
-        const uint32_t asrc = lds_addr(reinterpret_cast<const char*>(&alpha_lds[i16]));
-        asm volatile("ds_read_b32 %0, %4\n\tds_read_b32 %1, %4 offset:64\n\tds_read_b32 %2, %4 offset:128\n\t"
-                     "ds_read_b32 %3, %4 offset:192\n\ts_waitcnt lgkmcnt(0)"
-                     : "=&v"(al[0]), "=&v"(al[1]), "=&v"(al[2]), "=&v"(al[3])
-                     : "v"(asrc));
-        const uint32_t osrc = lds_addr(reinterpret_cast<const char*>(&odd_lds[0]));
-        u32x4 o4;
-        asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(o4) : "v"(osrc));
+    skey = tbeg < n1 ? k1lo + tbeg * 32 : (tbeg - n1) * 32;
+    __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));  // page numbers (and Q)
+    uint32_t okq[AHEAD];
+    uint32_t src[SH::LPT];
 #pragma unroll
-        for (int nb = 0; nb < 4; ++nb) odd[nb] = __builtin_amdgcn_readfirstlane(static_cast<int>(o4[nb]));
+    for (int i = 0; i < AHEAD; ++i) {
+      okq[i] = 0;
+      if (tbeg + i < tend) {
+        int page;
+        asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(page) : "v"(page_addr(tbeg + i)));
+        from = froms[i];
+        okq[i] = address_tile(page, within[i], src);
+        attn_static_for<0, SH::LPT>([&](auto IC) { copy(src, ring(i) + wave * 1024, IC); });
       }
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(al[0] != 1.0f || al[1] != 1.0f || al[2] != 1.0f || al[3] != 1.0f) != 0, 0)) {
-#pragma unroll
-        for (int j = 0; j < MBW; ++j)
-#pragma unroll
-          for (int nb = 0; nb < 4; ++nb) oacc[j][nb] = oacc[j][nb] * al[nb];
-      }
-      if (__builtin_expect((odd[0] | odd[1] | odd[2] | odd[3]) != 0, 0)) {
-        clean_tile(t);
-        attn_tile_barrier();
-      }
-      pv(t);
-      okmask = ok_next;
     }
+    uint32_t in_next = within[AHEAD];
+    from = froms[AHEAD];
+    if (tbeg + AHEAD <= tend) __builtin_amdgcn_s_waitcnt(vm_lgkm0((AHEAD - 1) * (SH::CH / SH::NT)));
+    else __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
+    attn_tile_barrier();  // the first tile landed
+    f32x4 st[RB][2];
+    float ref[RB];
+    qk(0, st, [] {}, [](auto) {});
+    softmax_begin(tbeg, okq[0], st, ref, tbeg & 1);
+#pragma unroll
+    for (int i = 0; i < 8 * RB; ++i) softmax_exp(i, st, ref);
+    softmax_end(st, tbeg & 1);
+    int slot = 0;  // of tile t
+    // MORE: a tile t + 1; COPY: a tile t + AHEAD
+    auto iteration = [&](int t, auto MORE, auto COPY) {
+      constexpr bool more = decltype(MORE)::value, ahead = decltype(COPY)::value;
+      // tile t + 1 (and the page numbers of tile t + AHEAD) landed; with three tiles ahead the copies of the last stay in
+      // flight.  Behind the barrier: every wave's, and every wave's P of tile t.
+      if (AHEAD >= 3 && ahead) __builtin_amdgcn_s_waitcnt(vm_lgkm0(SH::CH / SH::NT));
+      else __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
+      attn_tile_barrier();
+      const int next = slot + 1 == NS ? 0 : slot + 1, last_slot = slot == 0 ? NS - 1 : slot - 1;
+      int flags = 0;
+      uint32_t ok_new = 0;
+      char* dst = ring(last_slot) + wave * 1024;
+      auto start = [&] {
+        u32x4 fl;
+        int page;
+        asm volatile("ds_read_b32 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(page), "=&v"(fl)
+                     : "v"(page_addr(t + AHEAD)), "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[t & 1][0]))));
+        flags = __builtin_amdgcn_readfirstlane(static_cast<int>(fl[0] | fl[1] | fl[2] | fl[3]));
+        if constexpr (ahead) {
+          ok_new = address_tile(page, in_next, src);
+          in_next = fetch_pages();  // (past the share's end: the same page again, not used)
+        }
+      };
+      if constexpr (more) {
+        // (the copies spread over the k-steps: in one go each waits for the one before to leave the queue)
+        qk(next, st, start, [&](auto KC) {
+          constexpr int ks = decltype(KC)::value;
+          if constexpr (ahead) {
+            constexpr int first = ks * SH::LPT / KS, end = (ks + 1) * SH::LPT / KS;
+            attn_static_for<first, end>([&](auto IC) { copy(src, dst, IC); });
+          }
+        });
+      } else {
+        start();
+      }
+      if constexpr (ahead) from = from_next;
+      if (__builtin_expect(flags != 0, 0)) {
+        if (flags >= kMoved) {
+          // a wave's alpha is of this tile where the wave says so
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float al;
+            int f;
+            asm volatile("ds_read_b32 %0, %2\n\tds_read_b32 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(al), "=&v"(f)
+                         : "v"(lds_addr(reinterpret_cast<const char*>(&alpha_lds[t & 1][nb * 16 + i16]))),
+                           "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[t & 1][nb / RB]))));
+            al = f & (kMoved << (nb % RB)) ? al : 1.0f;
+#pragma unroll
+            for (int j = 0; j < MBW; ++j) oacc[j][nb] = oacc[j][nb] * al;
+          }
+        }
+        if (flags & kOdd) {
+          clean_tile(slot);
+          attn_tile_barrier();
+        }
+      }
+      constexpr bool BESIDE = RB == 1 || D < 576;  // (registers)
+      constexpr int EPB = MBW > 2 ? (8 * RB + MBW - 3) / (MBW > 2 ? MBW - 2 : 1) : 8 * RB;  // weights beside an output block
+      if constexpr (more && !BESIDE) {
+        softmax_begin(t + 1, okq[1 % AHEAD], st, ref, (t + 1) & 1);
+#pragma unroll
+        for (int i = 0; i < 8 * RB; ++i) softmax_exp(i, st, ref);
+        softmax_end(st, (t + 1) & 1);
+      }
+      pv(slot, t & 1, [&](auto JC) {
+        constexpr int j = decltype(JC)::value;
+        if constexpr (more && BESIDE) {
+          if constexpr (j == 0) softmax_begin(t + 1, okq[1 % AHEAD], st, ref, (t + 1) & 1);
+          constexpr int first = MBW > 2 ? (j - 1) * EPB : 0;
+          if constexpr (j > 0 || MBW == 1) {
+#pragma unroll
+            for (int i = first < 0 ? 0 : first; i < first + EPB && i < 8 * RB; ++i) softmax_exp(i, st, ref);
+          }
+          if constexpr (j + 1 == MBW) softmax_end(st, (t + 1) & 1);
+        }
+      });
+#pragma unroll
+      for (int i = 0; i + 1 < AHEAD; ++i) okq[i] = okq[i + 1];
+      okq[AHEAD - 1] = ok_new;
+      slot = next;
+    };
+    int t = tbeg;
+    for (; t + AHEAD < tend; ++t) iteration(t, std::true_type{}, std::true_type{});
+    for (; t + 1 < tend; ++t) iteration(t, std::true_type{}, std::false_type{});
+    iteration(t, std::false_type{}, std::false_type{});
   }
-
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");  // (the last MFMAs' wait states, see mfma_result_fence)
 
   // ---- the result ----------------------------------------------------------------
-  float l_tot = l_run;
-  {
-    const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_tot), __float_as_uint(l_tot), false, false);
-    l_tot = __uint_as_float(r16[0]) + __uint_as_float(r16[1]);
-    const SwapPair r32 = permlane32_swap(__float_as_uint(l_tot), __float_as_uint(l_tot));
-    l_tot = __uint_as_float(r32.x) + __uint_as_float(r32.y);
+  float l_tot[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_run[b]), __float_as_uint(l_run[b]), false, false);
+    l_tot[b] = __uint_as_float(r16[0]) + __uint_as_float(r16[1]);
+    const SwapPair r32 = permlane32_swap(__float_as_uint(l_tot[b]), __float_as_uint(l_tot[b]));
+    l_tot[b] = __uint_as_float(r32.x) + __uint_as_float(r32.y);
   }
   const int64_t flat0 = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(item.first)) * a.H + row0;  // first row of o
   if (shares > 1) {
     const int64_t slot = __builtin_amdgcn_readfirstlane(item.slot);
-    if (g == 0) a.part_ml[slot * kPagedRows + lrow] = float2{m_ref, l_tot};
-    float* po = a.part_o + slot * kPagedRows * D;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+      if (g == 0) a.part_ml[slot * M + (wave * RB + b) * 16 + i16] = float2{m_ref[b], l_tot[b]};
+    float* po = a.part_o + slot * M * D;
 #pragma unroll
     for (int j = 0; j < MBW; ++j) {
       const int mbi = j * kAttnWaves + wave;
       if (SH::MBT % kAttnWaves == 0 || mbi < SH::MBT) {
 #pragma unroll
-        for (int nb = 0; nb < 4; ++nb)
+        for (int nb = 0; nb < NB; ++nb)
           if (nb * 16 < nrows) *reinterpret_cast<f32x4*>(po + (nb * 16 + i16) * D + mbi * 16 + 4 * g) = oacc[j][nb];
       }
     }
@@ -602,150 +792,201 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     }
     return;
   }
-  {
-    const float sink = live ? a.sink[head] : kNever;
+  float* scale_lds = alpha_lds[0];
+  __syncthreads();  // every wave has left the last tile and its alpha
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int lrow = (wave * RB + b) * 16 + i16;
+    const bool live = lrow < nrows;
+    const float sink = live ? a.sink[(row0 + lrow) % a.H] : kNever;
     const float sink2 = sink * kLog2e;
-    const float m_fin = __builtin_fmaxf(m_ref, sink2);
-    const float ref = m_fin == kNever ? 0.f : m_fin;
-    const float resc = __builtin_amdgcn_exp2f(m_ref - ref);
-    const float l_fin = l_tot * resc + __builtin_amdgcn_exp2f(sink2 - ref);
+    const float m_fin = __builtin_fmaxf(m_ref[b], sink2);
+    const float top = m_fin == kNever ? 0.f : m_fin;
+    const float resc = __builtin_amdgcn_exp2f(m_ref[b] - top);
+    const float l_fin = l_tot[b] * resc + __builtin_amdgcn_exp2f(sink2 - top);
     if (g == 0) {
       scale_lds[lrow] = l_fin == 0.f ? 0.f : resc / l_fin;
       if (live)
-        a.lse[flat0 + lrow] = l_fin == 0.f ? -1.0e30f : l_tot == 0.f ? sink : (__builtin_amdgcn_logf(l_fin) + ref) * kLn2;
+        a.lse[flat0 + lrow] = l_fin == 0.f ? -1.0e30f : l_tot[b] == 0.f ? sink : (__builtin_amdgcn_logf(l_fin) + top) * kLn2;
     }
   }
-  __syncthreads();  // scales published, every wave has left the last tile
-  // staged row by row in the tiles' LDS, chunk c of row r at c ^ (r & 7), then written in one piece: the rows follow each
-  // other in o
-  float sc[4];
+  __syncthreads();  // scales published
+  // staged 64 rows at a time in the tiles' LDS, chunk c of row r at c ^ (r & 7), then written in one piece: the rows follow
+  // each other in o
 #pragma unroll
-  for (int nb = 0; nb < 4; ++nb) sc[nb] = scale_lds[nb * 16 + i16];
+  for (int half = 0; half < RB; ++half) {
+    float sc[4];
 #pragma unroll
-  for (int j = 0; j < MBW; ++j) {
-    const int mbi = j * kAttnWaves + wave;
-    if (SH::MBT % kAttnWaves == 0 || mbi < SH::MBT) {
+    for (int nb = 0; nb < 4; ++nb) sc[nb] = scale_lds[(4 * half + nb) * 16 + i16];
 #pragma unroll
-      for (int nb = 0; nb < 4; ++nb) {
-        const int row = nb * 16 + i16;
-        uint2 w;
-        w.x = pack2<F16>(oacc[j][nb][0] * sc[nb], oacc[j][nb][1] * sc[nb]);
-        w.y = pack2<F16>(oacc[j][nb][2] * sc[nb], oacc[j][nb][3] * sc[nb]);
-        *reinterpret_cast<uint2*>(kv_lds + kv_off<D>(row, 2 * mbi + (g >> 1)) + 8 * (g & 1)) = w;
+    for (int j = 0; j < MBW; ++j) {
+      const int mbi = j * kAttnWaves + wave;
+      if (SH::MBT % kAttnWaves == 0 || mbi < SH::MBT) {
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb) {
+          const f32x4 v = oacc[j][4 * half + nb] * sc[nb];
+          uint2 w;
+          w.x = pack2<F16>(v[0], v[1]);
+          w.y = pack2<F16>(v[2], v[3]);
+          *reinterpret_cast<uint2*>(kv_lds + kv_off<D>(nb * 16 + i16, 2 * mbi + (g >> 1)) + 8 * (g & 1)) = w;
+        }
       }
     }
+    __syncthreads();
+    char* obase = reinterpret_cast<char*>(a.o + (flat0 + 64 * half) * D);
+    const int n = min(nrows - 64 * half, 64);
+    for (int e = threadIdx.x; e < n * SH::CPR; e += kPagedThreads)
+      *reinterpret_cast<u32x4*>(obase + static_cast<int64_t>(e) * 16) =
+          *reinterpret_cast<const u32x4*>(kv_lds + kv_off<D>(e / SH::CPR, e % SH::CPR));
+    if (half + 1 < RB) __syncthreads();
   }
-  __syncthreads();
-  char* obase = reinterpret_cast<char*>(a.o + flat0 * D);
-  for (int e = threadIdx.x; e < nrows * SH::CPR; e += kPagedThreads)
-    *reinterpret_cast<u32x4*>(obase + static_cast<int64_t>(e) * 16) =
-        *reinterpret_cast<const u32x4*>(kv_lds + kv_off<D>(e / SH::CPR, e % SH::CPR));
 }
 
-// Joins the shares of the split row blocks: a wave for each row, lanes along the dimensions.  Bound: the partial outputs,
-// read once (they fit the last-level cache).
+// Joins the shares of the split row blocks.  A thread takes four dimensions of a row and every fourth share, eight of them
+// in flight, with a running maximum; the four threads of a place join theirs in LDS.  Bound: the partial outputs, read
+// once (they fit the last-level cache).
 template <bool F16>
-__global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnArgs a, int D) {
+__global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnArgs a, int D, int M) {
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float lds[3][6][64];
+  const int at = threadIdx.x & 63, part = threadIdx.x >> 6;
   const int count = a.rec[0];
+  const int vec = D / 4;
+  const int e = static_cast<int>(blockIdx.x) * 64 + at;  // (a block's places fill whole workgroups: 64 divides M)
+  const int row = e / vec, d = (e - row * vec) * 4;
   for (int b = blockIdx.y; b < count; b += gridDim.y) {
     const int4 rec = *reinterpret_cast<const int4*>(a.rec + 4 + 4 * static_cast<int64_t>(b));
-    const int row = blockIdx.x * 4 + wave;
-    if (row >= rec.w) continue;
-    const int64_t flat = static_cast<int64_t>(rec.z) + row;
-    const float sink = a.sink[flat % a.H];
-    const float sink2 = sink * kLog2e;
-    const float2* ml = a.part_ml + static_cast<int64_t>(rec.x) * kPagedRows + row;
-    float m = sink2;
-    for (int i = 0; i < rec.y; ++i) m = __builtin_fmaxf(m, ml[static_cast<int64_t>(i) * kPagedRows].x);
-    const float ref = m == kNever ? 0.f : m;
-    float keys = 0.f;
-    for (int i = 0; i < rec.y; ++i) {
-      const float2 v = ml[static_cast<int64_t>(i) * kPagedRows];
-      keys = __builtin_fmaf(v.y, __builtin_amdgcn_exp2f(v.x - ref), keys);
-    }
-    const float l = keys + __builtin_amdgcn_exp2f(sink2 - ref);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int d = lane * 4; d < D; d += 256) {
-      const float* po = a.part_o + (static_cast<int64_t>(rec.x) * kPagedRows + row) * D + d;
-      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int i0 = 0; i0 < rec.y; i0 += 8) {
+    if (static_cast<int>(blockIdx.x) * 64 / vec >= rec.w) continue;  // (the same in every thread)
+    const bool live = row < rec.w;
+    float m = kNever, l = 0.f;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      const float2* ml = a.part_ml + static_cast<int64_t>(rec.x) * M + row;
+      const float* po = a.part_o + (static_cast<int64_t>(rec.x) * M + row) * D + d;
+      for (int i0 = part; i0 < rec.y; i0 += 32) {
+        float2 v[8];
         f32x4 x[8];
-        float w[8];
+        float top = m;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          const int i = i0 + u < rec.y ? i0 + u : rec.y - 1;
-          x[u] = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * kPagedRows * D);
-          w[u] = ml[static_cast<int64_t>(i) * kPagedRows].x;
+          const int i = i0 + 4 * u < rec.y ? i0 + 4 * u : i0;
+          v[u] = ml[static_cast<int64_t>(i) * M];
+          x[u] = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * M * D);
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (i0 + u >= rec.y) continue;
-          const float e = __builtin_amdgcn_exp2f(w[u] - ref);
+        for (int u = 0; u < 8; ++u) top = __builtin_fmaxf(top, v[u].x);
+        const float ref = top == kNever ? 0.f : top;
+        const float s = __builtin_amdgcn_exp2f(m - ref);
+        l *= s;
+        acc *= s;
+        m = top;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(x[u][c], e, acc[c]);
+        for (int u = 0; u < 8; ++u) {
+          const float w = i0 + 4 * u < rec.y ? __builtin_amdgcn_exp2f(v[u].x - ref) : 0.f;
+          if (i0 + 4 * u < rec.y) {
+            l = __builtin_fmaf(v[u].y, w, l);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(x[u][c], w, acc[c]);
+          }
         }
       }
+    }
+    if (part > 0) {
+      float* p = &lds[part - 1][0][at];
+      p[0] = m;
+      p[64] = l;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) p[64 * (2 + c)] = acc[c];
+    }
+    __syncthreads();
+    if (part == 0 && live) {
+      const int64_t flat = static_cast<int64_t>(rec.z) + row;
+      const float sink = a.sink[flat % a.H];
+      const float sink2 = sink * kLog2e;
+      float top = __builtin_fmaxf(m, sink2);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) top = __builtin_fmaxf(top, lds[q][0][at]);
+      const float ref = top == kNever ? 0.f : top;
+      float w = __builtin_amdgcn_exp2f(m - ref);
+      float keys = l * w;
+      acc *= w;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        w = __builtin_amdgcn_exp2f(lds[q][0][at] - ref);
+        keys = __builtin_fmaf(lds[q][1][at], w, keys);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(lds[q][2 + c][at], w, acc[c]);
+      }
+      const float all = keys + __builtin_amdgcn_exp2f(sink2 - ref);
+      const float inv = all == 0.f ? 0.f : 1.f / all;
       uint2 o;
       o.x = pack2<F16>(acc[0] * inv, acc[1] * inv);
       o.y = pack2<F16>(acc[2] * inv, acc[3] * inv);
       *reinterpret_cast<uint2*>(a.o + flat * D + d) = o;
+      if (d == 0)
+        a.lse[flat] = all == 0.f ? -1.0e30f : keys == 0.f ? sink : (__builtin_amdgcn_logf(all) + ref) * kLn2;
     }
-    if (lane == 0)
-      a.lse[flat] = l == 0.f ? -1.0e30f : keys == 0.f ? sink : (__builtin_amdgcn_logf(l) + ref) * kLn2;
+    __syncthreads();  // the next block's partial sums take the same LDS
   }
-}
-
-template <int D>
-static int launch_paged_attn_d(bool f16, const PagedAttnArgs& a, int64_t blocks, int64_t split_blocks, hipStream_t st) {
-  if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true>), dim3(static_cast<unsigned>(blocks)), dim3(kPagedThreads), 0, st, a);
-  else hipLaunchKernelGGL((paged_attn_kernel<D, false>), dim3(static_cast<unsigned>(blocks)), dim3(kPagedThreads), 0, st, a);
-  int rc = check_launch("paged_attn_kernel");
-  if (rc || !a.part_o) return rc;
-  const dim3 grid(kPagedRows / 4, static_cast<unsigned>(split_blocks));
-  if (f16) hipLaunchKernelGGL(paged_combine_kernel<true>, grid, dim3(kPagedThreads), 0, st, a, D);
-  else hipLaunchKernelGGL(paged_combine_kernel<false>, grid, dim3(kPagedThreads), 0, st, a, D);
-  return check_launch("paged_combine_kernel");
 }
 
 static bool served(int64_t D) { return D == 32 || D == 64 || D == 128 || D == 256 || D == 512 || D == 576; }
 
 // Sizes of a call, from what the host knows.
-struct PagedPlan {
-  int64_t blocks;        // row blocks at most
-  int64_t want;          // workgroups that run at once
+struct PagedSizes {
+  int rb;                // row blocks of 16 of a wave
+  int64_t blocks;        // row blocks of a workgroup at most
+  int want_log2;         // workgroups that run at once
   int64_t grid;          // workgroups
   int64_t items;         // partial outputs at most, 0: no row block is split
   int64_t split_blocks;  // split row blocks at most
   int64_t bytes;         // scratch
+  int behind;            // tokens of a row block before its last one at most
 };
-constexpr int kLeastTiles = 4;  // tiles of a share at least
+constexpr int kLeastTiles = 8;  // tiles of a share at least
 
-static PagedPlan paged_plan_of(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys1, int64_t keys2) {
-  PagedPlan p{};
-  // a request's last row block is part empty unless 64 divides n H
-  int64_t g = kPagedRows;
+static PagedSizes paged_sizes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys1, int64_t keys2) {
+  PagedSizes p{};
+  p.rb = 1;
+  const int64_t M = 64 * p.rb;
+  // a request's last row block is part empty unless M divides n H
+  int64_t g = M;
   while (H % g) g /= 2;
-  p.blocks = (N * H + (R < N ? R : N) * (kPagedRows - g)) / kPagedRows;
-  p.want = 256 * per_cu(static_cast<int>(D));
-  p.grid = 2 * p.blocks <= p.want ? p.want : p.blocks + p.want;
+  p.blocks = (N * H + (R < N ? R : N) * (M - g)) / M;
+  p.want_log2 = 8 + (D >= 512 ? 0 : D >= 128 ? 1 : 2);
+  const int64_t want = int64_t{1} << p.want_log2;
+  p.grid = 2 * p.blocks <= want ? want : p.blocks + want;
   // tiles of a row block at most
-  const int64_t span = kPagedRows / H + 1 + window;
+  const int64_t span = M / H + 1 + window;
+  p.behind = static_cast<int>((M - 1) / H);
   const int64_t tiles = ((window < keys1 && span < keys1 ? span : keys1) + 31) / 32 + (keys2 + 31) / 32;
   if (tiles <= kLeastTiles) {
     p.grid = p.blocks;
     return p;
   }
   // shares of split row blocks: sum of ceil(tiles / c) <= 2 sum tiles / c <= 2 want, where tiles > c >= U / want
-  p.items = 2 * p.want;
+  p.items = 2 * want;
   const int64_t each = p.blocks * ((tiles + kLeastTiles - 1) / kLeastTiles);
   if (each < p.items) p.items = each;
   p.split_blocks = p.items / 2;
   if (p.blocks < p.split_blocks) p.split_blocks = p.blocks;
-  if (2 * p.blocks <= p.want && each < p.grid) p.grid = each;
-  p.bytes = p.items * kPagedRows * (D * 4 + 8) + 16 * (p.split_blocks + 1);
+  if (2 * p.blocks <= want && each < p.grid) p.grid = each;
+  p.bytes = p.items * M * (D * 4 + 8) + 16 * (p.split_blocks + 1);
   return p;
+}
+
+template <int D>
+static int launch_paged_attn_d(bool f16, const PagedAttnArgs& a, const PagedSizes& p, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(p.grid < 1 ? 1 : p.grid)), block(kPagedThreads);
+  if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true, 1>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((paged_attn_kernel<D, false, 1>), grid, block, 0, st, a);
+  const int rc = check_launch("paged_attn_kernel");
+  if (rc || !a.part_o) return rc;
+  const int M = 64 * p.rb;
+  const dim3 cgrid(static_cast<unsigned>(M * (D / 4) / 64), static_cast<unsigned>(p.split_blocks));
+  if (f16) hipLaunchKernelGGL(paged_combine_kernel<true>, cgrid, block, 0, st, a, D, M);
+  else hipLaunchKernelGGL(paged_combine_kernel<false>, cgrid, block, 0, st, a, D, M);
+  return check_launch("paged_combine_kernel");
 }
 
 }  // namespace si
@@ -763,7 +1004,7 @@ extern "C" int64_t si_paged_attn_fwd_scratch_bytes(int64_t N, int64_t H, int64_t
   if (N <= 0 || H <= 0 || R <= 0 || window < 0 || keys < 0 || keys2 < 0 || !served(D) || N > lim || H > lim ||
       N * H > lim || R > lim)
     return 0;
-  return paged_plan_of(N, H, D, R, window == 0 || window > lim ? lim : window, keys < lim ? keys : lim,
+  return paged_sizes(N, H, D, R, window == 0 || window > lim ? lim : window, keys < lim ? keys : lim,
                        keys2 < lim ? keys2 : lim).bytes;
 }
 
@@ -790,11 +1031,12 @@ static int set_cache(PagedCache& c, const void* base, const int64_t* strides, in
   c.tstride = tstride;
   c.pstride = static_cast<uint32_t>(strides[0] / 8);
   c.rstride = static_cast<uint32_t>(strides[1] / 8);
-  c.P = static_cast<int>(P);
   c.pages = P > 0 ? static_cast<int>(pages) : 0;
+  c.keys = static_cast<int>(cache_keys(pages, P, ps));
   c.ps = static_cast<uint32_t>(ps);
   c.magic = 0;
   c.shift = 0;
+  c.one = ps == 1 ? ~0u : 0u;
   if (ps > 1) {
     // l = ceil(log2 ps): magic = ceil(2^(31 + l) / ps) is below 2^32 and exceeds 2^(31 + l) / ps by less than one, so
     // for key < 2^31 the product is off by less than 2^31 <= 2^(31 + l) / ps and the quotient is exact
@@ -851,26 +1093,27 @@ extern "C" int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const 
   a.H = static_cast<int>(H);
   a.R = static_cast<int>(R);
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  PagedPlan p = paged_plan_of(N, H, D, R > 0 ? R : 1, a.window, cache_keys(pages, P, page_size),
-                              ratio > 0 ? cache_keys(pages2, P2, page_size2) : 0);
-  a.want = static_cast<int>(p.want);
+  PagedSizes p = paged_sizes(N, H, D, R > 0 ? R : 1, a.window, cache_keys(pages, P, page_size),
+                             ratio > 0 ? cache_keys(pages2, P2, page_size2) : 0);
+  a.want_log2 = p.want_log2;
   a.least = kLeastTiles;
+  a.behind = p.behind;
   if (p.bytes > 0 && scratch && scratch_bytes >= p.bytes) {
+    const int64_t M = 64 * p.rb;
     a.part_o = static_cast<float*>(scratch);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + p.items * kPagedRows * D);
-    a.rec = reinterpret_cast<int32_t*>(a.part_ml + p.items * kPagedRows);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + p.items * M * D);
+    a.rec = reinterpret_cast<int32_t*>(a.part_ml + p.items * M);
   } else {
     p.grid = p.blocks;
   }
-  if (p.grid < 1) p.grid = 1;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool f16 = qkv_dtype == SI_DTYPE_F16;
   switch (D) {
-    case 32: return launch_paged_attn_d<32>(f16, a, p.grid, p.split_blocks, st);
-    case 64: return launch_paged_attn_d<64>(f16, a, p.grid, p.split_blocks, st);
-    case 128: return launch_paged_attn_d<128>(f16, a, p.grid, p.split_blocks, st);
-    case 256: return launch_paged_attn_d<256>(f16, a, p.grid, p.split_blocks, st);
-    case 512: return launch_paged_attn_d<512>(f16, a, p.grid, p.split_blocks, st);
-    default: return launch_paged_attn_d<576>(f16, a, p.grid, p.split_blocks, st);
+    case 32: return launch_paged_attn_d<32>(f16, a, p, st);
+    case 64: return launch_paged_attn_d<64>(f16, a, p, st);
+    case 128: return launch_paged_attn_d<128>(f16, a, p, st);
+    case 256: return launch_paged_attn_d<256>(f16, a, p, st);
+    case 512: return launch_paged_attn_d<512>(f16, a, p, st);
+    default: return launch_paged_attn_d<576>(f16, a, p, st);
   }
 }

@@ -19,6 +19,7 @@ graph and replayed with other lengths.  Lengths stay below 2^31.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -41,33 +42,60 @@ class PagedPlan(NamedTuple):
     free_next: torch.Tensor  # [1] int32: position in the free list after this step
 
 
-def _int32(t: torch.Tensor, name: str, shape) -> torch.Tensor:
-    if t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
-    assert tuple(t.shape) == tuple(shape), f"{name} must be {list(shape)}, got {list(t.shape)}"
-    return t.to(torch.int32).contiguous()
+def _check_devices(dev: torch.device, **tensors) -> None:
+    """Every tensor on ``dev``, a GPU; its names are looked at only where one is not."""
+    at = dev.index
+    for t in tensors.values():
+        if t is not None and t.get_device() != at:
+            _check_device(dev, **tensors)
 
 
-def _check_table(table: torch.Tensor, name: str, R: int) -> None:
-    if table.dtype != torch.int32:
+def _int32(t: torch.Tensor, name: str, n: int) -> torch.Tensor:
+    assert t.dim() == 1 and t.shape[0] == n, f"{name} must be [{n}], got {list(t.shape)}"
+    if t.dtype is not torch.int32:
+        if t.dtype is not torch.int64:
+            raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _table_stride(table: torch.Tensor, name: str, R: int) -> int:
+    """Stride of the rows of a ``[R, P]`` block table."""
+    if table.dtype is not torch.int32:
         raise ValueError(f"{name} must be int32, got {table.dtype}")
     assert table.dim() == 2 and table.shape[0] == R, f"{name} must be [{R}, P], got {list(table.shape)}"
-    if table.shape[1] > 1 and table.stride(1) != 1:
+    s, one = table.stride()
+    if one != 1 and table.shape[1] > 1:
         raise ValueError(f"{name} needs contiguous rows")
+    return s if R > 1 else table.shape[1]
 
 
-def _check_cache(cache: torch.Tensor, name: str) -> None:
-    assert cache.dim() == 3, f"{name} must be [pages, page_size, width]"
-    if cache.shape[1] < 1:
-        raise ValueError(f"{name} needs a page size of at least 1")
+def _check_slots(slots: torch.Tensor, n: int) -> torch.Tensor:
+    if slots.dtype is not torch.int64:
+        raise ValueError(f"slots must be int64, got {slots.dtype}")
+    assert slots.dim() == 1 and slots.shape[0] == n, f"slots must be [{n}], got {list(slots.shape)}"
+    return slots if slots.is_contiguous() else slots.contiguous()
 
 
-def _cache_strides(t: torch.Tensor):
+def _cache_strides(cache: torch.Tensor, name: str):
     """Page, row and element stride, with those that a size of one leaves free as for packed rows."""
-    n, p, w = t.shape
-    sw = t.stride(2) if w > 1 else 1
-    sp = t.stride(1) if p > 1 else w
-    return (t.stride(0) if n > 1 else sp * p, sp, sw)
+    assert cache.dim() == 3, f"{name} must be [pages, page_size, width]"
+    n, p, w = cache.shape
+    if p < 1:
+        raise ValueError(f"{name} needs a page size of at least 1")
+    s = cache.stride()
+    if n > 1 and p > 1 and w > 1:
+        return s
+    sw = s[2] if w > 1 else 1
+    sp = s[1] if p > 1 else w
+    return (s[0] if n > 1 else sp * p, sp, sw)
+
+
+def _check_apart(strides, pages: int, page_size: int, width: int) -> None:
+    """A cache that is written: no two rows share memory."""
+    sp, sr, se = strides
+    if se != 1 or sr < width or (pages > 1 and sp < sr * (page_size - 1) + width):
+        raise ValueError("the cache's rows must be contiguous and apart")
 
 
 def paged_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -91,28 +119,26 @@ def paged_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     """
     assert ctx_lens.is_cuda
     dev = ctx_lens.device
-    _check_device(dev, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_start=free_start)
+    _check_devices(dev, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_start=free_start)
     assert ctx_lens.dim() == 1 and free_pages.dim() == 1
-    R = ctx_lens.shape[0]
-    ctx, new = _int32(ctx_lens, "ctx_lens", (R,)), _int32(new_lens, "new_lens", (R,))
-    _check_table(block_table, "block_table", R)
-    free_pages = _int32(free_pages, "free_pages", free_pages.shape)
+    R, F = ctx_lens.shape[0], free_pages.shape[0]
+    ctx, new = _int32(ctx_lens, "ctx_lens", R), _int32(new_lens, "new_lens", R)
+    stride, P = _table_stride(block_table, "block_table", R), block_table.shape[1]
+    free_pages = _int32(free_pages, "free_pages", F)
     if free_start is not None:
-        free_start = _int32(free_start, "free_start", (1,))
+        free_start = _int32(free_start, "free_start", 1)
     if page_size < 1 or ratio < 1 or num_rows < 0:
         raise ValueError(f"page_size and ratio must be positive and num_rows not negative, got {page_size}, {ratio}, {num_rows}")
-    P = block_table.shape[1]
-    i32 = {"dtype": torch.int32, "device": dev}
-    cu, seq, nxt = torch.empty(R + 1, **i32), torch.empty(R, **i32), torch.empty(1, **i32)
-    req, pos = torch.empty(num_rows, **i32), torch.empty(num_rows, **i32)
-    slots = torch.empty(num_rows, dtype=torch.int64, device=dev)
     L = _lib.load()
     with _lib.on_device(dev):
-        rc = L.si_paged_plan(ctx.data_ptr(), new.data_ptr(), R, ratio, block_table.data_ptr(),
-                             block_table.stride(0) if R > 1 else P, P, free_pages.data_ptr(), free_pages.shape[0],
-                             None if free_start is None else free_start.data_ptr(), page_size, num_rows, cu.data_ptr(),
-                             seq.data_ptr(), slots.data_ptr(), req.data_ptr(), pos.data_ptr(), nxt.data_ptr(),
-                             _lib.stream_ptr(dev))
+        # (one allocation for the five int32 lists: each is 2 us)
+        lists = torch.empty(2 * (R + 1 + num_rows), dtype=torch.int32, device=dev)
+        cu, seq, nxt, req, pos = torch.unsafe_split_with_sizes(lists, [R + 1, R, 1, num_rows, num_rows])
+        slots = torch.empty(num_rows, dtype=torch.int64, device=dev)
+        rc = L.si_paged_plan(ctx.data_ptr(), new.data_ptr(), R, ratio, block_table.data_ptr(), stride, P,
+                             free_pages.data_ptr(), F, None if free_start is None else free_start.data_ptr(), page_size,
+                             num_rows, cu.data_ptr(), seq.data_ptr(), slots.data_ptr(), req.data_ptr(), pos.data_ptr(),
+                             nxt.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc)
     return PagedPlan(cu, seq, slots, req, pos, nxt)
 
@@ -125,26 +151,24 @@ def paged_write(rows: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) ->
     """
     assert rows.is_cuda
     dev = rows.device
-    _check_device(dev, cache=cache, slots=slots)
-    _check_cache(cache, "cache")
-    assert rows.dim() == 2 and rows.shape[1] == cache.shape[2], "rows must be [N, width of the cache]"
-    if rows.dtype != cache.dtype:
-        raise ValueError(f"rows and cache must share one type, got {rows.dtype} and {cache.dtype}")
-    if slots.dtype != torch.int64:
-        raise ValueError(f"slots must be int64, got {slots.dtype}")
-    assert tuple(slots.shape) == (rows.shape[0],), "slots must be [N]"
+    _check_devices(dev, cache=cache, slots=slots)
+    st = _cache_strides(cache, "cache")
     pages, ps, width = cache.shape
-    sp, sr, se = _cache_strides(cache)
-    if se != 1 or sr < width or (pages > 1 and sp < sr * (ps - 1) + width):
-        raise ValueError("the cache's rows must be contiguous and apart")
-    if rows.shape[1] > 1 and rows.stride(1) != 1:
+    assert rows.dim() == 2 and rows.shape[1] == width, "rows must be [N, width of the cache]"
+    if rows.dtype is not cache.dtype:
+        raise ValueError(f"rows and cache must share one type, got {rows.dtype} and {cache.dtype}")
+    N = rows.shape[0]
+    slots = _check_slots(slots, N)
+    _check_apart(st, pages, ps, width)
+    rs, one = rows.stride()
+    if (one != 1 and width > 1) or rs < 0:
         rows = rows.contiguous()
-    slots = slots.contiguous()
+        rs = width
     size = cache.element_size()
     L = _lib.load()
     with _lib.on_device(dev):
-        rc = L.si_paged_write(rows.data_ptr(), rows.stride(0) * size, slots.data_ptr(), rows.shape[0], width * size,
-                              cache.data_ptr(), sp * size, sr * size, pages, ps, _lib.stream_ptr(dev))
+        rc = L.si_paged_write(rows.data_ptr(), rs * size, slots.data_ptr(), N, width * size, cache.data_ptr(), st[0] * size,
+                              st[1] * size, pages, ps, _lib.stream_ptr(dev))
     _lib.check(rc)
     return cache
 
@@ -170,49 +194,46 @@ def paged_compress(c_a: torch.Tensor, z_a: torch.Tensor, b_a: torch.Tensor, bloc
     """
     assert c_a.is_cuda
     dev = c_a.device
-    _check_device(dev, z_a=z_a, b_a=b_a, block_table=block_table, request=request, positions=positions, cache=cache,
-                  slots=slots, c_b=c_b, z_b=z_b, b_b=b_b)
+    _check_devices(dev, z_a=z_a, b_a=b_a, block_table=block_table, request=request, positions=positions, cache=cache,
+                   slots=slots, c_b=c_b, z_b=z_b, b_b=b_b)
+    dtype = c_a.dtype
     dt = _dtype_code(c_a)
-    given = [t is not None for t in (c_b, z_b, b_b)]
-    if any(given) and not all(given):
+    overlap = c_b is not None
+    if overlap != (z_b is not None) or overlap != (b_b is not None):
         raise ValueError("overlapping entries need c_b, z_b and b_b")
-    overlap = all(given)
-    _check_cache(c_a, "c_a")
-    _check_cache(cache, "cache")
+    st = [_cache_strides(c_a, "c_a")]
     pages, ps, C = c_a.shape
     for n, t in (("z_a", z_a), ("c_b", c_b), ("z_b", z_b)):
-        if t is not None and (t.shape != c_a.shape or t.dtype != c_a.dtype):
-            raise ValueError(f"{n} must match c_a")
-    if cache.dtype != c_a.dtype or cache.shape[2] != C:
+        if t is not None:
+            if t.shape != c_a.shape or t.dtype is not dtype:
+                raise ValueError(f"{n} must match c_a")
+            st.append(_cache_strides(t, n))
+    st.append(_cache_strides(cache, "cache"))
+    epages, eps, width = cache.shape
+    if cache.dtype is not dtype or width != C:
         raise ValueError("cache must have the streams' type and width")
+    if any(s[2] != 1 for s in st):
+        raise ValueError("the streams and the cache need a contiguous last dimension")
+    _check_apart(st[-1], epages, eps, C)
     m = b_a.shape[0]
     if b_a.dim() != 2 or b_a.shape[1] != C or m < 1 or (overlap and b_b.shape != b_a.shape):
         raise ValueError(f"biases must be [m, {C}]")
-    E = request.shape[0]
-    request, positions = _int32(request, "request", (E,)), _int32(positions, "positions", (E,))
-    if slots.dtype != torch.int64:
-        raise ValueError(f"slots must be int64, got {slots.dtype}")
-    assert tuple(slots.shape) == (E,), "slots must be [E]"
-    slots = slots.contiguous()
-    R = block_table.shape[0]
-    _check_table(block_table, "block_table", R)
-    st = [_cache_strides(t) for t in (c_a, z_a, c_b, z_b, cache) if t is not None]
-    if any(s[2] != 1 for s in st):
-        raise ValueError("the streams and the cache need a contiguous last dimension")
-    sp, sr, _ = st[-1]
-    if sr < C or (cache.shape[0] > 1 and sp < sr * (cache.shape[1] - 1) + C):
-        raise ValueError("the cache's rows must be apart")
-    ba = b_a.to(torch.float32).contiguous()
-    bb = b_b.to(torch.float32).contiguous() if overlap else None
+    E, R = request.shape[0], block_table.shape[0]
+    request, positions = _int32(request, "request", E), _int32(positions, "positions", E)
+    slots = _check_slots(slots, E)
+    stride = _table_stride(block_table, "block_table", R)
+    ba = b_a if b_a.dtype is torch.float32 else b_a.float()
+    ba = ba if ba.is_contiguous() else ba.contiguous()
+    bb = b_b.float().contiguous() if overlap else None
     st = [_lib.int64s(*s) for s in st]
     L = _lib.load()
     with _lib.on_device(dev):
         rc = L.si_paged_compress(
             c_a.data_ptr(), st[0], z_a.data_ptr(), st[1], ba.data_ptr(), c_b.data_ptr() if overlap else None,
             st[2] if overlap else None, z_b.data_ptr() if overlap else None, st[3] if overlap else None,
-            bb.data_ptr() if overlap else None, dt, pages, ps, C, m, block_table.data_ptr(), block_table.stride(0), R,
+            bb.data_ptr() if overlap else None, dt, pages, ps, C, m, block_table.data_ptr(), stride, R,
             block_table.shape[1], request.data_ptr(), positions.data_ptr(), slots.data_ptr(), E, cache.data_ptr(), st[-1],
-            cache.shape[0], cache.shape[1], _lib.stream_ptr(dev))
+            epages, eps, _lib.stream_ptr(dev))
     _lib.check(rc)
     return cache
 
@@ -242,56 +263,55 @@ def paged_attn_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
       ``o = 0`` and ``lse = sink`` (or ``-1e30`` if the sink is ``-inf``).  A value that is not finite reaches the rows that
       see its key and no others.
     """
-    assert q.is_cuda and kv_cache.is_cuda
+    assert q.is_cuda
     dev = q.device
-    _check_device(dev, kv_cache=kv_cache, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, attn_sink=attn_sink,
-                  kv2_cache=kv2_cache, block_table2=block_table2)
+    _check_devices(dev, kv_cache=kv_cache, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, attn_sink=attn_sink,
+                   kv2_cache=kv2_cache, block_table2=block_table2)
     assert q.dim() == 3, "q must be [N, H, D]"
     N, H, D = q.shape
-    assert q.dtype in (torch.bfloat16, torch.float16), f"q must be bf16 or fp16, got {q.dtype}"
-    assert attn_sink.dtype == torch.float32 and attn_sink.shape == (H,)
+    dtype = q.dtype
+    assert dtype is torch.bfloat16 or dtype is torch.float16, f"q must be bf16 or fp16, got {dtype}"
+    assert attn_sink.dtype is torch.float32 and attn_sink.dim() == 1 and attn_sink.shape[0] == H, "attn_sink must be [H] fp32"
     if D not in SUPPORTED_D:
         raise ValueError(f"D ({D}) must be one of {SUPPORTED_D}")
     if window is not None and window < 1:
         raise ValueError(f"window must be positive, got {window}")
-    second = [t is not None for t in (kv2_cache, block_table2, ratio)]
-    if any(second) and not all(second):
+    two = kv2_cache is not None
+    if two != (block_table2 is not None) or two != (ratio is not None):
         raise ValueError("a second cache needs kv2_cache, block_table2 and ratio")
-    if all(second) and ratio < 1:
+    if two and ratio < 1:
         raise ValueError(f"ratio must be positive, got {ratio}")
     R = block_table.shape[0]
-    st = [None, None]
-    for i, (n, c, t) in enumerate((("kv", kv_cache, block_table), ("kv2", kv2_cache, block_table2))):
-        if c is None:
-            continue
-        _check_cache(c, f"{n}_cache")
-        assert c.dtype == q.dtype and c.shape[2] == D, f"{n}_cache must have q's type and width"
-        _check_table(t, f"{n}'s block table", R)
-        s = _cache_strides(c)
-        if s[2] != 1 or (s[0] | s[1]) % 8 or c.data_ptr() % 16:
-            raise ValueError(f"{n}_cache needs a contiguous last dimension and rows that start at multiples of 16 bytes")
-        st[i] = _lib.int64s(*s)
-    cu, lens = _int32(cu_q, "cu_q", (R + 1,)), _int32(seq_lens, "seq_lens", (R,))
-    if softmax_scale is None:
-        softmax_scale = D ** -0.5
+
+    def cache_args(cache, table, name):
+        assert cache.dtype is dtype and cache.shape[-1] == D, f"{name}_cache must have q's type and width"
+        s = _cache_strides(cache, f"{name}_cache")
+        p = cache.data_ptr()
+        if s[2] != 1 or (s[0] | s[1]) % 8 or p % 16:
+            raise ValueError(f"{name}_cache needs a contiguous last dimension and rows that start at multiples of 16 bytes")
+        pages, ps, _ = cache.shape
+        return (p, _lib.int64s(*s), pages, ps, table.data_ptr(), _table_stride(table, f"{name}'s block table", R),
+                table.shape[1])
+
+    c1 = cache_args(kv_cache, block_table, "kv")
+    c2 = cache_args(kv2_cache, block_table2, "kv2") if two else (None, None, 0, 1, None, 0, 0)
+    cu, lens = _int32(cu_q, "cu_q", R + 1), _int32(seq_lens, "seq_lens", R)
     q = q if _aligned(q) else q.contiguous()
-    attn_sink = attn_sink.contiguous()
-    o = torch.empty((N, H, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((N, H), dtype=torch.float32, device=dev)
-    two = all(second)
-    keys = block_table.shape[1] * kv_cache.shape[1]
-    keys2 = block_table2.shape[1] * kv2_cache.shape[1] if two else 0
+    attn_sink = attn_sink if attn_sink.is_contiguous() else attn_sink.contiguous()
+    window, ratio = window or 0, ratio or 0
     L = _lib.load()
     with _lib.on_device(dev):
-        scratch, nscratch = _lib.scratch(L.si_paged_attn_fwd_scratch_bytes(N, H, D, R, window or 0, keys, keys2), dev)
-        rc = L.si_paged_attn_fwd(
-            q.data_ptr(), _lib.strides(q), kv_cache.data_ptr(), st[0], kv_cache.shape[0], kv_cache.shape[1],
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-            kv2_cache.data_ptr() if two else None, st[1], kv2_cache.shape[0] if two else 0,
-            kv2_cache.shape[1] if two else 1, block_table2.data_ptr() if two else None,
-            block_table2.stride(0) if two else 0, block_table2.shape[1] if two else 0, window or 0, ratio or 0,
-            cu.data_ptr(), lens.data_ptr(), attn_sink.data_ptr(), N, H, D, R, float(softmax_scale), _lib.qkv_dtype(q),
-            o.data_ptr(), lse.data_ptr(), None if scratch is None else scratch.data_ptr(), nscratch,
-            _lib.stream_ptr(dev))
+        o = torch.empty((N, H, D), dtype=dtype, device=dev)
+        lse = torch.empty((N, H), dtype=torch.float32, device=dev)
+        scratch, nscratch = _lib.scratch(_attn_scratch(N, H, D, R, window, c1[3] * c1[6], c2[3] * c2[6]), dev)
+        rc = L.si_paged_attn_fwd(q.data_ptr(), _lib.strides(q), *c1, *c2, window, ratio, cu.data_ptr(), lens.data_ptr(),
+                                 attn_sink.data_ptr(), N, H, D, R, D ** -0.5 if softmax_scale is None else float(softmax_scale),
+                                 _lib.qkv_dtype(q), o.data_ptr(), lse.data_ptr(),
+                                 None if scratch is None else scratch.data_ptr(), nscratch, _lib.stream_ptr(dev))
     _lib.check(rc)
     return o, lse
+
+
+@functools.lru_cache(maxsize=1024)
+def _attn_scratch(*sizes) -> int:
+    return _lib.load().si_paged_attn_fwd_scratch_bytes(*sizes)
