@@ -35,7 +35,7 @@ struct PagedAttnArgs {
   float* lse;        // [N,H] contiguous
   int N, H, R;
   float scale_log2;
-  int want_log2;     // workgroups to fill the GPU with: 2^want_log2
+  int want;          // workgroups that run at once
   int least;         // fewest tiles of a share
   int behind;        // tokens of a row block before its last one at most
   float* part_o;     // [items, M, D]; null: rows are not split

@@ -192,7 +192,7 @@ __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, P
     // (rounded up: fp32 sums of whole numbers, at most 2^-20 too small over the few thousand additions of a call)
     units = ((units_lds[0] + units_lds[1]) + (units_lds[2] + units_lds[3])) * (1.0f + 0x1p-16f);
     const int all = (blocks_lds[0] + blocks_lds[1]) + (blocks_lds[2] + blocks_lds[3]);
-    const int want = 1 << a.want_log2;
+    const int want = a.want;
     const float least = static_cast<float>(a.least);
     auto tiles_of = [&](float x) { return static_cast<uint32_t>(__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(x), least), 0x1p30f)); };
     const float each = units / static_cast<float>(want);
@@ -275,9 +275,7 @@ __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, P
 }
 
 // Resident workgroups of a CU: 216 registers of a wave hold Q^T and O^T at D = 576, 96 at D = 256.
-constexpr int per_cu(int D) { return D >= 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
-// Tiles resident in LDS.
-constexpr int ring_slots(int D, int RB) { return D == 576 && RB == 2 ? 3 : 4; }
+constexpr int per_cu(int D, bool PAIR) { return D >= 512 ? (PAIR ? 2 : 1) : D == 256 ? 2 : D == 128 ? 3 : 4; }
 
 constexpr float kNever = -__builtin_inff();
 constexpr int kOdd = 1;    // a masked score that is not finite
@@ -298,20 +296,22 @@ __device__ __forceinline__ bf16x8 finite_or_zero(bf16x8 x) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// RB: blocks of 16 rows of a wave (rows of a workgroup: 64 RB).
-template <int D, bool F16, int RB>
-__global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(PagedAttnArgs a) {
+// RB: blocks of 16 rows of a wave (rows of a workgroup: 64 RB).  PAIR: the steps of a tile one after the other, for two
+// workgroups on a CU.
+template <int D, bool F16, int RB, bool PAIR>
+__global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_kernel(PagedAttnArgs a) {
   using SH = AttnShape<D>;
   constexpr int KS = SH::KS, MBW = SH::MBW, ROW = SH::ROW;
   constexpr int M = 64 * RB, NB = 4 * RB;          // rows and row blocks of the workgroup
-  constexpr int NS = ring_slots(D, RB), AHEAD = NS - 1;  // tiles in LDS, and copied ahead of P V
+  constexpr int NS = PAIR ? 2 : 4, AHEAD = NS - 1;  // tiles in LDS, and copied ahead of P V
+  constexpr int NP = PAIR ? 1 : 2, PAGES = PAIR ? 2 : 4;  // P's and page numbers' buffers
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
   static_assert(NS * SH::TILE >= 64 * ROW, "the output is staged 64 rows at a time");
   __shared__ __attribute__((aligned(16))) char kv_lds[NS * SH::TILE];
-  __shared__ __attribute__((aligned(16))) char p_lds[2][NB * 64 * 16];
-  __shared__ __attribute__((aligned(16))) float alpha_lds[2][M];
-  __shared__ __attribute__((aligned(16))) int flag_lds[2][4];  // kOdd, kMoved of this tile, by wave
-  __shared__ __attribute__((aligned(16))) int page_lds[kAttnWaves][4][64];  // page numbers of four tiles, by wave
+  __shared__ __attribute__((aligned(16))) char p_lds[NP][NB * 64 * 16];
+  __shared__ __attribute__((aligned(16))) float alpha_lds[NP][M];
+  __shared__ __attribute__((aligned(16))) int flag_lds[NP][4];  // kOdd, kMoved of this tile, by wave
+  __shared__ __attribute__((aligned(16))) int page_lds[kAttnWaves][PAGES][64];  // page numbers of the next tiles, by wave
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -335,20 +335,36 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
   }
   if (!work) return;
 
-  const int row0 = __builtin_amdgcn_readfirstlane(item.block) * M;  // within the request
-  const int nrows = min(__builtin_amdgcn_readfirstlane(item.n) * a.H - row0, M);
-  const int pos0 = __builtin_amdgcn_readfirstlane(item.len - item.n);
-  const int req = __builtin_amdgcn_readfirstlane(item.req);
-  const int shares = __builtin_amdgcn_readfirstlane(item.shares);
+  // (scalars from here on: as the vector registers they come in they would stay there to the end)
+  scalar_tie(item.first);
+  scalar_tie(item.n);
+  scalar_tie(item.len);
+  scalar_tie(item.req);
+  scalar_tie(item.block);
+  scalar_tie(item.share);
+  scalar_tie(item.shares);
+  scalar_tie(item.slot);
+  scalar_tie(item.rec);
+  const int row0 = item.block * M;  // within the request
+  const int nrows = min(item.n * a.H - row0, M);
+  const int pos0 = item.len - item.n;
+  const int req = item.req, shares = item.shares, share = item.share;
   const int pa = pos0 + row0 / a.H, pb = pos0 + (row0 + nrows - 1) / a.H;  // first and last token
   // tiles of this row block: the window's, then the second cache's; and this share of them
   const int k1lo = win_lo(a, pa), k1hi = win_hi(a, pb);
   const int k2hi = ent_hi(a, pb);
   const int n1 = k1hi > k1lo ? ceil_div32(k1hi - k1lo) : 0;
   const int ntiles = n1 + ceil_div32(k2hi);
-  const int share = __builtin_amdgcn_readfirstlane(item.share);
   const int tbeg = static_cast<int>(static_cast<int64_t>(ntiles) * share / shares);
   const int tend = static_cast<int>(static_cast<int64_t>(ntiles) * (share + 1) / shares);
+
+  // (Lane addresses are worked out anew for each tile where registers are short: an opaque copy of the lane number keeps
+  // the compiler from hoisting them.)
+  auto lane_now = [&]() __attribute__((always_inline)) {
+    int ln = lane;
+    if constexpr (PAIR) reg_tie(ln);
+    return ln;
+  };
 
   // ---- copies ----------------------------------------------------------------
   // Lanes l and l + 32 resolve key l of a tile; a key past the tile's last one stands in for by that one (it is masked,
@@ -362,7 +378,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
   CacheView view;            // of the next tile to fetch page numbers for
   CacheBase from, from_next; // of the tile to copy, and of the one after it
   int fkey = 0, fend = 0, ftile = tbeg;
-  auto enter = [&](int t) {  // moves the view to tile t
+  auto enter = [&](int t) __attribute__((always_inline)) {  // moves the view to tile t
     const bool second = t >= n1;
     view = CacheView{pick(second, view1.table, view2.table), pick(second, view1.ps, view2.ps),
                      pick(second, view1.rstride, view2.rstride), pick(second, view1.magic, view2.magic),
@@ -372,59 +388,68 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     fkey = second ? (t - n1) * 32 : k1lo + t * 32;
     fend = second ? k2hi : k1hi;
   };
-  auto fetch_pages = [&] {
+  auto fetch_pages = [&]() __attribute__((always_inline)) {
     if (__builtin_expect(ftile == n1, 0) && ntiles > n1) enter(n1);
-    const uint32_t key = static_cast<uint32_t>(min(fkey + (lane & 31), fend - 1));
+    const uint32_t key = static_cast<uint32_t>(min(fkey + (lane_now() & 31), fend - 1));
     const uint32_t col = view.page_of(key);
     __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(view.table + col),
-                                     (lds_void_t*)&page_lds[wave][ftile & 3][0], 4, 0, 0);
+                                     (lds_void_t*)&page_lds[wave][ftile % PAGES][0], 4, 0, 0);
     ++ftile;
     fkey += 32;
     return (key - col * view.ps) * view.rstride;
   };
-  // This lane's key and chunk of copy i, kept where registers allow.
-  constexpr bool KEEP = RB == 1;
-  int src_lane[KEEP ? SH::LPT : 1];
-  uint32_t src_chunk[KEEP ? SH::LPT : 1];
-  if constexpr (KEEP) {
-#pragma unroll
-    for (int i = 0; i < SH::LPT; ++i) {
-      const int e = i * SH::NT + static_cast<int>(threadIdx.x), k = e / SH::CPR;
-      src_lane[i] = (k & 31) * 4;
-      src_chunk[i] = static_cast<uint32_t>((e % SH::CPR) ^ kv_swz<D>(k));
-    }
-  }
-  auto copy_lane = [&](int i, int ln) {
-    if constexpr (KEEP) return src_lane[i];
-    else return ((i * SH::NT + wave * 64 + ln) / SH::CPR & 31) * 4;
+  // A tile's copies, LPT of a wave.  At D >= 256 wave w copies keys 8w .. 8w + 7, 64 chunks of 16 bytes at a time: copy i
+  // holds the end of key A(i) and, from lane B(i) on, the start of the next, so the two rows are scalars; the swizzle of key
+  // 8w + j is j.  Below, a copy spans more keys and each lane gets its row by a lane exchange; copies go over the waves.
+  constexpr bool BY_WAVE = D >= 256;
+  constexpr int FSWZ = SH::FMASK;
+  constexpr int CPR = SH::CPR, LPT = SH::LPT;
+  static_assert(!BY_WAVE || LPT * 64 == 8 * CPR, "a wave's copies are its eight rows");
+  struct Sources {
+    uint32_t row[LPT < 8 ? 8 : LPT];  // rows of the wave's keys, or of this lane's copies, in 16-byte units
   };
-  auto copy_chunk = [&](int i, int ln) {
-    if constexpr (KEEP) return src_chunk[i];
-    const int e = i * SH::NT + wave * 64 + ln;
-    return static_cast<uint32_t>((e % SH::CPR) ^ kv_swz<D>(e / SH::CPR));
-  };
-  // Sources of a tile's copies, in 16-byte units; returns which of its keys have a page.
-  auto address_tile = [&](int page, uint32_t within, uint32_t (&src)[SH::LPT]) {
+  // Sources of the tile whose page numbers are `page`; returns which of its keys have a page.
+  auto address_tile = [&](int page, uint32_t within, Sources& y) __attribute__((always_inline)) {
     const bool ok = static_cast<uint32_t>(page) < from.pages;
-    const uint32_t off = ok ? static_cast<uint32_t>(page) * from.pstride + within : 0u;
-    int ln = lane;
-    reg_tie(ln);
+    const uint32_t row = ok ? static_cast<uint32_t>(page) * from.pstride + within : 0u;
+    if constexpr (BY_WAVE) {
 #pragma unroll
-    for (int i = 0; i < SH::LPT; ++i)
-      src[i] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(copy_lane(i, ln), static_cast<int>(off)));
+      for (int j = 0; j < 8; ++j)
+        y.row[j] = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(row), wave * 8 + j));
+    } else {
+#pragma unroll
+      for (int i = 0; i < LPT; ++i)
+        y.row[i] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(
+            ((i * SH::NT + wave * 64 + lane_now()) / CPR & 31) * 4, static_cast<int>(row)));
+    }
     return static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
   };
-  auto copy = [&](const uint32_t (&src)[SH::LPT], char* dst, auto IC) {
+  auto copy = [&](const Sources& y, char* tile, auto IC) __attribute__((always_inline)) {
     constexpr int i = decltype(IC)::value;
-    if (SH::CH % SH::NT == 0 || i + 1 < SH::LPT || i * SH::NT + wave * 64 < SH::CH) {
-      int ln = lane;
-      reg_tie(ln);
-      const char* at = from.base + (static_cast<uint64_t>(src[i] + copy_chunk(i, ln)) << 4);
-      __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint16_t*>(at), (lds_void_t*)(dst + i * (SH::NT * 16)), 16, 0, 0);
+    uint32_t src;
+    char* dst;
+    if constexpr (BY_WAVE) {
+      constexpr int A = 64 * i / CPR, OFF = 64 * i - CPR * A, B = CPR - OFF;  // lanes [0, B): key A, the others the next
+      const int ln = lane_now();
+      if constexpr (B >= 64) {
+        src = y.row[A] + static_cast<uint32_t>((ln + OFF) ^ (FSWZ & A));
+      } else {
+        const uint32_t one = y.row[A] + static_cast<uint32_t>((ln + OFF) ^ (FSWZ & A));
+        const uint32_t two = y.row[A + 1 < 8 ? A + 1 : 7] + static_cast<uint32_t>((ln - B) ^ (FSWZ & (A + 1)));
+        src = ln < B ? one : two;
+      }
+      dst = tile + wave * (LPT * 1024) + i * 1024;
+    } else {
+      const int e = i * SH::NT + wave * 64 + lane_now();
+      src = y.row[i] + static_cast<uint32_t>((e % CPR) ^ kv_swz<D>(e / CPR));
+      dst = tile + wave * 1024 + i * (SH::NT * 16);
     }
+    if (BY_WAVE || SH::CH % SH::NT == 0 || i + 1 < LPT || i * SH::NT + wave * 64 < SH::CH)
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint16_t*>(from.base + (static_cast<uint64_t>(src) << 4)),
+                                       (lds_void_t*)dst, 16, 0, 0);
   };
-  auto ring = [&](int slot) { return kv_lds + slot * SH::TILE; };
-  auto page_addr = [&](int t) { return lds_addr(reinterpret_cast<const char*>(&page_lds[wave][t & 3][0])) + lane * 4; };
+  auto ring = [&](int slot) __attribute__((always_inline)) { return kv_lds + slot * SH::TILE; };
+  auto page_addr = [&](int t) __attribute__((always_inline)) { return lds_addr(reinterpret_cast<const char*>(&page_lds[wave][t % PAGES][0])) + lane_now() * 4; };
   // (the first tiles' page numbers are on their way while Q is addressed; tiles past the share's end are not used)
   uint32_t within[AHEAD + 1];
   CacheBase froms[AHEAD + 1];
@@ -438,7 +463,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
   }
 
   // ---- this lane's rows: their Q^T fragments and the keys they see ----------------
-  int lo1[RB], cnt1[RB], cnt2[RB];
+  int rpos[RB];  // position, -1: no row
   bf16x8 qf[RB][KS];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -446,10 +471,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     const bool live = lrow < nrows;
     const int tok = live ? (row0 + lrow) / a.H : 0;
     const int head = live ? row0 + lrow - tok * a.H : 0;
-    const int pos = pos0 + tok;
-    lo1[b] = live ? win_lo(a, pos) : 0;
-    cnt1[b] = live ? max(win_hi(a, pos) - win_lo(a, pos), 0) : 0;
-    cnt2[b] = live ? ent_hi(a, pos) : 0;
+    rpos[b] = live ? pos0 + tok : -1;
     const uint16_t* qrow = a.q + (static_cast<int64_t>(item.first) + tok) * a.qst + head * a.qsh;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -461,16 +483,14 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
   // ---- S^T -------------------------------------------------------------------
   // A-fragment addresses: key 16mb + i16, chunk 4ks + g; with f = kv_swz(i16), (4ks + g) ^ f = 4 (ks ^ (f >> 2)) +
   // (g ^ (f & 3)), so the offset is a per-lane base (one per parity of ks) plus 64 ks + 16 ROW mb.
-  const int qf_swz = kv_swz<D>(i16);
-  const int qbase = i16 * ROW + 16 * (g ^ (qf_swz & 3));
-  const int qadj = 64 * (qf_swz >> 2);
-  constexpr int QPD = KS < 4 ? KS : 4;
+  constexpr int QPD0 = PAIR ? 2 : 4, QPD = KS < QPD0 ? KS : QPD0;
   // start() runs behind the first fragments' reads, beside(ks) among the MFMAs of k-step ks.
-  auto qk = [&](int slot, f32x4 (&st)[RB][2], auto&& start, auto&& beside) {
-    const uint32_t tile = lds_addr(ring(slot));
-    const uint32_t qa_e = tile + qbase + qadj, qa_o = tile + qbase - qadj;
+  auto qk = [&](int slot, f32x4 (&st)[RB][2], auto&& start, auto&& beside) __attribute__((always_inline)) {
+    const int ln = lane_now(), key = ln & 15, f = kv_swz<D>(key);
+    const uint32_t at = lds_addr(ring(slot)) + key * ROW + 16 * ((ln >> 4) ^ (f & 3));
+    const uint32_t qa_e = at + 64 * (f >> 2), qa_o = at - 64 * (f >> 2);
     bf16x8 kq[QPD][2];
-    auto issue = [&](auto KC) {
+    auto issue = [&](auto KC) __attribute__((always_inline)) {
       constexpr int ks = decltype(KC)::value;
       const uint32_t base = (ks & 1) ? qa_o : qa_e;
       kq[ks % QPD][0] = ld128<64 * ks>(base);
@@ -498,6 +518,15 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
   int all1lo = win_lo(a, pb), all1hi = nrows == M ? win_hi(a, pa) : -1;
   int all2hi = nrows == M ? ent_hi(a, pa) : -1;
   float scale = a.scale_log2 == 0.f ? 1.0f : __builtin_fabsf(a.scale_log2);
+  // (what masks need of the arguments, kept out of the loop as scalar loads)
+  int window = a.window, cap1 = a.c1.keys, cap2 = a.c2.keys, ratio = a.ratio;
+  scalar_tie(window);
+  scalar_tie(cap1);
+  scalar_tie(cap2);
+  scalar_tie(ratio);
+  auto ent_end = [&](int p) __attribute__((always_inline)) {  // as ent_hi; only tiles of the second cache ask
+    return p < 0 ? 0 : min(static_cast<int>(static_cast<uint32_t>(p + 1) / static_cast<uint32_t>(ratio)), cap2);
+  };
   scalar_tie(all1lo);
   scalar_tie(all1hi);
   scalar_tie(all2hi);
@@ -515,8 +544,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     l_run[b] = 0.f;
   }
   int skey = 0;  // first key of the next tile to mask
-  const uint32_t pdst = lds_addr(&p_lds[0][(wave * RB * 64 + lane) * 16]);
-  auto softmax_begin = [&](int t, uint32_t okmask, f32x4 (&st)[RB][2], float (&ref)[RB], int pbuf) {
+  auto softmax_begin = [&](int t, uint32_t okmask, f32x4 (&st)[RB][2], float (&ref)[RB], int pbuf) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < RB; ++b) mfma_result_fence(st[b][0], st[b][1]);
     if (t == n1) skey = 0;
@@ -526,14 +554,17 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     int flags = 0;
     if (!full) {
       bool odd = false;
+      const int g4 = 4 * (lane_now() >> 4);
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        const int lo = skey - (second ? 0 : lo1[b]), cnt = second ? cnt2[b] : cnt1[b];
+        const int end = second ? ent_end(rpos[b]) : max(min(rpos[b] + 1, cap1), 0);
+        const int begin = second ? 0 : max(max(rpos[b] + 1, 0) - window, 0);
+        const int lo = skey - begin, cnt = max(end - begin, 0);
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int kk = 16 * mb + 4 * g + r;
+            const int kk = 16 * mb + g4 + r;
             const bool ok = static_cast<uint32_t>(kk + lo) < static_cast<uint32_t>(cnt) && ((okmask >> kk) & 1);
             const bool fin = __builtin_fabsf(st[b][mb][r]) < __builtin_inff();
             odd = odd || (!ok && !fin);
@@ -559,7 +590,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
         const float alpha = raise && !first ? __builtin_amdgcn_exp2f(m_ref[b] - tmax) : 1.0f;
         if (raise) m_ref[b] = tmax;
         l_run[b] *= alpha;
-        const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][(wave * RB + b) * 16 + i16]));
+        const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][(wave * RB + b) * 16 + (lane_now() & 15)]));
         asm volatile("ds_write_b32 %0, %1" ::"v"(adst), "v"(alpha) : "memory");  // (the four lanes of a row write the same)
         if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) flags |= kMoved << b;
       }
@@ -568,18 +599,19 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     const uint32_t fdst = lds_addr(reinterpret_cast<const char*>(&flag_lds[pbuf][wave]));
     asm volatile("ds_write_b32 %0, %1" ::"v"(fdst), "v"(flags) : "memory");
   };
-  auto softmax_exp = [&](int i, f32x4 (&st)[RB][2], const float (&ref)[RB]) {  // i of 8 RB weights
+  auto softmax_exp = [&](int i, f32x4 (&st)[RB][2], const float (&ref)[RB]) __attribute__((always_inline)) {  // i of 8 RB weights
     const int b = i >> 3, mb = (i >> 2) & 1, r = i & 3;
     st[b][mb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][mb][r], scale, -ref[b]));
   };
-  auto softmax_end = [&](const f32x4 (&p)[RB][2], int pbuf) {
+  auto softmax_end = [&](const f32x4 (&p)[RB][2], int pbuf) __attribute__((always_inline)) {
+    const uint32_t pdst = lds_addr(&p_lds[pbuf][(wave * RB * 64 + lane_now()) * 16]);
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       l_run[b] += ((p[b][0][0] + p[b][0][1]) + (p[b][0][2] + p[b][0][3])) + ((p[b][1][0] + p[b][1][1]) + (p[b][1][2] + p[b][1][3]));
       // P^T B-fragment: k-slots 8g+0..3 <-> keys 4g+0..3, 8g+4..7 <-> keys 16+4g+0..3
       const u32x4 w = u32x4{pack2<F16>(p[b][0][0], p[b][0][1]), pack2<F16>(p[b][0][2], p[b][0][3]),
                             pack2<F16>(p[b][1][0], p[b][1][1]), pack2<F16>(p[b][1][2], p[b][1][3])};
-      asm volatile("ds_write_b128 %0, %1" ::"v"(pdst + pbuf * (NB * 1024) + b * 1024), "v"(w) : "memory");
+      asm volatile("ds_write_b128 %0, %1" ::"v"(pdst + b * 1024), "v"(w) : "memory");
     }
   };
 
@@ -591,13 +623,14 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     for (int nb = 0; nb < NB; ++nb) oacc[j][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   // V^T transposing reads: source lane (g, i16) points at key 4g + (i16 >> 2) (+16 for k-slots 4..7), dims d0 + 4 (i16 & 3)
   // with d0 = 16 (4j + wave); chunk 8j + x, x = 2 wave + ((i16 & 3) >> 1) < 8, swizzles to 8j + (x ^ f): a fixed base + 128 j.
-  const int tkey = 4 * g + (i16 >> 2);
-  const int tx = 2 * wave + ((i16 & 3) >> 1);
-  const int tbase = tkey * ROW + 16 * ((tx ^ kv_swz<D>(tkey)) & (SH::CPR - 1)) + 8 * (i16 & 1);
   // V^T blocks go through a queue VQ deep; between(j) runs among the MFMAs of output block j.
-  constexpr int VQ = MBW < 3 ? MBW : (RB == 1 ? 4 : 3) < MBW ? (RB == 1 ? 4 : 3) : MBW;
-  auto pv = [&](int slot, int pbuf, auto&& between) {
-    const uint32_t psrc = lds_addr(&p_lds[0][0]) + pbuf * (NB * 1024) + lane * 16;
+  constexpr int VQ0 = PAIR ? 2 : RB == 1 ? 4 : 3, VQ = VQ0 < MBW ? VQ0 : MBW;
+  auto pv = [&](int slot, int pbuf, auto&& between) __attribute__((always_inline)) {
+    const int ln = lane_now();
+    const int tkey = 4 * (ln >> 4) + ((ln & 15) >> 2);
+    const int tx = 2 * wave + ((ln & 3) >> 1);
+    const int tbase = tkey * ROW + 16 * ((tx ^ kv_swz<D>(tkey)) & (SH::CPR - 1)) + 8 * (ln & 1);
+    const uint32_t psrc = lds_addr(&p_lds[pbuf][0]) + ln * 16;
     bf16x8 pf[NB];
     attn_static_for<0, NB>([&](auto NC) {
       constexpr int nb = decltype(NC)::value;
@@ -605,7 +638,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     });
     const uint32_t ta = lds_addr(ring(slot)) + tbase;
     v4i16 lo[VQ], hi[VQ];
-    auto issue = [&](auto JC) {
+    auto issue = [&](auto JC) __attribute__((always_inline)) {
       constexpr int j = decltype(JC)::value;
       lo[j % VQ] = tr_read<128 * j>(ta);
       hi[j % VQ] = tr_read<16 * ROW + 128 * j>(ta);
@@ -628,7 +661,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     });
   };
   // Values of a tile that are not finite become zero, in its LDS (every wave has done with its scores).
-  auto clean_tile = [&](int slot) {
+  auto clean_tile = [&](int slot) __attribute__((always_inline)) {
     const uint32_t tile = lds_addr(ring(slot));
     for (int e = threadIdx.x; e < SH::CH; e += kPagedThreads) {
       bf16x8 x;
@@ -638,15 +671,38 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     }
   };
 
+  // What the waves' flags of a tile ask for before its P V.
+  auto settle = [&](int flags, int pbuf, int slot) __attribute__((always_inline)) {
+    if (flags >= kMoved) {
+      // a wave's alpha is of this tile where the wave says so
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float al;
+        int f;
+        asm volatile("ds_read_b32 %0, %2\n\tds_read_b32 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(al), "=&v"(f)
+                     : "v"(lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][nb * 16 + i16]))),
+                       "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[pbuf][nb / RB]))));
+        al = f & (kMoved << (nb % RB)) ? al : 1.0f;
+#pragma unroll
+        for (int j = 0; j < MBW; ++j) oacc[j][nb] = oacc[j][nb] * al;
+      }
+    }
+    if (flags & kOdd) {
+      clean_tile(slot);
+      attn_tile_barrier();
+    }
+  };
+
   // ---- the tiles -------------------------------------------------------------
   // Iteration t: P V of tile t beside S^T and softmax of tile t + 1, one barrier.  Tile t lives in slot t - tbeg mod NS,
   // its P in p_lds[t & 1].  The copies of tile t + AHEAD go out at the start, into the slot of tile t - 1, which every
   // wave has left; they land by the start of iteration t + AHEAD - 1.
-  if (tbeg < tend) {
+  if (!PAIR && tbeg < tend) {
     skey = tbeg < n1 ? k1lo + tbeg * 32 : (tbeg - n1) * 32;
     __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));  // page numbers (and Q)
     uint32_t okq[AHEAD];
-    uint32_t src[SH::LPT];
+    Sources src;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       okq[i] = 0;
@@ -655,7 +711,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
         asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(page) : "v"(page_addr(tbeg + i)));
         from = froms[i];
         okq[i] = address_tile(page, within[i], src);
-        attn_static_for<0, SH::LPT>([&](auto IC) { copy(src, ring(i) + wave * 1024, IC); });
+        attn_static_for<0, SH::LPT>([&](auto IC) { copy(src, ring(i), IC); });
       }
     }
     uint32_t in_next = within[AHEAD];
@@ -672,7 +728,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     softmax_end(st, tbeg & 1);
     int slot = 0;  // of tile t
     // MORE: a tile t + 1; COPY: a tile t + AHEAD
-    auto iteration = [&](int t, auto MORE, auto COPY) {
+    auto iteration = [&](int t, auto MORE, auto COPY) __attribute__((always_inline)) {
       constexpr bool more = decltype(MORE)::value, ahead = decltype(COPY)::value;
       // tile t + 1 (and the page numbers of tile t + AHEAD) landed; with three tiles ahead the copies of the last stay in
       // flight.  Behind the barrier: every wave's, and every wave's P of tile t.
@@ -682,8 +738,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
       const int next = slot + 1 == NS ? 0 : slot + 1, last_slot = slot == 0 ? NS - 1 : slot - 1;
       int flags = 0;
       uint32_t ok_new = 0;
-      char* dst = ring(last_slot) + wave * 1024;
-      auto start = [&] {
+      char* dst = ring(last_slot);
+      auto start = [&]() __attribute__((always_inline)) {
         u32x4 fl;
         int page;
         asm volatile("ds_read_b32 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
@@ -708,27 +764,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
         start();
       }
       if constexpr (ahead) from = from_next;
-      if (__builtin_expect(flags != 0, 0)) {
-        if (flags >= kMoved) {
-          // a wave's alpha is of this tile where the wave says so
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            float al;
-            int f;
-            asm volatile("ds_read_b32 %0, %2\n\tds_read_b32 %1, %3\n\ts_waitcnt lgkmcnt(0)"
-                         : "=&v"(al), "=&v"(f)
-                         : "v"(lds_addr(reinterpret_cast<const char*>(&alpha_lds[t & 1][nb * 16 + i16]))),
-                           "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[t & 1][nb / RB]))));
-            al = f & (kMoved << (nb % RB)) ? al : 1.0f;
-#pragma unroll
-            for (int j = 0; j < MBW; ++j) oacc[j][nb] = oacc[j][nb] * al;
-          }
-        }
-        if (flags & kOdd) {
-          clean_tile(slot);
-          attn_tile_barrier();
-        }
-      }
+      if (__builtin_expect(flags != 0, 0)) settle(flags, t & 1, slot);
       constexpr bool BESIDE = RB == 1 || D < 576;  // (registers)
       constexpr int EPB = MBW > 2 ? (8 * RB + MBW - 3) / (MBW > 2 ? MBW - 2 : 1) : 8 * RB;  // weights beside an output block
       if constexpr (more && !BESIDE) {
@@ -759,6 +795,55 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     for (; t + 1 < tend; ++t) iteration(t, std::true_type{}, std::false_type{});
     iteration(t, std::false_type{}, std::false_type{});
   }
+  // PAIR: one tile ahead in LDS, a tile's steps one after the other, two barriers; the other workgroup of the CU fills the
+  // gaps.
+  if (PAIR && tbeg < tend) {
+    skey = tbeg < n1 ? k1lo + tbeg * 32 : (tbeg - n1) * 32;
+    __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));  // page numbers (and Q)
+    uint32_t ok;
+    {
+      int page;
+      asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(page) : "v"(page_addr(tbeg)));
+      from = froms[0];
+      Sources src;
+      ok = address_tile(page, within[0], src);
+      attn_static_for<0, SH::LPT>([&](auto IC) { copy(src, ring(0), IC); });
+    }
+    uint32_t in_next = within[1];
+    from = froms[1];
+    for (int t = tbeg; t < tend; ++t) {
+      const int slot = (t - tbeg) & 1;
+      __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
+      attn_tile_barrier();  // tile t landed, every wave has left tile t - 1 and its P
+      uint32_t ok_next = 0;
+      {
+        f32x4 st[RB][2];
+        float ref[RB];
+        qk(slot, st, [] {}, [](auto) {});
+        softmax_begin(t, ok, st, ref, 0);
+#pragma unroll
+        for (int i = 0; i < 8 * RB; ++i) softmax_exp(i, st, ref);
+        softmax_end(st, 0);
+      }
+      if (t + 1 < tend) {
+        int page;
+        asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(page) : "v"(page_addr(t + 1)));
+        Sources src;
+        ok_next = address_tile(page, in_next, src);
+        attn_static_for<0, SH::LPT>([&](auto IC) { copy(src, ring(slot ^ 1), IC); });
+        in_next = fetch_pages();  // (past the share's end: the same page again, not used)
+        from = from_next;
+      }
+      attn_tile_barrier();  // P published
+      u32x4 fl;
+      asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(fl)
+                   : "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[0][0]))));
+      const int flags = __builtin_amdgcn_readfirstlane(static_cast<int>(fl[0] | fl[1] | fl[2] | fl[3]));
+      if (__builtin_expect(flags != 0, 0)) settle(flags, 0, slot);
+      pv(slot, 0, [](auto) {});
+      ok = ok_next;
+    }
+  }
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");  // (the last MFMAs' wait states, see mfma_result_fence)
 
   // ---- the result ----------------------------------------------------------------
@@ -770,9 +855,9 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
     const SwapPair r32 = permlane32_swap(__float_as_uint(l_tot[b]), __float_as_uint(l_tot[b]));
     l_tot[b] = __uint_as_float(r32.x) + __uint_as_float(r32.y);
   }
-  const int64_t flat0 = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(item.first)) * a.H + row0;  // first row of o
+  const int64_t flat0 = static_cast<int64_t>(item.first) * a.H + row0;  // first row of o
   if (shares > 1) {
-    const int64_t slot = __builtin_amdgcn_readfirstlane(item.slot);
+    const int64_t slot = item.slot;
 #pragma unroll
     for (int b = 0; b < RB; ++b)
       if (g == 0) a.part_ml[slot * M + (wave * RB + b) * 16 + i16] = float2{m_ref[b], l_tot[b]};
@@ -842,91 +927,99 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D)) void paged_attn_kernel(Pa
   }
 }
 
-// Joins the shares of the split row blocks.  A thread takes four dimensions of a row and every fourth share, eight of them
-// in flight, with a running maximum; the four threads of a place join theirs in LDS.  Bound: the partial outputs, read
-// once (they fit the last-level cache).
-template <bool F16>
+// Joins the shares of the split row blocks.  A thread takes four dimensions of a row and every PARTS-th share, up to
+// sixteen in flight, with a running maximum; with four parts the four threads of a place join theirs in LDS.  Bound: the
+// partial outputs, read once (they fit the last-level cache).
+template <bool F16, int PARTS>
 __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnArgs a, int D, int M) {
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  __shared__ float lds[3][6][64];
-  const int at = threadIdx.x & 63, part = threadIdx.x >> 6;
+  constexpr int U = PARTS == 1 ? 16 : 8, PLACES = kPagedThreads / PARTS;
+  __shared__ float lds[PARTS > 1 ? PARTS - 1 : 1][6][PARTS > 1 ? PLACES : 1];
   const int count = a.rec[0];
   const int vec = D / 4;
-  const int e = static_cast<int>(blockIdx.x) * 64 + at;  // (a block's places fill whole workgroups: 64 divides M)
+  const int at = threadIdx.x % PLACES, part = threadIdx.x / PLACES;
+  const int e = static_cast<int>(blockIdx.x) * PLACES + at;
   const int row = e / vec, d = (e - row * vec) * 4;
   for (int b = blockIdx.y; b < count; b += gridDim.y) {
     const int4 rec = *reinterpret_cast<const int4*>(a.rec + 4 + 4 * static_cast<int64_t>(b));
-    if (static_cast<int>(blockIdx.x) * 64 / vec >= rec.w) continue;  // (the same in every thread)
-    const bool live = row < rec.w;
+    if (static_cast<int>(blockIdx.x) * PLACES / vec >= rec.w) continue;  // (the same in every thread)
     float m = kNever, l = 0.f;
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const float2* ml = a.part_ml + static_cast<int64_t>(rec.x) * M + row;
-      const float* po = a.part_o + (static_cast<int64_t>(rec.x) * M + row) * D + d;
-      for (int i0 = part; i0 < rec.y; i0 += 32) {
-        float2 v[8];
-        f32x4 x[8];
-        float top = m;
+    const int64_t first = static_cast<int64_t>(rec.x) * M + (row < rec.w ? row : 0);
+    const float2* ml = a.part_ml + first;
+    const float* po = a.part_o + first * D + d;
+    for (int i0 = part; i0 < rec.y; i0 += U * PARTS) {
+      float2 v[U];
+      f32x4 x[U];
+      float top = m;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int i = i0 + 4 * u < rec.y ? i0 + 4 * u : i0;
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * PARTS;
+        if (i < rec.y) {  // (the same in a whole wave)
           v[u] = ml[static_cast<int64_t>(i) * M];
           x[u] = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * M * D);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) top = __builtin_fmaxf(top, v[u].x);
-        const float ref = top == kNever ? 0.f : top;
-        const float s = __builtin_amdgcn_exp2f(m - ref);
-        l *= s;
-        acc *= s;
-        m = top;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float w = i0 + 4 * u < rec.y ? __builtin_amdgcn_exp2f(v[u].x - ref) : 0.f;
-          if (i0 + 4 * u < rec.y) {
-            l = __builtin_fmaf(v[u].y, w, l);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(x[u][c], w, acc[c]);
-          }
+        } else {
+          v[u] = float2{kNever, 0.f};
+          x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
       }
-    }
-    if (part > 0) {
-      float* p = &lds[part - 1][0][at];
-      p[0] = m;
-      p[64] = l;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) p[64 * (2 + c)] = acc[c];
-    }
-    __syncthreads();
-    if (part == 0 && live) {
-      const int64_t flat = static_cast<int64_t>(rec.z) + row;
-      const float sink = a.sink[flat % a.H];
-      const float sink2 = sink * kLog2e;
-      float top = __builtin_fmaxf(m, sink2);
-#pragma unroll
-      for (int q = 0; q < 3; ++q) top = __builtin_fmaxf(top, lds[q][0][at]);
+      for (int u = 0; u < U; ++u) top = __builtin_fmaxf(top, v[u].x);
       const float ref = top == kNever ? 0.f : top;
-      float w = __builtin_amdgcn_exp2f(m - ref);
-      float keys = l * w;
-      acc *= w;
+      const float s = __builtin_amdgcn_exp2f(m - ref);
+      l *= s;
+      acc *= s;
+      m = top;
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        w = __builtin_amdgcn_exp2f(lds[q][0][at] - ref);
-        keys = __builtin_fmaf(lds[q][1][at], w, keys);
+      for (int u = 0; u < U; ++u) {
+        const float w = __builtin_amdgcn_exp2f(v[u].x - ref);
+        l = __builtin_fmaf(v[u].y, w, l);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(lds[q][2 + c][at], w, acc[c]);
+        for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(x[u][c], w, acc[c]);
       }
-      const float all = keys + __builtin_amdgcn_exp2f(sink2 - ref);
-      const float inv = all == 0.f ? 0.f : 1.f / all;
-      uint2 o;
-      o.x = pack2<F16>(acc[0] * inv, acc[1] * inv);
-      o.y = pack2<F16>(acc[2] * inv, acc[3] * inv);
-      *reinterpret_cast<uint2*>(a.o + flat * D + d) = o;
-      if (d == 0)
-        a.lse[flat] = all == 0.f ? -1.0e30f : keys == 0.f ? sink : (__builtin_amdgcn_logf(all) + ref) * kLn2;
     }
-    __syncthreads();  // the next block's partial sums take the same LDS
+    if constexpr (PARTS > 1) {
+      __syncthreads();  // (the last block's partial sums have been read)
+      if (part > 0) {
+        lds[part - 1][0][at] = m;
+        lds[part - 1][1][at] = l;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) lds[part - 1][2 + c][at] = acc[c];
+      }
+      __syncthreads();
+      if (part == 0) {
+        float top = m;
+#pragma unroll
+        for (int q = 0; q + 1 < PARTS; ++q) top = __builtin_fmaxf(top, lds[q][0][at]);
+        const float ref = top == kNever ? 0.f : top;
+        float w = __builtin_amdgcn_exp2f(m - ref);
+        l *= w;
+        acc *= w;
+#pragma unroll
+        for (int q = 0; q + 1 < PARTS; ++q) {
+          w = __builtin_amdgcn_exp2f(lds[q][0][at] - ref);
+          l = __builtin_fmaf(lds[q][1][at], w, l);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(lds[q][2 + c][at], w, acc[c]);
+        }
+        m = top;
+      }
+    }
+    if (part > 0 || row >= rec.w) continue;
+    const int64_t flat = static_cast<int64_t>(rec.z) + row;
+    const float sink = a.sink[flat % a.H];
+    const float sink2 = sink * kLog2e;
+    const float top = __builtin_fmaxf(m, sink2);
+    const float ref = top == kNever ? 0.f : top;
+    const float w = __builtin_amdgcn_exp2f(m - ref);
+    const float keys = l * w;
+    const float all = keys + __builtin_amdgcn_exp2f(sink2 - ref);
+    const float inv = all == 0.f ? 0.f : w / all;
+    uint2 o;
+    o.x = pack2<F16>(acc[0] * inv, acc[1] * inv);
+    o.y = pack2<F16>(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2*>(a.o + flat * D + d) = o;
+    if (d == 0) a.lse[flat] = all == 0.f ? -1.0e30f : keys == 0.f ? sink : (__builtin_amdgcn_logf(all) + ref) * kLn2;
   }
 }
 
@@ -935,8 +1028,9 @@ static bool served(int64_t D) { return D == 32 || D == 64 || D == 128 || D == 25
 // Sizes of a call, from what the host knows.
 struct PagedSizes {
   int rb;                // row blocks of 16 of a wave
+  bool pair;             // two workgroups on a CU (D >= 512)
   int64_t blocks;        // row blocks of a workgroup at most
-  int want_log2;         // workgroups that run at once
+  int64_t want;          // workgroups that run at once
   int64_t grid;          // workgroups
   int64_t items;         // partial outputs at most, 0: no row block is split
   int64_t split_blocks;  // split row blocks at most
@@ -953,8 +1047,8 @@ static PagedSizes paged_sizes(int64_t N, int64_t H, int64_t D, int64_t R, int64_
   int64_t g = M;
   while (H % g) g /= 2;
   p.blocks = (N * H + (R < N ? R : N) * (M - g)) / M;
-  p.want_log2 = 8 + (D >= 512 ? 0 : D >= 128 ? 1 : 2);
-  const int64_t want = int64_t{1} << p.want_log2;
+  p.pair = D >= 512 && p.blocks >= 512;
+  const int64_t want = p.want = 256 * per_cu(static_cast<int>(D), p.pair);
   p.grid = 2 * p.blocks <= want ? want : p.blocks + want;
   // tiles of a row block at most
   const int64_t span = M / H + 1 + window;
@@ -978,14 +1072,29 @@ static PagedSizes paged_sizes(int64_t N, int64_t H, int64_t D, int64_t R, int64_
 template <int D>
 static int launch_paged_attn_d(bool f16, const PagedAttnArgs& a, const PagedSizes& p, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.grid < 1 ? 1 : p.grid)), block(kPagedThreads);
-  if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true, 1>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((paged_attn_kernel<D, false, 1>), grid, block, 0, st, a);
+  if (D >= 512 && p.pair) {
+    if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true, 1, (D >= 512)>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<D, false, 1, (D >= 512)>), grid, block, 0, st, a);
+  } else {
+    if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true, 1, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<D, false, 1, false>), grid, block, 0, st, a);
+  }
   const int rc = check_launch("paged_attn_kernel");
   if (rc || !a.part_o) return rc;
   const int M = 64 * p.rb;
-  const dim3 cgrid(static_cast<unsigned>(M * (D / 4) / 64), static_cast<unsigned>(p.split_blocks));
-  if (f16) hipLaunchKernelGGL(paged_combine_kernel<true>, cgrid, block, 0, st, a, D, M);
-  else hipLaunchKernelGGL(paged_combine_kernel<false>, cgrid, block, 0, st, a, D, M);
+  // One thread a place where those fill the GPU, four where they do not (us, one and
+  // four: 64 blocks of up to 5 shares, D = 576, 6.8 and 9.3; 4 blocks of 33 shares 7.2 and 6.7; 32 blocks of up to 64 shares of
+  // 16 rows, D = 128, 8.7 and 7.8).
+  const int64_t places = static_cast<int64_t>(M) * (D / 4);
+  const bool four = p.split_blocks * places < (int64_t{1} << 18);
+  const dim3 cgrid(static_cast<unsigned>((places * (four ? 4 : 1) + kPagedThreads - 1) / kPagedThreads), static_cast<unsigned>(p.split_blocks));
+  if (four) {
+    if (f16) hipLaunchKernelGGL((paged_combine_kernel<true, 4>), cgrid, block, 0, st, a, D, M);
+    else hipLaunchKernelGGL((paged_combine_kernel<false, 4>), cgrid, block, 0, st, a, D, M);
+  } else {
+    if (f16) hipLaunchKernelGGL((paged_combine_kernel<true, 1>), cgrid, block, 0, st, a, D, M);
+    else hipLaunchKernelGGL((paged_combine_kernel<false, 1>), cgrid, block, 0, st, a, D, M);
+  }
   return check_launch("paged_combine_kernel");
 }
 
@@ -1095,7 +1204,7 @@ extern "C" int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const 
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   PagedSizes p = paged_sizes(N, H, D, R > 0 ? R : 1, a.window, cache_keys(pages, P, page_size),
                              ratio > 0 ? cache_keys(pages2, P2, page_size2) : 0);
-  a.want_log2 = p.want_log2;
+  a.want = static_cast<int>(p.want);
   a.least = kLeastTiles;
   a.behind = p.behind;
   if (p.bytes > 0 && scratch && scratch_bytes >= p.bytes) {
