@@ -256,9 +256,11 @@ static int launch_write(WriteArgs a, int64_t n, int64_t row_bytes, hipStream_t s
 //   out[c] = sum_j v_j[c] e^(z_j[c] + bias_j[c]) / sum_j e^(z_j[c] + bias_j[c]),
 // channel by channel; a token without a page counts as absent.
 //
-// A thread takes 16 (or 8) bytes of channels and every PARTS-th token, keeps the running maximum, denominator and
-// numerator of each channel in fp32 registers, and the PARTS threads of a channel group join theirs by lane exchanges
-// and one LDS step.  Eight neighbouring threads read 128 consecutive bytes of a row.  Bound: the two streams' bytes.
+// The workgroup looks up where its tokens' rows are once, into LDS.  Then a thread takes 16 (or 8) bytes of channels and
+// every PARTS-th token, keeps the running maximum, denominator and numerator of each channel in fp32 registers, and the
+// PARTS threads of a channel group join theirs by lane exchanges and one LDS step.  Eight neighbouring threads read 128
+// consecutive bytes of a row.  Bound: the two streams' bytes.  (With the lookups in every thread and a rescale in every join
+// it was bound by its 2,300 instructions a thread: 64K tokens, C = 576, 64 us.)
 // ---------------------------------------------------------------------------
 struct CompressArgs {
   const char *ca, *za, *cb, *zb;        // streams, [pages, ps, C]
@@ -276,83 +278,83 @@ struct CompressArgs {
   int groups;                           // channel groups of 8 threads
 };
 
+template <int DT>
+struct Elem;
+template <>
+struct Elem<0> {
+  typedef float T;
+};
+template <>
+struct Elem<1> {
+  typedef __bf16 T;
+};
+template <>
+struct Elem<2> {
+  typedef _Float16 T;
+};
 template <int DT, int N>
-struct Piece;  // N elements of type DT (0 fp32, 1 bf16, 2 fp16)
-template <int N>
-struct Piece<0, N> {
-  static __device__ __forceinline__ void load(const char* p, float (&v)[N]) {
-    if constexpr (N == 4) {
-      const f32x4 w = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = w[e];
-    } else {
-      v[0] = *reinterpret_cast<const float*>(p);
-    }
-  }
-  static __device__ __forceinline__ void store(char* p, const float (&v)[N]) {
-    if constexpr (N == 4) *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-    else *reinterpret_cast<float*>(p) = v[0];
-  }
-};
-template <typename T, int N>
-struct Piece16 {
+struct Piece {  // N elements of type DT (0 fp32, 1 bf16, 2 fp16), as they lie in memory
+  typedef typename Elem<DT>::T T;
   typedef T vec __attribute__((ext_vector_type(N)));
-  static __device__ __forceinline__ void load(const char* p, float (&v)[N]) {
-    if constexpr (N == 1) {
-      v[0] = static_cast<float>(*reinterpret_cast<const T*>(p));
-    } else {
-      const vec w = *reinterpret_cast<const vec*>(p);
+  vec w;
+  __device__ __forceinline__ void load(const char* p) { w = *reinterpret_cast<const vec*>(p); }
+  __device__ __forceinline__ void fill(float x) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = static_cast<float>(w[e]);
-    }
+    for (int e = 0; e < N; ++e) w[e] = static_cast<T>(x);
   }
+  __device__ __forceinline__ float at(int e) const { return static_cast<float>(w[e]); }
   static __device__ __forceinline__ void store(char* p, const float (&v)[N]) {  // rounds to nearest even
-    if constexpr (N == 1) {
-      *reinterpret_cast<T*>(p) = static_cast<T>(v[0]);
-    } else {
-      vec w;
+    vec w;
 #pragma unroll
-      for (int e = 0; e < N; ++e) w[e] = static_cast<T>(v[e]);
-      *reinterpret_cast<vec*>(p) = w;
-    }
+    for (int e = 0; e < N; ++e) w[e] = static_cast<T>(v[e]);
+    *reinterpret_cast<vec*>(p) = w;
   }
 };
-template <int N>
-struct Piece<1, N> : Piece16<__bf16, N> {};
-template <int N>
-struct Piece<2, N> : Piece16<_Float16, N> {};
 
-// Joins two partial (maximum, denominator, numerator) triples; -inf maxima (nothing seen) weigh nothing.
-__device__ __forceinline__ void pool_join(float& mx, float& den, float& num, float mx2, float den2, float num2) {
-  const float m = __builtin_fmaxf(mx, mx2);
-  const float ref = m == -__builtin_inff() ? 0.f : m;
-  const float s = __expf(mx - ref), s2 = __expf(mx2 - ref);
-  den = den * s + den2 * s2;
-  num = num * s + num2 * s2;
-  mx = m;
+// The value of the lane D away.
+template <int D>
+__device__ __forceinline__ float lane_away(float x) {
+  return __uint_as_float(lane_xor_u32<D>(__float_as_uint(x)));
 }
 
 template <int DT, int N, int PARTS>
-__global__ __launch_bounds__(256) void paged_compress_kernel(CompressArgs a) {
+__global__ __launch_bounds__(256, 4) void paged_compress_kernel(CompressArgs a) {
+  static_assert(PARTS == 4 || PARTS == 32, "lanes 8 and 16 apart, or all of a workgroup");
   constexpr int U = 4;                       // tokens of a thread in flight
   constexpr int SIZE = DT == 0 ? 4 : 2;
   constexpr int ITEMS = 32 / PARTS;          // entries of a workgroup
-  constexpr int WPARTS = PARTS < 8 ? PARTS : 8;  // parts of one wave
+  constexpr int ROWS = 256 / ITEMS;          // tokens of an entry looked up at a time
+  constexpr float kLog2e = 1.4426950408889634f;
+  __shared__ const char* row_lds[3][256];    // of each token: content and gate (null: no page), bias
   const int vg = threadIdx.x & 7;
   const int part = (threadIdx.x >> 3) % PARTS;
   const int item = (threadIdx.x >> 3) / PARTS;
   const int64_t group = blockIdx.x % a.groups;
-  const int64_t e = static_cast<int64_t>(blockIdx.x / a.groups) * ITEMS + item;
+  const int64_t e0 = static_cast<int64_t>(blockIdx.x / a.groups) * ITEMS;
   const int64_t c = (group * 8 + vg) * N;
-  int r = -1, ent = -1;
-  int64_t slot = -1;
-  if (e < a.E) {
-    r = a.request[e];
+  // entry `i` of the workgroup: its request, or -1
+  auto entry = [&](int i, int& ent, int64_t& slot) {
+    const int64_t e = e0 + i;
+    if (e >= a.E) return -1;
+    const int r = a.request[e];
     ent = a.entry[e];
     slot = a.slots[e];
-  }
-  const bool live = r >= 0 && r < a.R && ent >= 0 && slot >= 0 && slot < a.nslots && c < a.C;
-  if (PARTS == 32 && !(r >= 0 && r < a.R && ent >= 0 && slot >= 0 && slot < a.nslots)) return;  // (the same in every thread)
+    return r >= 0 && r < a.R && ent >= 0 && slot >= 0 && slot < a.nslots ? r : -1;
+  };
+  int ent = 0;
+  int64_t slot = 0;
+  const bool there = entry(item, ent, slot) >= 0;
+  if (ITEMS == 1 && !there) return;  // (the same in every thread)
+  const bool live = there && c < a.C;
+  const int64_t most = a.overlap ? 2 * a.m : a.m;
+  const int64_t rows = a.overlap && ent > 0 ? 2 * a.m : a.m;
+  // the token that this thread looks up, of entry `look`
+  const int look = threadIdx.x / ROWS;
+  int lent = 0;
+  int64_t lslot = 0;
+  const int lreq = ITEMS == 1 ? a.request[e0] : entry(look, lent, lslot);
+  if (ITEMS == 1) lent = ent;
+  const int64_t lrows = a.overlap && lent > 0 ? 2 * a.m : a.m;
   float mx[N], den[N], num[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -361,92 +363,102 @@ __global__ __launch_bounds__(256) void paged_compress_kernel(CompressArgs a) {
     num[i] = 0.f;
   }
   bool any = false;
-  if (live) {
-    const int32_t* trow = a.table + r * a.tstride;
-    const int64_t rows = a.overlap && ent > 0 ? 2 * a.m : a.m;
-    for (int64_t j0 = part; j0 < rows; j0 += PARTS * U) {
-      float z[U][N], v[U][N], b[U][N];
+  for (int64_t base = 0; base < most; base += ROWS) {
+    if (base > 0) __syncthreads();  // (the last tokens' rows have been read)
+    {
+      const int64_t j = base + threadIdx.x % ROWS;
+      const char *zrow = nullptr, *crow = nullptr, *brow = nullptr;
+      if (lreq >= 0 && j < lrows) {
+        const bool second = j >= a.m;  // stream b: the block before
+        const int64_t jj = second ? j - a.m : j;
+        int64_t at = (static_cast<int64_t>(lent) - (second ? 1 : 0)) * a.m + jj;
+        int64_t col;
+        if (at <= 0x7fffffff) {
+          col = static_cast<uint32_t>(at) / static_cast<uint32_t>(a.ps);
+        } else {
+          col = at / a.ps;
+        }
+        at -= col * a.ps;
+        const int64_t page = col < a.P ? a.table[lreq * a.tstride + col] : -1;
+        if (page >= 0 && page < a.pages) {
+          const int st = second ? 2 : 0;
+          crow = (second ? a.cb : a.ca) + (page * a.pstride[st] + at * a.rstride[st]) * SIZE;
+          zrow = (second ? a.zb : a.za) + (page * a.pstride[st + 1] + at * a.rstride[st + 1]) * SIZE;
+          brow = reinterpret_cast<const char*>((second ? a.bb : a.ba) + jj * a.C);
+        }
+      }
+      row_lds[0][threadIdx.x] = crow;
+      row_lds[1][threadIdx.x] = zrow;
+      row_lds[2][threadIdx.x] = brow;
+    }
+    __syncthreads();
+    const int here = live ? static_cast<int>(rows - base < ROWS ? rows - base : ROWS) : 0;
+    for (int j0 = part; j0 < here; j0 += PARTS * U) {
+      Piece<DT, N> zp[U], vp[U];
+      Piece<0, N> bp[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t j = j0 + u * PARTS;
-        bool there = j < rows;
-        int64_t at = 0, page = 0;
-        int st = 0;
-        int64_t jj = 0;
-        if (there) {
-          st = j >= a.m ? 2 : 0;  // stream b: the block before
-          jj = st ? j - a.m : j;
-          at = (static_cast<int64_t>(ent) - (st ? 1 : 0)) * a.m + jj;
-          int64_t col;
-          if (at <= 0x7fffffff) {
-            const uint32_t q = static_cast<uint32_t>(at) / static_cast<uint32_t>(a.ps);
-            col = q;
-            at -= static_cast<int64_t>(q) * a.ps;
-          } else {
-            col = at / a.ps;
-            at -= col * a.ps;
-          }
-          there = col < a.P;
-          if (there) {
-            page = trow[col];
-            there = page >= 0 && page < a.pages;
-          }
-        }
-        if (there) {
+        const int j = j0 + u * PARTS;
+        const char* crow = j < here ? row_lds[0][item * ROWS + (j & (ROWS - 1))] : nullptr;
+        if (crow) {
           any = true;
-          const char* zp = st ? a.zb : a.za;
-          const char* vp = st ? a.cb : a.ca;
-          const float* bp = (st ? a.bb : a.ba) + jj * a.C + c;
-          Piece<DT, N>::load(zp + (page * a.pstride[st + 1] + at * a.rstride[st + 1] + c) * SIZE, z[u]);
-          Piece<DT, N>::load(vp + (page * a.pstride[st] + at * a.rstride[st] + c) * SIZE, v[u]);
-          if constexpr (N == 1) {
-            b[u][0] = bp[0];
-          } else {
-#pragma unroll
-            for (int i = 0; i < N; i += 4) {
-              const f32x4 w = *reinterpret_cast<const f32x4*>(bp + i);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) b[u][i + q] = w[q];
-            }
-          }
+          zp[u].load(row_lds[1][item * ROWS + (j & (ROWS - 1))] + c * SIZE);
+          vp[u].load(crow + c * SIZE);
+          bp[u].load(row_lds[2][item * ROWS + (j & (ROWS - 1))] + c * 4);
         } else {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            z[u][i] = -__builtin_inff();
-            v[u][i] = 0.f;
-            b[u][i] = 0.f;
-          }
+          zp[u].fill(-__builtin_inff());
+          vp[u].fill(0.f);
+          bp[u].fill(0.f);
         }
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        float m = mx[i];
+        float m = mx[i], z[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          z[u][i] += b[u][i];
-          m = __builtin_fmaxf(m, z[u][i]);
+          z[u] = zp[u].at(i) + bp[u].at(i);
+          m = __builtin_fmaxf(m, z[u]);
         }
-        const float ref = m == -__builtin_inff() ? 0.f : m;
-        const float s = __expf(mx[i] - ref);
+        const float ref = m == -__builtin_inff() ? 0.f : m * kLog2e;
+        const float s = __builtin_amdgcn_exp2f(__builtin_fmaf(mx[i], kLog2e, -ref));
         den[i] *= s;
         num[i] *= s;
         mx[i] = m;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const float w = __expf(z[u][i] - ref);
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(z[u], kLog2e, -ref));
           den[i] += w;
-          num[i] += w * v[u][i];
+          num[i] = __builtin_fmaf(w, vp[u].at(i), num[i]);
         }
       }
     }
   }
-  // join the parts: lanes 8, 16, 32 apart, then the waves of an entry
+  // Join the parts: lanes 8, 16, 32 apart, the maxima first, so that a thread rescales its sums once; then the waves of an
+  // entry.  (With a rescale in every step, 96 of a thread's 128 exponentials were the joins': 64K tokens 64 us.)
+  float top[N];
 #pragma unroll
-  for (int d = 8; d < 8 * WPARTS; d *= 2) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      pool_join(mx[i], den[i], num[i], __shfl_xor(mx[i], d), __shfl_xor(den[i], d), __shfl_xor(num[i], d));
-    any = any | (__shfl_xor(static_cast<int>(any), d) != 0);
+  for (int i = 0; i < N; ++i) {
+    top[i] = __builtin_fmaxf(mx[i], lane_away<8>(mx[i]));
+    top[i] = __builtin_fmaxf(top[i], lane_away<16>(top[i]));
+    if constexpr (PARTS >= 8) top[i] = __builtin_fmaxf(top[i], lane_away<32>(top[i]));
+    const float w = top[i] == -__builtin_inff() ? 0.f : __expf(mx[i] - top[i]);
+    den[i] *= w;
+    num[i] *= w;
+    den[i] += lane_away<8>(den[i]);
+    num[i] += lane_away<8>(num[i]);
+    den[i] += lane_away<16>(den[i]);
+    num[i] += lane_away<16>(num[i]);
+    if constexpr (PARTS >= 8) {
+      den[i] += lane_away<32>(den[i]);
+      num[i] += lane_away<32>(num[i]);
+    }
+  }
+  {
+    float seen = any ? 1.f : 0.f;
+    seen += lane_away<8>(seen);
+    seen += lane_away<16>(seen);
+    if constexpr (PARTS >= 8) seen += lane_away<32>(seen);
+    any = seen != 0.f;
   }
   if constexpr (PARTS > 8) {
     constexpr int WAVES = PARTS / 8;
@@ -455,7 +467,7 @@ __global__ __launch_bounds__(256) void paged_compress_kernel(CompressArgs a) {
     if ((threadIdx.x & 63) < 8) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        lds[wave][vg][i] = mx[i];
+        lds[wave][vg][i] = top[i];
         lds[wave][vg][N + i] = den[i];
         lds[wave][vg][2 * N + i] = num[i];
       }
@@ -463,12 +475,24 @@ __global__ __launch_bounds__(256) void paged_compress_kernel(CompressArgs a) {
     }
     __syncthreads();
     if (threadIdx.x < 8) {
-      for (int w = 1; w < WAVES; ++w) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          pool_join(mx[i], den[i], num[i], lds[w][vg][i], lds[w][vg][N + i], lds[w][vg][2 * N + i]);
-        any = any || lds[w][vg][3 * N] != 0.f;
+      for (int i = 0; i < N; ++i) {
+        float m = top[i];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) m = __builtin_fmaxf(m, lds[w][vg][i]);
+        const float ref = m == -__builtin_inff() ? 0.f : m;
+        const float s = __expf(top[i] - ref);
+        den[i] *= s;
+        num[i] *= s;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) {
+          const float sw = __expf(lds[w][vg][i] - ref);
+          den[i] += lds[w][vg][N + i] * sw;
+          num[i] += lds[w][vg][2 * N + i] * sw;
+        }
       }
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) any = any || lds[w][vg][3 * N] != 0.f;
     }
   }
   if (live && part == 0) {
