@@ -88,7 +88,8 @@ __device__ __forceinline__ T pick(bool second, T x, T y) {
 // and `want` workgroups, a row block is cut into ceil(tiles / c) shares; c is the smallest of four steps from U / want to
 // 2 U / want with which all shares run at once.  With more row blocks than that, c = 2 U / want cuts only requests
 // far longer than the average, which would otherwise end last on their own.
-// Every workgroup does these sums itself, with lane-shift scans in 32 bits.
+// Every workgroup does these sums itself, with lane-shift scans in 32 bits, and where there are at most 64 requests every
+// wave, without a barrier.
 // ---------------------------------------------------------------------------
 struct PagedReq {
   int first, n, len;  // first row of q, new tokens, entries of the first cache
@@ -161,12 +162,75 @@ __device__ __forceinline__ float wave_sum_last(float x) {
   return x;
 }
 
+constexpr int kSteps = 4;
+// Tiles of a share: the steps to try, from the sum of blocks x tiles (rounded up: fp32 sums of whole numbers, at most 2^-20
+// too small over the few thousand additions of a call).
+struct ShareSteps {
+  uint32_t step[kSteps];
+  float units;
+  uint32_t least;
+  __device__ __forceinline__ uint32_t tiles_of(float x) const {
+    return static_cast<uint32_t>(__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(x), static_cast<float>(least)), 0x1p30f));
+  }
+  __device__ __forceinline__ ShareSteps(const PagedAttnArgs& a, float sum)
+      : units(sum * (1.0f + 0x1p-16f)), least(static_cast<uint32_t>(a.least)) {
+    const float each = units / static_cast<float>(a.want);
+    step[0] = tiles_of(each);
+    step[1] = tiles_of(1.25f * each);
+    step[2] = tiles_of(1.5f * each);
+    step[3] = tiles_of(2.f * each);
+  }
+  // The smallest step whose shares (fits[]) all run at once, for `all` < want row blocks; at the least the one that always
+  // does: sum of ceil(tiles / c) <= units / c + blocks <= want.
+  __device__ __forceinline__ uint32_t pick(const int (&fits)[kSteps], int all, int want) const {
+    uint32_t c = tiles_of(units / static_cast<float>(want - all));
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i)
+      if (fits[i] <= want) c = step[i];
+    return c;
+  }
+};
+
+// For up to 64 requests, one to a lane, every wave for itself: no LDS and no barrier.
+template <int M>
+__device__ __forceinline__ bool paged_schedule_wave(const PagedAttnArgs& a, int id, PagedItem& it) {
+  const int lane = threadIdx.x & 63;
+  PagedReq q{};
+  if (lane < a.R) q = paged_req<M>(a, lane);
+  auto last = [](int x) { return __builtin_amdgcn_readlane(x, kWave - 1); };
+  uint32_t c = kWhole;
+  if (a.part_o) {
+    const float sum = wave_sum_last(static_cast<float>(q.blocks) * static_cast<float>(q.tiles));
+    const ShareSteps steps(a, __uint_as_float(static_cast<uint32_t>(last(static_cast<int>(__float_as_uint(sum))))));
+    const int all = last(wave_scan(q.blocks));
+    c = steps.step[kSteps - 1];
+    if (all < a.want) {
+      int fits[kSteps];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) fits[i] = last(wave_scan(q.blocks * shares_of(q.tiles, steps.step[i])));
+      c = steps.pick(fits, all, a.want);
+    }
+  }
+  const int s = shares_of(q.tiles, c);
+  const int items = q.blocks * s, parts = s > 1 ? items : 0, recs = s > 1 ? q.blocks : 0;
+  const int end = wave_scan(items), end_parts = wave_scan(parts), end_recs = wave_scan(recs);
+  if (a.part_o && id == 0 && threadIdx.x == kWave - 1) a.rec[0] = end_recs;
+  if (id >= last(end)) return false;
+  const int r = __builtin_ctzll(__builtin_amdgcn_ballot_w64(id < end));  // the first request that ends behind it
+  auto at = [&](int x) { return __builtin_amdgcn_readlane(x, r); };
+  const int shares = at(s), k = id - at(end - items), block = k / shares;
+  // (the last row blocks see the most keys: they start first)
+  it = PagedItem{at(q.first), at(q.n), at(q.len), r, at(q.blocks) - 1 - block, k - block * shares, shares,
+                 at(end_parts - parts) + k, at(end_recs - recs) + block};
+  return true;
+}
+
 // This workgroup's item, or false.  All threads call it.
 template <int M>
 __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, PagedItem& it) {
-  constexpr int W = kPagedThreads / kWave, STEPS = 4;
+  constexpr int W = kPagedThreads / kWave;
   __shared__ float units_lds[W];
-  __shared__ int blocks_lds[W], fits_lds[W][STEPS], sums_lds[3][W];
+  __shared__ int blocks_lds[W], fits_lds[W][kSteps], sums_lds[3][W];
   __shared__ PagedItem found;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.R + kPagedThreads - 1) / kPagedThreads;
@@ -189,33 +253,25 @@ __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, P
       blocks_lds[wave] = blocks;
     }
     __syncthreads();
-    // (rounded up: fp32 sums of whole numbers, at most 2^-20 too small over the few thousand additions of a call)
-    units = ((units_lds[0] + units_lds[1]) + (units_lds[2] + units_lds[3])) * (1.0f + 0x1p-16f);
+    const ShareSteps steps(a, (units_lds[0] + units_lds[1]) + (units_lds[2] + units_lds[3]));
     const int all = (blocks_lds[0] + blocks_lds[1]) + (blocks_lds[2] + blocks_lds[3]);
-    const int want = a.want;
-    const float least = static_cast<float>(a.least);
-    auto tiles_of = [&](float x) { return static_cast<uint32_t>(__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(x), least), 0x1p30f)); };
-    const float each = units / static_cast<float>(want);
-    const uint32_t steps[STEPS] = {tiles_of(each), tiles_of(1.25f * each), tiles_of(1.5f * each), tiles_of(2.f * each)};
-    c = steps[STEPS - 1];
-    if (all < want) {
-      int n[STEPS] = {};
+    c = steps.step[kSteps - 1];
+    if (all < a.want) {
+      int n[kSteps] = {};
       for (int r = r0; r < r1; ++r) {
         const PagedReq q = req(r);
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) n[i] += q.blocks * shares_of(q.tiles, steps[i]);
+        for (int i = 0; i < kSteps; ++i) n[i] += q.blocks * shares_of(q.tiles, steps.step[i]);
       }
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
+      for (int i = 0; i < kSteps; ++i) {
         n[i] = wave_scan(n[i]);
         if (lane == kWave - 1) fits_lds[wave][i] = n[i];
       }
       __syncthreads();
-      // (sum of ceil(tiles / c) <= units / c + blocks <= want)
-      c = tiles_of(units / static_cast<float>(want - all));
 #pragma unroll
-      for (int i = STEPS - 1; i >= 0; --i)
-        if ((fits_lds[0][i] + fits_lds[1][i]) + (fits_lds[2][i] + fits_lds[3][i]) <= want) c = steps[i];
+      for (int i = 0; i < kSteps; ++i) n[i] = (fits_lds[0][i] + fits_lds[1][i]) + (fits_lds[2][i] + fits_lds[3][i]);
+      c = steps.pick(n, all, a.want);
     }
   }
   int items = 0, parts = 0, recs = 0;
@@ -320,7 +376,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   const int last = a.R > 0 ? a.cu[a.R] : 0;
 
   PagedItem item;
-  const bool work = paged_schedule<M>(a, xcd_block_order(), item);
+  const int id = xcd_block_order();
+  const bool work = a.R <= kWave ? paged_schedule_wave<M>(a, id, item) : paged_schedule<M>(a, id, item);
   // Rows of no request: as a row without a key.
   {
     const int end = last < 0 ? 0 : (last < a.N ? last : a.N);
