@@ -366,6 +366,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   __shared__ __attribute__((aligned(16))) char kv_lds[NS * SH::TILE];
   __shared__ __attribute__((aligned(16))) char p_lds[NP][NB * 64 * 16];
   __shared__ __attribute__((aligned(16))) float alpha_lds[NP][M];
+  __shared__ float sink_lds[M];  // of each row, for the end
   __shared__ __attribute__((aligned(16))) int flag_lds[NP][4];  // kOdd, kMoved of this tile, by wave
   __shared__ __attribute__((aligned(16))) int page_lds[kAttnWaves][PAGES][64];  // page numbers of the next tiles, by wave
 
@@ -521,6 +522,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
 
   // ---- this lane's rows: their Q^T fragments and the keys they see ----------------
   int rpos[RB];  // position, -1: no row
+  const float* sink_at[RB];
   bf16x8 qf[RB][KS];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -529,19 +531,41 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     const int tok = live ? (row0 + lrow) / a.H : 0;
     const int head = live ? row0 + lrow - tok * a.H : 0;
     rpos[b] = live ? pos0 + tok : -1;
+    sink_at[b] = a.sink + head;
+    // (a row past the block's last one reads the first one's Q; nothing of it is used)
     const uint16_t* qrow = a.q + (static_cast<int64_t>(item.first) + tok) * a.qst + head * a.qsh;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      qf[b][ks] = live && a.scale_log2 != 0.f ? *reinterpret_cast<const bf16x8*>(qrow + ks * 32 + g * 8) : bf16x8{};
-      if (__builtin_expect(a.scale_log2 < 0.f, 0)) qf[b][ks] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, qf[b][ks]) ^ 0x80008000u);
-    }
+    for (int ks = 0; ks < KS; ++ks) qf[b][ks] = *reinterpret_cast<const bf16x8*>(qrow + ks * 32 + g * 8);
   }
+  // The page numbers, asked for before these KS * RB loads, have landed; the loads may be in flight.
+  __builtin_amdgcn_s_waitcnt(vm_lgkm0(KS * RB));
+  // Sinks, kept in LDS for the end (each row's is read back by the lane that wrote it).
+  float sink_v[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) sink_v[b] = *sink_at[b];
+  auto sink_to_lds = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const uint32_t dst = lds_addr(reinterpret_cast<const char*>(&sink_lds[(wave * RB + b) * 16 + i16]));
+      asm volatile("ds_write_b32 %0, %1" ::"v"(dst), "v"(sink_v[b]) : "memory");  // (the four lanes of a row write the same)
+    }
+  };
 
   // ---- S^T -------------------------------------------------------------------
   // A-fragment addresses: key 16mb + i16, chunk 4ks + g; with f = kv_swz(i16), (4ks + g) ^ f = 4 (ks ^ (f >> 2)) +
   // (g ^ (f & 3)), so the offset is a per-lane base (one per parity of ks) plus 64 ks + 16 ROW mb.
   constexpr int QPD0 = PAIR ? 2 : 4, QPD = KS < QPD0 ? KS : QPD0;
   // start() runs behind the first fragments' reads, beside(ks) among the MFMAs of k-step ks.
+  auto scale_q = [&]() __attribute__((always_inline)) {  // (scale is positive below)
+    if (__builtin_expect(a.scale_log2 <= 0.f, 0)) {
+      const uint32_t keep = a.scale_log2 == 0.f ? 0u : ~0u, flip = a.scale_log2 == 0.f ? 0u : 0x80008000u;
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          qf[b][ks] = __builtin_bit_cast(bf16x8, (__builtin_bit_cast(u32x4, qf[b][ks]) & keep) ^ flip);
+    }
+  };
   auto qk = [&](int slot, f32x4 (&st)[RB][2], auto&& start, auto&& beside) __attribute__((always_inline)) {
     const int ln = lane_now(), key = ln & 15, f = kv_swz<D>(key);
     const uint32_t at = lds_addr(ring(slot)) + key * ROW + 16 * ((ln >> 4) ^ (f & 3));
@@ -757,7 +781,6 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // wave has left; they land by the start of iteration t + AHEAD - 1.
   if (!PAIR && tbeg < tend) {
     skey = tbeg < n1 ? k1lo + tbeg * 32 : (tbeg - n1) * 32;
-    __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));  // page numbers (and Q)
     uint32_t okq[AHEAD];
     Sources src;
 #pragma unroll
@@ -778,6 +801,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     attn_tile_barrier();  // the first tile landed
     f32x4 st[RB][2];
     float ref[RB];
+    sink_to_lds();
+    scale_q();
     qk(0, st, [] {}, [](auto) {});
     softmax_begin(tbeg, okq[0], st, ref, tbeg & 1);
 #pragma unroll
@@ -852,11 +877,11 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     for (; t + 1 < tend; ++t) iteration(t, std::true_type{}, std::false_type{});
     iteration(t, std::false_type{}, std::false_type{});
   }
+  if (tbeg >= tend) sink_to_lds();
   // PAIR: one tile ahead in LDS, a tile's steps one after the other, two barriers; the other workgroup of the CU fills the
   // gaps.
   if (PAIR && tbeg < tend) {
     skey = tbeg < n1 ? k1lo + tbeg * 32 : (tbeg - n1) * 32;
-    __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));  // page numbers (and Q)
     uint32_t ok;
     {
       int page;
@@ -868,6 +893,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     }
     uint32_t in_next = within[1];
     from = froms[1];
+    sink_to_lds();
+    scale_q();
     for (int t = tbeg; t < tend; ++t) {
       const int slot = (t - tbeg) & 1;
       __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
@@ -940,7 +967,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   for (int b = 0; b < RB; ++b) {
     const int lrow = (wave * RB + b) * 16 + i16;
     const bool live = lrow < nrows;
-    const float sink = live ? a.sink[(row0 + lrow) % a.H] : kNever;
+    const float sink = sink_lds[lrow];
     const float sink2 = sink * kLog2e;
     const float m_fin = __builtin_fmaxf(m_ref[b], sink2);
     const float top = m_fin == kNever ? 0.f : m_fin;
