@@ -34,15 +34,18 @@ namespace si {
 template <typename T>
 __device__ __forceinline__ void scalar_tie(T& x) {
   static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two registers");
+  // (readfirstlane on both sides: the asm needs a scalar, and its result does not count as uniform by itself)
+  auto tied = [](uint32_t w) {
+    w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w)));
+    asm volatile("" : "+s"(w));
+    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w)));
+  };
   if constexpr (sizeof(T) == 4) {
-    x = __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+    x = __builtin_bit_cast(T, tied(__builtin_bit_cast(uint32_t, x)));
   } else {
     const uint64_t w = __builtin_bit_cast(uint64_t, x);
-    const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w)));
-    const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w >> 32)));
-    x = __builtin_bit_cast(T, hi << 32 | lo);
+    x = __builtin_bit_cast(T, static_cast<uint64_t>(tied(static_cast<uint32_t>(w >> 32))) << 32 | tied(static_cast<uint32_t>(w)));
   }
-  asm volatile("" : "+s"(x));
 }
 
 // A cache as one workgroup reads it.
@@ -445,6 +448,17 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
                           pick(second, base1.pages, base2.pages)};
     fkey = second ? (t - n1) * 32 : k1lo + t * 32;
     fend = second ? k2hi : k1hi;
+    scalar_tie(view.table);
+    scalar_tie(view.ps);
+    scalar_tie(view.rstride);
+    scalar_tie(view.magic);
+    scalar_tie(view.shift);
+    scalar_tie(view.one);
+    scalar_tie(from_next.base);
+    scalar_tie(from_next.pstride);
+    scalar_tie(from_next.pages);
+    scalar_tie(fkey);
+    scalar_tie(fend);
   };
   auto fetch_pages = [&]() __attribute__((always_inline)) {
     if (__builtin_expect(ftile == n1, 0) && ntiles > n1) enter(n1);
@@ -511,13 +525,12 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // (the first tiles' page numbers are on their way while Q is addressed; tiles past the share's end are not used)
   uint32_t within[AHEAD + 1];
   CacheBase froms[AHEAD + 1];
-  if (tbeg < tend) {
-    enter(tbeg);
+  enter(tbeg);
 #pragma unroll
-    for (int i = 0; i <= AHEAD; ++i) {
-      if (tbeg + i < tend) within[i] = fetch_pages();
-      froms[i] = from_next;
-    }
+  for (int i = 0; i <= AHEAD; ++i) {
+    within[i] = 0;
+    if (tbeg + i < tend) within[i] = fetch_pages();
+    froms[i] = from_next;
   }
 
   // ---- this lane's rows: their Q^T fragments and the keys they see ----------------
@@ -914,7 +927,10 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
         asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(page) : "v"(page_addr(t + 1)));
         Sources src;
         ok_next = address_tile(page, in_next, src);
-        attn_static_for<0, SH::LPT>([&](auto IC) { copy(src, ring(slot ^ 1), IC); });
+        attn_static_for<0, SH::LPT>([&](auto IC) {
+          copy(src, ring(slot ^ 1), IC);
+          __builtin_amdgcn_sched_barrier(0);  // (one address at a time: registers)
+        });
         in_next = fetch_pages();  // (past the share's end: the same page again, not used)
         from = from_next;
       }
