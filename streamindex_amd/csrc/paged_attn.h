@@ -36,13 +36,15 @@ struct PagedAttnArgs {
   int N, H, R;
   float scale_log2;
   int want;          // workgroups that run at once
-  int least;         // fewest tiles of a share
+  float part_cost;   // of a partial output, in tiles
   int behind;        // tokens of a row block before its last one at most
-  float* part_o;     // [items, M, D]; null: rows are not split
-  float2* part_ml;   // [items, M]
+  float* part_o;     // [items, kRows / 16, D / 16, 64, 4]: blocks of 16 rows x 16 dimensions as a wave holds them; null:
+                     // rows are not split
+  float2* part_ml;   // [items, kRows]
   int32_t* rec;      // [0]: split row blocks; then 4 each: first item, shares, first row, rows
 };
 
 constexpr int kPagedThreads = 256;
+constexpr int kRows = 64;  // (token, head) rows of a workgroup
 
 }  // namespace si

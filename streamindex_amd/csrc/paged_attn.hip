@@ -4,14 +4,23 @@
 // four neighbouring tokens, so every key row that is fetched serves 64 query rows whatever the head count.  It walks
 // the keys that any of its rows sees, 32 at a time, the window's first:
 //   * the tile's rows are copied from their pages straight into LDS (global_load_lds, 16 bytes a lane, no staging
-//     registers), one tile ahead of use, two tiles resident; the page numbers are fetched one tile further ahead;
+//     registers), the page numbers fetched a tile before their copies;
 //   * S^T = K Q^T on 16x16x32 MFMAs, keys on M: wave w takes rows 16w .. 16w+15, Q^T stays in registers;
 //   * the online softmax is in-lane (a lane holds eight keys of one row) plus two lane exchanges when a maximum moves,
 //     which it does only once a score exceeds it by 2^64 (fp16: 2^8), so the accumulator is rarely rescaled;
 //   * P^T goes through LDS, and O^T += V^T P^T with the output dimensions dealt to the waves.
 // P is rounded to the element type for the matrix core, the denominator sums the unrounded values in fp32.
-// At D >= 512 two workgroups fit a CU (79 KB of LDS each); they run out of step, so one's copies, softmax and barriers
-// fall behind the other's MFMAs.
+//
+// Two ways through the tiles.  With four tiles in LDS (one workgroup a CU at D >= 512, two at 256, three at 128, four
+// below), the softmax of tile t + 1 runs among the MFMAs of tile t's P V, its copies three tiles ahead, one barrier a tile.
+// PAIR: two tiles in LDS, a tile's steps one after the other, two workgroups a CU, whose copies, prologues and ends fall
+// behind each other's MFMAs: taken where there are more row blocks than CUs, at D >= 512 (us, PAIR and not, D = 576: 256 row
+// blocks of 11 tiles 66 and 33, of 254 tiles 330 and 346; 320 of them 44 and 57, 549 and 661; 1,024 84 and 109, 1,171 and
+// 1,411).  At D = 256, 512 row blocks of up to 288 tiles run 314 us without and 338 with three a CU as PAIR allows there.
+//
+// Bound, long keys: the LDS, which every K tile leaves four times (each wave's S^T) and once more as V, beside its copy: at
+// D = 576 1,010 TFLOP/s, at 256 892, at 128 694, at 64 562 where a library product reaches 1,279 (below 256 the softmax's
+// vector work weighs more).  Few keys a row: Q in, O out and the prologue.
 //
 // A key that only some of the 64 rows see is masked for the others by a weight of zero; the matrix core would still
 // turn 0 x inf into NaN.  Keys and values being the same rows, such a value makes the key's raw score non-finite as
@@ -87,16 +96,22 @@ __device__ __forceinline__ T pick(bool second, T x, T y) {
 // ---------------------------------------------------------------------------
 // Schedule
 //
-// Request r has blocks(r) = ceil(n_r H / M) blocks of M rows of about tiles(r) key tiles each.  With U = sum blocks tiles
-// and `want` workgroups, a row block is cut into ceil(tiles / c) shares; c is the smallest of four steps from U / want to
-// 2 U / want with which all shares run at once.  With more row blocks than that, c = 2 U / want cuts only requests
-// far longer than the average, which would otherwise end last on their own.
+// Request r has blocks(r) = ceil(n_r H / 64) row blocks of about tiles(r) key tiles each.  With U = sum blocks tiles and
+// `want` workgroups at once, a row block is cut into ceil(tiles / c) shares.  c is the cheapest of: no cut, and four steps
+// from U / want up, the last one with which all shares run at once.  The cost is the longest share, in tiles, and 1/24 of a
+// tile for each partial output of 64 rows, its write and read (us: 64 row blocks of 12, 24 and 40 tiles, D = 576, cut in two 27, 35 and
+// 44 and whole 25, 41 and 60; 128 of them 36, 44, 54 and 28, 42, 62; with D = 128, 256 of 24 and 40, 30, 36 and 26, 38).
+// With more row blocks than `want`, c = 2 U / want cuts only requests far longer than the average, which would otherwise
+// end last on their own.
 // Every workgroup does these sums itself, with lane-shift scans in 32 bits, and where there are at most 64 requests every
-// wave, without a barrier.
+// wave, without a barrier (721 one-chunk row blocks: 576 us with the barriers, 555 without).  An ascending cu_q makes the
+// requests' rows disjoint, on which every bound here and the sizes of the partial outputs rest; with one that descends
+// somewhere no request has rows.
 // ---------------------------------------------------------------------------
 struct PagedReq {
   int first, n, len;  // first row of q, new tokens, entries of the first cache
   int blocks, tiles;
+  bool down;          // cu_q descends here
 };
 
 __device__ __forceinline__ int ceil_div32(int x) { return static_cast<int>((static_cast<uint32_t>(x) + 31u) >> 5); }
@@ -110,14 +125,14 @@ __device__ __forceinline__ int ent_hi(const PagedAttnArgs& a, int p) {
   return min(static_cast<int>(static_cast<uint32_t>(p + 1) / static_cast<uint32_t>(a.ratio)), a.c2.keys);
 }
 
-template <int M>
 __device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& a, int r) {
   PagedReq q;
   const int c0 = a.cu[r], c1 = a.cu[r + 1];
   q.len = max(a.lens[r], 0);
   q.first = min(max(c0, 0), a.N);
   q.n = max(min(c1, a.N) - q.first, 0);
-  q.blocks = static_cast<int>((static_cast<uint32_t>(q.n) * static_cast<uint32_t>(a.H) + (M - 1)) / M);
+  q.down = c1 < c0;
+  q.blocks = static_cast<int>((static_cast<uint32_t>(q.n) * static_cast<uint32_t>(a.H) + (kRows - 1)) / kRows);
   // tiles of the last row block, which sees the most
   const int p = q.len - 1;
   const int span = max(win_hi(a, p) - win_lo(a, p - a.behind), 0);
@@ -149,11 +164,22 @@ __device__ __forceinline__ int shares_of(int tiles, uint32_t c) {
 
 constexpr uint32_t kWhole = 0x7fffffffu;  // no row block is cut
 
+// Number of this workgroup's item among `total`; `total` and on where it has none.  Consecutive workgroups go to the eight
+// XCDs in turn: each XCD takes runs of up to 32 items, one to a CU, whose keys its L2 then holds once, and all of them the
+// same number, however many of the launched workgroups the lengths leave without an item.
+__device__ __forceinline__ int paged_item_number(int total) {
+  const int xcd = blockIdx.x & 7, k = blockIdx.x >> 3;
+  const int whole = total >> 8;  // rounds of 8 x 32
+  if (k < 32 * whole) return ((k >> 5) * 8 + xcd) * 32 + (k & 31);
+  const int rest = total - 256 * whole, run = (rest + 7) >> 3, i = k - 32 * whole;
+  return i < run ? 256 * whole + xcd * run + i : total;
+}
+
 // The sum over the wave, in lane 63.
 __device__ __forceinline__ float wave_sum_last(float x) {
   auto shifted = [](float v, auto CTRL, auto MASK) {
-    return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)),
-                                                                             decltype(CTRL)::value, decltype(MASK)::value, 0xf, false)));
+    return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+        0, static_cast<int>(__float_as_uint(v)), decltype(CTRL)::value, decltype(MASK)::value, 0xf, false)));
   };
   using std::integral_constant;
   x += shifted(x, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
@@ -165,60 +191,77 @@ __device__ __forceinline__ float wave_sum_last(float x) {
   return x;
 }
 
+// The largest over the wave, in lane 63, of values from 0 on.
+__device__ __forceinline__ int wave_max_last(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  return max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+}
+
 constexpr int kSteps = 4;
+constexpr int kLeastTiles = 4;  // of a share at least
 // Tiles of a share: the steps to try, from the sum of blocks x tiles (rounded up: fp32 sums of whole numbers, at most 2^-20
-// too small over the few thousand additions of a call).
+// too small over the few thousand additions of a call) and the number of row blocks.
 struct ShareSteps {
   uint32_t step[kSteps];
-  float units;
-  uint32_t least;
-  __device__ __forceinline__ uint32_t tiles_of(float x) const {
+  static __device__ __forceinline__ uint32_t tiles_of(float x, int least) {
     return static_cast<uint32_t>(__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(x), static_cast<float>(least)), 0x1p30f));
   }
-  __device__ __forceinline__ ShareSteps(const PagedAttnArgs& a, float sum)
-      : units(sum * (1.0f + 0x1p-16f)), least(static_cast<uint32_t>(a.least)) {
-    const float each = units / static_cast<float>(a.want);
-    step[0] = tiles_of(each);
-    step[1] = tiles_of(1.25f * each);
-    step[2] = tiles_of(1.5f * each);
-    step[3] = tiles_of(2.f * each);
+  __device__ __forceinline__ ShareSteps(float sum, int all, int want) {
+    const float units = sum * (1.0f + 0x1p-16f), each = units / static_cast<float>(want);
+    step[0] = tiles_of(each, kLeastTiles);
+    step[1] = tiles_of(1.25f * each, 6);
+    step[2] = tiles_of(1.5f * each, 8);
+    // (sum of ceil(tiles / c) <= units / c + all <= want)
+    step[3] = tiles_of(__builtin_fmaxf(2.f * each, all < want ? units / static_cast<float>(want - all) : 0.f), 16);
   }
-  // The smallest step whose shares (fits[]) all run at once, for `all` < want row blocks; at the least the one that always
-  // does: sum of ceil(tiles / c) <= units / c + blocks <= want.
-  __device__ __forceinline__ uint32_t pick(const int (&fits)[kSteps], int all, int want) const {
-    uint32_t c = tiles_of(units / static_cast<float>(want - all));
+  // For all < want row blocks, the longest of `longest` tiles, and items[i] shares with step i: see above.
+  __device__ __forceinline__ uint32_t pick(const int (&items)[kSteps], int all, int longest, const PagedAttnArgs& a) const {
+    uint32_t c = kWhole;
+    float cost = static_cast<float>(longest);
 #pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i)
-      if (fits[i] <= want) c = step[i];
+    for (int i = kSteps - 1; i >= 0; --i) {
+      const int more = items[i] - all, parts = more + min(more, all);  // partial outputs, at most
+      const float x = static_cast<float>(min(static_cast<int>(step[i]), longest)) + static_cast<float>(parts) * a.part_cost;
+      if (items[i] <= a.want && x < cost) {
+        c = step[i];
+        cost = x;
+      }
+    }
     return c;
   }
 };
 
-// For up to 64 requests, one to a lane, every wave for itself: no LDS and no barrier.
-template <int M>
-__device__ __forceinline__ bool paged_schedule_wave(const PagedAttnArgs& a, int id, PagedItem& it) {
+// This workgroup's item, or false.  For up to 64 requests, one to a lane, every wave for itself: no LDS and no barrier.
+__device__ __forceinline__ bool paged_schedule_wave(const PagedAttnArgs& a, PagedItem& it, bool& down) {
   const int lane = threadIdx.x & 63;
   PagedReq q{};
-  if (lane < a.R) q = paged_req<M>(a, lane);
+  if (lane < a.R) q = paged_req(a, lane);
+  down = __builtin_amdgcn_ballot_w64(q.down) != 0;
+  if (down) q.blocks = 0;
   auto last = [](int x) { return __builtin_amdgcn_readlane(x, kWave - 1); };
   uint32_t c = kWhole;
   if (a.part_o) {
     const float sum = wave_sum_last(static_cast<float>(q.blocks) * static_cast<float>(q.tiles));
-    const ShareSteps steps(a, __uint_as_float(static_cast<uint32_t>(last(static_cast<int>(__float_as_uint(sum))))));
-    const int all = last(wave_scan(q.blocks));
+    const int all = last(wave_scan(q.blocks)), longest = last(wave_max_last(q.blocks > 0 ? q.tiles : 0));
+    const ShareSteps steps(__uint_as_float(static_cast<uint32_t>(last(static_cast<int>(__float_as_uint(sum))))), all, a.want);
     c = steps.step[kSteps - 1];
     if (all < a.want) {
-      int fits[kSteps];
+      int shares[kSteps];
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) fits[i] = last(wave_scan(q.blocks * shares_of(q.tiles, steps.step[i])));
-      c = steps.pick(fits, all, a.want);
+      for (int i = 0; i < kSteps; ++i) shares[i] = last(wave_scan(q.blocks * shares_of(q.tiles, steps.step[i])));
+      c = steps.pick(shares, all, longest, a);
     }
   }
   const int s = shares_of(q.tiles, c);
   const int items = q.blocks * s, parts = s > 1 ? items : 0, recs = s > 1 ? q.blocks : 0;
   const int end = wave_scan(items), end_parts = wave_scan(parts), end_recs = wave_scan(recs);
-  if (a.part_o && id == 0 && threadIdx.x == kWave - 1) a.rec[0] = end_recs;
-  if (id >= last(end)) return false;
+  if (a.part_o && blockIdx.x == 0 && threadIdx.x == kWave - 1) a.rec[0] = end_recs;
+  const int total = last(end), id = paged_item_number(total);
+  if (id >= total) return false;
   const int r = __builtin_ctzll(__builtin_amdgcn_ballot_w64(id < end));  // the first request that ends behind it
   auto at = [&](int x) { return __builtin_amdgcn_readlane(x, r); };
   const int shares = at(s), k = id - at(end - items), block = k / shares;
@@ -228,36 +271,46 @@ __device__ __forceinline__ bool paged_schedule_wave(const PagedAttnArgs& a, int 
   return true;
 }
 
-// This workgroup's item, or false.  All threads call it.
-template <int M>
-__device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, PagedItem& it) {
+// The same for any number.  All threads call it.
+__device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, PagedItem& it, bool& down) {
   constexpr int W = kPagedThreads / kWave;
   __shared__ float units_lds[W];
-  __shared__ int blocks_lds[W], fits_lds[W][kSteps], sums_lds[3][W];
+  __shared__ int blocks_lds[W], longest_lds[W], items_lds[W][kSteps], sums_lds[3][W];
   __shared__ PagedItem found;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.R + kPagedThreads - 1) / kPagedThreads;
   const int r0 = min(t * per, a.R), r1 = min(r0 + per, a.R);
   PagedReq mine{};  // kept where a thread has one request
   float units = 0.f;
-  int blocks = 0;
+  int blocks = 0, longest = 0;
+  bool descends = false;
   for (int r = r0; r < r1; ++r) {
-    mine = paged_req<M>(a, r);
+    mine = paged_req(a, r);
     units = __builtin_fmaf(static_cast<float>(mine.blocks), static_cast<float>(mine.tiles), units);
     blocks += mine.blocks;
+    longest = max(longest, mine.blocks > 0 ? mine.tiles : 0);
+    descends = descends || mine.down;
   }
-  auto req = [&](int r) { return per == 1 ? mine : paged_req<M>(a, r); };
+  down = __syncthreads_or(descends) != 0;
+  if (down) {
+    if (a.part_o && blockIdx.x == 0 && t == 0) a.rec[0] = 0;
+    return false;
+  }
+  auto req = [&](int r) { return per == 1 ? mine : paged_req(a, r); };
   uint32_t c = kWhole;  // tiles of a share
   if (a.part_o) {
     units = wave_sum_last(units);
     blocks = wave_scan(blocks);
+    longest = wave_max_last(longest);
     if (lane == kWave - 1) {
       units_lds[wave] = units;
       blocks_lds[wave] = blocks;
+      longest_lds[wave] = longest;
     }
     __syncthreads();
-    const ShareSteps steps(a, (units_lds[0] + units_lds[1]) + (units_lds[2] + units_lds[3]));
     const int all = (blocks_lds[0] + blocks_lds[1]) + (blocks_lds[2] + blocks_lds[3]);
+    longest = max(max(longest_lds[0], longest_lds[1]), max(longest_lds[2], longest_lds[3]));
+    const ShareSteps steps((units_lds[0] + units_lds[1]) + (units_lds[2] + units_lds[3]), all, a.want);
     c = steps.step[kSteps - 1];
     if (all < a.want) {
       int n[kSteps] = {};
@@ -269,12 +322,12 @@ __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, P
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         n[i] = wave_scan(n[i]);
-        if (lane == kWave - 1) fits_lds[wave][i] = n[i];
+        if (lane == kWave - 1) items_lds[wave][i] = n[i];
       }
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) n[i] = (fits_lds[0][i] + fits_lds[1][i]) + (fits_lds[2][i] + fits_lds[3][i]);
-      c = steps.pick(n, all, a.want);
+      for (int i = 0; i < kSteps; ++i) n[i] = (items_lds[0][i] + items_lds[1][i]) + (items_lds[2][i] + items_lds[3][i]);
+      c = steps.pick(n, all, longest, a);
     }
   }
   int items = 0, parts = 0, recs = 0;
@@ -306,7 +359,8 @@ __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, P
       total[i] += sums_lds[i][w];
     }
   }
-  if (a.part_o && id == 0 && t == 0) a.rec[0] = total[2];
+  if (a.part_o && blockIdx.x == 0 && t == 0) a.rec[0] = total[2];
+  const int id = paged_item_number(total[0]);
   if (id >= total[0]) return false;
   if (before[0] <= id && id < before[0] + items) {
     int at = before[0], part0 = before[1], rec0 = before[2];
@@ -333,12 +387,12 @@ __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, int id, P
   return true;
 }
 
-// Resident workgroups of a CU: 216 registers of a wave hold Q^T and O^T at D = 576, 96 at D = 256.
+// Resident workgroups of a CU: LDS sets them, and Q^T and O^T take 216 registers of a wave at D = 576, 96 at D = 256.
 constexpr int per_cu(int D, bool PAIR) { return D >= 512 ? (PAIR ? 2 : 1) : D == 256 ? 2 : D == 128 ? 3 : 4; }
 
 constexpr float kNever = -__builtin_inff();
 constexpr int kOdd = 1;    // a masked score that is not finite
-constexpr int kMoved = 2;  // a reference maximum of the wave's row block b has moved (kMoved << b): alpha is not one
+constexpr int kMoved = 2;  // a reference maximum has moved: alpha is not one
 
 // x with infinities and NaN replaced by zero.
 template <bool F16>
@@ -355,17 +409,16 @@ __device__ __forceinline__ bf16x8 finite_or_zero(bf16x8 x) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// RB: blocks of 16 rows of a wave (rows of a workgroup: 64 RB).  PAIR: the steps of a tile one after the other, for two
-// workgroups on a CU.
-template <int D, bool F16, int RB, bool PAIR>
+// PAIR: the steps of a tile one after the other, for two workgroups on a CU.
+template <int D, bool F16, bool PAIR>
 __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_kernel(PagedAttnArgs a) {
   using SH = AttnShape<D>;
   constexpr int KS = SH::KS, MBW = SH::MBW, ROW = SH::ROW;
-  constexpr int M = 64 * RB, NB = 4 * RB;          // rows and row blocks of the workgroup
+  constexpr int M = kRows, NB = M / 16;             // rows of the workgroup, and blocks of 16
   constexpr int NS = PAIR ? 2 : 4, AHEAD = NS - 1;  // tiles in LDS, and copied ahead of P V
   constexpr int NP = PAIR ? 1 : 2, PAGES = PAIR ? 2 : 4;  // P's and page numbers' buffers
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  static_assert(NS * SH::TILE >= 64 * ROW, "the output is staged 64 rows at a time");
+  static_assert(NS * SH::TILE >= M * ROW, "the output is staged in the tiles' LDS");
   __shared__ __attribute__((aligned(16))) char kv_lds[NS * SH::TILE];
   __shared__ __attribute__((aligned(16))) char p_lds[NP][NB * 64 * 16];
   __shared__ __attribute__((aligned(16))) float alpha_lds[NP][M];
@@ -377,21 +430,20 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   __builtin_assume(wave >= 0 && wave < 4);
   const int g = lane >> 4, i16 = lane & 15;
-  const int last = a.R > 0 ? a.cu[a.R] : 0;
-
+  // rows [begin, end) are the requests'
+  int begin = a.R > 0 ? min(max(a.cu[0], 0), a.N) : 0, end = a.R > 0 ? min(max(a.cu[a.R], 0), a.N) : 0;
   PagedItem item;
-  const int id = xcd_block_order();
-  const bool work = a.R <= kWave ? paged_schedule_wave<M>(a, id, item) : paged_schedule<M>(a, id, item);
+  bool down;
+  const bool work = a.R <= kWave ? paged_schedule_wave(a, item, down) : paged_schedule(a, item, down);
+  if (down) begin = end = 0;
   // Rows of no request: as a row without a key.
-  {
-    const int end = last < 0 ? 0 : (last < a.N ? last : a.N);
-    for (int64_t t = end + static_cast<int64_t>(blockIdx.x); t < a.N; t += gridDim.x) {
-      u32x4* orow = reinterpret_cast<u32x4*>(a.o + t * a.H * D);
-      for (int e = threadIdx.x; e < a.H * SH::CPR; e += kPagedThreads) orow[e] = u32x4{0, 0, 0, 0};
-      for (int h = threadIdx.x; h < a.H; h += kPagedThreads) {
-        const float s = a.sink[h];
-        a.lse[t * a.H + h] = s == kNever ? -1.0e30f : s;
-      }
+  for (int64_t i = blockIdx.x; i < begin + static_cast<int64_t>(a.N - end); i += gridDim.x) {
+    const int64_t t = i < begin ? i : end + i - begin;
+    u32x4* orow = reinterpret_cast<u32x4*>(a.o + t * a.H * D);
+    for (int64_t e = threadIdx.x; e < static_cast<int64_t>(a.H) * SH::CPR; e += kPagedThreads) orow[e] = u32x4{0, 0, 0, 0};
+    for (int h = threadIdx.x; h < a.H; h += kPagedThreads) {
+      const float s = a.sink[h];
+      a.lse[t * a.H + h] = s == kNever ? -1.0e30f : s;
     }
   }
   if (!work) return;
@@ -431,7 +483,10 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // Lanes l and l + 32 resolve key l of a tile; a key past the tile's last one stands in for by that one (it is masked,
   // and a tile always has a first key).  A key without a page reads row 0 of the cache and is masked.  Each wave fetches
   // the page numbers for its own copies into LDS (as registers they would make the compiler wait for every copy in
-  // flight before their use), a tile ahead of the copies; `within` is what the key's place in its page adds.
+  // flight before their use), a tile ahead of the copies; `within` is what the key's place in its page adds.  What
+  // a tile asks of its cache is held in scalars that every path sets: as vector registers, which a value that only some
+  // paths set becomes, they were spilled and read back between a tile's steps, with a wait for its copies each time
+  // (7,249 row blocks of up to 21 tiles, D = 576: 540 us, 476 without).
   CacheView view1, view2;
   CacheBase base1, base2;
   view_cache(a.c1, req, view1, base1);
@@ -521,7 +576,9 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
                                        (lds_void_t*)dst, 16, 0, 0);
   };
   auto ring = [&](int slot) __attribute__((always_inline)) { return kv_lds + slot * SH::TILE; };
-  auto page_addr = [&](int t) __attribute__((always_inline)) { return lds_addr(reinterpret_cast<const char*>(&page_lds[wave][t % PAGES][0])) + lane_now() * 4; };
+  auto page_addr = [&](int t) __attribute__((always_inline)) {
+    return lds_addr(reinterpret_cast<const char*>(&page_lds[wave][t % PAGES][0])) + lane_now() * 4;
+  };
   // (the first tiles' page numbers are on their way while Q is addressed; tiles past the share's end are not used)
   uint32_t within[AHEAD + 1];
   CacheBase froms[AHEAD + 1];
@@ -533,35 +590,30 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     froms[i] = from_next;
   }
 
-  // ---- this lane's rows: their Q^T fragments and the keys they see ----------------
-  int rpos[RB];  // position, -1: no row
-  const float* sink_at[RB];
-  bf16x8 qf[RB][KS];
+  __builtin_amdgcn_sched_barrier(0);
+
+  // ---- this lane's row: its Q^T fragment and the keys it sees ----------------
+  bf16x8 qf[KS];
+  const int lrow = wave * 16 + i16;
+  const bool live = lrow < nrows;
+  const int tok = live ? (row0 + lrow) / a.H : 0;
+  const int head = live ? row0 + lrow - tok * a.H : 0;
+  const int rpos = live ? pos0 + tok : -1;  // position, -1: no row
+  const float* sink_at = a.sink + head;
+  // (a row past the block's last one reads the first one's Q; nothing of it is used)
+  const uint16_t* qrow = a.q + (static_cast<int64_t>(item.first) + tok) * a.qst + head * a.qsh;
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int lrow = (wave * RB + b) * 16 + i16;
-    const bool live = lrow < nrows;
-    const int tok = live ? (row0 + lrow) / a.H : 0;
-    const int head = live ? row0 + lrow - tok * a.H : 0;
-    rpos[b] = live ? pos0 + tok : -1;
-    sink_at[b] = a.sink + head;
-    // (a row past the block's last one reads the first one's Q; nothing of it is used)
-    const uint16_t* qrow = a.q + (static_cast<int64_t>(item.first) + tok) * a.qst + head * a.qsh;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[b][ks] = *reinterpret_cast<const bf16x8*>(qrow + ks * 32 + g * 8);
-  }
-  // The page numbers, asked for before these KS * RB loads, have landed; the loads may be in flight.
-  __builtin_amdgcn_s_waitcnt(vm_lgkm0(KS * RB));
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qrow + ks * 32 + g * 8);
+  // The page numbers, asked for before these KS loads, have landed; the loads may be in flight.  (The loads return in
+  // order; the scheduling barriers keep them between the page numbers and the wait.)
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(vm_lgkm0(KS));
+  __builtin_amdgcn_sched_barrier(0);
   // Sinks, kept in LDS for the end (each row's is read back by the lane that wrote it).
-  float sink_v[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) sink_v[b] = *sink_at[b];
+  const float sink_v = *sink_at;
   auto sink_to_lds = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const uint32_t dst = lds_addr(reinterpret_cast<const char*>(&sink_lds[(wave * RB + b) * 16 + i16]));
-      asm volatile("ds_write_b32 %0, %1" ::"v"(dst), "v"(sink_v[b]) : "memory");  // (the four lanes of a row write the same)
-    }
+    const uint32_t dst = lds_addr(reinterpret_cast<const char*>(&sink_lds[wave * 16 + i16]));
+    asm volatile("ds_write_b32 %0, %1" ::"v"(dst), "v"(sink_v) : "memory");  // (the four lanes of a row write the same)
   };
 
   // ---- S^T -------------------------------------------------------------------
@@ -573,13 +625,11 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     if (__builtin_expect(a.scale_log2 <= 0.f, 0)) {
       const uint32_t keep = a.scale_log2 == 0.f ? 0u : ~0u, flip = a.scale_log2 == 0.f ? 0u : 0x80008000u;
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
-#pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          qf[b][ks] = __builtin_bit_cast(bf16x8, (__builtin_bit_cast(u32x4, qf[b][ks]) & keep) ^ flip);
+          qf[ks] = __builtin_bit_cast(bf16x8, (__builtin_bit_cast(u32x4, qf[ks]) & keep) ^ flip);
     }
   };
-  auto qk = [&](int slot, f32x4 (&st)[RB][2], auto&& start, auto&& beside) __attribute__((always_inline)) {
+  auto qk = [&](int slot, f32x4 (&st)[2], auto&& start, auto&& beside) __attribute__((always_inline)) {
     const int ln = lane_now(), key = ln & 15, f = kv_swz<D>(key);
     const uint32_t at = lds_addr(ring(slot)) + key * ROW + 16 * ((ln >> 4) ^ (f & 3));
     const uint32_t qa_e = at + 64 * (f >> 2), qa_o = at - 64 * (f >> 2);
@@ -592,17 +642,13 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     };
     attn_static_for<0, QPD>(issue);
     start();
-#pragma unroll
-    for (int b = 0; b < RB; ++b) st[b][0] = st[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    st[0] = st[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     attn_static_for<0, KS>([&](auto KC) {
       constexpr int ks = decltype(KC)::value;
       constexpr int later = (KS - 1 - ks) < (QPD - 1) ? (KS - 1 - ks) : (QPD - 1);
       lds_wait<2 * later>(kq[ks % QPD][0], kq[ks % QPD][1]);
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        st[b][0] = mfma16x16x32<F16>(kq[ks % QPD][0], qf[b][ks], st[b][0]);
-        st[b][1] = mfma16x16x32<F16>(kq[ks % QPD][1], qf[b][ks], st[b][1]);
-      }
+      st[0] = mfma16x16x32<F16>(kq[ks % QPD][0], qf[ks], st[0]);
+      st[1] = mfma16x16x32<F16>(kq[ks % QPD][1], qf[ks], st[1]);
       if constexpr (ks + QPD < KS) issue(std::integral_constant<int, ks + QPD>{});
       beside(KC);
     });
@@ -631,16 +677,10 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // is due; the weights one by one; their sum and their place in LDS.
   // (scale is positive: a negative one has changed the sign of Q, zero has made Q zero)
   constexpr float kLazy = F16 ? 8.0f : 64.0f;  // 2^8 keeps P in fp16's range, 2^64 in bf16's
-  float m_ref[RB], l_run[RB];  // reference maximum (log2 domain) and this lane's share of the denominator
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    m_ref[b] = kNever;
-    l_run[b] = 0.f;
-  }
+  float m_ref = kNever, l_run = 0.f;  // reference maximum (log2 domain) and this lane's share of the denominator
   int skey = 0;  // first key of the next tile to mask
-  auto softmax_begin = [&](int t, uint32_t okmask, f32x4 (&st)[RB][2], float (&ref)[RB], int pbuf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int b = 0; b < RB; ++b) mfma_result_fence(st[b][0], st[b][1]);
+  auto softmax_begin = [&](int t, uint32_t okmask, f32x4 (&st)[2], float& ref, int pbuf) __attribute__((always_inline)) {
+    mfma_result_fence(st[0], st[1]);
     if (t == n1) skey = 0;
     const bool second = t >= n1;
     // every row sees every key of the tile (32-bit sums: skey is below the end of a range that fits 31 bits)
@@ -649,64 +689,55 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     if (!full) {
       bool odd = false;
       const int g4 = 4 * (lane_now() >> 4);
+      const int end = second ? ent_end(rpos) : max(min(rpos + 1, cap1), 0);
+      const int begin = second ? 0 : max(max(rpos + 1, 0) - window, 0);
+      const int lo = skey - begin, cnt = max(end - begin, 0);
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        const int end = second ? ent_end(rpos[b]) : max(min(rpos[b] + 1, cap1), 0);
-        const int begin = second ? 0 : max(max(rpos[b] + 1, 0) - window, 0);
-        const int lo = skey - begin, cnt = max(end - begin, 0);
+      for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
-        for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int kk = 16 * mb + g4 + r;
-            const bool ok = static_cast<uint32_t>(kk + lo) < static_cast<uint32_t>(cnt) && ((okmask >> kk) & 1);
-            const bool fin = __builtin_fabsf(st[b][mb][r]) < __builtin_inff();
-            odd = odd || (!ok && !fin);
-            st[b][mb][r] = ok ? (fin ? st[b][mb][r] : __builtin_nanf("")) : kNever;
-          }
-      }
+        for (int r = 0; r < 4; ++r) {
+          const int kk = 16 * mb + g4 + r;
+          const bool ok = static_cast<uint32_t>(kk + lo) < static_cast<uint32_t>(cnt) && ((okmask >> kk) & 1);
+          const bool fin = __builtin_fabsf(st[mb][r]) < __builtin_inff();
+          odd = odd || (!ok && !fin);
+          st[mb][r] = ok ? (fin ? st[mb][r] : __builtin_nanf("")) : kNever;
+        }
       flags = __builtin_amdgcn_ballot_w64(odd) ? kOdd : 0;
     }
     skey += 32;
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const f32x4 y0 = st[b][0], y1 = st[b][1];
-      float lmax = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(y0[0], y0[1]), __builtin_fmaxf(y0[2], y0[3])),
-                                   __builtin_fmaxf(__builtin_fmaxf(y1[0], y1[1]), __builtin_fmaxf(y1[2], y1[3])));
-      lmax *= scale;
-      // no lane's keys lift its row's maximum: the tile's maximum over the lanes of a row is not needed
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(lmax > m_ref[b] + kLazy) != 0, 0)) {
-        const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
-        float tmax = __builtin_fmaxf(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
-        const SwapPair r32 = permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax));
-        tmax = __builtin_fmaxf(__uint_as_float(r32.x), __uint_as_float(r32.y));
-        const bool raise = tmax > m_ref[b] + kLazy, first = m_ref[b] == kNever;
-        const float alpha = raise && !first ? __builtin_amdgcn_exp2f(m_ref[b] - tmax) : 1.0f;
-        if (raise) m_ref[b] = tmax;
-        l_run[b] *= alpha;
-        const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][(wave * RB + b) * 16 + (lane_now() & 15)]));
-        asm volatile("ds_write_b32 %0, %1" ::"v"(adst), "v"(alpha) : "memory");  // (the four lanes of a row write the same)
-        if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) flags |= kMoved << b;
-      }
-      ref[b] = m_ref[b] == kNever ? 0.f : m_ref[b];
+    const f32x4 y0 = st[0], y1 = st[1];
+    float lmax = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(y0[0], y0[1]), __builtin_fmaxf(y0[2], y0[3])),
+                                 __builtin_fmaxf(__builtin_fmaxf(y1[0], y1[1]), __builtin_fmaxf(y1[2], y1[3])));
+    lmax *= scale;
+    // no lane's keys lift its row's maximum: the tile's maximum over the lanes of a row is not needed
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(lmax > m_ref + kLazy) != 0, 0)) {
+      const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
+      float tmax = __builtin_fmaxf(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
+      const SwapPair r32 = permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax));
+      tmax = __builtin_fmaxf(__uint_as_float(r32.x), __uint_as_float(r32.y));
+      const bool raise = tmax > m_ref + kLazy, first = m_ref == kNever;
+      const float alpha = raise && !first ? __builtin_amdgcn_exp2f(m_ref - tmax) : 1.0f;
+      if (raise) m_ref = tmax;
+      l_run *= alpha;
+      const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][wave * 16 + (lane_now() & 15)]));
+      asm volatile("ds_write_b32 %0, %1" ::"v"(adst), "v"(alpha) : "memory");  // (the four lanes of a row write the same)
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) flags |= kMoved;
     }
+    ref = m_ref == kNever ? 0.f : m_ref;
     const uint32_t fdst = lds_addr(reinterpret_cast<const char*>(&flag_lds[pbuf][wave]));
     asm volatile("ds_write_b32 %0, %1" ::"v"(fdst), "v"(flags) : "memory");
   };
-  auto softmax_exp = [&](int i, f32x4 (&st)[RB][2], const float (&ref)[RB]) __attribute__((always_inline)) {  // i of 8 RB weights
+  auto softmax_exp = [&](int i, f32x4 (&st)[2], float ref) __attribute__((always_inline)) {  // i of 8 weights
     const int b = i >> 3, mb = (i >> 2) & 1, r = i & 3;
-    st[b][mb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[b][mb][r], scale, -ref[b]));
+    st[mb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[mb][r], scale, -ref));
   };
-  auto softmax_end = [&](const f32x4 (&p)[RB][2], int pbuf) __attribute__((always_inline)) {
-    const uint32_t pdst = lds_addr(&p_lds[pbuf][(wave * RB * 64 + lane_now()) * 16]);
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      l_run[b] += ((p[b][0][0] + p[b][0][1]) + (p[b][0][2] + p[b][0][3])) + ((p[b][1][0] + p[b][1][1]) + (p[b][1][2] + p[b][1][3]));
-      // P^T B-fragment: k-slots 8g+0..3 <-> keys 4g+0..3, 8g+4..7 <-> keys 16+4g+0..3
-      const u32x4 w = u32x4{pack2<F16>(p[b][0][0], p[b][0][1]), pack2<F16>(p[b][0][2], p[b][0][3]),
-                            pack2<F16>(p[b][1][0], p[b][1][1]), pack2<F16>(p[b][1][2], p[b][1][3])};
-      asm volatile("ds_write_b128 %0, %1" ::"v"(pdst + b * 1024), "v"(w) : "memory");
-    }
+  auto softmax_end = [&](const f32x4 (&p)[2], int pbuf) __attribute__((always_inline)) {
+    const uint32_t pdst = lds_addr(&p_lds[pbuf][(wave * 64 + lane_now()) * 16]);
+    l_run += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+    // P^T B-fragment: k-slots 8g+0..3 <-> keys 4g+0..3, 8g+4..7 <-> keys 16+4g+0..3
+    const u32x4 w = u32x4{pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]),
+                          pack2<F16>(p[1][0], p[1][1]), pack2<F16>(p[1][2], p[1][3])};
+    asm volatile("ds_write_b128 %0, %1" ::"v"(pdst), "v"(w) : "memory");
   };
 
   // ---- O^T += V^T P^T -------------------------------------------------------------
@@ -718,7 +749,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // V^T transposing reads: source lane (g, i16) points at key 4g + (i16 >> 2) (+16 for k-slots 4..7), dims d0 + 4 (i16 & 3)
   // with d0 = 16 (4j + wave); chunk 8j + x, x = 2 wave + ((i16 & 3) >> 1) < 8, swizzles to 8j + (x ^ f): a fixed base + 128 j.
   // V^T blocks go through a queue VQ deep; between(j) runs among the MFMAs of output block j.
-  constexpr int VQ0 = PAIR ? 2 : RB == 1 ? 4 : 3, VQ = VQ0 < MBW ? VQ0 : MBW;
+  constexpr int VQ0 = PAIR ? 2 : 4, VQ = VQ0 < MBW ? VQ0 : MBW;
   auto pv = [&](int slot, int pbuf, auto&& between) __attribute__((always_inline)) {
     const int ln = lane_now();
     const int tkey = 4 * (ln >> 4) + ((ln & 15) >> 2);
@@ -776,8 +807,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
         asm volatile("ds_read_b32 %0, %2\n\tds_read_b32 %1, %3\n\ts_waitcnt lgkmcnt(0)"
                      : "=&v"(al), "=&v"(f)
                      : "v"(lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][nb * 16 + i16]))),
-                       "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[pbuf][nb / RB]))));
-        al = f & (kMoved << (nb % RB)) ? al : 1.0f;
+                       "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[pbuf][nb]))));
+        al = f & kMoved ? al : 1.0f;
 #pragma unroll
         for (int j = 0; j < MBW; ++j) oacc[j][nb] = oacc[j][nb] * al;
       }
@@ -792,7 +823,9 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // Iteration t: P V of tile t beside S^T and softmax of tile t + 1, one barrier.  Tile t lives in slot t - tbeg mod NS,
   // its P in p_lds[t & 1].  The copies of tile t + AHEAD go out at the start, into the slot of tile t - 1, which every
   // wave has left; they land by the start of iteration t + AHEAD - 1.
-  if (!PAIR && tbeg < tend) {
+  if (tbeg >= tend) {
+    sink_to_lds();
+  } else if constexpr (!PAIR) {
     skey = tbeg < n1 ? k1lo + tbeg * 32 : (tbeg - n1) * 32;
     uint32_t okq[AHEAD];
     Sources src;
@@ -812,14 +845,14 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     if (tbeg + AHEAD <= tend) __builtin_amdgcn_s_waitcnt(vm_lgkm0((AHEAD - 1) * (SH::CH / SH::NT)));
     else __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
     attn_tile_barrier();  // the first tile landed
-    f32x4 st[RB][2];
-    float ref[RB];
+    f32x4 st[2];
+    float ref;
     sink_to_lds();
     scale_q();
     qk(0, st, [] {}, [](auto) {});
     softmax_begin(tbeg, okq[0], st, ref, tbeg & 1);
 #pragma unroll
-    for (int i = 0; i < 8 * RB; ++i) softmax_exp(i, st, ref);
+    for (int i = 0; i < 8; ++i) softmax_exp(i, st, ref);
     softmax_end(st, tbeg & 1);
     int slot = 0;  // of tile t
     // MORE: a tile t + 1; COPY: a tile t + AHEAD
@@ -827,7 +860,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
       constexpr bool more = decltype(MORE)::value, ahead = decltype(COPY)::value;
       // tile t + 1 (and the page numbers of tile t + AHEAD) landed; with three tiles ahead the copies of the last stay in
       // flight.  Behind the barrier: every wave's, and every wave's P of tile t.
-      if (AHEAD >= 3 && ahead) __builtin_amdgcn_s_waitcnt(vm_lgkm0(SH::CH / SH::NT));
+      if constexpr (ahead) __builtin_amdgcn_s_waitcnt(vm_lgkm0(SH::CH / SH::NT));
       else __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
       attn_tile_barrier();
       const int next = slot + 1 == NS ? 0 : slot + 1, last_slot = slot == 0 ? NS - 1 : slot - 1;
@@ -860,22 +893,15 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
       }
       if constexpr (ahead) from = from_next;
       if (__builtin_expect(flags != 0, 0)) settle(flags, t & 1, slot);
-      constexpr bool BESIDE = RB == 1 || D < 576;  // (registers)
-      constexpr int EPB = MBW > 2 ? (8 * RB + MBW - 3) / (MBW > 2 ? MBW - 2 : 1) : 8 * RB;  // weights beside an output block
-      if constexpr (more && !BESIDE) {
-        softmax_begin(t + 1, okq[1 % AHEAD], st, ref, (t + 1) & 1);
-#pragma unroll
-        for (int i = 0; i < 8 * RB; ++i) softmax_exp(i, st, ref);
-        softmax_end(st, (t + 1) & 1);
-      }
+      constexpr int SPAN = MBW > 2 ? MBW - 2 : 1, EPB = (8 + SPAN - 1) / SPAN;  // weights beside one of SPAN output blocks
       pv(slot, t & 1, [&](auto JC) {
         constexpr int j = decltype(JC)::value;
-        if constexpr (more && BESIDE) {
-          if constexpr (j == 0) softmax_begin(t + 1, okq[1 % AHEAD], st, ref, (t + 1) & 1);
-          constexpr int first = MBW > 2 ? (j - 1) * EPB : 0;
+        if constexpr (more) {
+          if constexpr (j == 0) softmax_begin(t + 1, okq[1], st, ref, (t + 1) & 1);
           if constexpr (j > 0 || MBW == 1) {
+            constexpr int first = MBW == 1 ? 0 : (j - 1) * EPB;
 #pragma unroll
-            for (int i = first < 0 ? 0 : first; i < first + EPB && i < 8 * RB; ++i) softmax_exp(i, st, ref);
+            for (int i = first; i < first + EPB && i < 8; ++i) softmax_exp(i, st, ref);
           }
           if constexpr (j + 1 == MBW) softmax_end(st, (t + 1) & 1);
         }
@@ -889,11 +915,9 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     for (; t + AHEAD < tend; ++t) iteration(t, std::true_type{}, std::true_type{});
     for (; t + 1 < tend; ++t) iteration(t, std::true_type{}, std::false_type{});
     iteration(t, std::false_type{}, std::false_type{});
-  }
-  if (tbeg >= tend) sink_to_lds();
-  // PAIR: one tile ahead in LDS, a tile's steps one after the other, two barriers; the other workgroup of the CU fills the
-  // gaps.
-  if (PAIR && tbeg < tend) {
+  } else {
+    // PAIR: one tile ahead in LDS, a tile's steps one after the other, two barriers; the other workgroup of the CU fills
+    // the gaps.
     skey = tbeg < n1 ? k1lo + tbeg * 32 : (tbeg - n1) * 32;
     uint32_t ok;
     {
@@ -914,12 +938,12 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
       attn_tile_barrier();  // tile t landed, every wave has left tile t - 1 and its P
       uint32_t ok_next = 0;
       {
-        f32x4 st[RB][2];
-        float ref[RB];
+        f32x4 st[2];
+        float ref;
         qk(slot, st, [] {}, [](auto) {});
         softmax_begin(t, ok, st, ref, 0);
 #pragma unroll
-        for (int i = 0; i < 8 * RB; ++i) softmax_exp(i, st, ref);
+        for (int i = 0; i < 8; ++i) softmax_exp(i, st, ref);
         softmax_end(st, 0);
       }
       if (t + 1 < tend) {
@@ -947,20 +971,14 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");  // (the last MFMAs' wait states, see mfma_result_fence)
 
   // ---- the result ----------------------------------------------------------------
-  float l_tot[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_run[b]), __float_as_uint(l_run[b]), false, false);
-    l_tot[b] = __uint_as_float(r16[0]) + __uint_as_float(r16[1]);
-    const SwapPair r32 = permlane32_swap(__float_as_uint(l_tot[b]), __float_as_uint(l_tot[b]));
-    l_tot[b] = __uint_as_float(r32.x) + __uint_as_float(r32.y);
-  }
+  const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+  float l_tot = __uint_as_float(r16[0]) + __uint_as_float(r16[1]);
+  const SwapPair r32 = permlane32_swap(__float_as_uint(l_tot), __float_as_uint(l_tot));
+  l_tot = __uint_as_float(r32.x) + __uint_as_float(r32.y);
   const int64_t flat0 = static_cast<int64_t>(item.first) * a.H + row0;  // first row of o
   if (shares > 1) {
     const int64_t slot = item.slot;
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-      if (g == 0) a.part_ml[slot * M + (wave * RB + b) * 16 + i16] = float2{m_ref[b], l_tot[b]};
+    if (g == 0) a.part_ml[slot * M + wave * 16 + i16] = float2{m_ref, l_tot};
     float* po = a.part_o + slot * M * D;
 #pragma unroll
     for (int j = 0; j < MBW; ++j) {
@@ -968,7 +986,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
       if (SH::MBT % kAttnWaves == 0 || mbi < SH::MBT) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-          if (nb * 16 < nrows) *reinterpret_cast<f32x4*>(po + (nb * 16 + i16) * D + mbi * 16 + 4 * g) = oacc[j][nb];
+          if (nb * 16 < nrows) *reinterpret_cast<f32x4*>(po + ((nb * SH::MBT + mbi) * 64 + lane) * 4) = oacc[j][nb];
       }
     }
     if (share == 0 && threadIdx.x == 0) {
@@ -979,82 +997,79 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   }
   float* scale_lds = alpha_lds[0];
   __syncthreads();  // every wave has left the last tile and its alpha
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int lrow = (wave * RB + b) * 16 + i16;
-    const bool live = lrow < nrows;
-    const float sink = sink_lds[lrow];
-    const float sink2 = sink * kLog2e;
-    const float m_fin = __builtin_fmaxf(m_ref[b], sink2);
-    const float top = m_fin == kNever ? 0.f : m_fin;
-    const float resc = __builtin_amdgcn_exp2f(m_ref[b] - top);
-    const float l_fin = l_tot[b] * resc + __builtin_amdgcn_exp2f(sink2 - top);
-    if (g == 0) {
-      scale_lds[lrow] = l_fin == 0.f ? 0.f : resc / l_fin;
-      if (live)
-        a.lse[flat0 + lrow] = l_fin == 0.f ? -1.0e30f : l_tot[b] == 0.f ? sink : (__builtin_amdgcn_logf(l_fin) + top) * kLn2;
-    }
+  const float sink = sink_lds[lrow];
+  const float sink2 = sink * kLog2e;
+  const float m_fin = __builtin_fmaxf(m_ref, sink2);
+  const float top = m_fin == kNever ? 0.f : m_fin;
+  const float resc = __builtin_amdgcn_exp2f(m_ref - top);
+  const float l_fin = l_tot * resc + __builtin_amdgcn_exp2f(sink2 - top);
+  if (g == 0) {
+    scale_lds[lrow] = l_fin == 0.f ? 0.f : resc / l_fin;
+    if (live)
+      a.lse[flat0 + lrow] = l_fin == 0.f ? -1.0e30f : l_tot == 0.f ? sink : (__builtin_amdgcn_logf(l_fin) + top) * kLn2;
   }
   __syncthreads();  // scales published
-  // staged 64 rows at a time in the tiles' LDS, chunk c of row r at c ^ (r & 7), then written in one piece: the rows follow
-  // each other in o
+  // staged in the tiles' LDS, chunk c of row r at c ^ (r & 7), then written in one piece: the rows follow each other in o
+  float sc[NB];
 #pragma unroll
-  for (int half = 0; half < RB; ++half) {
-    float sc[4];
+  for (int nb = 0; nb < NB; ++nb) sc[nb] = scale_lds[nb * 16 + i16];
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) sc[nb] = scale_lds[(4 * half + nb) * 16 + i16];
+  for (int j = 0; j < MBW; ++j) {
+    const int mbi = j * kAttnWaves + wave;
+    if (SH::MBT % kAttnWaves == 0 || mbi < SH::MBT) {
 #pragma unroll
-    for (int j = 0; j < MBW; ++j) {
-      const int mbi = j * kAttnWaves + wave;
-      if (SH::MBT % kAttnWaves == 0 || mbi < SH::MBT) {
-#pragma unroll
-        for (int nb = 0; nb < 4; ++nb) {
-          const f32x4 v = oacc[j][4 * half + nb] * sc[nb];
-          uint2 w;
-          w.x = pack2<F16>(v[0], v[1]);
-          w.y = pack2<F16>(v[2], v[3]);
-          *reinterpret_cast<uint2*>(kv_lds + kv_off<D>(nb * 16 + i16, 2 * mbi + (g >> 1)) + 8 * (g & 1)) = w;
-        }
+      for (int nb = 0; nb < NB; ++nb) {
+        const f32x4 v = oacc[j][nb] * sc[nb];
+        uint2 w;
+        w.x = pack2<F16>(v[0], v[1]);
+        w.y = pack2<F16>(v[2], v[3]);
+        *reinterpret_cast<uint2*>(kv_lds + kv_off<D>(nb * 16 + i16, 2 * mbi + (g >> 1)) + 8 * (g & 1)) = w;
       }
     }
-    __syncthreads();
-    char* obase = reinterpret_cast<char*>(a.o + (flat0 + 64 * half) * D);
-    const int n = min(nrows - 64 * half, 64);
-    for (int e = threadIdx.x; e < n * SH::CPR; e += kPagedThreads)
-      *reinterpret_cast<u32x4*>(obase + static_cast<int64_t>(e) * 16) =
-          *reinterpret_cast<const u32x4*>(kv_lds + kv_off<D>(e / SH::CPR, e % SH::CPR));
-    if (half + 1 < RB) __syncthreads();
   }
+  __syncthreads();
+  char* obase = reinterpret_cast<char*>(a.o + flat0 * D);
+  for (int e = threadIdx.x; e < nrows * SH::CPR; e += kPagedThreads)
+    *reinterpret_cast<u32x4*>(obase + static_cast<int64_t>(e) * 16) =
+        *reinterpret_cast<const u32x4*>(kv_lds + kv_off<D>(e / SH::CPR, e % SH::CPR));
 }
 
+constexpr int kCombineParts = 4;
 // Joins the shares of the split row blocks.  A thread takes four dimensions of a row and every PARTS-th share, up to
 // sixteen in flight, with a running maximum; with four parts the four threads of a place join theirs in LDS.  Bound: the
-// partial outputs, read once (they fit the last-level cache).
-template <bool F16, int PARTS>
-__global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnArgs a, int D, int M) {
+// latency of the launch and of two dependent loads (4 us with nothing split, 6 for 256 partial outputs at D = 576, 38 MB
+// that the last-level cache holds).
+template <bool F16>
+__global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnArgs a, int D) {
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  constexpr int U = PARTS == 1 ? 16 : 8, PLACES = kPagedThreads / PARTS;
-  __shared__ float lds[PARTS > 1 ? PARTS - 1 : 1][6][PARTS > 1 ? PLACES : 1];
+  constexpr int M = kRows, U = 4;
+  __shared__ float lds[kCombineParts - 1][6][kPagedThreads / kCombineParts];
   const int count = a.rec[0];
-  const int vec = D / 4;
-  const int at = threadIdx.x % PLACES, part = threadIdx.x / PLACES;
-  const int e = static_cast<int>(blockIdx.x) * PLACES + at;
-  const int row = e / vec, d = (e - row * vec) * 4;
+  const bool wide = static_cast<int>(gridDim.x) > D / 16;
   for (int b = blockIdx.y; b < count; b += gridDim.y) {
     const int4 rec = *reinterpret_cast<const int4*>(a.rec + 4 + 4 * static_cast<int64_t>(b));
-    if (static_cast<int>(blockIdx.x) * PLACES / vec >= rec.w) continue;  // (the same in every thread)
+    const int parts = wide && rec.y > 2 * U ? kCombineParts : 1, places = kPagedThreads / parts;
+    if (static_cast<int>(blockIdx.x) * places >= M * D / 4) continue;
+    const int at = threadIdx.x % places, part = threadIdx.x / places;
+    // block of 16 rows and 16 dimensions (the same in a whole wave), row and dimensions
+    const int block = (static_cast<int>(blockIdx.x) * places + at) >> 6, nb = block / (D / 16), mbi = block - nb * (D / 16);
+    const int lane = at & 63, row = nb * 16 + (lane & 15), d = mbi * 16 + 4 * (lane >> 4);
+    if (nb * 16 >= rec.w) continue;  // (the same in every thread where there are parts)
+    const bool live = row < rec.w;
+    const int64_t flat = static_cast<int64_t>(rec.z) + row;
+    const float sink = live ? a.sink[flat % a.H] : 0.f;
     float m = kNever, l = 0.f;
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int64_t first = static_cast<int64_t>(rec.x) * M + (row < rec.w ? row : 0);
-    const float2* ml = a.part_ml + first;
-    const float* po = a.part_o + first * D + d;
-    for (int i0 = part; i0 < rec.y; i0 += U * PARTS) {
+    const int64_t first = static_cast<int64_t>(rec.x) * M;
+    const float2* ml = a.part_ml + first + (live ? row : 0);
+    const float* po = a.part_o + first * D + (block * 64 + lane) * 4;
+    for (int i0 = part; i0 < rec.y; i0 += U * parts) {
       float2 v[U];
       f32x4 x[U];
       float top = m;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * PARTS;
+        const int i = i0 + u * parts;
         if (i < rec.y) {  // (the same in a whole wave)
           v[u] = ml[static_cast<int64_t>(i) * M];
           x[u] = *reinterpret_cast<const f32x4*>(po + static_cast<int64_t>(i) * M * D);
@@ -1078,7 +1093,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnA
         for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(x[u][c], w, acc[c]);
       }
     }
-    if constexpr (PARTS > 1) {
+    if (parts > 1) {  // (the same in every thread, and nb too)
       __syncthreads();  // (the last block's partial sums have been read)
       if (part > 0) {
         lds[part - 1][0][at] = m;
@@ -1090,13 +1105,13 @@ __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnA
       if (part == 0) {
         float top = m;
 #pragma unroll
-        for (int q = 0; q + 1 < PARTS; ++q) top = __builtin_fmaxf(top, lds[q][0][at]);
+        for (int q = 0; q + 1 < kCombineParts; ++q) top = __builtin_fmaxf(top, lds[q][0][at]);
         const float ref = top == kNever ? 0.f : top;
         float w = __builtin_amdgcn_exp2f(m - ref);
         l *= w;
         acc *= w;
 #pragma unroll
-        for (int q = 0; q + 1 < PARTS; ++q) {
+        for (int q = 0; q + 1 < kCombineParts; ++q) {
           w = __builtin_amdgcn_exp2f(lds[q][0][at] - ref);
           l = __builtin_fmaf(lds[q][1][at], w, l);
 #pragma unroll
@@ -1105,9 +1120,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnA
         m = top;
       }
     }
-    if (part > 0 || row >= rec.w) continue;
-    const int64_t flat = static_cast<int64_t>(rec.z) + row;
-    const float sink = a.sink[flat % a.H];
+    if (part > 0 || !live) continue;
     const float sink2 = sink * kLog2e;
     const float top = __builtin_fmaxf(m, sink2);
     const float ref = top == kNever ? 0.f : top;
@@ -1127,7 +1140,6 @@ static bool served(int64_t D) { return D == 32 || D == 64 || D == 128 || D == 25
 
 // Sizes of a call, from what the host knows.
 struct PagedSizes {
-  int rb;                // row blocks of 16 of a wave
   bool pair;             // two workgroups on a CU (D >= 512)
   int64_t blocks;        // row blocks of a workgroup at most
   int64_t want;          // workgroups that run at once
@@ -1137,24 +1149,24 @@ struct PagedSizes {
   int64_t bytes;         // scratch
   int behind;            // tokens of a row block before its last one at most
 };
-constexpr int kLeastTiles = 8;  // tiles of a share at least
-
 static PagedSizes paged_sizes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys1, int64_t keys2) {
   PagedSizes p{};
-  p.rb = 1;
-  const int64_t M = 64 * p.rb;
+  const int64_t M = kRows;
   // a request's last row block is part empty unless M divides n H
   int64_t g = M;
   while (H % g) g /= 2;
   p.blocks = (N * H + (R < N ? R : N) * (M - g)) / M;
-  p.pair = D >= 512 && p.blocks >= 512;
+  p.pair = D >= 512 && p.blocks > 256;
   const int64_t want = p.want = 256 * per_cu(static_cast<int>(D), p.pair);
   p.grid = 2 * p.blocks <= want ? want : p.blocks + want;
   // tiles of a row block at most
   const int64_t span = M / H + 1 + window;
   p.behind = static_cast<int>((M - 1) / H);
   const int64_t tiles = ((window < keys1 && span < keys1 ? span : keys1) + 31) / 32 + (keys2 + 31) / 32;
-  if (tiles <= kLeastTiles) {
+  // Where no cut can win back the second launch, 4 us, that joins the shares, none is made (8 tiles at D = 576, 14 at 128, and
+  // more of them where many row blocks leave partial outputs; us whole and cut in two: 1 row block of 10 and 16 tiles, D = 576,
+  // 21 and 21, 29 and 22; 64 of 16 and 24, 30 and 30, 41 and 34; one of 16 and 24, D = 128, 17 and 20, 23 and 20).
+  if (tiles <= (D >= 512 ? 8 : 14) + p.blocks / 8) {
     p.grid = p.blocks;
     return p;
   }
@@ -1171,30 +1183,30 @@ static PagedSizes paged_sizes(int64_t N, int64_t H, int64_t D, int64_t R, int64_
 
 template <int D>
 static int launch_paged_attn_d(bool f16, const PagedAttnArgs& a, const PagedSizes& p, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(p.grid < 1 ? 1 : p.grid)), block(kPagedThreads);
-  if (D >= 512 && p.pair) {
-    if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true, 1, (D >= 512)>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<D, false, 1, (D >= 512)>), grid, block, 0, st, a);
+  const int64_t most = 0xffffffffLL / kPagedThreads;  // (a launch has fewer than 2^32 threads)
+  if (p.grid + 7 > most) return set_error(SI_ERR_UNSUPPORTED, "too many rows for one launch");
+  // (whole rounds of the XCDs: see paged_item_number)
+  const dim3 grid(static_cast<unsigned>(((p.grid < 1 ? 1 : p.grid) + 7) & ~int64_t{7})), block(kPagedThreads);
+  auto launch = [&](auto PAIR) {
+    constexpr bool pair = decltype(PAIR)::value;
+    if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true, pair>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<D, false, pair>), grid, block, 0, st, a);
+  };
+  if constexpr (D >= 512) {
+    if (p.pair) launch(std::true_type{});
+    else launch(std::false_type{});
   } else {
-    if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true, 1, false>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_kernel<D, false, 1, false>), grid, block, 0, st, a);
+    launch(std::false_type{});
   }
   const int rc = check_launch("paged_attn_kernel");
   if (rc || !a.part_o) return rc;
-  const int M = 64 * p.rb;
-  // One thread a place where those fill the GPU, four where they do not (us, one and
-  // four: 64 blocks of up to 5 shares, D = 576, 6.8 and 9.3; 4 blocks of 33 shares 7.2 and 6.7; 32 blocks of up to 64 shares of
-  // 16 rows, D = 128, 8.7 and 7.8).
-  const int64_t places = static_cast<int64_t>(M) * (D / 4);
-  const bool four = p.split_blocks * places < (int64_t{1} << 18);
-  const dim3 cgrid(static_cast<unsigned>((places * (four ? 4 : 1) + kPagedThreads - 1) / kPagedThreads), static_cast<unsigned>(p.split_blocks));
-  if (four) {
-    if (f16) hipLaunchKernelGGL((paged_combine_kernel<true, 4>), cgrid, block, 0, st, a, D, M);
-    else hipLaunchKernelGGL((paged_combine_kernel<false, 4>), cgrid, block, 0, st, a, D, M);
-  } else {
-    if (f16) hipLaunchKernelGGL((paged_combine_kernel<true, 1>), cgrid, block, 0, st, a, D, M);
-    else hipLaunchKernelGGL((paged_combine_kernel<false, 1>), cgrid, block, 0, st, a, D, M);
-  }
+  // One thread a place, or up to four for blocks of many shares where the workgroups that others leave idle are few (us, 2
+  // shares, D = 576: 24 blocks 5.2 with them and 4.3 without, 33 blocks 6.4 and 4.5; but 32 blocks of up to 59 shares, D = 128, 6
+  // and 12).
+  const bool wide = D / 16 * kCombineParts * p.split_blocks < 4096;
+  const dim3 cgrid(static_cast<unsigned>(D / 16 * (wide ? kCombineParts : 1)), static_cast<unsigned>(p.split_blocks));
+  if (f16) hipLaunchKernelGGL(paged_combine_kernel<true>, cgrid, block, 0, st, a, D);
+  else hipLaunchKernelGGL(paged_combine_kernel<false>, cgrid, block, 0, st, a, D);
   return check_launch("paged_combine_kernel");
 }
 
@@ -1305,10 +1317,10 @@ extern "C" int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const 
   PagedSizes p = paged_sizes(N, H, D, R > 0 ? R : 1, a.window, cache_keys(pages, P, page_size),
                              ratio > 0 ? cache_keys(pages2, P2, page_size2) : 0);
   a.want = static_cast<int>(p.want);
-  a.least = kLeastTiles;
   a.behind = p.behind;
+  a.part_cost = static_cast<float>(N * H) / (24.f * kRows * static_cast<float>(p.blocks));
   if (p.bytes > 0 && scratch && scratch_bytes >= p.bytes) {
-    const int64_t M = 64 * p.rb;
+    const int64_t M = kRows;
     a.part_o = static_cast<float*>(scratch);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + p.items * M * D);
     a.rec = reinterpret_cast<int32_t*>(a.part_ml + p.items * M);

@@ -13,6 +13,8 @@
 
 namespace si {
 
+constexpr int64_t kMostBlocks = 0xffffffffLL / 256;  // of 256 threads: a launch has fewer than 2^32
+
 // ---------------------------------------------------------------------------
 // Plan
 //
@@ -245,7 +247,7 @@ static int launch_write(WriteArgs a, int64_t n, int64_t row_bytes, hipStream_t s
   a.vec = static_cast<uint32_t>(row_bytes / static_cast<int64_t>(sizeof(V)));
   a.total = n * a.vec;
   const int64_t blocks = (a.total + 256 * kWriteUnroll - 1) / (256 * kWriteUnroll);
-  if (blocks > 0x7fffffffLL) return set_error(SI_ERR_UNSUPPORTED, "tensor too large");
+  if (blocks > kMostBlocks) return set_error(SI_ERR_UNSUPPORTED, "tensor too large");
   hipLaunchKernelGGL(paged_write_kernel<V>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
   return check_launch("paged_write_kernel");
 }
@@ -509,7 +511,7 @@ static int launch_paged_compress_p(CompressArgs a, hipStream_t st) {
   constexpr int ITEMS = 32 / PARTS;
   const int64_t groups = (a.C / N + 7) / 8;
   const int64_t blocks = (a.E + ITEMS - 1) / ITEMS * groups;
-  if (blocks > 0x7fffffffLL) return set_error(SI_ERR_UNSUPPORTED, "tensor too large");
+  if (blocks > kMostBlocks) return set_error(SI_ERR_UNSUPPORTED, "tensor too large");
   a.groups = static_cast<int>(groups);
   hipLaunchKernelGGL((paged_compress_kernel<DT, N, PARTS>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
   return check_launch("paged_compress_kernel");

@@ -90,7 +90,7 @@ def flash_hca_paged_forward(
     """One serving step of an HCA layer: :func:`flash_hca_forward` for a ragged batch of new tokens over a paged cache.
 
     Writes the new tokens' rows into their pages, pools the compressed entries that they complete and attends to the
-    window and to every legal entry.
+    window and to every legal entry.  Forward only.
 
     Args:
       q: ``[N, n_h, d]`` bf16 or fp16 RoPE-rotated queries of the new tokens.

@@ -14,7 +14,7 @@ prompt, and the earlier ones in a cache:
 A cache is ``[pages, page_size, width]``; a page holds consecutive entries of one request, ``block_table[r, i]`` is the
 page of request r's entries ``i * page_size`` and on (negative where there is none), and ``slot = page * page_size +
 offset`` names a row of the cache.  Lengths, tables and plans are read on the GPU alone, so a step can be captured into a
-graph and replayed with other lengths.  Lengths stay below 2^31.
+graph and replayed with other lengths.  Lengths stay below 2^31.  None of these has a gradient.
 """
 
 from __future__ import annotations
@@ -254,12 +254,13 @@ def paged_attn_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
         row for key and value, shared by the heads; rows 16-byte aligned.
       block_table: ``[R, P]`` int32.  Keys whose page is negative, past the cache or past the table are masked: pages
         that the window has left may be given back.
-      cu_q: ``[R + 1]`` int32 from 0, ascending; seq_lens: ``[R]`` int32; attn_sink: ``[H]`` fp32.
+      cu_q: ``[R + 1]`` int32, ascending (if it descends anywhere, no request has rows); seq_lens: ``[R]`` int32;
+        attn_sink: ``[H]`` fp32.
       softmax_scale: defaults to ``D ** -0.5``.
       window: earlier tokens seen, the token itself included (None: all).
       kv2_cache, block_table2, ratio: the compressed entries, one for ``ratio`` tokens.
     Returns:
-      ``(o [N, H, D] in q's type, lse [N, H] fp32)``.  A row without a key, those behind the last request among them, gets
+      ``(o [N, H, D] in q's type, lse [N, H] fp32)``.  A row without a key, those of no request among them, gets
       ``o = 0`` and ``lse = sink`` (or ``-1e30`` if the sink is ``-inf``).  A value that is not finite reaches the rows that
       see its key and no others.
     """

@@ -544,6 +544,33 @@ def test_attn_no_rows():
     assert not o.any() and torch.equal(lse, s.sink.expand(1, 4))
 
 
+@pytest.mark.parametrize("R", [64, 65, 257, 600])
+def test_attn_many_requests(R):
+    """One long request among short ones, its keys split over workgroups: each way of working out the shares."""
+    s = Step([(5000, 1) if r == R // 2 else (r % 40, r % 2) for r in range(R)], 4, 64, seed=R)
+    s.check(s.run())
+
+
+def test_attn_rows_in_front():
+    """Rows before the first request are rows without a key, as those behind the last."""
+    s = Step([(300, 3), (0, 2)], 4, 64)
+    want = s.run()
+    q = torch.cat([torch.full_like(s.q[:2], math.nan), s.q, torch.full_like(s.q[:1], math.nan)])
+    o, lse = paged_attn_fwd(q, s.kv, s.table, s.cu + 2, s.seq, s.sink)
+    assert torch.equal(o[2:7], want[0]) and torch.equal(lse[2:7], want[1])
+    rest = [0, 1, 7]
+    assert not o[rest].any() and torch.equal(lse[rest], s.sink.expand(3, 4))
+
+
+@pytest.mark.parametrize("R", [3, 70, 300])
+def test_attn_descending_rows(R):
+    """Requests whose rows overlap (cu_q descends) would have more row blocks than the call has room for: none has any."""
+    s = Step([(4000, 1)] * R, 64, 64)
+    s.cu = i32([0, R] * (R // 2 + 1))[:R + 1]
+    o, lse = s.run()
+    assert not o.any() and torch.equal(lse, s.sink.expand(R, 64))
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
