@@ -13,13 +13,11 @@
 //
 // Two ways through the tiles.  With four tiles in LDS (one workgroup a CU at D >= 512, two at 256, three at 128, four
 // below), the softmax of tile t + 1 runs among the MFMAs of tile t's P V, its copies three tiles ahead, one barrier a tile.
-// PAIR: two tiles in LDS, a tile's steps one after the other, two workgroups a CU, whose copies, prologues and ends fall
-// behind each other's MFMAs: taken where there are more row blocks than CUs, at D >= 512 (us, PAIR and not, D = 576: 256 row
-// blocks of 11 tiles 66 and 33, of 254 tiles 330 and 346; 320 of them 44 and 57, 549 and 661; 1,024 84 and 109, 1,171 and
-// 1,411).  At D = 256, 512 row blocks of up to 288 tiles run 314 us without and 338 with three a CU as PAIR allows there.
+// PAIR: two tiles in LDS, a tile's steps one after the other, one workgroup more a CU, whose copies, prologues and ends
+// fall behind each other's MFMAs: for many row blocks, from D = 128 on (pair_from below).
 //
 // Bound, long keys: the LDS, which every K tile leaves four times (each wave's S^T) and once more as V, beside its copy: at
-// D = 576 1,010 TFLOP/s, at 256 892, at 128 694, at 64 562 where a library product reaches 1,279 (below 256 the softmax's
+// D = 576 1,020 TFLOP/s, at 256 920, at 128 724, at 64 573 where a library product reaches 1,279 (below 256 the softmax's
 // vector work weighs more).  Few keys a row: Q in, O out and the prologue.
 //
 // A key that only some of the 64 rows see is masked for the others by a weight of zero; the matrix core would still
@@ -30,6 +28,7 @@
 // Few rows over many keys: each workgroup works out from the requests' lengths how many shares a row block's tiles are
 // cut into (Schedule below) and which share is its own; shares leave fp32 partial outputs that a second kernel joins.
 // Nothing of the lengths is read on the host.
+#include <cstdint>
 #include <string>
 #include <type_traits>
 
@@ -388,7 +387,12 @@ __device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, PagedItem
 }
 
 // Resident workgroups of a CU: LDS sets them, and Q^T and O^T take 216 registers of a wave at D = 576, 96 at D = 256.
-constexpr int per_cu(int D, bool PAIR) { return D >= 512 ? (PAIR ? 2 : 1) : D == 256 ? 2 : D == 128 ? 3 : 4; }
+constexpr int per_cu(int D, bool PAIR) { return (D >= 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4) + (PAIR ? 1 : 0); }
+// Row blocks from which PAIR is taken (us, PAIR and not, rows of 250 to 290 tiles and of 12: D = 576, 256 row blocks 330 and 346,
+// 66 and 33, 320 of them 549 and 661, 44 and 57, 1,024 1,171 and 1,411, 84 and 109; D = 256, 1,024 689 and 650, 46 and 46, 1,536
+// 933 and 982, 58 and 65, 4,096 2,755 and 2,926, 144 and 162; D = 128, 1,536 653 and 644, 41 and 43, 2,048 842 and 877, 50 and
+// 54; D = 64, 4,096 1,150 and 1,113, 63 and 67).
+constexpr int64_t pair_from(int64_t D) { return D >= 512 ? 257 : D == 256 ? 1025 : D == 128 ? 1537 : INT64_MAX; }
 
 constexpr float kNever = -__builtin_inff();
 constexpr int kOdd = 1;    // a masked score that is not finite
@@ -409,7 +413,7 @@ __device__ __forceinline__ bf16x8 finite_or_zero(bf16x8 x) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// PAIR: the steps of a tile one after the other, for two workgroups on a CU.
+// PAIR: the steps of a tile one after the other, for one workgroup more on a CU.
 template <int D, bool F16, bool PAIR>
 __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_kernel(PagedAttnArgs a) {
   using SH = AttnShape<D>;
@@ -916,7 +920,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     for (; t + 1 < tend; ++t) iteration(t, std::true_type{}, std::false_type{});
     iteration(t, std::false_type{}, std::false_type{});
   } else {
-    // PAIR: one tile ahead in LDS, a tile's steps one after the other, two barriers; the other workgroup of the CU fills
+    // PAIR: one tile ahead in LDS, a tile's steps one after the other, two barriers; the other workgroups of the CU fill
     // the gaps.
     skey = tbeg < n1 ? k1lo + tbeg * 32 : (tbeg - n1) * 32;
     uint32_t ok;
@@ -1140,7 +1144,7 @@ static bool served(int64_t D) { return D == 32 || D == 64 || D == 128 || D == 25
 
 // Sizes of a call, from what the host knows.
 struct PagedSizes {
-  bool pair;             // two workgroups on a CU (D >= 512)
+  bool pair;             // the kernel with PAIR
   int64_t blocks;        // row blocks of a workgroup at most
   int64_t want;          // workgroups that run at once
   int64_t grid;          // workgroups
@@ -1156,7 +1160,7 @@ static PagedSizes paged_sizes(int64_t N, int64_t H, int64_t D, int64_t R, int64_
   int64_t g = M;
   while (H % g) g /= 2;
   p.blocks = (N * H + (R < N ? R : N) * (M - g)) / M;
-  p.pair = D >= 512 && p.blocks > 256;
+  p.pair = p.blocks >= pair_from(D);
   const int64_t want = p.want = 256 * per_cu(static_cast<int>(D), p.pair);
   p.grid = 2 * p.blocks <= want ? want : p.blocks + want;
   // tiles of a row block at most
@@ -1192,7 +1196,7 @@ static int launch_paged_attn_d(bool f16, const PagedAttnArgs& a, const PagedSize
     if (f16) hipLaunchKernelGGL((paged_attn_kernel<D, true, pair>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((paged_attn_kernel<D, false, pair>), grid, block, 0, st, a);
   };
-  if constexpr (D >= 512) {
+  if constexpr (pair_from(D) < INT64_MAX) {
     if (p.pair) launch(std::true_type{});
     else launch(std::false_type{});
   } else {

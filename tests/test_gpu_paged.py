@@ -551,6 +551,35 @@ def test_attn_many_requests(R):
     s.check(s.run())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,H,lens", [
+    (576, 64, [(1000, 200), (0, 150), (77, 1)]), (512, 32, [(40, 700)]), (576, 100, [(0, 170), (333, 31)]),
+    (256, 64, [(500, 900), (3, 200)]), (128, 128, [(700, 600), (0, 250)]), (128, 24, [(90, 4400)]),
+])
+@pytest.mark.parametrize("window,ratio", [(None, None), (60, 8)])
+def test_attn_many_rows(D, H, lens, window, ratio, dtype):
+    """More row blocks than run at once; every ninth token is compared."""
+    s = Step(lens, H, D, window=window, ratio=ratio, dtype=dtype, pad=3, spread=3.0)
+    t = torch.arange(s.N)
+    s.check(s.run(), skip=set(t[t % 9 != 4].tolist()))
+
+
+@pytest.mark.parametrize("D,n", [(576, 400), (256, 1200), (128, 1700)])
+def test_attn_many_rows_missing_and_not_finite(D, n):
+    """Pages that are missing and a value that is not finite, where there are more row blocks than run at once."""
+    s = Step([(150, n)], 64, D, page=16)
+    s.table[0, 3:7] = -1
+    s.table[0, 20] = s.kv.shape[0]
+    o, lse = got = s.run()
+    t = torch.arange(n)
+    s.check(got, skip=set(t[t % 9 != 4].tolist()))
+    k = 150 + n // 2
+    s.kv[s.table[0, k // 16].long(), k % 16, 5] = math.inf
+    o2, lse2 = s.run()
+    assert torch.equal(o2[: n // 2], o[: n // 2]) and torch.equal(lse2[: n // 2], lse[: n // 2])
+    assert torch.isnan(o2[n // 2:]).any(-1).all()
+
+
 def test_attn_rows_in_front():
     """Rows before the first request are rows without a key, as those behind the last."""
     s = Step([(300, 3), (0, 2)], 4, 64)
