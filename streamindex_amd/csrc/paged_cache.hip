@@ -260,9 +260,10 @@ static int launch_write(WriteArgs a, int64_t n, int64_t row_bytes, hipStream_t s
 //
 // The workgroup looks up where its tokens' rows are once, into LDS.  Then a thread takes 16 (or 8) bytes of channels and
 // every PARTS-th token, keeps the running maximum, denominator and numerator of each channel in fp32 registers, and the
-// PARTS threads of a channel group join theirs by lane exchanges and one LDS step.  Eight neighbouring threads read 128
-// consecutive bytes of a row.  Bound: the two streams' bytes.  (With the lookups in every thread and a rescale in every join
-// it was bound by its 2,300 instructions a thread: 64K tokens, C = 576, 64 us.)
+// PARTS threads of a channel group join theirs by lane exchanges and, at 32, one LDS step.  Eight neighbouring threads read
+// 128 consecutive bytes of a row.  Bound: the two streams' bytes for 4-byte elements (454 MB in 85 us, 5.3 TB/s); with 2-byte
+// ones as many values come in half the bytes, and the vector work, an exponential and ten instructions a value, weighs as
+// much (149 MB in 39 us, 3.8 TB/s; 227 MB in 51 us, 4.5 TB/s).
 // ---------------------------------------------------------------------------
 struct CompressArgs {
   const char *ca, *za, *cb, *zb;        // streams, [pages, ps, C]
@@ -321,7 +322,7 @@ __device__ __forceinline__ float lane_away(float x) {
 
 template <int DT, int N, int PARTS>
 __global__ __launch_bounds__(256, 4) void paged_compress_kernel(CompressArgs a) {
-  static_assert(PARTS == 4 || PARTS == 32, "lanes 8 and 16 apart, or all of a workgroup");
+  static_assert(PARTS == 1 || PARTS == 4 || PARTS == 8 || PARTS == 32, "8 lanes, half a wave, a wave or a workgroup to an entry");
   constexpr int U = 4;                       // tokens of a thread in flight
   constexpr int SIZE = DT == 0 ? 4 : 2;
   constexpr int ITEMS = 32 / PARTS;          // entries of a workgroup
@@ -436,26 +437,26 @@ __global__ __launch_bounds__(256, 4) void paged_compress_kernel(CompressArgs a) 
     }
   }
   // Join the parts: lanes 8, 16, 32 apart, the maxima first, so that a thread rescales its sums once; then the waves of an
-  // entry.  (With a rescale in every step, 96 of a thread's 128 exponentials were the joins': 64K tokens 64 us.)
+  // entry.  (With a rescale in every step, 96 of a thread's 128 exponentials were the joins', with 32 parts.)
   float top[N];
+  if constexpr (PARTS > 1) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    top[i] = __builtin_fmaxf(mx[i], lane_away<8>(mx[i]));
-    top[i] = __builtin_fmaxf(top[i], lane_away<16>(top[i]));
-    if constexpr (PARTS >= 8) top[i] = __builtin_fmaxf(top[i], lane_away<32>(top[i]));
-    const float w = top[i] == -__builtin_inff() ? 0.f : __expf(mx[i] - top[i]);
-    den[i] *= w;
-    num[i] *= w;
-    den[i] += lane_away<8>(den[i]);
-    num[i] += lane_away<8>(num[i]);
-    den[i] += lane_away<16>(den[i]);
-    num[i] += lane_away<16>(num[i]);
-    if constexpr (PARTS >= 8) {
-      den[i] += lane_away<32>(den[i]);
-      num[i] += lane_away<32>(num[i]);
+    for (int i = 0; i < N; ++i) {
+      top[i] = __builtin_fmaxf(mx[i], lane_away<8>(mx[i]));
+      top[i] = __builtin_fmaxf(top[i], lane_away<16>(top[i]));
+      if constexpr (PARTS >= 8) top[i] = __builtin_fmaxf(top[i], lane_away<32>(top[i]));
+      const float w = top[i] == -__builtin_inff() ? 0.f : __expf(mx[i] - top[i]);
+      den[i] *= w;
+      num[i] *= w;
+      den[i] += lane_away<8>(den[i]);
+      num[i] += lane_away<8>(num[i]);
+      den[i] += lane_away<16>(den[i]);
+      num[i] += lane_away<16>(num[i]);
+      if constexpr (PARTS >= 8) {
+        den[i] += lane_away<32>(den[i]);
+        num[i] += lane_away<32>(num[i]);
+      }
     }
-  }
-  {
     float seen = any ? 1.f : 0.f;
     seen += lane_away<8>(seen);
     seen += lane_away<16>(seen);
@@ -518,7 +519,14 @@ static int launch_paged_compress_p(CompressArgs a, hipStream_t st) {
 }
 template <int DT, int N>
 static int launch_paged_compress_n(const CompressArgs& a, hipStream_t st) {
-  return (a.overlap ? 2 : 1) * a.m >= 64 ? launch_paged_compress_p<DT, N, 32>(a, st) : launch_paged_compress_p<DT, N, 4>(a, st);
+  // Parts of an entry, that is threads of a channel: the fewer, the less is spent on joining them; the more, the more loads of
+  // few entries are in flight (us, C = 576, bf16: 8 tokens, 7,000 entries, 1 and 4 parts 30 and 47; 16, 6,000, 50 and 59; 32,
+  // 1,000 entries, fp32, C = 500, 35 and 31; 128, 512 entries, 8 and 32 parts 39 and 48; 256 of which
+  // two are there, as a decode step of 256 requests has them, 11 and 7).
+  const int64_t tokens = (a.overlap ? 2 : 1) * a.m;
+  if (tokens <= 16) return launch_paged_compress_p<DT, N, 1>(a, st);
+  if (tokens < 64) return launch_paged_compress_p<DT, N, 4>(a, st);
+  return a.E * ((a.C / N + 7) / 8) >= 4096 ? launch_paged_compress_p<DT, N, 8>(a, st) : launch_paged_compress_p<DT, N, 32>(a, st);
 }
 template <int DT>
 static int launch_paged_compress(const CompressArgs& a, hipStream_t st) {

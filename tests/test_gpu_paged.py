@@ -201,6 +201,10 @@ COMPRESS = [
     (33, 5, False, 4, [(0, 6), (9, 10)], 1),
     (8, 1, True, 3, [(0, 5), (1, 2)], 4),
     (128, 200, True, 64, [(0, 1), (1, 3)], 64),
+    (576, 128, False, 64, [(0, 300), (5, 160), (3, 3)], 64),
+    (500, 50, True, 16, [(0, 90), (1, 61)], 7),
+    (100, 20, True, 32, [(0, 7), (4, 9)], 5),
+    (72, 33, False, 10, [(0, 400)], 64),
 ]
 
 
