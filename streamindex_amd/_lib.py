@@ -130,14 +130,17 @@ def load() -> ctypes.CDLL:
 _STRIDES = {}  # strides -> the array the library reads (it never writes one)
 
 
-def strides(t: torch.Tensor):
-    s = t.stride()
+def stride_array(s):
     arr = _STRIDES.get(s)
     if arr is None:
         if len(_STRIDES) >= 4096:
             _STRIDES.clear()
         arr = _STRIDES[s] = (ctypes.c_int64 * len(s))(*s)
     return arr
+
+
+def strides(t: torch.Tensor):
+    return stride_array(t.stride())
 
 
 def int64s(*vals):
@@ -170,11 +173,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 _HERE = contextlib.nullcontext()
+# (without the Python around it: 0.3 us a call less; a GPU tensor is at hand, so the runtime is up)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device(device: torch.device):
     """``torch.cuda.device(device)``, free where it already is the current one."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _current_device() else torch.cuda.device(device)
 
 
 def scratch(nbytes: int, device: torch.device):

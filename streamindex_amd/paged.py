@@ -42,14 +42,6 @@ class PagedPlan(NamedTuple):
     free_next: torch.Tensor  # [1] int32: position in the free list after this step
 
 
-def _check_devices(dev: torch.device, **tensors) -> None:
-    """Every tensor on ``dev``, a GPU; its names are looked at only where one is not."""
-    at = dev.index
-    for t in tensors.values():
-        if t is not None and t.get_device() != at:
-            _check_device(dev, **tensors)
-
-
 def _int32(t: torch.Tensor, name: str, n: int) -> torch.Tensor:
     assert t.dim() == 1 and t.shape[0] == n, f"{name} must be [{n}], got {list(t.shape)}"
     if t.dtype is not torch.int32:
@@ -119,7 +111,10 @@ def paged_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     """
     assert ctx_lens.is_cuda
     dev = ctx_lens.device
-    _check_devices(dev, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_start=free_start)
+    at = dev.index
+    if not (new_lens.get_device() == block_table.get_device() == free_pages.get_device() == at
+            and (free_start is None or free_start.get_device() == at)):
+        _check_device(dev, new_lens=new_lens, block_table=block_table, free_pages=free_pages, free_start=free_start)
     assert ctx_lens.dim() == 1 and free_pages.dim() == 1
     R, F = ctx_lens.shape[0], free_pages.shape[0]
     ctx, new = _int32(ctx_lens, "ctx_lens", R), _int32(new_lens, "new_lens", R)
@@ -151,7 +146,8 @@ def paged_write(rows: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) ->
     """
     assert rows.is_cuda
     dev = rows.device
-    _check_devices(dev, cache=cache, slots=slots)
+    if not cache.get_device() == slots.get_device() == dev.index:
+        _check_device(dev, cache=cache, slots=slots)
     st = _cache_strides(cache, "cache")
     pages, ps, width = cache.shape
     assert rows.dim() == 2 and rows.shape[1] == width, "rows must be [N, width of the cache]"
@@ -194,13 +190,17 @@ def paged_compress(c_a: torch.Tensor, z_a: torch.Tensor, b_a: torch.Tensor, bloc
     """
     assert c_a.is_cuda
     dev = c_a.device
-    _check_devices(dev, z_a=z_a, b_a=b_a, block_table=block_table, request=request, positions=positions, cache=cache,
-                   slots=slots, c_b=c_b, z_b=z_b, b_b=b_b)
+    if not (z_a.get_device() == b_a.get_device() == block_table.get_device() == request.get_device()
+            == positions.get_device() == cache.get_device() == slots.get_device() == dev.index):
+        _check_device(dev, z_a=z_a, b_a=b_a, block_table=block_table, request=request, positions=positions, cache=cache,
+                      slots=slots)
     dtype = c_a.dtype
     dt = _dtype_code(c_a)
     overlap = c_b is not None
     if overlap != (z_b is not None) or overlap != (b_b is not None):
         raise ValueError("overlapping entries need c_b, z_b and b_b")
+    if overlap:
+        _check_device(dev, c_b=c_b, z_b=z_b, b_b=b_b)
     st = [_cache_strides(c_a, "c_a")]
     pages, ps, C = c_a.shape
     for n, t in (("z_a", z_a), ("c_b", c_b), ("z_b", z_b)):
@@ -225,7 +225,7 @@ def paged_compress(c_a: torch.Tensor, z_a: torch.Tensor, b_a: torch.Tensor, bloc
     ba = b_a if b_a.dtype is torch.float32 else b_a.float()
     ba = ba if ba.is_contiguous() else ba.contiguous()
     bb = b_b.float().contiguous() if overlap else None
-    st = [_lib.int64s(*s) for s in st]
+    st = [_lib.stride_array(s) for s in st]
     L = _lib.load()
     with _lib.on_device(dev):
         rc = L.si_paged_compress(
@@ -266,8 +266,9 @@ def paged_attn_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     """
     assert q.is_cuda
     dev = q.device
-    _check_devices(dev, kv_cache=kv_cache, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, attn_sink=attn_sink,
-                   kv2_cache=kv2_cache, block_table2=block_table2)
+    if not (kv_cache.get_device() == block_table.get_device() == cu_q.get_device() == seq_lens.get_device()
+            == attn_sink.get_device() == dev.index):
+        _check_device(dev, kv_cache=kv_cache, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, attn_sink=attn_sink)
     assert q.dim() == 3, "q must be [N, H, D]"
     N, H, D = q.shape
     dtype = q.dtype
@@ -280,6 +281,8 @@ def paged_attn_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     two = kv2_cache is not None
     if two != (block_table2 is not None) or two != (ratio is not None):
         raise ValueError("a second cache needs kv2_cache, block_table2 and ratio")
+    if two and not kv2_cache.get_device() == block_table2.get_device() == dev.index:
+        _check_device(dev, kv2_cache=kv2_cache, block_table2=block_table2)
     if two and ratio < 1:
         raise ValueError(f"ratio must be positive, got {ratio}")
     R = block_table.shape[0]
@@ -291,7 +294,7 @@ def paged_attn_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
         if s[2] != 1 or (s[0] | s[1]) % 8 or p % 16:
             raise ValueError(f"{name}_cache needs a contiguous last dimension and rows that start at multiples of 16 bytes")
         pages, ps, _ = cache.shape
-        return (p, _lib.int64s(*s), pages, ps, table.data_ptr(), _table_stride(table, f"{name}'s block table", R),
+        return (p, _lib.stride_array(s), pages, ps, table.data_ptr(), _table_stride(table, f"{name}'s block table", R),
                 table.shape[1])
 
     c1 = cache_args(kv_cache, block_table, "kv")
