@@ -103,7 +103,7 @@ __device__ __forceinline__ T pick(bool second, T x, T y) {
 // With more row blocks than `want`, c = 2 U / want cuts only requests far longer than the average, which would otherwise
 // end last on their own.
 // Every workgroup does these sums itself, with lane-shift scans in 32 bits, and where there are at most 64 requests every
-// wave, without a barrier (721 one-chunk row blocks: 576 us with the barriers, 555 without).  An ascending cu_q makes the
+// wave, without a barrier (7,149 row blocks: 576 us with the barriers, 555 without).  An ascending cu_q makes the
 // requests' rows disjoint, on which every bound here and the sizes of the partial outputs rest; with one that descends
 // somewhere no request has rows.
 // ---------------------------------------------------------------------------
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // flight before their use), a tile ahead of the copies; `within` is what the key's place in its page adds.  What
   // a tile asks of its cache is held in scalars that every path sets: as vector registers, which a value that only some
   // paths set becomes, they were spilled and read back between a tile's steps, with a wait for its copies each time
-  // (7,249 row blocks of up to 21 tiles, D = 576: 540 us, 476 without).
+  // (7,149 row blocks of up to 17 tiles, D = 576: 540 us, 476 without).
   CacheView view1, view2;
   CacheBase base1, base2;
   view_cache(a.c1, req, view1, base1);
