@@ -165,7 +165,8 @@ constexpr uint32_t kWhole = 0x7fffffffu;  // no row block is cut
 
 // Number of this workgroup's item among `total`; `total` and on where it has none.  Consecutive workgroups go to the eight
 // XCDs in turn: each XCD takes runs of up to 32 items, one to a CU, whose keys its L2 then holds once, and all of them the
-// same number, however many of the launched workgroups the lengths leave without an item.
+// same number, however many of the launched workgroups the lengths leave without an item.  (512 row blocks of 288 tiles, D =
+// 256: runs of 32 319 us, of 64 332, of 16 321.)
 __device__ __forceinline__ int paged_item_number(int total) {
   const int xcd = blockIdx.x & 7, k = blockIdx.x >> 3;
   const int whole = total >> 8;  // rounds of 8 x 32

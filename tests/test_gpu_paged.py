@@ -604,6 +604,49 @@ def test_attn_descending_rows(R):
     assert not o.any() and torch.equal(lse, s.sink.expand(R, 64))
 
 
+def test_attn_shared_pages():
+    """Requests that share their pages, by equal table rows and by one row expanded; lengths as int64 and strided."""
+    s = Step([(70, 2), (70, 2), (70, 2)], 8, 128, window=50, ratio=4)
+    s.table[1:] = s.table[0]
+    s.table2[1:] = s.table2[0]
+    s.q[2:] = s.q[:2].repeat(2, 1, 1)
+    o, lse = s.run()
+    assert torch.equal(o[:2], o[2:4]) and torch.equal(o[:2], o[4:]) and torch.equal(lse[:2], lse[4:])
+    s.check((o, lse))
+    s.table, s.table2 = s.table[:1].expand(3, -1), s.table2[:1].expand(3, -1)
+    s.cu, s.seq = s.cu.long(), torch.stack([s.seq.long(), s.seq.long() * 0], 1)[:, 0]
+    o2, lse2 = s.run()
+    assert torch.equal(o2, o) and torch.equal(lse2, lse)
+
+
+def test_write_views():
+    """Rows expanded, every other slot of a list, a cache that is a slice of wider rows."""
+    g = torch.Generator().manual_seed(8)
+    wide = torch.zeros(5, 8, 96, dtype=torch.bfloat16, device=DEV)
+    row = torch.randn(1, 32, generator=g).to(torch.bfloat16).to(DEV)
+    slots = torch.randperm(40, generator=g).to(DEV)
+    paged_write(row.expand(20, 32), wide[..., 32:64], slots[::2])
+    want = torch.zeros(40, 96, dtype=torch.bfloat16, device=DEV)
+    want[slots[::2], 32:64] = row
+    assert torch.equal(wide.view(40, 96), want)
+
+
+def test_compress_twice_the_same_and_shared():
+    """An entry given twice, to two slots, and requests that share their pages: the same bits each."""
+    g = torch.Generator().manual_seed(9)
+    C, m, page = 64, 8, 16
+    x = torch.randn(4, page, 2 * C, generator=g).to(torch.bfloat16).to(DEV)
+    bias = torch.randn(m, C, generator=g).to(DEV)
+    table = i32([[2, 0, 3]]).expand(3, -1)
+    cache = torch.zeros(2, 8, C, dtype=torch.bfloat16, device=DEV)
+    paged_compress(x[..., :C], x[..., C:], bias, table, torch.tensor([0, 1, 2, 0], device=DEV), i32([4, 4, 4, 4]), cache,
+                   torch.tensor([1, 9, 4, 14], device=DEV))
+    out = cache.view(16, C)
+    assert out[1].any() and all(torch.equal(out[1], out[i]) for i in (9, 4, 14))
+    rest = [i for i in range(16) if i not in (1, 4, 9, 14)]
+    assert not out[rest].any()
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
