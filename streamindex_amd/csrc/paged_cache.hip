@@ -424,14 +424,16 @@ __global__ __launch_bounds__(256, 4) void paged_compress_kernel(CompressArgs a) 
           z[u] = zp[u].at(i) + bp[u].at(i);
           m = __builtin_fmaxf(m, z[u]);
         }
-        const float ref = m == -__builtin_inff() ? 0.f : m * kLog2e;
-        const float s = __builtin_amdgcn_exp2f(__builtin_fmaf(mx[i], kLog2e, -ref));
+        // (the difference comes first: m kLog2e overflows for a gate masked with the type's lowest value, and its rounding would
+        // differ from part to part)
+        const float ref = m == -__builtin_inff() ? 0.f : m;
+        const float s = __builtin_amdgcn_exp2f((mx[i] - ref) * kLog2e);
         den[i] *= s;
         num[i] *= s;
         mx[i] = m;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(z[u], kLog2e, -ref));
+          const float w = __builtin_amdgcn_exp2f((z[u] - ref) * kLog2e);
           den[i] += w;
           num[i] = __builtin_fmaf(w, vp[u].at(i), num[i]);
         }

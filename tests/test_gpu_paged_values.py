@@ -1,0 +1,98 @@
+"""GPU parity of the paged serving operators at values far from the usual ones, against 64-bit floats.
+
+Tolerances (u = eps / 2 of the type):
+* a compressed entry: u |ref| + 2^-18 sum w |v| / sum w.  The gates are chosen so that gate + bias is exact in fp32; their
+  differences from the maximum are then exact or off by 2^-24 of themselves, and a weight e^-d by d e^-d 2^-24 < 2^-25 and an
+  exponential's 2^-22.  The rest is fp32 sums, at most 2^5 additions along a path, twice.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from streamindex_amd import paged_compress
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+# ---------------------------------------------------------------------------
+# compress
+# ---------------------------------------------------------------------------
+def gate_masks(E, n):
+    """Tokens ``[E, n]`` to mask: some of an entry's first, all, all but one, every other one, every fourth kept."""
+    j, e = torch.arange(n), torch.arange(E)[:, None] % 7
+    kinds = [j < n // 2, j < 4, j >= 0, j < n - 1, j % 2 == 0, j % 4 != 3, j >= 1]
+    return torch.stack([torch.where(e[:, 0] == i, 1, 0)[:, None] * k[None] for i, k in enumerate(kinds)]).sum(0).bool()
+
+
+def check_gates(dtype, C, m, overlap, E, make):
+    """``make(z [E, tokens, C]) -> z``: the gates of each entry's tokens, the block before first, before the bias."""
+    g = torch.Generator().manual_seed(m + E)
+    page, epage, k = 16, 8, 2 if overlap else 1
+    S = E * m
+    pages = -(-S // page)
+    x = torch.zeros(pages * page, 2 * k * C, dtype=dtype)
+    bias = [(torch.randn(m, C, generator=g) * 64).round() / 64 for _ in range(k)]
+    for s in range(k):  # content and gate of stream a, then of b
+        x[:S, 2 * s * C:(2 * s + 1) * C] = torch.randn(S, C, generator=g).to(dtype)
+        z = make((torch.randn(E, m, C, generator=g) * 64).round() / 64)
+        x[:S, (2 * s + 1) * C:(2 * s + 2) * C] = z.reshape(S, C).to(dtype)
+    perm = torch.randperm(pages, generator=g)
+    store = torch.empty(pages, page, 2 * k * C, dtype=dtype)
+    store[perm] = x.view(pages, page, -1)
+    store, x, bias = store.to(DEV), x.to(DEV), [b.to(DEV) for b in bias]
+    cache = torch.zeros(-(-E // epage), epage, C, dtype=dtype, device=DEV)
+    ent = torch.arange(E, device=DEV)
+    more = {"c_b": store[..., 2 * C:3 * C], "z_b": store[..., 3 * C:], "b_b": bias[1]} if overlap else {}
+    paged_compress(store[..., :C], store[..., C:2 * C], bias[0], perm.to(torch.int32).to(DEV).view(1, -1),
+                   torch.zeros(E, dtype=torch.int32, device=DEV), ent.to(torch.int32), cache, ent, **more)
+    v, z = x[:S, :C].view(E, m, C).double(), x[:S, C:2 * C].view(E, m, C).double() + bias[0].double()
+    if overlap:
+        vb, zb = x[:S, 2 * C:3 * C].view(E, m, C).double(), x[:S, 3 * C:].view(E, m, C).double() + bias[1].double()
+        v = torch.cat([torch.cat([vb[:1] * 0, vb[:-1]]), v], 1)
+        z = torch.cat([torch.cat([torch.full_like(zb[:1], -math.inf), zb[:-1]]), z], 1)
+    w = torch.softmax(z, 1)
+    want, mag = (w * v).sum(1), (w * v.abs()).sum(1)
+    err = (cache.view(-1, C)[:E].double() - want).abs()
+    tol = half_step(dtype) * want.abs() + 2.0**-18 * mag + torch.finfo(dtype).smallest_normal
+    ok = (err <= tol) | (want.isnan() & err.isnan())  # (every gate -inf: NaN, as a softmax's)
+    assert ok.all(), (int((~ok).sum()), float((err - tol).nan_to_num(nan=math.inf).max()))
+    return want
+
+
+# few tokens an entry; some; many of few entries; many of many entries
+GATES = [(72, 8, False, 40), (33, 4, True, 50), (100, 50, False, 20), (64, 16, True, 30), (576, 128, False, 30), (128, 200, True, 9),
+         (576, 64, False, 600), (500, 100, False, 700)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("C,m,overlap,E", GATES)
+@pytest.mark.parametrize("value", ["lowest", "lowest and -inf"])
+def test_compress_masked_gates(dtype, C, m, overlap, E, value):
+    """Gates masked with the type's lowest value weigh nothing beside others, and all the same where an entry has no others."""
+    masked = gate_masks(E, m)[..., None].expand(E, m, C)
+
+    def make(z):
+        z = torch.where(masked, torch.finfo(dtype).min, z)
+        if value != "lowest":
+            z[:, ::3] = -math.inf
+        return z
+
+    want = check_gates(dtype, C, m, overlap, E, make)
+    assert not want.isnan().any() or value != "lowest"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("C,m,overlap,E", GATES)
+@pytest.mark.parametrize("offset", [32, -1000, 10000])
+def test_compress_gates_far_from_zero(dtype, C, m, overlap, E, offset):
+    """A common offset changes nothing but what the type can hold of the gates."""
+    check_gates(dtype, C, m, overlap, E, lambda z: z + offset)
