@@ -498,7 +498,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   view_cache(a.c2, req, view2, base2);
   CacheView view;            // of the next tile to fetch page numbers for
   CacheBase from, from_next; // of the tile to copy, and of the one after it
-  int fkey = 0, fend = 0, ftile = tbeg;
+  uint32_t fkey = 0, fend = 0;  // (unsigned: a tile past the last key of 2^31 - 1 begins behind 31 bits)
+  int ftile = tbeg;
   auto enter = [&](int t) __attribute__((always_inline)) {  // moves the view to tile t
     const bool second = t >= n1;
     view = CacheView{pick(second, view1.table, view2.table), pick(second, view1.ps, view2.ps),
@@ -506,8 +507,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
                      pick(second, view1.shift, view2.shift), pick(second, view1.one, view2.one)};
     from_next = CacheBase{pick(second, base1.base, base2.base), pick(second, base1.pstride, base2.pstride),
                           pick(second, base1.pages, base2.pages)};
-    fkey = second ? (t - n1) * 32 : k1lo + t * 32;
-    fend = second ? k2hi : k1hi;
+    fkey = second ? static_cast<uint32_t>(t - n1) * 32u : static_cast<uint32_t>(k1lo) + static_cast<uint32_t>(t) * 32u;
+    fend = static_cast<uint32_t>(second ? k2hi : k1hi);
     scalar_tie(view.table);
     scalar_tie(view.ps);
     scalar_tie(view.rstride);
@@ -522,7 +523,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   };
   auto fetch_pages = [&]() __attribute__((always_inline)) {
     if (__builtin_expect(ftile == n1, 0) && ntiles > n1) enter(n1);
-    const uint32_t key = static_cast<uint32_t>(min(fkey + (lane_now() & 31), fend - 1));
+    const uint32_t key = min(fkey + static_cast<uint32_t>(lane_now() & 31), fend - 1);
     const uint32_t col = view.page_of(key);
     __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(view.table + col),
                                      (lds_void_t*)&page_lds[wave][ftile % PAGES][0], 4, 0, 0);
@@ -709,7 +710,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
         }
       flags = __builtin_amdgcn_ballot_w64(odd) ? kOdd : 0;
     }
-    skey += 32;
+    skey = static_cast<int>(static_cast<uint32_t>(skey) + 32u);  // (may leave 31 bits behind the last tile)
     const f32x4 y0 = st[0], y1 = st[1];
     float lmax = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(y0[0], y0[1]), __builtin_fmaxf(y0[2], y0[3])),
                                  __builtin_fmaxf(__builtin_fmaxf(y1[0], y1[1]), __builtin_fmaxf(y1[2], y1[3])));

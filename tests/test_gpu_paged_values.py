@@ -15,6 +15,8 @@ import torch
 
 from streamindex_amd import paged_compress
 
+from tests.test_gpu_paged import Step
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
@@ -96,3 +98,17 @@ def test_compress_masked_gates(dtype, C, m, overlap, E, value):
 def test_compress_gates_far_from_zero(dtype, C, m, overlap, E, offset):
     """A common offset changes nothing but what the type can hold of the gates."""
     check_gates(dtype, C, m, overlap, E, lambda z: z + offset)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("D,H,lens,window", [
+    (32, 16, [(2**31 - 4, 3), (2**31 - 40, 1), (2**31 - 2**18 - 2, 5)], 100), (32, 1, [(2**31 - 2, 1), (2**31 - 33, 1)], 1),
+    (64, 64, [(2**31 - 130, 129)], 2000), (128, 64, [(2**31 - 1601, 1600)], 60),
+])
+def test_attn_positions_near_the_largest(D, H, lens, window):
+    """Positions up to 2^31 - 2 under a block table that names 2^31 keys: the tile past the last key is not looked up."""
+    s = Step(lens, H, D, window=window, page=2**18)
+    t = torch.arange(s.N)
+    s.check(s.run(), skip=set(t[(t % 97 != 5) & (s.N > 200)].tolist()))
