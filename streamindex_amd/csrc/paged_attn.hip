@@ -23,7 +23,8 @@
 // A key that only some of the 64 rows see is masked for the others by a weight of zero; the matrix core would still
 // turn 0 x inf into NaN.  Keys and values being the same rows, such a value makes the key's raw score non-finite as
 // well, so on a masked non-finite score the tile's values that are not finite are zeroed in LDS before P V; a row that
-// does see such a key gets a weight of NaN there, and with it its output.
+// does see such a key gets a weight of NaN there, and with it its output.  A score of -inf from finite values, a key of the
+// type's lowest ones say, is a weight of zero.
 //
 // Few rows over many keys: each workgroup works out from the requests' lengths how many shares a row block's tiles are
 // cut into (Schedule below) and which share is its own; shares leave fp32 partial outputs that a second kernel joins.
@@ -685,6 +686,13 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   constexpr float kLazy = F16 ? 8.0f : 64.0f;  // 2^8 keeps P in fp16's range, 2^64 in bf16's
   float m_ref = kNever, l_run = 0.f;  // reference maximum (log2 domain) and this lane's share of the denominator
   int skey = 0;  // first key of the next tile to mask
+  // This lane's row sees key kk of the tile that begins at key `first` where kk + lo, unsigned, is below cnt.
+  auto seen_keys = [&](bool second, int first, int& lo, int& cnt) __attribute__((always_inline)) {
+    const int end = second ? ent_end(rpos) : max(min(rpos + 1, cap1), 0);
+    const int begin = second ? 0 : max(max(rpos + 1, 0) - window, 0);
+    lo = first - begin;
+    cnt = max(end - begin, 0);
+  };
   auto softmax_begin = [&](int t, uint32_t okmask, f32x4 (&st)[2], float& ref, int pbuf) __attribute__((always_inline)) {
     mfma_result_fence(st[0], st[1]);
     if (t == n1) skey = 0;
@@ -695,9 +703,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     if (!full) {
       bool odd = false;
       const int g4 = 4 * (lane_now() >> 4);
-      const int end = second ? ent_end(rpos) : max(min(rpos + 1, cap1), 0);
-      const int begin = second ? 0 : max(max(rpos + 1, 0) - window, 0);
-      const int lo = skey - begin, cnt = max(end - begin, 0);
+      int lo, cnt;
+      seen_keys(second, skey, lo, cnt);
 #pragma unroll
       for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
@@ -706,7 +713,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
           const bool ok = static_cast<uint32_t>(kk + lo) < static_cast<uint32_t>(cnt) && ((okmask >> kk) & 1);
           const bool fin = __builtin_fabsf(st[mb][r]) < __builtin_inff();
           odd = odd || (!ok && !fin);
-          st[mb][r] = ok ? (fin ? st[mb][r] : __builtin_nanf("")) : kNever;
+          st[mb][r] = ok ? st[mb][r] : kNever;
         }
       flags = __builtin_amdgcn_ballot_w64(odd) ? kOdd : 0;
     }
@@ -791,9 +798,34 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
       between(JC);
     });
   };
-  // Values of a tile that are not finite become zero, in its LDS (every wave has done with its scores).
-  auto clean_tile = [&](int slot) __attribute__((always_inline)) {
+  // A masked key of the tile has a score that is not finite.  Values that are not finite become zero, in the tile's LDS (every
+  // wave has done with its scores), and a row that sees such a key gets a weight of NaN for it (it may be 0 so far, from a
+  // score of -inf).  A key of finite values whose score has left fp32's range keeps its weight: 0, or NaN.
+  auto clean_tile = [&](int t, uint32_t okmask, int slot, int pbuf) __attribute__((always_inline)) {
     const uint32_t tile = lds_addr(ring(slot));
+    const int ln = lane_now(), g4 = 4 * (ln >> 4);
+    uint32_t bad = 0;
+    for (int c = ln >> 5; c < SH::CPR; c += 2) {  // lanes l and l + 32 look through key l
+      bf16x8 x;
+      asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(x) : "v"(tile + (ln & 31) * ROW + c * 16));
+      const u32x4 d = __builtin_bit_cast(u32x4, x) ^ __builtin_bit_cast(u32x4, finite_or_zero<F16>(x));
+      bad |= (d[0] | d[1]) | (d[2] | d[3]);
+    }
+    const uint64_t both = __builtin_amdgcn_ballot_w64(bad != 0);
+    const uint32_t keys = (static_cast<uint32_t>(both) | static_cast<uint32_t>(both >> 32)) & okmask;
+    const bool second = t >= n1;
+    int lo, cnt;
+    seen_keys(second, second ? (t - n1) * 32 : k1lo + t * 32, lo, cnt);
+    const uint32_t pat = lds_addr(&p_lds[pbuf][(wave * 64 + ln) * 16]);
+    u32x4 w;
+    asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(w) : "v"(pat));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {  // (a weight of 0x7fff is NaN in both types)
+      const int kk = 16 * (i >> 2) + g4 + (i & 3);
+      if (((keys >> kk) & 1) && static_cast<uint32_t>(kk + lo) < static_cast<uint32_t>(cnt)) w[i >> 1] |= i & 1 ? 0x7fff0000u : 0x7fffu;
+    }
+    asm volatile("ds_write_b128 %0, %1" ::"v"(pat), "v"(w) : "memory");
+    attn_tile_barrier();  // every wave has looked through the tile
     for (int e = threadIdx.x; e < SH::CH; e += kPagedThreads) {
       bf16x8 x;
       asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(x) : "v"(tile + e * 16));
@@ -803,8 +835,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   };
 
   // What the waves' flags of a tile ask for before its P V.
-  auto settle = [&](int flags, int pbuf, int slot) __attribute__((always_inline)) {
-    if (flags >= kMoved) {
+  auto settle = [&](int flags, int t, uint32_t okmask, int pbuf, int slot) __attribute__((always_inline)) {
+    if (flags & kMoved) {
       // a wave's alpha is of this tile where the wave says so
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -820,7 +852,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
       }
     }
     if (flags & kOdd) {
-      clean_tile(slot);
+      clean_tile(t, okmask, slot, pbuf);
       attn_tile_barrier();
     }
   };
@@ -898,7 +930,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
         start();
       }
       if constexpr (ahead) from = from_next;
-      if (__builtin_expect(flags != 0, 0)) settle(flags, t & 1, slot);
+      if (__builtin_expect(flags != 0, 0)) settle(flags, t, okq[0], t & 1, slot);
       constexpr int SPAN = MBW > 2 ? MBW - 2 : 1, EPB = (8 + SPAN - 1) / SPAN;  // weights beside one of SPAN output blocks
       pv(slot, t & 1, [&](auto JC) {
         constexpr int j = decltype(JC)::value;
@@ -969,7 +1001,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
       asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(fl)
                    : "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[0][0]))));
       const int flags = __builtin_amdgcn_readfirstlane(static_cast<int>(fl[0] | fl[1] | fl[2] | fl[3]));
-      if (__builtin_expect(flags != 0, 0)) settle(flags, 0, slot);
+      if (__builtin_expect(flags != 0, 0)) settle(flags, t, ok, 0, slot);
       pv(slot, 0, [](auto) {});
       ok = ok_next;
     }

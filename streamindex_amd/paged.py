@@ -262,7 +262,7 @@ def paged_attn_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     Returns:
       ``(o [N, H, D] in q's type, lse [N, H] fp32)``.  A row without a key, those of no request among them, gets
       ``o = 0`` and ``lse = sink`` (or ``-1e30`` if the sink is ``-inf``).  A value that is not finite reaches the rows that
-      see its key and no others.
+      see its key and no others.  Scores are fp32: one below its range weighs nothing, one above it makes its row NaN.
     """
     assert q.is_cuda
     dev = q.device

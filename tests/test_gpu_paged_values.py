@@ -112,3 +112,71 @@ def test_attn_positions_near_the_largest(D, H, lens, window):
     s = Step(lens, H, D, window=window, page=2**18)
     t = torch.arange(s.N)
     s.check(s.run(), skip=set(t[(t % 97 != 5) & (s.N > 200)].tolist()))
+
+
+class Lowest(Step):
+    """Keys of the type's lowest value, at the positions ``at`` of each request and the entries ``at2``, and queries whose fp32
+    scores with them are -inf: they weigh nothing."""
+
+    def __init__(self, *args, at=(), at2=(), **kw):
+        super().__init__(*args, **kw)
+        self.q.abs_()
+        lowest = torch.finfo(self.dtype).min
+        for r, (c, n) in enumerate(self.lens):
+            self.lower(self.kv, self.table[r], at, c + n, lowest)
+            if self.ratio:
+                self.lower(self.kv2, self.table2[r], at2, (c + n) // self.ratio, lowest)
+
+    @staticmethod
+    def lower(cache, pages, at, end, lowest):
+        for p in {p % end for p in at} if end else ():
+            page = int(pages[p // cache.shape[1]])
+            if page >= 0:
+                cache[page, p % cache.shape[1]] = lowest
+
+    def keys(self, r, p):
+        k = super().keys(r, p)
+        return k[~(k == torch.finfo(self.dtype).min).all(1)]
+
+
+# positions: whole tiles, the tile that the chunk's rows see in part, the window's edge (counted from the end)
+@pytest.mark.parametrize("D,H,lens,kw", [
+    (64, 16, [(40, 9), (3, 1), (70, 2)], {}), (576, 64, [(40, 9), (100, 3)], {"window": 20, "ratio": 4, "page2": 8}),
+    (128, 24, [(9000, 2), (300, 1)], {}), (32, 1, [(200, 70)], {"window": 33}), (256, 64, [(90, 5)], {"ratio": 2}),
+    (128, 64, [(150, 1600)], {"window": 100}), (512, 64, [(150, 300)], {}), (576, 64, [(100, 300)], {"window": 40, "ratio": 8}),
+])
+def test_attn_keys_of_the_lowest_value(D, H, lens, kw):
+    """A finite key whose score leaves fp32 downwards weighs nothing, in tiles that every row sees whole and in others."""
+    s = Lowest(lens, H, D, at=(2, 33, -1, -4, -15, -19, -21, -36), at2=(0, 3, -1, -2), **kw)
+    t = torch.arange(s.N)
+    s.check(s.run(), skip=set(t[(t % 11 != 5) & (s.N > 200)].tolist()))
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D,H,lens", [(64, 16, [(60, 8), (33, 3)]), (576, 64, [(20000, 1), (70, 2)]), (128, 8, [(9000, 2)])])
+def test_attn_unused_rows_not_finite(value, D, H, lens):
+    """Values behind the last row and the last entry in their pages, in calls of one launch and where keys are split: nobody's."""
+    for kw in ({"window": 20, "ratio": 8}, {}):
+        s = Step(lens, H, D, page=48, page2=48, **kw)
+        want = s.run()
+        for cache, table, ends in ((s.kv, s.table, [c + n for c, n in lens]),
+                                   *([(s.kv2, s.table2, [(c + n) // 8 for c, n in lens])] if kw else [])):
+            for r, end in enumerate(ends):
+                if end % 48:
+                    cache[int(table[r, end // 48]), end % 48:] = value
+        got = s.run()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D,H,n", [(64, 16, 8), (576, 64, 300), (128, 64, 1700)])
+def test_attn_entry_not_finite(value, D, H, n):
+    """An entry that is not finite reaches the tokens from its last one on, whose earlier ones share its tile."""
+    s = Step([(60, n)], H, D, window=20, ratio=8)
+    want = s.run()
+    e = (60 + n // 2) // 8
+    s.kv2[int(s.table2[0, e // 16]), e % 16, 7] = value
+    o, lse = s.run()
+    first = 8 * (e + 1) - 1 - 60
+    assert torch.equal(o[:first], want[0][:first]) and torch.equal(lse[:first], want[1][:first])
+    assert o[first:, :, 7].isnan().all()
