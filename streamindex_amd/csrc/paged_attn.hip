@@ -7,7 +7,7 @@
 //     registers), the page numbers fetched a tile before their copies;
 //   * S^T = K Q^T on 16x16x32 MFMAs, keys on M: wave w takes rows 16w .. 16w+15, Q^T stays in registers;
 //   * the online softmax is in-lane (a lane holds eight keys of one row) plus two lane exchanges when a maximum moves,
-//     which it does only once a score exceeds it by 2^64 (fp16: 2^8), so the accumulator is rarely rescaled;
+//     which it does only once a weight exceeds the first by 2^64 (fp16: 2^4), so the accumulator is rarely rescaled;
 //   * P^T goes through LDS, and O^T += V^T P^T with the output dimensions dealt to the waves.
 // P is rounded to the element type for the matrix core, the denominator sums the unrounded values in fp32.
 //
@@ -683,8 +683,12 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // In steps that run among the MFMAs of the tile before: scores to log2 units and masks, a new reference maximum where one
   // is due; the weights one by one; their sum and their place in LDS.
   // (scale is positive: a negative one has changed the sign of Q, zero has made Q zero)
-  constexpr float kLazy = F16 ? 8.0f : 64.0f;  // 2^8 keeps P in fp16's range, 2^64 in bf16's
-  float m_ref = kNever, l_run = 0.f;  // reference maximum (log2 domain) and this lane's share of the denominator
+  // Weights are 2^(score - m_ref), with m_ref kHead below the row's maximum when it is set: P begins at 2^kHead, and the
+  // reference moves when a weight would pass 2^(kHead + kLazy).  fp16's normal numbers reach from 2^-14 to 2^15, so a weight
+  // of 2^-25 of the largest keeps its 11 bits (with kHead = 0 and kLazy = 8 it was zero in the numerator, 2.6 % of the mass
+  // of 2^20 such keys; us, 131,072 rows over 9,000 keys, D = 128, scores of deviation 1 and 8: 859, 867 then, 863, 888 now).
+  constexpr float kHead = F16 ? 11.0f : 0.0f, kLazy = F16 ? 4.0f : 64.0f;
+  float m_ref = kNever, l_run = 0.f;  // reference (log2 domain) and this lane's share of the denominator
   int skey = 0;  // first key of the next tile to mask
   // This lane's row sees key kk of the tile that begins at key `first` where kk + lo, unsigned, is below cnt.
   auto seen_keys = [&](bool second, int first, int& lo, int& cnt) __attribute__((always_inline)) {
@@ -723,14 +727,14 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
                                  __builtin_fmaxf(__builtin_fmaxf(y1[0], y1[1]), __builtin_fmaxf(y1[2], y1[3])));
     lmax *= scale;
     // no lane's keys lift its row's maximum: the tile's maximum over the lanes of a row is not needed
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(lmax > m_ref + kLazy) != 0, 0)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(lmax > m_ref + (kHead + kLazy)) != 0, 0)) {
       const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(lmax), __float_as_uint(lmax), false, false);
       float tmax = __builtin_fmaxf(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
       const SwapPair r32 = permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax));
       tmax = __builtin_fmaxf(__uint_as_float(r32.x), __uint_as_float(r32.y));
-      const bool raise = tmax > m_ref + kLazy, first = m_ref == kNever;
-      const float alpha = raise && !first ? __builtin_amdgcn_exp2f(m_ref - tmax) : 1.0f;
-      if (raise) m_ref = tmax;
+      const bool raise = tmax > m_ref + (kHead + kLazy), first = m_ref == kNever;
+      const float alpha = raise && !first ? __builtin_amdgcn_exp2f(m_ref - (tmax - kHead)) : 1.0f;
+      if (raise) m_ref = tmax - kHead;
       l_run *= alpha;
       const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][wave * 16 + (lane_now() & 15)]));
       asm volatile("ds_write_b32 %0, %1" ::"v"(adst), "v"(alpha) : "memory");  // (the four lanes of a row write the same)

@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from streamindex_amd import paged_compress
+from streamindex_amd import _lib, paged_attn_fwd, paged_compress
 
 from tests.test_gpu_paged import Step
 
@@ -180,3 +180,50 @@ def test_attn_entry_not_finite(value, D, H, n):
     first = 8 * (e + 1) - 1 - 60
     assert torch.equal(o[:first], want[0][:first]) and torch.equal(lse[:first], want[1][:first])
     assert o[first:, :, 7].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,H,N,keys,last", [
+    (64, 4, 1, 1 << 17, False), (64, 4, 1, 1 << 17, True), (576, 64, 1, 1 << 20, False), (128, 16, 3, 1 << 18, True),
+    (128, 64, 1600, 1 << 14, False), (256, 64, 1100, 1 << 13, False), (576, 64, 300, 1 << 15, False),
+])
+@pytest.mark.parametrize("split", [True, False])
+def test_attn_many_small_weights(monkeypatch, dtype, D, H, N, keys, last, split):
+    """One key far above all others, first or last: weights of 2^-25 of the largest count, however many keys share the page.
+
+    u |ref| + (u + 2 E + 2 a) sum p |v| / l: P keeps u of each of these weights, E as for any scores, and a bounds fp32 sums of
+    one addition a tile of 32 keys, (keys / 32) 2^-24."""
+    if not split:
+        monkeypatch.setattr(_lib, "scratch", lambda n, d: (None, 0))
+    page = 64
+    low = torch.ones(page, D, dtype=torch.float64)
+    low[0::2, 0], low[1::2, 0] = -1.0625, -1.0  # times 16: 17 and 16 below the top
+    low[1::2, 1] = -0.5
+    top = torch.zeros(1, D, dtype=torch.float64)
+    at = page - 1 if last else 0
+    one = torch.cat([low[:at], top, low[at + 1:]])
+    kv = torch.stack([one, low]).to(dtype).to(DEV)
+    q = torch.zeros(N, H, D, dtype=dtype, device=DEV)
+    q[..., 0] = 16
+    table = torch.ones(1, keys // page, dtype=torch.int32, device=DEV)
+    table[0, -1 if last else 0] = 0
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    sink = torch.full((H,), -math.inf, device=DEV)
+    o, lse = paged_attn_fwd(q, kv, table, i32([0, N]), i32([keys]), sink, 1.0)
+    p = torch.arange(keys - N, keys, dtype=torch.float64)
+    # the top is every token's where it is first, the last token's alone where it is last
+    w0 = (p == keys - 1).double() if last else torch.ones_like(p)
+    even = torch.floor(p / 2) + 1 - (0 if last else 1)  # keys at even and odd places that the token at p sees, without the top
+    odd = torch.floor((p + 1) / 2) - (w0 if last else 0)
+    we, wo = even * math.exp(-17), odd * math.exp(-16)
+    l = w0 + we + wo
+    ref = torch.ones(N, D, dtype=torch.float64) * ((we + wo) / l)[:, None]
+    mag = ref.clone()
+    ref[:, 0], mag[:, 0] = (-1.0625 * we - wo) / l, (1.0625 * we + wo) / l
+    ref[:, 1], mag[:, 1] = (we - 0.5 * wo) / l, (we + 0.5 * wo) / l
+    u, E, a = half_step(dtype), D * 2.0**-24 * 17 + 2.0**-20, keys / 32 * 2.0**-24
+    err = (o.double().cpu() - ref[:, None]).abs()
+    tol = u * ref.abs() + (u + 2 * E + 2 * a) * mag
+    assert (err <= tol[:, None]).all(), float((err / tol[:, None]).max())
+    el = (lse.double().cpu() - torch.log(l)[:, None]).abs()
+    assert (el <= E + a + 2.0**-20 * (1 + torch.log(l).abs()[:, None])).all(), float(el.max())
