@@ -143,6 +143,12 @@ def strides(t: torch.Tensor):
     return stride_array(t.stride())
 
 
+def packed(t: torch.Tensor) -> torch.Tensor:
+    """A copy with packed strides on a fresh allocation.  (``contiguous()`` returns a packed view at an odd place, and one
+    whose sizes of one hide odd strides, as it is.)"""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def int64s(*vals):
     return (ctypes.c_int64 * len(vals))(*vals)
 

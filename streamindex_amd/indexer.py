@@ -56,9 +56,9 @@ def _prep(q, k_idx, weights):
         return t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
 
     if not ok(q, 3):
-        q = q.contiguous()
+        q = _lib.packed(q)
     if not ok(k_idx, 2):
-        k_idx = k_idx.contiguous()
+        k_idx = _lib.packed(k_idx)
     return q, k_idx, weights
 
 
@@ -253,9 +253,9 @@ def indexer_topk_q(
     def ok(t):
         return t.stride(-1) == 1 and all(s % 16 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
 
-    q_fp4 = q_fp4 if ok(q_fp4) else q_fp4.contiguous()
+    q_fp4 = q_fp4 if ok(q_fp4) else _lib.packed(q_fp4)
     k8 = k_fp8.view(torch.uint8)
-    k8 = k8 if ok(k8) else k8.contiguous()
+    k8 = k8 if ok(k8) else _lib.packed(k8)
     q_scale = q_scale if q_scale.stride(-1) == 1 else q_scale.contiguous()
     out_idx = torch.empty((B, S, top_k), dtype=torch.int64, device=q_fp4.device)
     out_scores = torch.empty((B, S, top_k), dtype=torch.float32, device=q_fp4.device)

@@ -300,7 +300,7 @@ def paged_attn_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
     c1 = cache_args(kv_cache, block_table, "kv")
     c2 = cache_args(kv2_cache, block_table2, "kv2") if two else (None, None, 0, 1, None, 0, 0)
     cu, lens = _int32(cu_q, "cu_q", R + 1), _int32(seq_lens, "seq_lens", R)
-    q = q if _aligned(q) else q.contiguous()
+    q = q if _aligned(q) else _lib.packed(q)
     attn_sink = attn_sink if attn_sink.is_contiguous() else attn_sink.contiguous()
     window, ratio = window or 0, ratio or 0
     L = _lib.load()

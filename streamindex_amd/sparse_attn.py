@@ -87,13 +87,7 @@ def sparse_attn_fwd(
         softmax_scale = D ** -0.5
     K = topk_idxs.shape[-1]
 
-    def ok(t):
-        return t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
-
-    if not ok(q):
-        q = q.contiguous()
-    if not ok(kv):
-        kv = kv.contiguous()
+    q, kv = (t if _aligned(t) else _lib.packed(t) for t in (q, kv))
     attn_sink = attn_sink.contiguous()
     if row_len is not None:
         assert row_len.is_cuda and row_len.shape == (B, S), "row_len must be [B, S] on the GPU"
@@ -152,7 +146,7 @@ def sparse_attn_fwd_kv2(
     if softmax_scale is None:
         softmax_scale = D ** -0.5
     K = topk_idxs.shape[-1]
-    q, kv, kv2 = (t if _aligned(t) else t.contiguous() for t in (q, kv, kv2))
+    q, kv, kv2 = (t if _aligned(t) else _lib.packed(t) for t in (q, kv, kv2))
     attn_sink = attn_sink.contiguous()
     if row_len is not None:
         assert row_len.is_cuda and row_len.shape == (B, S), "row_len must be [B, S] on the GPU"
@@ -272,7 +266,7 @@ def sparse_attn_bwd(
         assert row_len.is_cuda and row_len.shape == (B, S), "row_len must be [B, S] on the GPU"
         if row_len.dtype != torch.int32:
             row_len = row_len.to(torch.int32)
-    q, kv, o, do = (t if _aligned(t) else t.contiguous() for t in (q, kv, o, do))
+    q, kv, o, do = (t if _aligned(t) else _lib.packed(t) for t in (q, kv, o, do))
     attn_sink = attn_sink.contiguous()
     dq = torch.empty((B, S, H, D), dtype=q.dtype, device=q.device)
     dkv = torch.empty((B, N_kv, D), dtype=kv.dtype, device=q.device)
