@@ -1203,7 +1203,7 @@ static PagedSizes paged_sizes(int64_t N, int64_t H, int64_t D, int64_t R, int64_
   p.grid = 2 * p.blocks <= want ? want : p.blocks + want;
   // tiles of a row block at most
   const int64_t span = M / H + 1 + window;
-  p.behind = static_cast<int>((M - 1) / H);
+  p.behind = static_cast<int>((M - 1 + H - g) / H);  // (a row block begins at any multiple of g heads of a token)
   const int64_t tiles = ((window < keys1 && span < keys1 ? span : keys1) + 31) / 32 + (keys2 + 31) / 32;
   // Where no cut can win back the second launch, 4 us, that joins the shares, none is made (8 tiles at D = 576, 14 at 128, and
   // more of them where many row blocks leave partial outputs; us whole and cut in two: 1 row block of 10 and 16 tiles, D = 576,

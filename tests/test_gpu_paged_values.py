@@ -227,3 +227,13 @@ def test_attn_many_small_weights(monkeypatch, dtype, D, H, N, keys, last, split)
     assert (err <= tol[:, None]).all(), float((err / tol[:, None]).max())
     el = (lse.double().cpu() - torch.log(l)[:, None]).abs()
     assert (el <= E + a + 2.0**-20 * (1 + torch.log(l).abs()[:, None])).all(), float(el.max())
+
+
+@pytest.mark.parametrize("H", [7, 24, 40, 100])
+@pytest.mark.parametrize("lens,kw", [
+    ([(3000, 9), (5, 4)], {"window": 31, "ratio": 2}), ([(4000, 12)], {"window": 700}), ([(2000, 3), (900, 30)], {"window": 96, "ratio": 8}),
+])
+def test_attn_row_blocks_that_begin_inside_a_token(H, lens, kw):
+    """Head counts that do not divide 64, with split keys: a row block spans one token more than its rows need."""
+    s = Step(lens, H, 128, **kw)
+    s.check(s.run())
