@@ -397,6 +397,14 @@ constexpr int per_cu(int D, bool PAIR) { return (D >= 512 ? 1 : D == 256 ? 2 : D
 constexpr int64_t pair_from(int64_t D) { return D >= 512 ? 257 : D == 256 ? 1025 : D == 128 ? 1537 : INT64_MAX; }
 
 constexpr float kNever = -__builtin_inff();
+// A sink in log2 units: finite where it outweighs everything (inf - inf would follow).  Finite ones below the range become
+// -inf, which weighs the same, nothing, beside a key, and a row whose keys weigh nothing takes its lse from the sink itself.
+__device__ __forceinline__ float sink_log2(float sink) {
+  constexpr float kMost = 3.4028234663852886e38f;
+  const float x = sink * 1.4426950408889634f;
+  return x > kMost ? kMost : x;  // (NaN stays)
+}
+__device__ __forceinline__ float lse_of_sink(float sink) { return sink == kNever ? -1.0e30f : sink; }
 constexpr int kOdd = 1;    // a masked score that is not finite
 constexpr int kMoved = 2;  // a reference maximum has moved: alpha is not one
 
@@ -423,7 +431,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   constexpr int M = kRows, NB = M / 16;             // rows of the workgroup, and blocks of 16
   constexpr int NS = PAIR ? 2 : 4, AHEAD = NS - 1;  // tiles in LDS, and copied ahead of P V
   constexpr int NP = PAIR ? 1 : 2, PAGES = PAIR ? 2 : 4;  // P's and page numbers' buffers
-  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  constexpr float kLn2 = 0.6931471805599453f;
   static_assert(NS * SH::TILE >= M * ROW, "the output is staged in the tiles' LDS");
   __shared__ __attribute__((aligned(16))) char kv_lds[NS * SH::TILE];
   __shared__ __attribute__((aligned(16))) char p_lds[NP][NB * 64 * 16];
@@ -448,8 +456,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
     u32x4* orow = reinterpret_cast<u32x4*>(a.o + t * a.H * D);
     for (int64_t e = threadIdx.x; e < static_cast<int64_t>(a.H) * SH::CPR; e += kPagedThreads) orow[e] = u32x4{0, 0, 0, 0};
     for (int h = threadIdx.x; h < a.H; h += kPagedThreads) {
-      const float s = a.sink[h];
-      a.lse[t * a.H + h] = s == kNever ? -1.0e30f : s;
+      a.lse[t * a.H + h] = lse_of_sink(a.sink[h]);
     }
   }
   if (!work) return;
@@ -1040,15 +1047,14 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   float* scale_lds = alpha_lds[0];
   __syncthreads();  // every wave has left the last tile and its alpha
   const float sink = sink_lds[lrow];
-  const float sink2 = sink * kLog2e;
+  const float sink2 = sink_log2(sink);
   const float m_fin = __builtin_fmaxf(m_ref, sink2);
   const float top = m_fin == kNever ? 0.f : m_fin;
-  const float resc = __builtin_amdgcn_exp2f(m_ref - top);
-  const float l_fin = l_tot * resc + __builtin_amdgcn_exp2f(sink2 - top);
+  const float resc = __builtin_amdgcn_exp2f(m_ref - top), keys = l_tot * resc;
+  const float l_fin = keys + __builtin_amdgcn_exp2f(sink2 - top);
   if (g == 0) {
-    scale_lds[lrow] = l_fin == 0.f ? 0.f : resc / l_fin;
-    if (live)
-      a.lse[flat0 + lrow] = l_fin == 0.f ? -1.0e30f : l_tot == 0.f ? sink : (__builtin_amdgcn_logf(l_fin) + top) * kLn2;
+    scale_lds[lrow] = keys == 0.f ? 0.f : resc / l_fin;
+    if (live) a.lse[flat0 + lrow] = keys == 0.f ? lse_of_sink(sink) : (__builtin_amdgcn_logf(l_fin) + top) * kLn2;
   }
   __syncthreads();  // scales published
   // staged in the tiles' LDS, chunk c of row r at c ^ (r & 7), then written in one piece: the rows follow each other in o
@@ -1083,7 +1089,7 @@ constexpr int kCombineParts = 4;
 // that the last-level cache holds).
 template <bool F16>
 __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnArgs a, int D) {
-  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  constexpr float kLn2 = 0.6931471805599453f;
   constexpr int M = kRows, U = 4;
   __shared__ float lds[kCombineParts - 1][6][kPagedThreads / kCombineParts];
   const int count = a.rec[0];
@@ -1163,18 +1169,18 @@ __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnA
       }
     }
     if (part > 0 || !live) continue;
-    const float sink2 = sink * kLog2e;
+    const float sink2 = sink_log2(sink);
     const float top = __builtin_fmaxf(m, sink2);
     const float ref = top == kNever ? 0.f : top;
     const float w = __builtin_amdgcn_exp2f(m - ref);
     const float keys = l * w;
     const float all = keys + __builtin_amdgcn_exp2f(sink2 - ref);
-    const float inv = all == 0.f ? 0.f : w / all;
+    const float inv = keys == 0.f ? 0.f : w / all;
     uint2 o;
     o.x = pack2<F16>(acc[0] * inv, acc[1] * inv);
     o.y = pack2<F16>(acc[2] * inv, acc[3] * inv);
     *reinterpret_cast<uint2*>(a.o + flat * D + d) = o;
-    if (d == 0) a.lse[flat] = all == 0.f ? -1.0e30f : keys == 0.f ? sink : (__builtin_amdgcn_logf(all) + ref) * kLn2;
+    if (d == 0) a.lse[flat] = keys == 0.f ? lse_of_sink(sink) : (__builtin_amdgcn_logf(all) + ref) * kLn2;
   }
 }
 

@@ -237,3 +237,32 @@ def test_attn_row_blocks_that_begin_inside_a_token(H, lens, kw):
     """Head counts that do not divide 64, with split keys: a row block spans one token more than its rows need."""
     s = Step(lens, H, 128, **kw)
     s.check(s.run())
+
+
+@pytest.mark.parametrize("D,H,lens", [(64, 8, [(40, 2), (9, 1)]), (576, 64, [(12000, 1), (100, 2)]), (128, 64, [(300, 1600)]), (32, 8, [(9000, 2)])])
+def test_attn_sinks_at_the_ends_of_their_range(D, H, lens):
+    """Sinks of fp32's lowest and largest values and infinite ones, for rows with keys, without any (no page) and of no request."""
+    f32 = torch.finfo(torch.float32)
+    s = Step(lens, H, D, pad=2)
+    s.sink[:6] = torch.tensor([f32.min, -math.inf, f32.max, 2.5e38, -2.5e38, 1.5])
+    t = torch.arange(s.N)
+    skip = set(t[(t % 97 != 5) & (s.N > 200) & (t < s.N - 2)].tolist())
+    empty = torch.where(s.sink == -math.inf, -1e30, s.sink)
+
+    def check(o, lse):
+        assert torch.equal(lse[-2:], empty.expand(2, H)) and not o[-2:].any()
+        inner = lse.clone()
+        inner[-2:] = s.sink  # (check() compares rows of no request with the sinks themselves)
+        s.check((o, inner), skip=skip)
+
+    check(*s.run())
+    want = s.run()
+    s.sink[0] = -math.inf  # the lowest value weighs as little beside a key
+    same = s.run()
+    assert torch.equal(same[0], want[0]) and torch.equal(same[1][:-2], want[1][:-2])
+    s.sink[0], s.table[:] = f32.min, -1
+    o, lse = s.run()
+    assert not o.any() and torch.equal(lse, empty.expand(s.N, H))
+    s.sink[:2] = torch.tensor([math.inf, math.nan])
+    o, lse = s.run()
+    assert not o[:, 0].any() and (lse[:, 0] == math.inf).all() and lse[:, 1].isnan().all()
