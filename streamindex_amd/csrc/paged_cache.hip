@@ -525,12 +525,18 @@ template <int DT, int N>
 static int launch_paged_compress_n(const CompressArgs& a, hipStream_t st) {
   // Parts of an entry, that is threads of a channel: the fewer, the less is spent on joining them; the more, the more loads of
   // few entries are in flight (us, C = 576, bf16: 8 tokens, 7,000 entries, 1 and 4 parts 30 and 47; 16, 6,000, 50 and 59; 32,
-  // 1,000 entries, fp32, C = 500, 35 and 31; 128, 512 entries, 8 and 32 parts 39 and 48; 256 of which
-  // two are there, as a decode step of 256 requests has them, 11 and 7).
+  // 1,000 entries, fp32, C = 500, 35 and 31).
   const int64_t tokens = (a.overlap ? 2 : 1) * a.m;
   if (tokens <= 16) return launch_paged_compress_p<DT, N, 1>(a, st);
   if (tokens < 64) return launch_paged_compress_p<DT, N, 4>(a, st);
-  return a.E * ((a.C / N + 7) / 8) >= 4096 ? launch_paged_compress_p<DT, N, 8>(a, st) : launch_paged_compress_p<DT, N, 32>(a, st);
+  // 8 or 32: a list of which few entries are there (a decode step's, one row a request) wants 32 at any length, one whose entries
+  // all are there 8 from some length on, sooner where entries have few tokens.  Only the length is known here, so the border
+  // lies where either choice loses about the same (us with 8 and 32, bf16, all entries there / one in 128: 64 tokens, C = 128,
+  // 256 rows 8.3, 8.7 / 6.8, 6.3, 1,024 rows 12.5, 20.2 / 7.4, 6.5; 128 tokens, C = 576, 128 rows 17.1, 16.7 / 10.1, 6.7, 256 rows
+  // 21.0, 24.8 / 10.2, 6.8, 512 rows 40.5, 50.1 / 10.9, 6.9; 200 tokens, C = 64, 1,024 rows 20.6, 18.1 / 16.2, 7.9, 4,096 rows 49.8,
+  // 63.1 / 16.3, 8.0; 512 tokens, C = 576, 128 rows 56.8, 45.2 / 29.5, 11.4).
+  const int64_t many = tokens < 176 ? 32 * (tokens - 48) : 4096;  // workgroups of 32 parts
+  return a.E * ((a.C / N + 7) / 8) >= many ? launch_paged_compress_p<DT, N, 8>(a, st) : launch_paged_compress_p<DT, N, 32>(a, st);
 }
 template <int DT>
 static int launch_paged_compress(const CompressArgs& a, hipStream_t st) {
