@@ -23,7 +23,7 @@ import torch
 from . import _lib
 from .csa import _launch_hca, _row_len
 from .paged import PagedPlan, paged_attn_fwd, paged_compress, paged_write
-from .sparse_attn import _aligned, _bwd_workspace, sparse_attn_bwd, sparse_attn_fwd_kv2
+from .sparse_attn import SUPPORTED_D, _aligned, _bwd_workspace, sparse_attn_bwd, sparse_attn_fwd_kv2
 
 __all__ = ["flash_hca_forward", "flash_hca_paged_forward", "build_hca_topk_idxs", "hca_row_len"]
 
@@ -100,14 +100,30 @@ def flash_hca_paged_forward(
         (:func:`streamindex_amd.paged.paged_plan`).  A page may be given back, and its table entry set to -1, once its
         tokens are behind the window and in a complete entry.
       entry_cache: ``[entry_pages, entry_page_size, d]``, updated in place; ``entry_table`` and ``entries`` its plan, made
-        with ``ratio=m'``.
+        with ``ratio=m'`` for the tokens that ``tokens`` holds (where its row lists were too short, ``tokens.seq_lens`` less
+        the earlier lengths).
       n_win: sliding-window size.  softmax_scale: defaults to ``d ** -0.5``.
     Returns:
       ``o: [N, n_h, d]`` in q's type, zero in rows behind the last request.
     """
-    d = q.shape[2]
-    if row_cache.dim() != 3 or row_cache.shape[2] != 3 * d:
-        raise ValueError(f"row_cache must be [pages, page_size, {3 * d}]")
+    assert q.is_cuda and q.dim() == 3, "q must be [N, n_h, d] on the GPU"
+    N, n_h, d = q.shape
+    # (what the attention would refuse, before anything is written)
+    if q.dtype not in (torch.bfloat16, torch.float16) or d not in SUPPORTED_D:
+        raise ValueError(f"q must be bf16 or fp16 of a width in {SUPPORTED_D}, got {q.dtype}, {d}")
+    for name, cache, width in (("row_cache", row_cache, 3 * d), ("entry_cache", entry_cache, d)):
+        if cache.dim() != 3 or cache.shape[2] != width or cache.dtype is not q.dtype:
+            raise ValueError(f"{name} must be [pages, page_size, {width}] of q's type")
+        s = cache.stride()
+        if (s[0] if cache.shape[0] > 1 else 0) % 8 or (s[1] if cache.shape[1] > 1 else 0) % 8 or cache.data_ptr() % 16:
+            raise ValueError(f"{name} needs rows that start at multiples of 16 bytes")
+    if rows.shape[0] != N or attn_sink.shape != (n_h,) or attn_sink.dtype is not torch.float32:
+        raise ValueError(f"rows must be [{N}, {3 * d}] and attn_sink [{n_h}] fp32")
+    R = block_table.shape[0]
+    if entry_table.shape[0] != R or tokens.seq_lens.shape[0] != R:
+        raise ValueError("block_table, entry_table and the plans must be of the same requests")
+    if n_win < 1:
+        raise ValueError(f"n_win must be positive, got {n_win}")
     paged_write(rows, row_cache, tokens.slots)
     kv, c, z = row_cache[..., :d], row_cache[..., d:2 * d], row_cache[..., 2 * d:]
     paged_compress(c, z, bias, block_table, entries.request, entries.positions, entry_cache, entries.slots)

@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from streamindex_amd import _lib, paged_attn_fwd, paged_compress
+from streamindex_amd import _lib, flash_hca_paged_forward, paged_attn_fwd, paged_compress, paged_plan
 
 from tests.test_gpu_paged import Step
 
@@ -266,3 +266,35 @@ def test_attn_sinks_at_the_ends_of_their_range(D, H, lens):
     s.sink[:2] = torch.tensor([math.inf, math.nan])
     o, lse = s.run()
     assert not o[:, 0].any() and (lse[:, 0] == math.inf).all() and lse[:, 1].isnan().all()
+
+
+# ---------------------------------------------------------------------------
+# the layer
+# ---------------------------------------------------------------------------
+def test_refused_step_writes_nothing():
+    """Each argument that the layer's last operator would refuse is refused before the first one writes."""
+    d, H, m, N = 64, 4, 4, 6
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    bf, f32 = torch.bfloat16, torch.float32
+    ones = lambda *s, t=bf: torch.ones(s, dtype=t, device=DEV)  # noqa: E731
+
+    def args(**kw):
+        table, etable = i32([[-1, -1], [-1, -1]]), i32([[-1], [-1]])
+        tok = paged_plan(i32([0, 0]), i32([4, 2]), table, i32([0, 1, 2]), 4, N)
+        ent = paged_plan(i32([0, 0]), i32([4, 2]), etable, i32([0, 1]), 4, 3, ratio=m)
+        a = dict(q=ones(N, H, d), rows=ones(N, 3 * d), bias=ones(m, d, t=f32), attn_sink=ones(H, t=f32),
+                 row_cache=ones(3, 4, 3 * d) * 0, block_table=table, tokens=tok, entry_cache=ones(2, 4, d) * 0,
+                 entry_table=etable, entries=ent, n_win=3)
+        a.update(kw)
+        return a
+
+    good = args()
+    assert flash_hca_paged_forward(**good).any() and good["row_cache"].any() and good["entry_cache"].any()
+    odd = torch.zeros(3, 4, 3 * d + 4, dtype=bf, device=DEV)[..., :3 * d]
+    for kw in ({"n_win": 0}, {"q": ones(N, H, d, t=f32)}, {"q": ones(N + 1, H, d)}, {"q": ones(N, H, 96)}, {"attn_sink": ones(H + 1, t=f32)},
+               {"attn_sink": ones(H)}, {"entry_cache": ones(2, 4, d + 8) * 0}, {"entry_cache": ones(2, 4, d, t=torch.float16) * 0},
+               {"entry_table": i32([[0]])}, {"row_cache": odd}, {"row_cache": ones(3, 4, 2 * d) * 0}):
+        a = args(**kw)
+        with pytest.raises(ValueError):
+            flash_hca_paged_forward(**a)
+        assert not a["row_cache"].any() and not a["entry_cache"].any(), kw
