@@ -436,7 +436,7 @@ int si_gated_pool(const void* kv, const void* score, void* out, int dtype, int64
  * r's entries i * page_size and on, negative where there is none, and
  * slot = page * page_size + offset names a row.  Tables are int32 with
  * contiguous rows table_stride elements apart; lengths are below 2^31 and are
- * read on the device only.
+ * read on the device only; a call has at most 2^30 requests.
  *
  * si_paged_plan: R requests with ctx_lens[r] tokens get new_lens[r] more (int32,
  * negative = 0).  Entries are tokens (ratio 1) or completed groups of ratio

@@ -1333,6 +1333,8 @@ extern "C" int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const 
                      "unsupported head dim D=" + std::to_string(D) + " (supported: 32, 64, 128, 256, 512, 576)");
   if (N > 0x7fffffff || H > 0x7fffffff || R > 0x7fffffff || N * H > 0x7fffffff || ratio > 0x7fffffff)
     return set_error(SI_ERR_UNSUPPORTED, "dimension exceeds int32");
+  // (a thread's share of the requests ends within 31 bits)
+  if (R > int64_t{1} << 30) return set_error(SI_ERR_UNSUPPORTED, "more than 2^30 requests");
   if (!q_strides) return set_error(SI_ERR_INVALID, "null stride argument");
   if (N > 0 && (!q || !attn_sink || !o || !lse || !cu_q || (R > 0 && !seq_lens)))
     return set_error(SI_ERR_INVALID, "null pointer argument");

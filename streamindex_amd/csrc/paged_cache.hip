@@ -557,6 +557,7 @@ static int launch_paged_compress(const CompressArgs& a, hipStream_t st) {
   return launch_paged_compress_n<DT, 1>(a, st);
 }
 
+constexpr int64_t kMostRequests = int64_t{1} << 30;  // (a thread's share of the requests ends within 31 bits)
 static bool too_big(int64_t x) { return x < 0 || x > 0x7fffffff; }
 
 }  // namespace si
@@ -572,6 +573,7 @@ extern "C" int si_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, i
     return set_error(SI_ERR_INVALID, "bad dimension");
   if (too_big(R) || too_big(P) || too_big(F) || too_big(rows) || too_big(ratio) || too_big(page_size))
     return set_error(SI_ERR_UNSUPPORTED, "dimension exceeds int32");
+  if (R > kMostRequests) return set_error(SI_ERR_UNSUPPORTED, "more than 2^30 requests");
   if (!cu || !free_next || (R > 0 && (!ctx_lens || !new_lens || !seq_lens)) || (R > 0 && P > 0 && !block_table) ||
       (F > 0 && !free_pages) || (rows > 0 && (!slots || !request || !positions)))
     return set_error(SI_ERR_INVALID, "null pointer argument");
