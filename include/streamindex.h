@@ -482,7 +482,8 @@ int si_paged_compress(const void* c_a, const int64_t* ca_strides, const void* z_
  * the last 1), the last at position seq_lens[r] - 1.  A token at position p sees
  * entries k of kv [pages, page_size, D] with p - window < k <= p (window 0: all
  * k <= p) and, with ratio > 0, entries i of kv2 with ratio (i + 1) - 1 <= p.
- * Keys without a page in [0, pages) are masked.  o [N,H,D] and lse [N,H]
+ * Keys without a page in [0, pages) are masked.  Scores are fp32: -inf weighs
+ * nothing, +inf and NaN make the row NaN.  o [N,H,D] and lse [N,H]
  * contiguous; rows of no request are written as rows without a key.  A cache
  * spans at most 64 GiB, its strides are multiples of 8 elements; N * H < 2^31.
  * scratch: as for si_sparse_attn_fwd_scratch, at least

@@ -16,9 +16,10 @@
 // PAIR: two tiles in LDS, a tile's steps one after the other, one workgroup more a CU, whose copies, prologues and ends
 // fall behind each other's MFMAs: for many row blocks, from D = 128 on (pair_from below).
 //
-// Bound, long keys: the LDS, which every K tile leaves four times (each wave's S^T) and once more as V, beside its copy: at
-// D = 576 1,020 TFLOP/s, at 256 920, at 128 724, at 64 573 where a library product reaches 1,279 (below 256 the softmax's
-// vector work weighs more).  Few keys a row: Q in, O out and the prologue.
+// Bound, long keys: the LDS, which every K tile leaves four times (each wave's S^T) and once more as V, beside its copy: one
+// request of 8,192 earlier tokens, 64 heads, 1,024 new ones at D = 576 1,130 TFLOP/s, at 512 1,055, 2,048 at 256 941, at 128 714,
+// 4,096 at 64 616, where a library product reaches 1,279 (below 256 the softmax's vector work weighs more).  Few keys a row:
+// Q in, O out and the prologue.
 //
 // A key that only some of the 64 rows see is masked for the others by a weight of zero; the matrix core would still
 // turn 0 x inf into NaN.  Keys and values being the same rows, such a value makes the key's raw score non-finite as
@@ -499,7 +500,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // flight before their use), a tile ahead of the copies; `within` is what the key's place in its page adds.  What
   // a tile asks of its cache is held in scalars that every path sets: as vector registers, which a value that only some
   // paths set becomes, they were spilled and read back between a tile's steps, with a wait for its copies each time
-  // (7,149 row blocks of up to 17 tiles, D = 576: 540 us, 476 without).
+  // (7,149 row blocks of up to 17 tiles, D = 576: 540 us, 476 without).  Five registers are still
+  // spilled with PAIR at D = 576: four are read back in a rescale of the accumulator only, one behind the last tile.
   CacheView view1, view2;
   CacheBase base1, base2;
   view_cache(a.c1, req, view1, base1);

@@ -25,7 +25,7 @@ constexpr int64_t kMostBlocks = 0xffffffffLL / 256;  // of 256 threads: a launch
 // One launch: every workgroup sums the lengths itself (R of them, L2-resident after the first) and then takes its share of
 // the rows and of the new pages, which it finds in the sums by bisection.  A row whose page is new computes that page
 // from the free list as well, so no workgroup reads what another one writes.  Bound: the latency of one chain of loads
-// and scans, 3.6 us for 64 rows of 64 requests and 9.2 for 65,536; a kernel for the sums and one for the rows would pay a
+// and scans, 3.7 us for 64 rows of 64 requests and 9.2 for 79,134 of 301; a kernel for the sums and one for the rows would pay a
 // second launch.
 // ---------------------------------------------------------------------------
 struct PlanArgs {
@@ -263,9 +263,10 @@ static int launch_write(WriteArgs a, int64_t n, int64_t row_bytes, hipStream_t s
 // The workgroup looks up where its tokens' rows are once, into LDS.  Then a thread takes 16 (or 8) bytes of channels and
 // every PARTS-th token, keeps the running maximum, denominator and numerator of each channel in fp32 registers, and the
 // PARTS threads of a channel group join theirs by lane exchanges and, at 32, one LDS step.  Eight neighbouring threads read
-// 128 consecutive bytes of a row.  Bound: the two streams' bytes for 4-byte elements (454 MB in 85 us, 5.3 TB/s); with 2-byte
-// ones as many values come in half the bytes, and the vector work, an exponential and ten instructions a value, weighs as
-// much (149 MB in 39 us, 3.8 TB/s; 227 MB in 51 us, 4.5 TB/s).
+// 128 consecutive bytes of a row.  Bound: the two streams' bytes for 4-byte elements (454 MB in 85 us, 5.3 TB/s).  With 2-byte
+// ones as many values come in half the bytes: 149 MB in 40 us, 3.7 TB/s.  Vector instructions, twenty a value with the
+// exponential, fill 66 % of the CUs' busy cycles there, and about 9 us do not grow with the entries (113 MB in 31.6 us, 226 MB in
+// 54.4: 5.0 TB/s between them): the launch, a chain of lookup, page and rows, and a second round of few workgroups.
 // ---------------------------------------------------------------------------
 struct CompressArgs {
   const char *ca, *za, *cb, *zb;        // streams, [pages, ps, C]

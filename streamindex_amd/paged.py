@@ -141,8 +141,8 @@ def paged_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
 def paged_write(rows: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
     """``cache[slots[t] // page_size, slots[t] % page_size] = rows[t]``; returns ``cache``, written in place.
 
-    ``rows [N, width]`` of the cache's type, ``slots [N]`` int64; a slot outside the cache (-1) writes nothing.  Slots
-    are distinct, as a plan's are: of a slot given twice each 16-byte piece is one of the two rows'.
+    ``rows [N, width]`` of the cache's type and not part of it, ``slots [N]`` int64; a slot outside the cache (-1) writes
+    nothing.  Slots are distinct, as a plan's are: of a slot given twice each 16-byte piece is one of the two rows'.
     """
     assert rows.is_cuda
     dev = rows.device
@@ -251,7 +251,7 @@ def paged_attn_fwd(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.T
 
     Args:
       q: ``[N, H, D]`` bf16 or fp16.  kv_cache: ``[pages, page_size, D]`` of q's type (the new tokens' rows included), one
-        row for key and value, shared by the heads; rows 16-byte aligned.
+        row for key and value, shared by the heads; rows 16-byte aligned, within 64 GiB of the first.
       block_table: ``[R, P]`` int32.  Keys whose page is negative, past the cache or past the table are masked: pages
         that the window has left may be given back.
       cu_q: ``[R + 1]`` int32, ascending (if it descends anywhere, no request has rows); seq_lens: ``[R]`` int32;
