@@ -9,13 +9,14 @@ Tolerances (u = eps / 2 of the type):
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
 
 from streamindex_amd import _lib, flash_hca_paged_forward, paged_attn_fwd, paged_compress, paged_plan
 
-from tests.test_gpu_paged import Step
+from tests.test_gpu_paged import Server, Step
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -298,3 +299,47 @@ def test_refused_step_writes_nothing():
         with pytest.raises(ValueError):
             flash_hca_paged_forward(**a)
         assert not a["row_cache"].any() and not a["entry_cache"].any(), kw
+
+
+@pytest.mark.parametrize("H,d,m,n_win,page,dtype", [
+    (64, 576, 16, 24, 64, torch.bfloat16), (8, 64, 8, 20, 7, torch.bfloat16), (24, 128, 5, 1, 3, torch.float16),
+])
+def test_serving_steps_against_the_definition(H, d, m, n_win, page, dtype):
+    """Chunks and decode steps of three requests: every entry and every output against 64-bit arithmetic over the tokens' own
+    rows, with the tolerances of an entry and of the attention (whose keys are the entries as they are cached)."""
+    R, total = 3, [5 * m + 3, 2, 4 * m]
+    g = torch.Generator().manual_seed(m)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(dtype).to(DEV)  # noqa: E731
+    bias, sink = torch.randn(m, d, generator=g).to(DEV), torch.randn(H, generator=g).to(DEV)
+    srv = Server(R, 150, page, 4, d, m, n_win, dtype, bias, sink, max(total))
+    q, x = [rnd(t, H, d) for t in total], [rnd(t, 3 * d) for t in total]
+    done, rng, u, scale = [0] * R, random.Random(m), half_step(dtype), d ** -0.5
+    while any(done[r] < total[r] for r in range(R)):
+        new = [min(total[r] - done[r], rng.choice([0, 1, 1, m + 2])) for r in range(R)]
+        if not any(new):
+            continue
+        o = srv.step(torch.cat([q[r][done[r]:done[r] + new[r]] for r in range(R)] + [rnd(1, H, d)]),
+                     torch.cat([x[r][done[r]:done[r] + new[r]] for r in range(R)] + [rnd(1, 3 * d)]),
+                     torch.tensor(new, dtype=torch.int32, device=DEV))
+        t = 0
+        for r in range(R):
+            rows = x[r].double()
+            ends = (done[r] + new[r]) // m
+            ents = [srv.ents[int(srv.etable[r, i // 4]), i % 4].double() for i in range(ends)]
+            for i in range(done[r] // m, ends):
+                v, z = rows[i * m:(i + 1) * m, d:2 * d], rows[i * m:(i + 1) * m, 2 * d:] + bias.double()
+                w = torch.softmax(z, 0)
+                tol = u * (w * v).sum(0).abs() + 2.0**-18 * (w * v.abs()).sum(0) + torch.finfo(dtype).smallest_normal
+                assert ((ents[i] - (w * v).sum(0)).abs() <= tol).all()
+            for p in range(done[r], done[r] + new[r]):
+                k = torch.cat([rows[max(0, p + 1 - n_win):p + 1, :d], *(e[None] for e in ents[:(p + 1) // m])])
+                qd = q[r][p].double()
+                s = qd @ k.t() * scale
+                E = d * 2.0**-24 * scale * (qd.abs() @ k.abs().t()).amax(1) + 2.0**-20
+                w = torch.softmax(torch.cat([s, sink.double()[:, None]], 1), 1)[:, :-1]
+                ref, mag = w @ k, w @ k.abs()
+                tol = u * ref.abs() + (u + 2 * E[:, None]) * mag * (1 + 2 * u) + torch.finfo(dtype).smallest_normal
+                assert ((o[t].double() - ref).abs() <= tol).all(), (r, p)
+                t += 1
+            done[r] += new[r]
+        assert not o[t:].any()
