@@ -7,7 +7,7 @@
 //     registers), the page numbers fetched a tile before their copies;
 //   * S^T = K Q^T on 16x16x32 MFMAs, keys on M: wave w takes rows 16w .. 16w+15, Q^T stays in registers;
 //   * the online softmax is in-lane (a lane holds eight keys of one row) plus two lane exchanges when a maximum moves,
-//     which it does only once a weight exceeds the first by 2^64 (fp16: 2^4), so the accumulator is rarely rescaled;
+//     which it does only once a weight exceeds the first by 2^32 (fp16: 2^4), so the accumulator is rarely rescaled;
 //   * P^T goes through LDS, and O^T += V^T P^T with the output dimensions dealt to the waves.
 // P is rounded to the element type for the matrix core, the denominator sums the unrounded values in fp32.
 //
@@ -693,10 +693,15 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // is due; the weights one by one; their sum and their place in LDS.
   // (scale is positive: a negative one has changed the sign of Q, zero has made Q zero)
   // Weights are 2^(score - m_ref), with m_ref kHead below the row's maximum when it is set: P begins at 2^kHead, and the
-  // reference moves when a weight would pass 2^(kHead + kLazy).  fp16's normal numbers reach from 2^-14 to 2^15, so a weight
-  // of 2^-25 of the largest keeps its 11 bits (with kHead = 0 and kLazy = 8 it was zero in the numerator, 2.6 % of the mass
-  // of 2^20 such keys; us, 131,072 rows over 9,000 keys, D = 128, scores of deviation 1 and 8: 859, 867 then, 863, 888 now).
-  constexpr float kHead = F16 ? 11.0f : 0.0f, kLazy = F16 ? 4.0f : 64.0f;
+  // reference moves when a weight would pass 2^(kHead + kLazy).
+  // fp16's normal numbers reach from 2^-14 to 2^15, so a weight of 2^-25 of the largest keeps its 11 bits (with P from 1 to 2^8
+  // it was zero in the numerator, 2.6 % of the mass of 2^20 such keys).
+  // bf16 has fp32's range: P begins at 2^-32 and never passes 1, so the reference is no lower than the largest weight, whose
+  // distance from a sink far above is then in range if the weight is (with P from 1 to 2^64, scores of -90 and -47 beside a sink
+  // of 0 gave zero); values below 2^-94 lose bits for it.
+  // (us, 131,072 rows over 9,000 keys, D = 128, scores of deviation 1 and 8: fp16 841, 869 with P from 1 to 2^8, 846, 889 now;
+  // bf16 831, 833 with P from 1 to 2^64, 837, 840 now, 836, 863 from 2^-16.)
+  constexpr float kHead = F16 ? 11.0f : -32.0f, kLazy = F16 ? 4.0f : 32.0f;
   float m_ref = kNever, l_run = 0.f;  // reference (log2 domain) and this lane's share of the denominator
   int skey = 0;  // first key of the next tile to mask
   // This lane's row sees key kk of the tile that begins at key `first` where kk + lo, unsigned, is below cnt.

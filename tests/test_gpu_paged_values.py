@@ -343,3 +343,47 @@ def test_serving_steps_against_the_definition(H, d, m, n_win, page, dtype):
                 t += 1
             done[r] += new[r]
         assert not o[t:].any()
+
+
+def scored(s, score):
+    """Queries of one and keys whose scores are ``score(r, k)``, for entries ``score(r, -1 - i)``, with sinks of zero."""
+    s.q.zero_()
+    s.q[..., 0] = 1
+    s.sink.zero_()
+    for r, (c, n) in enumerate(s.lens):
+        for cache, table, at in ((s.kv, s.table, range(c + n)), (s.kv2, s.table2, range((c + n) // s.ratio if s.ratio else 0))):
+            if len(at):
+                k = torch.tensor(at, device=DEV)
+                page = table[r, k // cache.shape[1]].long()
+                x = torch.tensor([score(r, i if cache is s.kv else -1 - i) for i in at], device=DEV, dtype=s.dtype)
+                cache[page[page >= 0], (k % cache.shape[1])[page >= 0], 0] = x[page >= 0]
+    return s
+
+
+@pytest.mark.parametrize("D,H,lens,kw,low,high", [
+    (64, 4, [(40, 3), (9, 1)], {"window": 1, "ratio": 8}, -90, -47), (576, 64, [(100, 300)], {"window": 2, "ratio": 4}, -90, -47),
+    (128, 64, [(100, 1600)], {"window": 1, "ratio": 16}, -90, -47), (512, 16, [(70, 2)], {"window": 3, "ratio": 4}, -89, -45.5),
+    (256, 8, [(50, 1)], {"window": 1, "ratio": 8}, -94, -86.5), (32, 8, [(20, 1)], {"window": 1, "ratio": 8}, -87, -87),
+    (64, 4, [(6000, 1)], {}, -130, -86), (576, 16, [(9000, 2)], {}, -128, -85),
+])
+def test_attn_small_beside_the_sink(D, H, lens, kw, low, high):
+    """Scores that begin far below the sink and rise by less than moves the reference: their weights are in fp32's range, whole
+    and joined, the difference of the first one from the sink is not."""
+    s = Step(lens, H, D, **kw)
+    end = lens[0][0] + lens[0][1]
+    scored(s, (lambda r, k: low if k >= 0 else high) if kw else lambda r, k: low + (high - low) * k / end)
+    t = torch.arange(s.N)
+    o, lse = s.run(softmax_scale=1.0)
+    s.check((o, lse), scale=1.0, skip=set(t[(t % 17 != 5) & (s.N > 200)].tolist()))
+    assert o.any(-1).all()
+
+
+@pytest.mark.parametrize("D,H,lens", [(64, 16, [(70, 3), (0, 2)]), (576, 64, [(5000, 1)]), (128, 64, [(40, 1600)])])
+@pytest.mark.parametrize("power", [-80, 90])
+def test_attn_small_and_large_values(D, H, lens, power):
+    """bf16 rows of about 2^power, with queries that bring their scores back to some."""
+    s = Step(lens, H, D)
+    s.kv *= 2.0**power
+    s.q *= 2.0**-power
+    t = torch.arange(s.N)
+    s.check(s.run(), skip=set(t[(t % 17 != 5) & (s.N > 200)].tolist()))
