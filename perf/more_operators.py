@@ -335,19 +335,19 @@ def _attn_plain(s):
 def run(s):
     c = s["case"]
     if own:
-        from streamindex_amd import norm_rotary, paged_attn_q_fwd, paged_write_q, rotary
+        import streamindex_amd as si
 
         if c["op"] == "rotary":
-            y = rotary(s["x"], s["pos"], s["freqs"], interleaved=not c["halves"], magnitude=s["magnitude"])
+            y = si.rotary(s["x"], s["pos"], s["freqs"], interleaved=not c["halves"], magnitude=s["magnitude"])
             return [y.detach(), *torch.autograd.grad(y, [s["x"]], s["dy"])] if c["train"] else y
         if c["op"] == "norm":
-            y = norm_rotary(s["x"], s["pos"], s["freqs"], s["weight"], eps=EPS, interleaved=not c["halves"], magnitude=s["magnitude"])
+            y = si.norm_rotary(s["x"], s["pos"], s["freqs"], s["weight"], eps=EPS, interleaved=not c["halves"], magnitude=s["magnitude"])
             leaves = [s["x"], s["weight"]] if c["weight"] else [s["x"]]
             return [y.detach(), *torch.autograd.grad(y, leaves, s["dy"])] if c["train"] else y
         if c["op"] == "write":
-            return list(paged_write_q(s["new"], s["codes"][:-1], s["scales"][:-1], s["slots"]))
+            return list(si.paged_write_q(s["new"], s["codes"][:-1], s["scales"][:-1], s["slots"]))
         more = {"kv2_cache": s["kv2"], "kv2_scales": s["scales2"], "block_table2": s["table2"], "ratio": c["ratio"]} if c["ratio"] else {}
-        return list(paged_attn_q_fwd(s["q"], s["kv"], s["scales"], s["table"], s["cu"], s["lens"], s["sink"], window=c["window"] or None, **more))
+        return list(si.paged_attn_q_fwd(s["q"], s["kv"], s["scales"], s["table"], s["cu"], s["lens"], s["sink"], window=c["window"] or None, **more))
     return {"norm": _norm_plain, "rotary": _rotary_plain, "write": _write_plain, "attn": _attn_plain}[c["op"]](s)
 
 
