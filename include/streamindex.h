@@ -501,6 +501,36 @@ int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* kv, c
                       int64_t scratch_bytes, void* stream);
 
 /*
+ * Norm and rotation of the rows x [T, H, D] (x_strides: token and head, in
+ * elements; the last dimension contiguous); no counterpart in the reference.
+ * norm: z = x (mean(x^2) + eps)^-1/2 weight (weight [D] fp32, NULL: ones), else
+ * z = x.  Then the pairs (a, b) of dimensions start .. start + 2 pairs - 1,
+ * neighbours or, with halves, (i, i + pairs), are turned by the angle
+ * t = p freqs[i]: m (a cos t - b sin t, a sin t + b cos t), m = magnitude,
+ * -t with inverse.  p of token t is positions[t % npos] (int32, or int64 with
+ * pos64), freqs [pairs] fp64 in radians; pairs 0: none.  y [T, H, D] contiguous.
+ * dtype 0 = fp32, 1 = bf16, 2 = fp16; D <= 1024.
+ */
+int si_norm_rotary(const void* x, const int64_t* x_strides, int norm, const float* weight, float eps,
+                   const void* positions, int pos64, int64_t npos, const double* freqs, int64_t pairs, int64_t start,
+                   int halves, float magnitude, int inverse, int64_t T, int64_t H, int64_t D, int dtype, void* y,
+                   void* stream);
+
+/*
+ * Gradients of si_norm_rotary with norm: dx [T, H, D] contiguous and, unless
+ * NULL, dweight [D] fp32 (with or without a weight), for which workspace holds
+ * at least si_norm_rotary_bwd_workspace_bytes(...) bytes; the same bits every
+ * time.  The gradient of the rotation alone is si_norm_rotary without norm and
+ * with inverse the other way round.
+ */
+int64_t si_norm_rotary_bwd_workspace_bytes(int64_t T, int64_t H, int64_t D, int64_t pairs);
+int si_norm_rotary_bwd(const void* dy, const int64_t* dy_strides, const void* x, const int64_t* x_strides,
+                       const float* weight, float eps, const void* positions, int pos64, int64_t npos,
+                       const double* freqs, int64_t pairs, int64_t start, int halves, float magnitude, int inverse,
+                       int64_t T, int64_t H, int64_t D, int dtype, void* dx, float* dweight, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/*
  * Synthetic inputs for benchmarks and tests (no counterpart in the reference,
  * whose harnesses draw with torch.randn on a CUDA generator,
  * eval/test_v4_indexer_parity.py:89-103): out[i] = N(0,1)[seed, stream, i]

@@ -16,7 +16,9 @@ Operators (hand-written HIP kernels behind the C ABI in
 * :func:`flash_hca_forward`, :func:`build_hca_topk_idxs` — HCA (window + every
   legal compressed entry);
 * :func:`paged_plan`, :func:`paged_write`, :func:`paged_compress`, :func:`paged_attn_fwd` — serving steps over a paged
-  cache, and :func:`flash_hca_paged_forward`, an HCA layer of them.
+  cache, and :func:`flash_hca_paged_forward`, an HCA layer of them;
+* :func:`rotary`, :func:`norm_rotary` — rotary positions of the heads' rows, alone and behind their norm, with gradients, and
+  :func:`rotary_freqs`.
 
 The same names are importable under the reference's module paths through the
 ``flash_sparse`` package (``flash_sparse.triton.chunked_indexer`` etc.).
@@ -28,6 +30,7 @@ from .sparse_attn import (build_inverted_topk, sparse_attn, sparse_attn_bwd, spa
                           sparse_attn_fwd_kv2, sparse_attn_kv2)
 from .csa import build_csa_topk_idxs, csa_topk_idxs, flash_csa_forward
 from .hca import build_hca_topk_idxs, flash_hca_forward, flash_hca_paged_forward
+from .rotary import norm_rotary, rotary, rotary_freqs
 from .paged import PagedPlan, paged_attn_fwd, paged_compress, paged_plan, paged_write
 
 __version__ = "0.1.0"
@@ -51,6 +54,9 @@ __all__ = [
     "paged_compress",
     "paged_attn_fwd",
     "flash_hca_paged_forward",
+    "rotary",
+    "norm_rotary",
+    "rotary_freqs",
     "flash_csa_forward",
     "build_csa_topk_idxs",
     "csa_topk_idxs",

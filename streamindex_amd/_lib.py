@@ -91,6 +91,11 @@ SIGNATURES = {
     "si_paged_attn_fwd": (_I32, [_P, _I64P, _P, _I64P, _I64, _I64, _P, _I64, _I64, _P, _I64P, _I64, _I64, _P, _I64, _I64,
                                  _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, ctypes.c_float, _I32,
                                  _P, _P, _P, _I64, _P]),
+    "si_norm_rotary": (_I32, [_P, _I64P, _I32, _P, ctypes.c_float, _P, _I32, _I64, _P, _I64, _I64, _I32, ctypes.c_float, _I32,
+                              _I64, _I64, _I64, _I32, _P, _P]),
+    "si_norm_rotary_bwd_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
+    "si_norm_rotary_bwd": (_I32, [_P, _I64P, _P, _I64P, _P, ctypes.c_float, _P, _I32, _I64, _P, _I64, _I64, _I32,
+                                  ctypes.c_float, _I32, _I64, _I64, _I64, _I32, _P, _P, _P, _I64, _P]),
     "si_fill_normal": (_I32, [_P, _I32, _I64, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_float, _P]),
     "si_sparse_attn_bwd_noalloc_scratch_bytes": (_I64, []),
     "si_sparse_attn_bwd_noalloc": (_I32, [_P, _I64P, _P, _I64P, _P, _P, _I32, _I64P, _P, _I64P, _P, _I64P, _P, _I64P,

@@ -1,0 +1,178 @@
+"""Rotary positions of the heads' rows, alone and behind their norm, on MI355X (gfx950 HIP kernels via the C ABI).
+
+Queries and keys come to the attention "RoPE-rotated" (``flash_sparse/csa.py:184``), as the reference's operators take them:
+
+* :func:`rotary` — the rotation, of neighbouring dimensions or of halves, of the whole head or a part of it;
+* :func:`norm_rotary` — each head's row over its root mean square, by a weight, then the rotation, in one pass;
+* :func:`rotary_freqs` — the frequencies, stretched for long contexts or not.
+
+Both have gradients, in x and the weight.  Angles are 64-bit, everything else fp32, rounded once to x's type.  The reference has
+no counterpart.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .quant import _dtype_code
+from .sparse_attn import _check_device
+
+__all__ = ["rotary", "norm_rotary", "rotary_freqs"]
+
+MOST_D = 1024
+
+
+def rotary_freqs(dims: int, base: float = 10000.0, *, factor: float = 1.0, original_length: int = 4096, fast: float = 32.0,
+                 slow: float = 1.0, device="cuda") -> torch.Tensor:
+    """Radians a position of each pair, ``base ** (-2 i / dims)``, ``[dims / 2]`` fp64.
+
+    ``factor > 1`` stretches a context of ``original_length`` tokens: pairs that turn fewer than ``slow`` times in it are
+    divided by ``factor``, those that turn more than ``fast`` times stay, and between them the share goes in a straight line
+    over the pairs.
+    """
+    if dims < 0 or dims % 2 or base <= 0 or factor < 1 or original_length < 1 or not fast > slow > 0:
+        raise ValueError(f"bad frequencies: dims={dims}, base={base}, factor={factor}, original_length={original_length}, "
+                         f"fast={fast}, slow={slow}")
+    f = [base ** (-2.0 * i / dims) for i in range(dims // 2)]
+    if factor > 1 and base > 1:
+        def pair(turns):  # that turns so often in original_length
+            return dims * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dims - 1)
+        share = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(dims // 2)]
+        f = [x * (1 - s) + x / factor * s for x, s in zip(f, share)]
+    return torch.tensor(f, dtype=torch.float64, device=device)
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *, interleaved: bool = True,
+           start: Optional[int] = None, magnitude: float = 1.0, inverse: bool = False) -> torch.Tensor:
+    """Rotates pairs of dimensions of every head by the token's position: with t = position * freqs[i],
+    ``(a, b) -> magnitude * (a cos t - b sin t, a sin t + b cos t)``.
+
+    Args:
+      x: ``[..., H, D]`` fp32, bf16 or fp16, ``D <= 1024``.
+      positions: int32 or int64, the sizes of x in front of the heads or the last of them (``[S]`` for ``[B, S, H, D]``);
+        negative ones turn backwards.
+      freqs: ``[dims / 2]`` radians a position (:func:`rotary_freqs`; fp32 ones are taken as they are, in 64 bits).
+      interleaved: pairs of neighbours ``(2i, 2i + 1)`` (True) or of halves ``(i, i + dims / 2)``.
+      start: the first of the ``dims`` rotary dimensions, those before and behind stay (default: the last of the head).
+      magnitude: of the rotary dimensions, as stretched contexts scale them.
+      inverse: turn the other way, as attention outputs are turned back.
+    Returns a new tensor of x's type and shape.  Gradient in x.
+    """
+    return _apply(x, positions, freqs, None, None, interleaved, start, magnitude, inverse)
+
+
+def norm_rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, weight: Optional[torch.Tensor] = None, *,
+                eps: float = 1e-6, interleaved: bool = True, start: Optional[int] = None, magnitude: float = 1.0,
+                inverse: bool = False) -> torch.Tensor:
+    """``rotary(x * (mean(x ** 2) + eps) ** -0.5 * weight, ...)``, the mean over each head's D, in one pass.
+
+    ``weight``: ``[D]``, None for ones; the other arguments are :func:`rotary`'s.  Gradients in x and the weight (the same
+    bits every time).
+    """
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    return _apply(x, positions, freqs, weight, float(eps), interleaved, start, magnitude, inverse)
+
+
+def _apply(x, positions, freqs, weight, eps, interleaved, start, magnitude, inverse):
+    assert x.is_cuda, "x must be on the GPU"
+    _check_device(x.device, positions=positions, freqs=freqs, weight=weight)
+    dt = _dtype_code(x)
+    lead, D = x.dim() - 2, x.shape[-1] if x.dim() else 0
+    if lead < 0:
+        raise ValueError(f"x must be [..., H, D], got {list(x.shape)}")
+    if freqs.dim() != 1 or not freqs.dtype.is_floating_point or freqs.requires_grad:
+        raise ValueError("freqs must be [dims / 2] floating point without gradient")
+    pairs = freqs.shape[0]
+    at = D - 2 * pairs if start is None else start
+    if D < 1 or D > MOST_D or at < 0 or at + 2 * pairs > D:
+        raise ValueError(f"the head needs 1 to {MOST_D} dimensions and the rotary ones within it, got {D} and {at} to {at + 2 * pairs}")
+    n = positions.dim()
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    if n > lead or positions.shape != x.shape[lead - n:lead]:
+        raise ValueError(f"positions must be {list(x.shape[:lead])} or its last sizes, got {list(positions.shape)}")
+    if weight is not None and weight.shape != (D,):
+        raise ValueError(f"weight must be [{D}], got {list(weight.shape)}")
+    positions = positions if positions.is_contiguous() else positions.contiguous()
+    freqs = freqs if freqs.dtype is torch.float64 and freqs.is_contiguous() else freqs.double().contiguous()
+    args = (eps, not interleaved, at, float(magnitude), bool(inverse), dt)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)):
+        return _RotaryFunc.apply(x, weight, positions, freqs, args)
+    return _forward(x, weight, positions, freqs, args)
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """``[T, H, D]`` with a contiguous last dimension: a view where there is one."""
+    x = x.reshape(-1, *x.shape[-2:]) if x.dim() != 3 else x
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _fp32(weight: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if weight is None:
+        return None
+    w = weight if weight.dtype is torch.float32 else weight.float()
+    return w if w.is_contiguous() else w.contiguous()
+
+
+def _forward(x, weight, positions, freqs, args):
+    eps, halves, start, magnitude, inverse, dt = args
+    dev = x.device
+    L = _lib.load()
+    with _lib.on_device(dev):
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        if x.numel() == 0:
+            return y
+        rows, w = _rows(x), _fp32(weight)
+        T, H, D = rows.shape
+        rc = L.si_norm_rotary(rows.data_ptr(), _lib.stride_array(rows.stride()), eps is not None, None if w is None else w.data_ptr(),
+                              eps or 0.0, positions.data_ptr(), positions.dtype is torch.int64, positions.numel(), freqs.data_ptr(),
+                              freqs.shape[0], start, halves, magnitude, inverse, T, H, D, dt, y.data_ptr(), _lib.stream_ptr(dev))
+    _lib.check(rc)
+    return y
+
+
+class _RotaryFunc(torch.autograd.Function):
+    """Norm (with ``eps``) and rotation; the backward keeps x for the norm and nothing for the rotation alone."""
+
+    @staticmethod
+    def forward(ctx, x, weight, positions, freqs, args):
+        norm = args[0] is not None
+        ctx.save_for_backward(positions, freqs, *((x, weight) if norm and weight is not None else (x,) if norm else ()))
+        ctx.args = args
+        return _forward(x.detach(), None if weight is None else weight.detach(), positions, freqs, args)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        positions, freqs, *saved = ctx.saved_tensors
+        eps, halves, start, magnitude, inverse, dt = ctx.args
+        if not saved:
+            return _forward(dy, None, positions, freqs, (None, halves, start, magnitude, not inverse, dt)), None, None, None, None
+        x, weight = saved[0], saved[1] if len(saved) > 1 else None
+        need_w = weight is not None and ctx.needs_input_grad[1]
+        dev = x.device
+        L = _lib.load()
+        with _lib.on_device(dev):
+            dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            D = x.shape[-1]
+            dw = torch.empty(D, dtype=torch.float32, device=dev) if need_w else None
+            if x.numel() == 0:
+                return dx, None if dw is None else dw.zero_().to(weight.dtype), None, None, None
+            rows, drows, w = _rows(x), _rows(dy), _fp32(weight)
+            T, H, _ = rows.shape
+            size = L.si_norm_rotary_bwd_workspace_bytes(T, H, D, freqs.shape[0]) if need_w else 0
+            ws = torch.empty(size, dtype=torch.uint8, device=dev) if need_w else None
+            rc = L.si_norm_rotary_bwd(
+                drows.data_ptr(), _lib.stride_array(drows.stride()), rows.data_ptr(), _lib.stride_array(rows.stride()),
+                None if w is None else w.data_ptr(), eps, positions.data_ptr(), positions.dtype is torch.int64, positions.numel(),
+                freqs.data_ptr(), freqs.shape[0], start, halves, magnitude, inverse, T, H, D, dt, dx.data_ptr(),
+                None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(), size, _lib.stream_ptr(dev))
+        _lib.check(rc)
+        return dx, None if dw is None else dw if weight.dtype is torch.float32 else dw.to(weight.dtype), None, None, None
