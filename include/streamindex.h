@@ -501,6 +501,21 @@ int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* kv, c
                       int64_t scratch_bytes, void* stream);
 
 /*
+ * Row t of rows ([n, D], dtype 0 = fp32, 1 = bf16, 2 = fp16, row_stride elements
+ * apart) to slots[t] of a cache in 8 bits: e4m3 codes (page_stride and
+ * slot_stride in bytes) and fp32 scales [pages, page_size / block] (scale_stride
+ * elements a page), one for `block` tokens.  The scale becomes the smallest power
+ * of two, from 2^-64 on, with 448 scale >= |x| for the finite x of the block's new
+ * rows, and no smaller than the one of the block's earlier tokens, those before its
+ * first new row, whose codes are rescaled where it grows.  Slots outside the
+ * cache write nothing; slots are distinct, and a block's rows follow each other
+ * in rising order, as a plan's do (fewer than 64 rows without a slot between).
+ */
+int si_paged_write_q(const void* rows, int64_t row_stride, int dtype, const int64_t* slots, int64_t n, int64_t D,
+                     void* codes, int64_t page_stride, int64_t slot_stride, float* scales, int64_t scale_stride,
+                     int64_t pages, int64_t page_size, int64_t block, void* stream);
+
+/*
  * Norm and rotation of the rows x [T, H, D] (x_strides: token and head, in
  * elements; the last dimension contiguous); no counterpart in the reference.
  * norm: z = x (mean(x^2) + eps)^-1/2 weight (weight [D] fp32, NULL: ones), else
