@@ -516,6 +516,24 @@ int si_paged_write_q(const void* rows, int64_t row_stride, int dtype, const int6
                      int64_t pages, int64_t page_size, int64_t block, void* stream);
 
 /*
+ * si_paged_attn_fwd over caches in 8 bits: kv, kv2 e4m3 codes [pages, page_size,
+ * D] (strides in bytes, multiples of 16) with fp32 scales [pages, page_size /
+ * block] (scale_stride elements a page); an entry is its code times its scale.
+ * q and o are of qkv_dtype.  A code of NaN reaches the rows that see its key and
+ * no others; scales of seen keys are finite.
+ */
+int64_t si_paged_attn_q_fwd_scratch_bytes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys,
+                                          int64_t keys2, int qkv_dtype);
+int si_paged_attn_q_fwd(const void* q, const int64_t* q_strides, const void* kv, const int64_t* kv_strides,
+                        const float* scales, int64_t scale_stride, int64_t block, int64_t pages, int64_t page_size,
+                        const int32_t* block_table, int64_t table_stride, int64_t P, const void* kv2,
+                        const int64_t* kv2_strides, const float* scales2, int64_t scale_stride2, int64_t block2,
+                        int64_t pages2, int64_t page_size2, const int32_t* block_table2, int64_t table_stride2,
+                        int64_t P2, int64_t window, int64_t ratio, const int32_t* cu_q, const int32_t* seq_lens,
+                        const float* attn_sink, int64_t N, int64_t H, int64_t D, int64_t R, float softmax_scale,
+                        int qkv_dtype, void* o, float* lse, void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
  * Norm and rotation of the rows x [T, H, D] (x_strides: token and head, in
  * elements; the last dimension contiguous); no counterpart in the reference.
  * norm: z = x (mean(x^2) + eps)^-1/2 weight (weight [D] fp32, NULL: ones), else

@@ -17,7 +17,7 @@ Operators (hand-written HIP kernels behind the C ABI in
   legal compressed entry);
 * :func:`paged_plan`, :func:`paged_write`, :func:`paged_compress`, :func:`paged_attn_fwd` — serving steps over a paged
   cache, and :func:`flash_hca_paged_forward`, an HCA layer of them;
-* :func:`paged_write_q` — the same over a cache held in 8 bits;
+* :func:`paged_write_q`, :func:`paged_attn_q_fwd` — write and attention over a cache held in 8 bits;
 * :func:`rotary`, :func:`norm_rotary` — rotary positions of the heads' rows, alone and behind their norm, with gradients, and
   :func:`rotary_freqs`.
 
@@ -33,7 +33,7 @@ from .csa import build_csa_topk_idxs, csa_topk_idxs, flash_csa_forward
 from .hca import build_hca_topk_idxs, flash_hca_forward, flash_hca_paged_forward
 from .rotary import norm_rotary, rotary, rotary_freqs
 from .paged import PagedPlan, paged_attn_fwd, paged_compress, paged_plan, paged_write
-from .paged_q import paged_write_q
+from .paged_q import paged_attn_q_fwd, paged_write_q
 
 __version__ = "0.1.0"
 
@@ -56,6 +56,7 @@ __all__ = [
     "paged_write_q",
     "paged_compress",
     "paged_attn_fwd",
+    "paged_attn_q_fwd",
     "flash_hca_paged_forward",
     "rotary",
     "norm_rotary",

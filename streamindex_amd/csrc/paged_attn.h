@@ -7,6 +7,8 @@
 // entries i of its second cache with ratio (i + 1) - 1 <= p.  Keys and values are the same rows, shared by the heads.
 #pragma once
 
+#include <hip/hip_runtime.h>
+
 #include "attn_common.h"
 #include "si_common.h"
 
@@ -46,5 +48,15 @@ struct PagedAttnArgs {
 
 constexpr int kPagedThreads = 256;
 constexpr int kRows = 64;  // (token, head) rows of a workgroup
+
+// Head dims served.
+bool paged_attn_served(int64_t D);
+// Keys that a block table row of P pages can name, at most 2^31 - 1.
+int64_t paged_cache_keys(int64_t pages, int64_t P, int64_t ps);
+// Checks a cache of `size`-byte elements and its block table, and sets c.
+int set_paged_cache(PagedCache& c, int size, const void* base, const int64_t* strides, int64_t pages, int64_t ps, int64_t D,
+                    const int32_t* table, int64_t tstride, int64_t P, int64_t R, const char* name);
+// Joins the shares of the split row blocks, of which there are at most split_blocks.
+int launch_paged_combine(bool f16, const PagedAttnArgs& a, int D, int64_t split_blocks, hipStream_t st);
 
 }  // namespace si

@@ -34,360 +34,10 @@
 #include <string>
 #include <type_traits>
 
-#include "paged_attn.h"
+#include "paged_attn_sched.h"
 #include "si_status.h"
 
 namespace si {
-
-// Keeps a wave-uniform value in scalar registers from here on: a kernel argument fetched again inside the tile loop would
-// be a scalar load in flight among the LDS reads, whose lgkmcnt waits count on completion in order.
-template <typename T>
-__device__ __forceinline__ void scalar_tie(T& x) {
-  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two registers");
-  // (readfirstlane on both sides: the asm needs a scalar, and its result does not count as uniform by itself)
-  auto tied = [](uint32_t w) {
-    w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w)));
-    asm volatile("" : "+s"(w));
-    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(w)));
-  };
-  if constexpr (sizeof(T) == 4) {
-    x = __builtin_bit_cast(T, tied(__builtin_bit_cast(uint32_t, x)));
-  } else {
-    const uint64_t w = __builtin_bit_cast(uint64_t, x);
-    x = __builtin_bit_cast(T, static_cast<uint64_t>(tied(static_cast<uint32_t>(w >> 32))) << 32 | tied(static_cast<uint32_t>(w)));
-  }
-}
-
-// A cache as one workgroup reads it.
-struct CacheView {
-  const int32_t* table;  // the request's row
-  uint32_t ps, rstride, magic, shift, one;
-  __device__ __forceinline__ uint32_t page_of(uint32_t key) const { return (__umulhi(key, magic) + (key & one)) >> shift; }
-};
-struct CacheBase {
-  const char* base;
-  uint32_t pstride, pages;
-};
-// (by value: a choice between two caches stays one between values at hand, not between addresses in memory)
-__device__ __forceinline__ void view_cache(PagedCache c, int req, CacheView& v, CacheBase& b) {
-  v.table = c.table + req * c.tstride;
-  v.ps = c.ps;
-  v.rstride = c.rstride;
-  v.magic = c.magic;
-  v.shift = c.shift;
-  v.one = c.one;
-  b.base = reinterpret_cast<const char*>(c.base);
-  b.pstride = c.pstride;
-  b.pages = static_cast<uint32_t>(c.pages);
-  scalar_tie(v.table);
-  scalar_tie(v.ps);
-  scalar_tie(v.rstride);
-  scalar_tie(v.magic);
-  scalar_tie(v.shift);
-  scalar_tie(v.one);
-  scalar_tie(b.base);
-  scalar_tie(b.pstride);
-  scalar_tie(b.pages);
-}
-template <typename T>
-__device__ __forceinline__ T pick(bool second, T x, T y) {
-  return second ? y : x;
-}
-
-// ---------------------------------------------------------------------------
-// Schedule
-//
-// Request r has blocks(r) = ceil(n_r H / 64) row blocks of about tiles(r) key tiles each.  With U = sum blocks tiles and
-// `want` workgroups at once, a row block is cut into ceil(tiles / c) shares.  c is the cheapest of: no cut, and four steps
-// from U / want up, the last one with which all shares run at once.  The cost is the longest share, in tiles, and 1/24 of a
-// tile for each partial output of 64 rows, its write and read (us: 64 row blocks of 12, 24 and 40 tiles, D = 576, cut in two 27, 35 and
-// 44 and whole 25, 41 and 60; 128 of them 36, 44, 54 and 28, 42, 62; with D = 128, 256 of 24 and 40, 30, 36 and 26, 38).
-// With more row blocks than `want`, c = 2 U / want cuts only requests far longer than the average, which would otherwise
-// end last on their own.
-// Every workgroup does these sums itself, with lane-shift scans in 32 bits, and where there are at most 64 requests every
-// wave, without a barrier (7,149 row blocks: 576 us with the barriers, 555 without).  An ascending cu_q makes the
-// requests' rows disjoint, on which every bound here and the sizes of the partial outputs rest; with one that descends
-// somewhere no request has rows.
-// ---------------------------------------------------------------------------
-struct PagedReq {
-  int first, n, len;  // first row of q, new tokens, entries of the first cache
-  int blocks, tiles;
-  bool down;          // cu_q descends here
-};
-
-__device__ __forceinline__ int ceil_div32(int x) { return static_cast<int>((static_cast<uint32_t>(x) + 31u) >> 5); }
-
-// Keys [lo, hi) of the first cache that a token at position p sees, and entries of the second.  Lengths are taken from 0 on,
-// so positions run from -N to 2^31 - 2 and nothing here leaves 32 bits.
-__device__ __forceinline__ int win_lo(const PagedAttnArgs& a, int p) { return max(max(p + 1, 0) - a.window, 0); }
-__device__ __forceinline__ int win_hi(const PagedAttnArgs& a, int p) { return max(min(p + 1, a.c1.keys), 0); }
-__device__ __forceinline__ int ent_hi(const PagedAttnArgs& a, int p) {
-  if (a.ratio == 0 || p < 0) return 0;
-  return min(static_cast<int>(static_cast<uint32_t>(p + 1) / static_cast<uint32_t>(a.ratio)), a.c2.keys);
-}
-
-__device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& a, int r) {
-  PagedReq q;
-  const int c0 = a.cu[r], c1 = a.cu[r + 1];
-  q.len = max(a.lens[r], 0);
-  q.first = min(max(c0, 0), a.N);
-  q.n = max(min(c1, a.N) - q.first, 0);
-  q.down = c1 < c0;
-  q.blocks = static_cast<int>((static_cast<uint32_t>(q.n) * static_cast<uint32_t>(a.H) + (kRows - 1)) / kRows);
-  // tiles of the last row block, which sees the most
-  const int p = q.len - 1;
-  const int span = max(win_hi(a, p) - win_lo(a, p - a.behind), 0);
-  q.tiles = max(ceil_div32(span) + ceil_div32(ent_hi(a, p)), 1);
-  return q;
-}
-
-struct PagedItem {  // what a workgroup does
-  int first, n, len;  // the request, as PagedReq
-  int req, block, share, shares;
-  int slot;           // its partial output, where shares > 1
-  int rec;            // number of its row block among the split ones
-};
-
-// Inclusive prefix sum over the wave: shifts within rows of 16 lanes, then the rows' last lanes to the rows behind.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
-  return x;
-}
-
-__device__ __forceinline__ int shares_of(int tiles, uint32_t c) {
-  return tiles <= 1 ? 1 : static_cast<int>((static_cast<uint32_t>(tiles) + c - 1) / c);
-}
-
-constexpr uint32_t kWhole = 0x7fffffffu;  // no row block is cut
-
-// Number of this workgroup's item among `total`; `total` and on where it has none.  Consecutive workgroups go to the eight
-// XCDs in turn: each XCD takes runs of up to 32 items, one to a CU, whose keys its L2 then holds once, and all of them the
-// same number, however many of the launched workgroups the lengths leave without an item.  (512 row blocks of 288 tiles, D =
-// 256: runs of 32 319 us, of 64 332, of 16 321.)
-__device__ __forceinline__ int paged_item_number(int total) {
-  const int xcd = blockIdx.x & 7, k = blockIdx.x >> 3;
-  const int whole = total >> 8;  // rounds of 8 x 32
-  if (k < 32 * whole) return ((k >> 5) * 8 + xcd) * 32 + (k & 31);
-  const int rest = total - 256 * whole, run = (rest + 7) >> 3, i = k - 32 * whole;
-  return i < run ? 256 * whole + xcd * run + i : total;
-}
-
-// The sum over the wave, in lane 63.
-__device__ __forceinline__ float wave_sum_last(float x) {
-  auto shifted = [](float v, auto CTRL, auto MASK) {
-    return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
-        0, static_cast<int>(__float_as_uint(v)), decltype(CTRL)::value, decltype(MASK)::value, 0xf, false)));
-  };
-  using std::integral_constant;
-  x += shifted(x, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
-  x += shifted(x, integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
-  x += shifted(x, integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
-  x += shifted(x, integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
-  x += shifted(x, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
-  x += shifted(x, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
-  return x;
-}
-
-// The largest over the wave, in lane 63, of values from 0 on.
-__device__ __forceinline__ int wave_max_last(int x) {
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
-  return max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
-}
-
-constexpr int kSteps = 4;
-constexpr int kLeastTiles = 4;  // of a share at least
-// Tiles of a share: the steps to try, from the sum of blocks x tiles (rounded up: fp32 sums of whole numbers, at most 2^-20
-// too small over the few thousand additions of a call) and the number of row blocks.
-struct ShareSteps {
-  uint32_t step[kSteps];
-  static __device__ __forceinline__ uint32_t tiles_of(float x, int least) {
-    return static_cast<uint32_t>(__builtin_fminf(__builtin_fmaxf(__builtin_ceilf(x), static_cast<float>(least)), 0x1p30f));
-  }
-  __device__ __forceinline__ ShareSteps(float sum, int all, int want) {
-    const float units = sum * (1.0f + 0x1p-16f), each = units / static_cast<float>(want);
-    step[0] = tiles_of(each, kLeastTiles);
-    step[1] = tiles_of(1.25f * each, 6);
-    step[2] = tiles_of(1.5f * each, 8);
-    // (sum of ceil(tiles / c) <= units / c + all <= want)
-    step[3] = tiles_of(__builtin_fmaxf(2.f * each, all < want ? units / static_cast<float>(want - all) : 0.f), 16);
-  }
-  // For all < want row blocks, the longest of `longest` tiles, and items[i] shares with step i: see above.
-  __device__ __forceinline__ uint32_t pick(const int (&items)[kSteps], int all, int longest, const PagedAttnArgs& a) const {
-    uint32_t c = kWhole;
-    float cost = static_cast<float>(longest);
-#pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i) {
-      const int more = items[i] - all, parts = more + min(more, all);  // partial outputs, at most
-      const float x = static_cast<float>(min(static_cast<int>(step[i]), longest)) + static_cast<float>(parts) * a.part_cost;
-      if (items[i] <= a.want && x < cost) {
-        c = step[i];
-        cost = x;
-      }
-    }
-    return c;
-  }
-};
-
-// This workgroup's item, or false.  For up to 64 requests, one to a lane, every wave for itself: no LDS and no barrier.
-__device__ __forceinline__ bool paged_schedule_wave(const PagedAttnArgs& a, PagedItem& it, bool& down) {
-  const int lane = threadIdx.x & 63;
-  PagedReq q{};
-  if (lane < a.R) q = paged_req(a, lane);
-  down = __builtin_amdgcn_ballot_w64(q.down) != 0;
-  if (down) q.blocks = 0;
-  auto last = [](int x) { return __builtin_amdgcn_readlane(x, kWave - 1); };
-  uint32_t c = kWhole;
-  if (a.part_o) {
-    const float sum = wave_sum_last(static_cast<float>(q.blocks) * static_cast<float>(q.tiles));
-    const int all = last(wave_scan(q.blocks)), longest = last(wave_max_last(q.blocks > 0 ? q.tiles : 0));
-    const ShareSteps steps(__uint_as_float(static_cast<uint32_t>(last(static_cast<int>(__float_as_uint(sum))))), all, a.want);
-    c = steps.step[kSteps - 1];
-    if (all < a.want) {
-      int shares[kSteps];
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) shares[i] = last(wave_scan(q.blocks * shares_of(q.tiles, steps.step[i])));
-      c = steps.pick(shares, all, longest, a);
-    }
-  }
-  const int s = shares_of(q.tiles, c);
-  const int items = q.blocks * s, parts = s > 1 ? items : 0, recs = s > 1 ? q.blocks : 0;
-  const int end = wave_scan(items), end_parts = wave_scan(parts), end_recs = wave_scan(recs);
-  if (a.part_o && blockIdx.x == 0 && threadIdx.x == kWave - 1) a.rec[0] = end_recs;
-  const int total = last(end), id = paged_item_number(total);
-  if (id >= total) return false;
-  const int r = __builtin_ctzll(__builtin_amdgcn_ballot_w64(id < end));  // the first request that ends behind it
-  auto at = [&](int x) { return __builtin_amdgcn_readlane(x, r); };
-  const int shares = at(s), k = id - at(end - items), block = k / shares;
-  // (the last row blocks see the most keys: they start first)
-  it = PagedItem{at(q.first), at(q.n), at(q.len), r, at(q.blocks) - 1 - block, k - block * shares, shares,
-                 at(end_parts - parts) + k, at(end_recs - recs) + block};
-  return true;
-}
-
-// The same for any number.  All threads call it.
-__device__ __forceinline__ bool paged_schedule(const PagedAttnArgs& a, PagedItem& it, bool& down) {
-  constexpr int W = kPagedThreads / kWave;
-  __shared__ float units_lds[W];
-  __shared__ int blocks_lds[W], longest_lds[W], items_lds[W][kSteps], sums_lds[3][W];
-  __shared__ PagedItem found;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int per = (a.R + kPagedThreads - 1) / kPagedThreads;
-  const int r0 = min(t * per, a.R), r1 = min(r0 + per, a.R);
-  PagedReq mine{};  // kept where a thread has one request
-  float units = 0.f;
-  int blocks = 0, longest = 0;
-  bool descends = false;
-  for (int r = r0; r < r1; ++r) {
-    mine = paged_req(a, r);
-    units = __builtin_fmaf(static_cast<float>(mine.blocks), static_cast<float>(mine.tiles), units);
-    blocks += mine.blocks;
-    longest = max(longest, mine.blocks > 0 ? mine.tiles : 0);
-    descends = descends || mine.down;
-  }
-  down = __syncthreads_or(descends) != 0;
-  if (down) {
-    if (a.part_o && blockIdx.x == 0 && t == 0) a.rec[0] = 0;
-    return false;
-  }
-  auto req = [&](int r) { return per == 1 ? mine : paged_req(a, r); };
-  uint32_t c = kWhole;  // tiles of a share
-  if (a.part_o) {
-    units = wave_sum_last(units);
-    blocks = wave_scan(blocks);
-    longest = wave_max_last(longest);
-    if (lane == kWave - 1) {
-      units_lds[wave] = units;
-      blocks_lds[wave] = blocks;
-      longest_lds[wave] = longest;
-    }
-    __syncthreads();
-    const int all = (blocks_lds[0] + blocks_lds[1]) + (blocks_lds[2] + blocks_lds[3]);
-    longest = max(max(longest_lds[0], longest_lds[1]), max(longest_lds[2], longest_lds[3]));
-    const ShareSteps steps((units_lds[0] + units_lds[1]) + (units_lds[2] + units_lds[3]), all, a.want);
-    c = steps.step[kSteps - 1];
-    if (all < a.want) {
-      int n[kSteps] = {};
-      for (int r = r0; r < r1; ++r) {
-        const PagedReq q = req(r);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) n[i] += q.blocks * shares_of(q.tiles, steps.step[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        n[i] = wave_scan(n[i]);
-        if (lane == kWave - 1) items_lds[wave][i] = n[i];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) n[i] = (items_lds[0][i] + items_lds[1][i]) + (items_lds[2][i] + items_lds[3][i]);
-      c = steps.pick(n, all, longest, a);
-    }
-  }
-  int items = 0, parts = 0, recs = 0;
-  for (int r = r0; r < r1; ++r) {
-    const PagedReq q = req(r);
-    const int s = shares_of(q.tiles, c);
-    items += q.blocks * s;
-    if (s > 1) {
-      parts += q.blocks * s;
-      recs += q.blocks;
-    }
-  }
-  int before[3];
-  const int x3[3] = {items, parts, recs};
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const int v = wave_scan(x3[i]);
-    if (lane == kWave - 1) sums_lds[i][wave] = v;
-    before[i] = v - x3[i];
-  }
-  __syncthreads();
-  int total[3];
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    total[i] = 0;
-#pragma unroll
-    for (int w = 0; w < kPagedThreads / kWave; ++w) {
-      if (w < wave) before[i] += sums_lds[i][w];
-      total[i] += sums_lds[i][w];
-    }
-  }
-  if (a.part_o && blockIdx.x == 0 && t == 0) a.rec[0] = total[2];
-  const int id = paged_item_number(total[0]);
-  if (id >= total[0]) return false;
-  if (before[0] <= id && id < before[0] + items) {
-    int at = before[0], part0 = before[1], rec0 = before[2];
-    for (int r = r0; r < r1; ++r) {
-      const PagedReq q = req(r);
-      const int s = shares_of(q.tiles, c);
-      const int n = q.blocks * s;
-      if (id < at + n) {
-        const int k = id - at;
-        const int block = k / s;
-        // (the last row blocks see the most keys: they start first)
-        found = PagedItem{q.first, q.n, q.len, r, q.blocks - 1 - block, k - block * s, s, part0 + k, rec0 + block};
-        break;
-      }
-      at += n;
-      if (s > 1) {
-        part0 += n;
-        rec0 += q.blocks;
-      }
-    }
-  }
-  __syncthreads();
-  it = found;
-  return true;
-}
 
 // Resident workgroups of a CU: LDS sets them, and Q^T and O^T take 216 registers of a wave at D = 576, 96 at D = 256.
 constexpr int per_cu(int D, bool PAIR) { return (D >= 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4) + (PAIR ? 1 : 0); }
@@ -396,18 +46,6 @@ constexpr int per_cu(int D, bool PAIR) { return (D >= 512 ? 1 : D == 256 ? 2 : D
 // 933 and 982, 58 and 65, 4,096 2,755 and 2,926, 144 and 162; D = 128, 1,536 653 and 644, 41 and 43, 2,048 842 and 877, 50 and
 // 54; D = 64, 4,096 1,150 and 1,113, 63 and 67).
 constexpr int64_t pair_from(int64_t D) { return D >= 512 ? 257 : D == 256 ? 1025 : D == 128 ? 1537 : INT64_MAX; }
-
-constexpr float kNever = -__builtin_inff();
-// A sink in log2 units: finite where it outweighs everything (inf - inf would follow).  Finite ones below the range become
-// -inf, which weighs the same, nothing, beside a key, and a row whose keys weigh nothing takes its lse from the sink itself.
-__device__ __forceinline__ float sink_log2(float sink) {
-  constexpr float kMost = 3.4028234663852886e38f;
-  const float x = sink * 1.4426950408889634f;
-  return x > kMost ? kMost : x;  // (NaN stays)
-}
-__device__ __forceinline__ float lse_of_sink(float sink) { return sink == kNever ? -1.0e30f : sink; }
-constexpr int kOdd = 1;    // a masked score that is not finite
-constexpr int kMoved = 2;  // a reference maximum has moved: alpha is not one
 
 // x with infinities and NaN replaced by zero.
 template <bool F16>
@@ -449,7 +87,7 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   int begin = a.R > 0 ? min(max(a.cu[0], 0), a.N) : 0, end = a.R > 0 ? min(max(a.cu[a.R], 0), a.N) : 0;
   PagedItem item;
   bool down;
-  const bool work = a.R <= kWave ? paged_schedule_wave(a, item, down) : paged_schedule(a, item, down);
+  const bool work = a.R <= kWave ? paged_schedule_wave<kAttnTK>(a, item, down) : paged_schedule<kAttnTK>(a, item, down);
   if (down) begin = end = 0;
   // Rows of no request: as a row without a key.
   for (int64_t i = blockIdx.x; i < begin + static_cast<int64_t>(a.N - end); i += gridDim.x) {
@@ -480,8 +118,8 @@ __global__ __launch_bounds__(kPagedThreads, per_cu(D, PAIR)) void paged_attn_ker
   // tiles of this row block: the window's, then the second cache's; and this share of them
   const int k1lo = win_lo(a, pa), k1hi = win_hi(a, pb);
   const int k2hi = ent_hi(a, pb);
-  const int n1 = k1hi > k1lo ? ceil_div32(k1hi - k1lo) : 0;
-  const int ntiles = n1 + ceil_div32(k2hi);
+  const int n1 = k1hi > k1lo ? key_tiles<kAttnTK>(k1hi - k1lo) : 0;
+  const int ntiles = n1 + key_tiles<kAttnTK>(k2hi);
   const int tbeg = static_cast<int>(static_cast<int64_t>(ntiles) * share / shares);
   const int tend = static_cast<int>(static_cast<int64_t>(ntiles) * (share + 1) / shares);
 
@@ -1191,7 +829,18 @@ __global__ __launch_bounds__(kPagedThreads) void paged_combine_kernel(PagedAttnA
   }
 }
 
-static bool served(int64_t D) { return D == 32 || D == 64 || D == 128 || D == 256 || D == 512 || D == 576; }
+int launch_paged_combine(bool f16, const PagedAttnArgs& a, int D, int64_t split_blocks, hipStream_t st) {
+  // One thread a place, or up to four for blocks of many shares where the workgroups that others leave idle are few (us, 2
+  // shares, D = 576: 24 blocks 5.2 with them and 4.3 without, 33 blocks 6.4 and 4.5; but 32 blocks of up to 59 shares, D = 128, 6
+  // and 12).
+  const bool wide = D / 16 * kCombineParts * split_blocks < 4096;
+  const dim3 block(kPagedThreads), cgrid(static_cast<unsigned>(D / 16 * (wide ? kCombineParts : 1)), static_cast<unsigned>(split_blocks));
+  if (f16) hipLaunchKernelGGL(paged_combine_kernel<true>, cgrid, block, 0, st, a, D);
+  else hipLaunchKernelGGL(paged_combine_kernel<false>, cgrid, block, 0, st, a, D);
+  return check_launch("paged_combine_kernel");
+}
+
+bool paged_attn_served(int64_t D) { return D == 32 || D == 64 || D == 128 || D == 256 || D == 512 || D == 576; }
 
 // Sizes of a call, from what the host knows.
 struct PagedSizes {
@@ -1255,37 +904,16 @@ static int launch_paged_attn_d(bool f16, const PagedAttnArgs& a, const PagedSize
   }
   const int rc = check_launch("paged_attn_kernel");
   if (rc || !a.part_o) return rc;
-  // One thread a place, or up to four for blocks of many shares where the workgroups that others leave idle are few (us, 2
-  // shares, D = 576: 24 blocks 5.2 with them and 4.3 without, 33 blocks 6.4 and 4.5; but 32 blocks of up to 59 shares, D = 128, 6
-  // and 12).
-  const bool wide = D / 16 * kCombineParts * p.split_blocks < 4096;
-  const dim3 cgrid(static_cast<unsigned>(D / 16 * (wide ? kCombineParts : 1)), static_cast<unsigned>(p.split_blocks));
-  if (f16) hipLaunchKernelGGL(paged_combine_kernel<true>, cgrid, block, 0, st, a, D);
-  else hipLaunchKernelGGL(paged_combine_kernel<false>, cgrid, block, 0, st, a, D);
-  return check_launch("paged_combine_kernel");
+  return launch_paged_combine(f16, a, D, p.split_blocks, st);
 }
 
-}  // namespace si
-
-using namespace si;
-
-static int64_t cache_keys(int64_t pages, int64_t P, int64_t ps) {
+int64_t paged_cache_keys(int64_t pages, int64_t P, int64_t ps) {
   const int64_t k = pages > 0 ? P * ps : 0;
   return k < 0x7fffffff ? k : 0x7fffffff;
 }
 
-extern "C" int64_t si_paged_attn_fwd_scratch_bytes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window,
-                                                   int64_t keys, int64_t keys2) {
-  const int64_t lim = 0x7fffffff;
-  if (N <= 0 || H <= 0 || R <= 0 || window < 0 || keys < 0 || keys2 < 0 || !served(D) || N > lim || H > lim ||
-      N * H > lim || R > lim)
-    return 0;
-  return paged_sizes(N, H, D, R, window == 0 || window > lim ? lim : window, keys < lim ? keys : lim,
-                       keys2 < lim ? keys2 : lim).bytes;
-}
-
-static int set_cache(PagedCache& c, const void* base, const int64_t* strides, int64_t pages, int64_t ps, int64_t D,
-                     const int32_t* table, int64_t tstride, int64_t P, int64_t R, const char* name) {
+int set_paged_cache(PagedCache& c, int size, const void* base, const int64_t* strides, int64_t pages, int64_t ps, int64_t D,
+                    const int32_t* table, int64_t tstride, int64_t P, int64_t R, const char* name) {
   const std::string n(name);
   if (!strides) return set_error(SI_ERR_INVALID, n + ": null stride argument");
   if (pages < 0 || ps <= 0 || P < 0) return set_error(SI_ERR_INVALID, n + ": bad dimension");
@@ -1293,11 +921,11 @@ static int set_cache(PagedCache& c, const void* base, const int64_t* strides, in
   if (R == 0) P = 0;
   if (pages > 0 && P > 0 && (!base || !table)) return set_error(SI_ERR_INVALID, n + ": null pointer argument");
   if (R > 1 && tstride < 0) return set_error(SI_ERR_INVALID, n + ": negative block table stride");
-  if (strides[2] != 1 || strides[0] < 0 || strides[1] < 0 || (strides[0] | strides[1]) % 8 ||
+  if (strides[2] != 1 || strides[0] < 0 || strides[1] < 0 || (strides[0] | strides[1]) % (16 / size) ||
       (reinterpret_cast<uintptr_t>(base) & 15))
     return set_error(SI_ERR_INVALID, n + " needs a contiguous last dimension, 16-byte rows and alignment");
   // (each factor below 2^31: no product overflows 64 bits before it is compared)
-  const int64_t lim = int64_t{1} << 35;  // 64 GiB in elements
+  const int64_t lim = (int64_t{1} << 36) / size;  // 64 GiB in elements
   if (pages > 0 && (strides[0] >= lim || strides[1] >= lim || (pages - 1) > (lim - 1) / (strides[0] > 0 ? strides[0] : 1) ||
                     (ps - 1) > (lim - 1) / (strides[1] > 0 ? strides[1] : 1) ||
                     (pages - 1) * strides[0] + (ps - 1) * strides[1] + D > lim))
@@ -1305,10 +933,10 @@ static int set_cache(PagedCache& c, const void* base, const int64_t* strides, in
   c.base = static_cast<const uint16_t*>(base);
   c.table = table;
   c.tstride = tstride;
-  c.pstride = static_cast<uint32_t>(strides[0] / 8);
-  c.rstride = static_cast<uint32_t>(strides[1] / 8);
+  c.pstride = static_cast<uint32_t>(strides[0] / (16 / size));
+  c.rstride = static_cast<uint32_t>(strides[1] / (16 / size));
   c.pages = P > 0 ? static_cast<int>(pages) : 0;
-  c.keys = static_cast<int>(cache_keys(pages, P, ps));
+  c.keys = static_cast<int>(paged_cache_keys(pages, P, ps));
   c.ps = static_cast<uint32_t>(ps);
   c.magic = 0;
   c.shift = 0;
@@ -1324,6 +952,20 @@ static int set_cache(PagedCache& c, const void* base, const int64_t* strides, in
   return SI_OK;
 }
 
+}  // namespace si
+
+using namespace si;
+
+extern "C" int64_t si_paged_attn_fwd_scratch_bytes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window,
+                                                   int64_t keys, int64_t keys2) {
+  const int64_t lim = 0x7fffffff;
+  if (N <= 0 || H <= 0 || R <= 0 || window < 0 || keys < 0 || keys2 < 0 || !paged_attn_served(D) || N > lim || H > lim ||
+      N * H > lim || R > lim)
+    return 0;
+  return paged_sizes(N, H, D, R, window == 0 || window > lim ? lim : window, keys < lim ? keys : lim,
+                       keys2 < lim ? keys2 : lim).bytes;
+}
+
 extern "C" int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* kv, const int64_t* kv_strides,
                                  int64_t pages, int64_t page_size, const int32_t* block_table, int64_t table_stride,
                                  int64_t P, const void* kv2, const int64_t* kv2_strides, int64_t pages2,
@@ -1335,7 +977,7 @@ extern "C" int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const 
   if (qkv_dtype != SI_DTYPE_BF16 && qkv_dtype != SI_DTYPE_F16)
     return set_error(SI_ERR_INVALID, "qkv_dtype must be SI_DTYPE_BF16 (0) or SI_DTYPE_F16 (1)");
   if (N < 0 || H <= 0 || D <= 0 || R < 0 || window < 0 || ratio < 0) return set_error(SI_ERR_INVALID, "bad dimension");
-  if (!served(D))
+  if (!paged_attn_served(D))
     return set_error(SI_ERR_UNSUPPORTED,
                      "unsupported head dim D=" + std::to_string(D) + " (supported: 32, 64, 128, 256, 512, 576)");
   if (N > 0x7fffffff || H > 0x7fffffff || R > 0x7fffffff || N * H > 0x7fffffff || ratio > 0x7fffffff)
@@ -1350,10 +992,10 @@ extern "C" int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const 
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(scratch)) & 15)
     return set_error(SI_ERR_INVALID, "q, o and scratch must be 16-byte aligned");
   PagedAttnArgs a{};
-  int rc = set_cache(a.c1, kv, kv_strides, pages, page_size, D, block_table, table_stride, P, R, "kv");
+  int rc = set_paged_cache(a.c1, 2, kv, kv_strides, pages, page_size, D, block_table, table_stride, P, R, "kv");
   if (rc) return rc;
   if (ratio > 0) {
-    rc = set_cache(a.c2, kv2, kv2_strides, pages2, page_size2, D, block_table2, table_stride2, P2, R, "kv2");
+    rc = set_paged_cache(a.c2, 2, kv2, kv2_strides, pages2, page_size2, D, block_table2, table_stride2, P2, R, "kv2");
     if (rc) return rc;
   }
   if (N == 0) return SI_OK;
@@ -1371,8 +1013,8 @@ extern "C" int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const 
   a.H = static_cast<int>(H);
   a.R = static_cast<int>(R);
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  PagedSizes p = paged_sizes(N, H, D, R > 0 ? R : 1, a.window, cache_keys(pages, P, page_size),
-                             ratio > 0 ? cache_keys(pages2, P2, page_size2) : 0);
+  PagedSizes p = paged_sizes(N, H, D, R > 0 ? R : 1, a.window, paged_cache_keys(pages, P, page_size),
+                             ratio > 0 ? paged_cache_keys(pages2, P2, page_size2) : 0);
   a.want = static_cast<int>(p.want);
   a.behind = p.behind;
   a.part_cost = static_cast<float>(N * H) / (24.f * kRows * static_cast<float>(p.blocks));
