@@ -23,8 +23,6 @@
 
 namespace si {
 
-constexpr int kQTile = 64;  // keys of a tile
-
 // Scales of a cache: [pages, keys of a page / block].
 struct QScales {
   const float* base;
@@ -40,22 +38,26 @@ struct PagedAttnQArgs {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
-template <int D, bool F16>
+// PAIR: tiles of 32 keys, a tile's steps one after the other, and one workgroup more a CU, which fills the gaps.
+template <int D, bool F16, bool PAIR>
 struct QShape {
+  static constexpr int TK = PAIR ? 32 : 64;      // keys of a tile
   static constexpr int CPR = D / 16;             // 16-byte chunks of a key row
   static constexpr int ROW = D;                  // bytes
-  static constexpr int TILE = kQTile * ROW;
-  static constexpr int WAVES = D == 32 ? 2 : 4;  // that copy a tile, KPW keys each
-  static constexpr int KPW = kQTile / WAVES;
-  static constexpr int LPT = KPW * CPR / 64;     // copies of such a wave
+  static constexpr int TILE = TK * ROW;
+  static constexpr int CH = TK * CPR;            // chunks of a tile
+  static constexpr int LPT = (CH + kPagedThreads - 1) / kPagedThreads;  // copies of a thread
+  static constexpr int LANDED = CH / kPagedThreads;                     // of every thread
   static constexpr int NG = D / 64;              // whole groups of 64 dimensions
-  static constexpr int PP = F16 ? 2 : 1;         // of P
+  static constexpr int PP = F16 ? 2 : 1;         // pieces of P
   static constexpr int MBT = D / 16;             // 16-dim output blocks
   static constexpr int MBW = (MBT + 3) / 4;      // per wave
-  static constexpr int NS = D == 512 && !F16 ? 4 : 3;  // tiles in LDS
+  static constexpr int NS = D == 512 && !F16 && !PAIR ? 4 : 3;  // tiles in LDS
 };
-// Workgroups of a CU: LDS sets them.
-constexpr int q_per_cu(int D, bool F16) { return D >= 512 ? 1 : D == 256 ? (F16 ? 1 : 2) : D == 128 ? (F16 ? 2 : 3) : F16 ? 3 : 4; }
+// Workgroups of a CU: LDS and registers set them.
+constexpr int q_per_cu(int D, bool F16, bool PAIR) {
+  return PAIR ? 2 : D >= 512 ? 1 : D == 256 ? (F16 ? 1 : 2) : D == 128 ? (F16 ? 2 : 3) : F16 ? 3 : 4;
+}
 
 // Chunk c of key k is stored at c ^ q_swz(k), so that both reads of a tile spread over the banks: 16 keys 16 mb + 0 .. 15 at one
 // chunk (S^T), and keys 4 g + 0 .. 3 and 16 + 4 g + 0 .. 3 at one chunk (V^T).
@@ -63,7 +65,7 @@ template <int D>
 __device__ __forceinline__ int q_swz(int k) {
   const int h = ((k >> 2) ^ (k >> 4)) & 1;
   if constexpr (D == 32) return h;
-  else if constexpr (QShape<D, false>::CPR % 8 == 0) return (k & 3) | (h << 2);
+  else if constexpr (D / 16 % 8 == 0) return (k & 3) | (h << 2);
   else return ((k >> 1) & 1) | (h << 1);
 }
 
@@ -109,23 +111,24 @@ struct QScaleView {
   uint32_t magic, shift, one, per_page;
 };
 
-template <int D, bool F16>
-__global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_kernel(PagedAttnQArgs args) {
-  using SH = QShape<D, F16>;
+template <int D, bool F16, bool PAIR>
+__global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_attn_q_kernel(PagedAttnQArgs args) {
+  using SH = QShape<D, F16, PAIR>;
   const PagedAttnArgs& a = args.a;
-  constexpr int TK = kQTile, MB = TK / 16, KSTEPS = TK / 32;
+  constexpr int TK = SH::TK, MB = TK / 16, KSTEPS = TK / 32;
   constexpr int MBW = SH::MBW, ROW = SH::ROW, NG = SH::NG, PP = SH::PP;
   constexpr int M = kRows, NB = M / 16;
-  constexpr int NS = SH::NS, AHEAD = NS - 1, PAGES = 4;
+  constexpr int NS = SH::NS, AHEAD = NS - 1, PAGES = 4, NP = PAIR ? 1 : 2;
   constexpr float kLn2 = 0.6931471805599453f;
-  static_assert(NS * SH::TILE >= M * D * 2, "the output is staged in the tiles' LDS");
+  constexpr int PARTS = NS * SH::TILE >= M * D * 2 ? 1 : 2;  // of the output, staged in the tiles' LDS
+  static_assert(NS * SH::TILE >= M * D * 2 / PARTS, "the output is staged in the tiles' LDS");
   __shared__ __attribute__((aligned(16))) char kv_lds[NS * SH::TILE];
-  __shared__ __attribute__((aligned(16))) char p_lds[2][PP][KSTEPS][NB * 64 * 16];
-  __shared__ __attribute__((aligned(16))) float alpha_lds[2][M];
+  __shared__ __attribute__((aligned(16))) char p_lds[NP][PP][KSTEPS][NB * 64 * 16];
+  __shared__ __attribute__((aligned(16))) float alpha_lds[NP][M];
   __shared__ float sink_lds[M];
-  __shared__ __attribute__((aligned(16))) int flag_lds[2][4];
-  __shared__ __attribute__((aligned(16))) int page_lds[kAttnWaves][PAGES][TK];
-  __shared__ __attribute__((aligned(16))) float scale_lds[kAttnWaves][NS][TK];
+  __shared__ __attribute__((aligned(16))) int flag_lds[NP][4];
+  __shared__ __attribute__((aligned(16))) int page_lds[kAttnWaves][PAGES][64];
+  __shared__ __attribute__((aligned(16))) float scale_lds[kAttnWaves][NS][64];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -166,8 +169,16 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
   const int tbeg = static_cast<int>(static_cast<int64_t>(ntiles) * share / shares);
   const int tend = static_cast<int>(static_cast<int64_t>(ntiles) * (share + 1) / shares);
 
+  // (Lane addresses are worked out anew for each tile where registers are short: an opaque copy of the lane number keeps
+  // the compiler from hoisting them.)
+  auto lane_now = [&]() __attribute__((always_inline)) {
+    int ln = lane;
+    if constexpr (PAIR) reg_tie(ln);
+    return ln;
+  };
+
   // ---- copies ----------------------------------------------------------------
-  // Lane l resolves key l of a tile (a key past the last one as that one, a key without a page as row 0; both are masked).
+  // Lane l resolves key l of a tile, or l mod 32 (a key past the last one as that one, a key without a page as row 0; both are masked).
   // Every wave fetches all page numbers and scales for itself, a tile and no tile ahead of its copies, into LDS.
   CacheView view1, view2;
   CacheBase base1, base2;
@@ -226,7 +237,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
   };
   auto fetch_pages = [&]() __attribute__((always_inline)) {
     if (__builtin_expect(ftile == n1, 0) && ntiles > n1) enter(n1);
-    const uint32_t key = min(fkey + static_cast<uint32_t>(lane), fend - 1);
+    const uint32_t key = min(fkey + static_cast<uint32_t>(lane_now() & (TK - 1)), fend - 1);
     const uint32_t col = view.page_of(key);
     __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(view.table + col),
                                      (lds_void_t*)&page_lds[wave][ftile % PAGES][0], 4, 0, 0);
@@ -238,14 +249,6 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
   struct Rows {
     uint32_t row[SH::LPT];  // of this lane's copies, 16-byte units
   };
-  // Where the wave's copy i takes key (64 i + lane) / CPR of its KPW, chunk (64 i + lane) % CPR behind the swizzle.
-  uint32_t ckey[SH::LPT], cchunk[SH::LPT];
-#pragma unroll
-  for (int i = 0; i < SH::LPT; ++i) {
-    const int e = 64 * i + lane, k = wave * SH::KPW + e / SH::CPR;
-    ckey[i] = static_cast<uint32_t>(k & (TK - 1)) * 4;
-    cchunk[i] = static_cast<uint32_t>((e % SH::CPR) ^ q_swz<D>(k));
-  }
   // Sources of the tile whose page numbers are `page`, its scales on their way; returns which keys have a page.
   auto address_tile = [&](int page, const Within& in, Rows& y, int slot) __attribute__((always_inline)) {
     const bool ok = static_cast<uint32_t>(page) < from.cache.pages;
@@ -254,22 +257,24 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
     const float* sc = from.scales + (ok ? static_cast<int64_t>(p) * from.sstride + in.block : 0);
     __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(sc), (lds_void_t*)&scale_lds[wave][slot][0], 4, 0, 0);
 #pragma unroll
-    for (int i = 0; i < SH::LPT; ++i)
-      y.row[i] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(static_cast<int>(ckey[i]), static_cast<int>(row)));
+    for (int i = 0; i < SH::LPT; ++i)  // the row of chunk 256 i + 64 wave + lane
+      y.row[i] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(
+          ((i * kPagedThreads + wave * 64 + lane_now()) / SH::CPR & (TK - 1)) * 4, static_cast<int>(row)));
     return __builtin_amdgcn_ballot_w64(ok);
   };
   auto copy = [&](const Rows& y, char* tile, auto IC) __attribute__((always_inline)) {
     constexpr int i = decltype(IC)::value;
-    const uint32_t src = y.row[i] + cchunk[i];
-    char* dst = tile + wave * (SH::LPT * 1024) + i * 1024;
-    if (SH::WAVES == 4 || wave < SH::WAVES)
+    const int e = i * kPagedThreads + wave * 64 + lane_now(), k = e / SH::CPR;
+    const uint32_t src = y.row[i] + static_cast<uint32_t>((e - k * SH::CPR) ^ q_swz<D>(k));
+    char* dst = tile + i * (kPagedThreads * 16) + wave * 1024;
+    if (SH::CH % kPagedThreads == 0 || i + 1 < SH::LPT || i * kPagedThreads + wave * 64 < SH::CH)
       __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(from.cache.base + (static_cast<uint64_t>(src) << 4)),
                                        (lds_void_t*)dst, 16, 0, 0);
   };
-  constexpr int LANDED = SH::WAVES == 4 ? SH::LPT : 0;  // copies that every wave has in flight for a tile
+  constexpr int LANDED = SH::LANDED;
   auto ring = [&](int slot) __attribute__((always_inline)) { return kv_lds + slot * SH::TILE; };
   auto page_addr = [&](int t) __attribute__((always_inline)) {
-    return lds_addr(reinterpret_cast<const char*>(&page_lds[wave][t % PAGES][0])) + lane * 4;
+    return lds_addr(reinterpret_cast<const char*>(&page_lds[wave][t % PAGES][0])) + lane_now() * 4;
   };
   Within within[AHEAD + 1];
   Source froms[AHEAD + 1];
@@ -335,23 +340,24 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
   // ---- S^T -------------------------------------------------------------------
   // Unit u: 16 keys of one group of 64 dimensions, groups outermost.  A-fragments: key 16 mb + i16, chunk 4 j + g (D = 32: half a
   // chunk).
-  constexpr int UNITS = QG * MB, QD = 4;
-  uint32_t kbase[2][2];  // by mb's and j's parity
-#pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int f = q_swz<D>(16 * b + i16);
-    const uint32_t at = i16 * ROW + (D == 32 ? 16 * ((g >> 1) ^ f) + 8 * (g & 1) : 16 * (g ^ (f & 3)));
-    kbase[b][0] = at + 64 * (f >> 2);
-    kbase[b][1] = at - 64 * (f >> 2);
-  }
+  constexpr int UNITS = QG * MB, QD = PAIR || UNITS < 4 ? 2 : 4;
   auto qk = [&](int slot, f32x4 (&st)[MB], f32x4 (&sc)[MB], auto&& start, auto&& beside) __attribute__((always_inline)) {
     const uint32_t tile = lds_addr(ring(slot));
-    const uint32_t sat = lds_addr(reinterpret_cast<const char*>(&scale_lds[wave][slot][0])) + 16 * g;
+    const int ln = lane_now(), lg = ln >> 4, lk = ln & 15;
+    uint32_t kbase[2][2];  // by mb's and j's parity
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int f = q_swz<D>(16 * b + lk);
+      const uint32_t at = tile + lk * ROW + (D == 32 ? 16 * ((lg >> 1) ^ f) + 8 * (lg & 1) : 16 * (lg ^ (f & 3)));
+      kbase[b][0] = at + 64 * (f >> 2);
+      kbase[b][1] = at - 64 * (f >> 2);
+    }
+    const uint32_t sat = lds_addr(reinterpret_cast<const char*>(&scale_lds[wave][slot][0])) + 16 * lg;
     i32x4 s4[MB];
     typename std::conditional<D == 32, i32x2, i32x4>::type k[QD];
     auto issue = [&](auto UC) __attribute__((always_inline)) {
       constexpr int u = decltype(UC)::value, j = u / MB, mb = u % MB;
-      const uint32_t at = tile + kbase[mb & 1][j & 1];
+      const uint32_t at = kbase[mb & 1][j & 1];
       if constexpr (D == 32) k[u % QD] = ldq64<16 * ROW * mb>(at);
       else k[u % QD] = ldq<64 * j + 16 * ROW * mb>(at);
     };
@@ -375,8 +381,8 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
       }
       beside(UC);
     });
-    static_assert(MB == 4, "four reads of scales");
-    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s4[0]), "+v"(s4[1]), "+v"(s4[2]), "+v"(s4[3]));
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s4[0]), "+v"(s4[1]));
+    if constexpr (MB == 4) asm volatile("" : "+v"(s4[MB - 2]), "+v"(s4[MB - 1]));
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) sc[mb] = __builtin_bit_cast(f32x4, s4[mb]);
   };
@@ -403,10 +409,10 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
   int skey = 0;
   auto softmax_begin = [&](int t, uint64_t okmask, f32x4 (&st)[MB], f32x4 (&sc)[MB], float& ref, int pbuf) __attribute__((always_inline)) {
     mfma_result_fence(st[0], st[1]);
-    mfma_result_fence(st[2], st[3]);
+    if constexpr (MB == 4) mfma_result_fence(st[MB - 2], st[MB - 1]);
     if (t == n1) skey = 0;
     const bool second = t >= n1;
-    const bool full = okmask == ~0ull && (second ? skey <= all2hi - TK : skey >= all1lo && skey <= all1hi - TK);
+    const bool full = (TK == 64 ? okmask == ~0ull : static_cast<uint32_t>(okmask) == ~0u) && (second ? skey <= all2hi - TK : skey >= all1lo && skey <= all1hi - TK);
     int flags = 0;
     float lmax = kNever;
     if (!full) {
@@ -414,12 +420,13 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
       const int end2 = second ? ent_end(rpos) : max(min(rpos + 1, cap1), 0);
       const int begin2 = second ? 0 : max(max(rpos + 1, 0) - window, 0);
       const int lo = skey - begin2, cnt = max(end2 - begin2, 0);
-      const uint64_t mine = okmask >> (4 * g);
+      const int g4 = 4 * (lane_now() >> 4);
+      const uint64_t mine = okmask >> g4;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool ok = static_cast<uint32_t>(16 * mb + 4 * g + r + lo) < static_cast<uint32_t>(cnt) && ((mine >> (16 * mb + r)) & 1);
+          const bool ok = static_cast<uint32_t>(16 * mb + g4 + r + lo) < static_cast<uint32_t>(cnt) && ((mine >> (16 * mb + r)) & 1);
           odd = odd || (!ok && !(__builtin_fabsf(st[mb][r]) < __builtin_inff()));
           st[mb][r] = ok ? st[mb][r] * (sc[mb][r] * rscale) : kNever;
           sc[mb][r] = ok ? sc[mb][r] : 0.f;  // (a masked key's scale may be anything)
@@ -445,7 +452,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
       const float alpha = raise && !first ? __builtin_amdgcn_exp2f(m_ref - (tmax - kHead)) : 1.0f;
       if (raise) m_ref = tmax - kHead;
       l_run *= alpha;
-      const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][wave * 16 + i16]));
+      const uint32_t adst = lds_addr(reinterpret_cast<const char*>(&alpha_lds[pbuf][wave * 16 + (lane_now() & 15)]));
       asm volatile("ds_write_b32 %0, %1" ::"v"(adst), "v"(alpha) : "memory");
       if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) flags |= kMoved;
     }
@@ -453,10 +460,11 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
     const uint32_t fdst = lds_addr(reinterpret_cast<const char*>(&flag_lds[pbuf][wave]));
     asm volatile("ds_write_b32 %0, %1" ::"v"(fdst), "v"(flags) : "memory");
   };
-  auto softmax_exp = [&](int i, f32x4 (&st)[MB], float ref) __attribute__((always_inline)) {  // i of 16 weights
+  auto softmax_exp = [&](int i, f32x4 (&st)[MB], float ref) __attribute__((always_inline)) {  // i of 4 MB weights
     st[i >> 2][i & 3] = __builtin_amdgcn_exp2f(st[i >> 2][i & 3] - ref);
   };
   auto softmax_end = [&](const f32x4 (&p)[MB], const f32x4 (&sc)[MB], int pbuf) __attribute__((always_inline)) {
+    const int ln16 = (wave * 64 + lane_now()) * 16;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) l_run += (p[mb][0] + p[mb][1]) + (p[mb][2] + p[mb][3]);
     // P^T B-fragment of k-step s: k-slots 8g+0..3 <-> keys 32s + 4g+0..3, 8g+4..7 <-> keys 32s + 16 + 4g+0..3
@@ -465,7 +473,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
       const f32x4 x = p[2 * s] * sc[2 * s], y = p[2 * s + 1] * sc[2 * s + 1];
       const u32x4 w = u32x4{f32x2_to_bf16x2(x[0], x[1]), f32x2_to_bf16x2(x[2], x[3]), f32x2_to_bf16x2(y[0], y[1]),
                             f32x2_to_bf16x2(y[2], y[3])};
-      asm volatile("ds_write_b128 %0, %1" ::"v"(lds_addr(&p_lds[pbuf][0][s][(wave * 64 + lane) * 16])), "v"(w) : "memory");
+      asm volatile("ds_write_b128 %0, %1" ::"v"(lds_addr(&p_lds[pbuf][0][s][ln16])), "v"(w) : "memory");
       if constexpr (PP == 2) {
         u32x4 v;
 #pragma unroll
@@ -473,7 +481,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
           const f32x4& z = c < 2 ? x : y;
           v[c] = f32x2_to_bf16x2(z[2 * (c & 1)] - elem_lo<false>(w[c]), z[2 * (c & 1) + 1] - elem_hi<false>(w[c]));
         }
-        asm volatile("ds_write_b128 %0, %1" ::"v"(lds_addr(&p_lds[pbuf][PP - 1][s][(wave * 64 + lane) * 16])), "v"(v) : "memory");
+        asm volatile("ds_write_b128 %0, %1" ::"v"(lds_addr(&p_lds[pbuf][PP - 1][s][ln16])), "v"(v) : "memory");
       }
     }
   };
@@ -485,18 +493,18 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) oacc[j][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
   // V^T reads: source lane (g, i16) points at key 4g + (x & 3) + 16 (x >> 2), x = i16 >> 1, half i16 & 1 of chunk 4 j + wave
-  uint32_t vbase[2];
-  {
-    const int x = i16 >> 1, key = 4 * g + (x & 3) + 16 * (x >> 2), f = q_swz<D>(key);
-    const uint32_t at = key * ROW + 16 * ((wave ^ (f & 3)) & (SH::CPR - 1 < 3 ? SH::CPR - 1 : 3)) + 8 * (i16 & 1);
-    vbase[0] = at + 64 * (f >> 2);
-    vbase[1] = at - 64 * (f >> 2);
-  }
-  constexpr int VQ = MBW < 3 ? MBW : 3;
+  constexpr int VQ0 = PAIR ? 2 : 3, VQ = VQ0 < MBW ? VQ0 : MBW;
   auto pv = [&](int slot, int pbuf, auto&& between) __attribute__((always_inline)) {
-    const uint32_t tile = lds_addr(ring(slot));
+    const int ln = lane_now();
+    uint32_t vbase[2];
+    {
+      const int x = (ln & 15) >> 1, key = 4 * (ln >> 4) + (x & 3) + 16 * (x >> 2), f = q_swz<D>(key);
+      const uint32_t at = lds_addr(ring(slot)) + key * ROW + 16 * ((wave ^ (f & 3)) & (SH::CPR < 4 ? SH::CPR - 1 : 3)) + 8 * (ln & 1);
+      vbase[0] = at + 64 * (f >> 2);
+      vbase[1] = at - 64 * (f >> 2);
+    }
     bf16x8 pf[PP][KSTEPS][NB];
-    const uint32_t psrc = lds_addr(&p_lds[pbuf][0][0][0]) + lane * 16;
+    const uint32_t psrc = lds_addr(&p_lds[pbuf][0][0][0]) + ln * 16;
     attn_static_for<0, PP * KSTEPS * NB>([&](auto NC) {
       constexpr int n = decltype(NC)::value;
       pf[n / (KSTEPS * NB)][n / NB % KSTEPS][n % NB] = ld128<1024 * n>(psrc);
@@ -506,14 +514,15 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
       constexpr int j = decltype(JC)::value;
       attn_static_for<0, KSTEPS>([&](auto SC) {
         constexpr int s = decltype(SC)::value;
-        v[j % VQ][s] = tr_read8<64 * j + 32 * ROW * s>(tile + vbase[j & 1]);
+        v[j % VQ][s] = tr_read8<64 * j + 32 * ROW * s>(vbase[j & 1]);
       });
     };
     attn_static_for<0, VQ>(issue);
     attn_static_for<0, MBW>([&](auto JC) {
       constexpr int j = decltype(JC)::value;
       constexpr int later = (MBW - 1 - j) < (VQ - 1) ? (MBW - 1 - j) : (VQ - 1);
-      asm volatile("s_waitcnt lgkmcnt(%2)" : "+v"(v[j % VQ][0]), "+v"(v[j % VQ][1]) : "n"(KSTEPS * later));
+      asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(v[j % VQ][0]) : "n"(KSTEPS * later));
+      if constexpr (KSTEPS == 2) reg_tie(v[j % VQ][KSTEPS - 1]);
       if constexpr (j == 0) {
 #pragma unroll
         for (int p = 0; p < PP; ++p)
@@ -576,7 +585,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
   // t - tbeg mod NS, its P in p_lds[t & 1].  The copies of tile t + AHEAD go out at the start, into the slot of tile t - 1.
   if (tbeg >= tend) {
     sink_to_lds();
-  } else {
+  } else if constexpr (!PAIR) {
     skey = tbeg < n1 ? k1lo + tbeg * TK : (tbeg - n1) * TK;
     if (tbeg + AHEAD <= tend) __builtin_amdgcn_s_waitcnt(vm_lgkm0((AHEAD - 1) * (LANDED + 1)));
     else __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
@@ -587,7 +596,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
     qk(0, st, sc, [] {}, [](auto) {});
     softmax_begin(tbeg, okq[0], st, sc, ref, tbeg & 1);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) softmax_exp(i, st, ref);
+    for (int i = 0; i < 4 * MB; ++i) softmax_exp(i, st, ref);
     softmax_end(st, sc, tbeg & 1);
     int slot = 0;  // of tile t
     auto iteration = [&](int t, auto MORE, auto COPY) __attribute__((always_inline)) {
@@ -646,6 +655,53 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
     for (; t + AHEAD < tend; ++t) iteration(t, std::true_type{}, std::true_type{});
     for (; t + 1 < tend; ++t) iteration(t, std::true_type{}, std::false_type{});
     iteration(t, std::false_type{}, std::false_type{});
+  } else {
+    // PAIR: two tiles ahead, two barriers a tile.  Tile t lives in slot t - tbeg mod 3; the copies of tile t + 2 go into the
+    // slot of tile t - 1.
+    skey = tbeg < n1 ? k1lo + tbeg * TK : (tbeg - n1) * TK;
+    sink_to_lds();
+    int slot = 0;
+    auto step = [&](int t, auto NEXT, auto COPY) __attribute__((always_inline)) {
+      constexpr bool next = decltype(NEXT)::value, ahead = decltype(COPY)::value;
+      // tile t and the page numbers of tile t + 2 have landed; the scales and copies of tile t + 1 may be in flight
+      __builtin_amdgcn_s_waitcnt(vm_lgkm0(next ? LANDED + 1 : 0));
+      attn_tile_barrier();  // every wave's, and every wave has left tile t - 1 and its P
+      {
+        f32x4 st[MB], sc[MB];
+        float ref;
+        qk(slot, st, sc, [] {}, [](auto) {});
+        softmax_begin(t, okq[0], st, sc, ref, 0);
+#pragma unroll
+        for (int i = 0; i < 4 * MB; ++i) softmax_exp(i, st, ref);
+        softmax_end(st, sc, 0);
+      }
+      okq[0] = okq[1];
+      if constexpr (ahead) {
+        const int last_slot = slot == 0 ? NS - 1 : slot - 1;
+        int page;
+        asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(page) : "v"(page_addr(t + 2)));
+        const Within in = in_next;
+        in_next = fetch_pages();  // (past the share's end: the same page again, not used)
+        okq[1] = address_tile(page, in, src, last_slot);
+        attn_static_for<0, SH::LPT>([&](auto IC) {
+          copy(src, ring(last_slot), IC);
+          __builtin_amdgcn_sched_barrier(0);  // (one address at a time: registers)
+        });
+        from = from_next;
+      }
+      attn_tile_barrier();  // P published
+      u32x4 fl;
+      asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(fl)
+                   : "v"(lds_addr(reinterpret_cast<const char*>(&flag_lds[0][0]))));
+      const int flags = __builtin_amdgcn_readfirstlane(static_cast<int>(fl[0] | fl[1] | fl[2] | fl[3]));
+      if (__builtin_expect(flags != 0, 0)) settle(flags, 0, slot);
+      pv(slot, 0, [](auto) {});
+      slot = slot + 1 == NS ? 0 : slot + 1;
+    };
+    int t = tbeg;
+    for (; t + 2 < tend; ++t) step(t, std::true_type{}, std::true_type{});
+    if (t + 1 < tend) step(t++, std::true_type{}, std::false_type{});
+    step(t, std::false_type{}, std::false_type{});
   }
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");  // (the last MFMAs' wait states, see mfma_result_fence)
 
@@ -688,32 +744,42 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16)) void paged_attn_q_
   }
   __syncthreads();  // scales published
   // staged in the tiles' LDS, then written in one piece: the rows follow each other in o
-  float osc[NB];
+  char* obase = reinterpret_cast<char*>(a.o + flat0 * D);
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) osc[nb] = out_scale[nb * 16 + i16];
+  for (int part = 0; part < PARTS; ++part) {
+    constexpr int R = M / PARTS;  // rows of a part
+    if (part > 0) {
+      if (part * R >= nrows) return;
+      __syncthreads();  // the part before has been read
+    }
 #pragma unroll
-  for (int j = 0; j < MBW; ++j) {
-    const int mbi = j * kAttnWaves + wave;
-    if (SH::MBT % kAttnWaves == 0 || mbi < SH::MBT) {
+    for (int nb = part * (NB / PARTS); nb < (part + 1) * (NB / PARTS); ++nb) {
+      const float osc = out_scale[nb * 16 + i16];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const f32x4 v = oacc[j][nb] * osc[nb];
-        uint2 w;
-        w.x = pack2<F16>(v[0], v[1]);
-        w.y = pack2<F16>(v[2], v[3]);
-        *reinterpret_cast<uint2*>(kv_lds + kv_off<D>(nb * 16 + i16, 2 * mbi + (g >> 1)) + 8 * (g & 1)) = w;
+      for (int j = 0; j < MBW; ++j) {
+        const int mbi = j * kAttnWaves + wave;
+        if (SH::MBT % kAttnWaves == 0 || mbi < SH::MBT) {
+          const f32x4 v = oacc[j][nb] * osc;
+          uint2 w;
+          w.x = pack2<F16>(v[0], v[1]);
+          w.y = pack2<F16>(v[2], v[3]);
+          *reinterpret_cast<uint2*>(kv_lds + kv_off<D>(nb * 16 + i16 - part * R, 2 * mbi + (g >> 1)) + 8 * (g & 1)) = w;
+        }
       }
     }
+    __syncthreads();
+    for (int e = threadIdx.x; e < min(nrows - part * R, R) * (D / 8); e += kPagedThreads)
+      *reinterpret_cast<u32x4*>(obase + static_cast<int64_t>(e + part * R * (D / 8)) * 16) =
+          *reinterpret_cast<const u32x4*>(kv_lds + kv_off<D>(e / (D / 8), e % (D / 8)));
   }
-  __syncthreads();
-  char* obase = reinterpret_cast<char*>(a.o + flat0 * D);
-  for (int e = threadIdx.x; e < nrows * (D / 8); e += kPagedThreads)
-    *reinterpret_cast<u32x4*>(obase + static_cast<int64_t>(e) * 16) =
-        *reinterpret_cast<const u32x4*>(kv_lds + kv_off<D>(e / (D / 8), e % (D / 8)));
 }
+
+// Row blocks from which PAIR is taken.
+constexpr int64_t q_pair_from(int64_t D, bool f16) { return D >= 512 ? 257 : INT64_MAX; }
 
 // Sizes of a call, from what the host knows.
 struct PagedQSizes {
+  bool pair;             // the kernel with PAIR
   int64_t blocks;        // row blocks of a workgroup at most
   int64_t want;          // workgroups that run at once
   int64_t grid;          // workgroups
@@ -729,11 +795,12 @@ static PagedQSizes q_sizes(int64_t N, int64_t H, int64_t D, bool f16, int64_t R,
   int64_t g = M;
   while (H % g) g /= 2;
   p.blocks = (N * H + (R < N ? R : N) * (M - g)) / M;
-  const int64_t want = p.want = 256 * q_per_cu(static_cast<int>(D), f16);
+  p.pair = p.blocks >= q_pair_from(D, f16);
+  const int64_t want = p.want = 256 * q_per_cu(static_cast<int>(D), f16, p.pair), tile = p.pair ? 32 : 64;
   p.grid = 2 * p.blocks <= want ? want : p.blocks + want;
   const int64_t span = M / H + 1 + window;
   p.behind = static_cast<int>((M - 1 + H - g) / H);  // (a row block begins at any multiple of g heads of a token)
-  const int64_t tiles = ((window < keys1 && span < keys1 ? span : keys1) + kQTile - 1) / kQTile + (keys2 + kQTile - 1) / kQTile;
+  const int64_t tiles = ((window < keys1 && span < keys1 ? span : keys1) + tile - 1) / tile + (keys2 + tile - 1) / tile;
   // Where no cut can win back the second launch that joins the shares, none is made.
   if (tiles <= (D >= 512 ? 8 : 14) + p.blocks / 8) {
     p.grid = p.blocks;
@@ -755,8 +822,18 @@ static int launch_paged_attn_q(bool f16, const PagedAttnQArgs& a, const PagedQSi
   if (p.grid + 7 > most) return set_error(SI_ERR_UNSUPPORTED, "too many rows for one launch");
   // (whole rounds of the XCDs: see paged_item_number)
   const dim3 grid(static_cast<unsigned>(((p.grid < 1 ? 1 : p.grid) + 7) & ~int64_t{7})), block(kPagedThreads);
-  if (f16) hipLaunchKernelGGL((paged_attn_q_kernel<D, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((paged_attn_q_kernel<D, false>), grid, block, 0, st, a);
+  auto launch = [&](auto F16) {
+    constexpr bool half = decltype(F16)::value;
+    if constexpr (q_pair_from(D, half) < INT64_MAX) {
+      if (p.pair) {
+        hipLaunchKernelGGL((paged_attn_q_kernel<D, half, true>), grid, block, 0, st, a);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((paged_attn_q_kernel<D, half, false>), grid, block, 0, st, a);
+  };
+  if (f16) launch(std::true_type{});
+  else launch(std::false_type{});
   const int rc = check_launch("paged_attn_q_kernel");
   if (rc || !a.a.part_o) return rc;
   return launch_paged_combine(f16, a.a, D, p.split_blocks, st);
