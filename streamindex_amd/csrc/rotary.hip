@@ -27,7 +27,7 @@ namespace si {
 
 constexpr int kRotThreads = 256;
 constexpr int64_t kRotMostD = 1024;
-constexpr int kRotTable = 48 * 1024;  // bytes of LDS for cosines and sines at most
+constexpr int kRotTable = 40 * 1024;  // bytes of LDS for cosines and sines at most
 
 struct RotArgs {
   const char* x;   // [T, H, D]; the forward's input
@@ -45,6 +45,7 @@ struct RotArgs {
   int iters;                   // groups of rows of a workgroup
   int per;                     // of them for each filling of the table
   int tokens;                  // of those at most
+  int weight_lds;              // floats of LDS for the weight, in front of the table
   float magnitude, sign, eps;
 };
 
@@ -153,6 +154,25 @@ struct RotPlace {
   }
 };
 
+// The weights from dimension e0 on.
+template <int V>
+__device__ __forceinline__ void rot_weights(const RotArgs& a, const float* weight, int e0, float (&w)[V]) {
+  if (!a.weight) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = 1.f;
+  } else if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      const f32x4 x = reinterpret_cast<const f32x4*>(weight + e0)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[4 * i + e] = x[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = weight[e0 + e];
+  }
+}
+
 // z turned, in place: v the piece's values; u those of its partner piece (halves).
 template <int V, bool PAIRS>
 __device__ __forceinline__ void rot_turn(const RotArgs& a, const RotPlace<V>& p, const float2* table, float (&v)[V],
@@ -176,11 +196,17 @@ __device__ __forceinline__ void rot_turn(const RotArgs& a, const RotPlace<V>& p,
   }
 }
 
-// Cosines and sines of the tokens from that of row row0 on, a.tokens of them, to LDS; all threads call it.  Returns the first.
-__device__ __forceinline__ int64_t rot_fill(const RotArgs& a, int64_t row0, float2* table) {
-  if (a.pairs == 0) return 0;
+// The weight, at first, and the cosines and sines of the tokens from that of row row0 on, a.tokens of them, to LDS; all threads
+// call it.  Returns the first token.
+__device__ __forceinline__ int64_t rot_fill(const RotArgs& a, int64_t row0, float* weight, float2* table, bool at_first) {
   const int64_t token0 = row0 / a.H, last = (a.rows - 1) / a.H;
-  __syncthreads();  // (the table has been used)
+  if (at_first) {
+    if (a.weight)
+      for (int e = threadIdx.x; e < a.D; e += kRotThreads) weight[e] = a.weight[e];
+  } else {
+    if (a.pairs == 0) return 0;
+    __syncthreads();  // (the table has been used)
+  }
   for (int i = threadIdx.x; i < a.tokens * a.pairs; i += kRotThreads) {
     const int64_t token = token0 + static_cast<uint32_t>(i) / static_cast<uint32_t>(a.pairs);
     if (token <= last) table[i] = rot_at(a, rot_pos(a, token), static_cast<int>(static_cast<uint32_t>(i) % static_cast<uint32_t>(a.pairs)));
@@ -191,7 +217,8 @@ __device__ __forceinline__ int64_t rot_fill(const RotArgs& a, int64_t row0, floa
 
 template <int DT, int V, int CPL, bool NORM>
 __global__ __launch_bounds__(kRotThreads) void norm_rotary_kernel(RotArgs a) {
-  extern __shared__ float2 rot_table[];
+  extern __shared__ __attribute__((aligned(16))) float rot_lds[];
+  float2* const all = reinterpret_cast<float2*>(rot_lds + a.weight_lds);
   const int lane = threadIdx.x & (a.lpr - 1), group = threadIdx.x >> a.log_lpr, groups = kRotThreads >> a.log_lpr;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.iters * groups;
   int64_t token0 = 0;
@@ -210,7 +237,7 @@ __global__ __launch_bounds__(kRotThreads) void norm_rotary_kernel(RotArgs a) {
       if (live && p.there) piece[c].load(x, at + p.e0);
       else piece[c].zero();
     }
-    if (it % a.per == 0) token0 = rot_fill(a, first, rot_table);
+    if (it % a.per == 0) token0 = rot_fill(a, first, rot_lds, all, it == 0);
     if (!live) continue;
     float r = 1.f;
     if constexpr (NORM) {
@@ -222,17 +249,18 @@ __global__ __launch_bounds__(kRotThreads) void norm_rotary_kernel(RotArgs a) {
       sum = rot_sum(sum, a.log_lpr);
       r = 1.0f / __builtin_sqrtf(sum / static_cast<float>(a.D) + a.eps);
     }
-    const float2* table = rot_table + static_cast<int>(token - token0) * a.pairs;
+    const float2* table = all + static_cast<int>(token - token0) * a.pairs;
     const int64_t to = row * a.D;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
       const RotPlace<V> p(a, lane, c);
       if (!p.there) continue;
-      float v[V], u[V];
+      float v[V], u[V], w[V];
+      if constexpr (NORM) rot_weights<V>(a, rot_lds, p.e0, w);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         v[e] = piece[c].at(e);
-        if constexpr (NORM) v[e] *= r * (a.weight ? a.weight[p.e0 + e] : 1.f);
+        if constexpr (NORM) v[e] *= r * w[e];
         u[e] = 0.f;
       }
       if (p.turned) {
@@ -240,10 +268,11 @@ __global__ __launch_bounds__(kRotThreads) void norm_rotary_kernel(RotArgs a) {
           const int other = a.halves ? p.partner : p.e0 + (((p.e0 - a.start) & 1) ? -1 : 1);
           RotPiece<DT, V> q;
           q.load(x, at + other);
+          if constexpr (NORM) rot_weights<V>(a, rot_lds, other, w);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             u[e] = q.at(e);
-            if constexpr (NORM) u[e] *= r * (a.weight ? a.weight[other + e] : 1.f);
+            if constexpr (NORM) u[e] *= r * w[e];
           }
         }
         rot_turn<V, (V > 1)>(a, p, table, v, u);
@@ -253,10 +282,12 @@ __global__ __launch_bounds__(kRotThreads) void norm_rotary_kernel(RotArgs a) {
   }
 }
 
-// The gradients of a normed row.  Partial sums of dw stay in registers over the workgroup's rows.
+// The gradients of a normed row.  Partial sums of dw stay in registers over the workgroup's rows; d is formed twice, from dy
+// as it was loaded, which costs less than its registers.
 template <int DT, int V, int CPL>
-__global__ __launch_bounds__(kRotThreads) void norm_rotary_bwd_kernel(RotArgs a) {
-  extern __shared__ float2 rot_table[];
+__global__ __launch_bounds__(kRotThreads, 2) void norm_rotary_bwd_kernel(RotArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float rot_lds[];
+  float2* const all = reinterpret_cast<float2*>(rot_lds + a.weight_lds);
   const int lane = threadIdx.x & (a.lpr - 1), group = threadIdx.x >> a.log_lpr, groups = kRotThreads >> a.log_lpr;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.iters * groups;
   int64_t token0 = 0;
@@ -284,17 +315,14 @@ __global__ __launch_bounds__(kRotThreads) void norm_rotary_bwd_kernel(RotArgs a)
         grad[c].zero();
       }
     }
-    if (it % a.per == 0) token0 = rot_fill(a, first, rot_table);
+    if (it % a.per == 0) token0 = rot_fill(a, first, rot_lds, all, it == 0);
     if (!live) continue;
-    const float2* table = rot_table + static_cast<int>(token - token0) * a.pairs;
-    float d[CPL][V], sum = 0.f, dot = 0.f;
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      const RotPlace<V> p(a, lane, c);
+    const float2* table = all + static_cast<int>(token - token0) * a.pairs;
+    auto gradient = [&](const RotPlace<V>& p, const RotPiece<DT, V>& g, float (&d)[V]) {
       float u[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        d[c][e] = grad[c].at(e);
+        d[e] = g.at(e);
         u[e] = 0.f;
       }
       if (p.turned) {
@@ -305,13 +333,22 @@ __global__ __launch_bounds__(kRotThreads) void norm_rotary_bwd_kernel(RotArgs a)
 #pragma unroll
           for (int e = 0; e < V; ++e) u[e] = q.at(e);
         }
-        rot_turn<V, (V > 1)>(a, p, table, d[c], u);
+        rot_turn<V, (V > 1)>(a, p, table, d, u);
       }
+    };
+    float sum = 0.f, dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+      const RotPlace<V> p(a, lane, c);
+      if (!p.there) continue;
+      float d[V], w[V];
+      gradient(p, grad[c], d);
+      rot_weights<V>(a, rot_lds, p.e0, w);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float x = piece[c].at(e), w = a.weight && p.there ? a.weight[p.e0 + e] : 1.f;
+        const float x = piece[c].at(e);
         sum = __builtin_fmaf(x, x, sum);
-        dot = __builtin_fmaf(d[c][e] * w, x, dot);
+        dot = __builtin_fmaf(d[e] * w[e], x, dot);
       }
     }
     sum = rot_sum(sum, a.log_lpr);
@@ -323,12 +360,14 @@ __global__ __launch_bounds__(kRotThreads) void norm_rotary_bwd_kernel(RotArgs a)
     for (int c = 0; c < CPL; ++c) {
       const RotPlace<V> p(a, lane, c);
       if (!p.there) continue;
-      float v[V];
+      float d[V], w[V], v[V];
+      gradient(p, grad[c], d);
+      rot_weights<V>(a, rot_lds, p.e0, w);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float x = piece[c].at(e), w = a.weight ? a.weight[p.e0 + e] : 1.f;
-        dw[c][e] = __builtin_fmaf(d[c][e], x * r, dw[c][e]);
-        v[e] = r * (d[c][e] * w - x * k);
+        const float x = piece[c].at(e);
+        dw[c][e] = __builtin_fmaf(d[e], x * r, dw[c][e]);
+        v[e] = r * (d[e] * w[e] - x * k);
       }
       rot_store<DT, V>(a.out, to + p.e0, v);
     }
@@ -357,8 +396,18 @@ __global__ __launch_bounds__(256) void norm_rotary_dw_kernel(const float* part, 
   __shared__ float lds[16][17];
   const int e = threadIdx.x & 15, k = threadIdx.x >> 4, d = blockIdx.x * 16 + e;
   float s = 0.f;
-  if (d < D)
-    for (int i = k; i < parts; i += 16) s += part[static_cast<int64_t>(i) * D + d];
+  if (d < D) {
+    constexpr int U = 8;  // in flight
+    int i = k;
+    for (; i + 16 * (U - 1) < parts; i += 16 * U) {
+      float x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = part[static_cast<int64_t>(i + 16 * u) * D + d];
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += x[u];
+    }
+    for (; i < parts; i += 16) s += part[static_cast<int64_t>(i) * D + d];
+  }
   lds[k][e] = s;
   __syncthreads();
   if (k == 0 && d < D) {
@@ -383,6 +432,8 @@ static RotPlan rot_plan(int64_t rows, int64_t H, int64_t D, int64_t pairs, int v
   p.log_lpr = 0;
   while ((int64_t{9} << p.log_lpr) < n && p.log_lpr < 6) ++p.log_lpr;
   while (p.log_lpr < 3 && (int64_t{1} << p.log_lpr) < n) ++p.log_lpr;  // (128 bytes of a row at once)
+  // few rows: shorter chains, more workgroups
+  while (p.log_lpr < 6 && (int64_t{1} << p.log_lpr) < n && rows <= int64_t{512} * (kRotThreads >> p.log_lpr) / 2) ++p.log_lpr;
   // tokens of k rows that follow each other at most
   auto tokens = [&](int64_t k) { return k % H == 0 || H % k == 0 ? (k + H - 1) / H : (k - 2) / H + 2; };
   while (p.log_lpr < 6 && tokens(kRotThreads >> p.log_lpr) * pairs * 8 > kRotTable) ++p.log_lpr;  // (4 rows of 512 pairs fit)
@@ -390,8 +441,8 @@ static RotPlan rot_plan(int64_t rows, int64_t H, int64_t D, int64_t pairs, int v
   const int64_t cpl = (n + p.lpr - 1) / p.lpr;
   p.cpl = cpl <= 1 ? 1 : cpl <= 2 ? 2 : cpl <= 4 ? 4 : cpl <= 9 ? 9 : 16;
   const int64_t groups = kRotThreads / p.lpr, all = (rows + groups - 1) / groups;
-  // backward: at most 1,024 workgroups, whose sums of dw are joined; forward: up to 8 groups of rows, for weights read once
-  int64_t iters = bwd ? (all + 1023) / 1024 : all / 4096, per;
+  // backward: at most 512 workgroups, two a CU, whose sums of dw are joined; forward: up to 8 groups of rows
+  int64_t iters = bwd ? (all + 511) / 512 : all / 4096, per;
   per = iters = iters < 1 ? 1 : iters > 8 && !bwd ? 8 : iters;
   while (per > 1 && tokens(per * groups) * pairs * 8 > kRotTable / 3) per = (per + 1) / 2;
   p.per = static_cast<int>(per);
@@ -484,6 +535,7 @@ static void rot_args(RotArgs& a, const RotPlan& p, const float* weight, const vo
   a.log_lpr = p.log_lpr;
   a.iters = p.iters;
   a.per = p.per;
+  a.weight_lds = weight ? static_cast<int>((D + 3) / 4 * 4) : 0;
   a.tokens = p.tokens;
 }
 
@@ -509,7 +561,7 @@ extern "C" int si_norm_rotary(const void* x, const int64_t* x_strides, int norm,
   return rot_dispatch(dtype, p, [&](auto DT, auto V, auto CPL) {
     constexpr int dt = decltype(DT)::value, v = decltype(V)::value, cpl = decltype(CPL)::value;
     const dim3 grid(static_cast<unsigned>(p.blocks)), block(kRotThreads);
-    const size_t lds = static_cast<size_t>(p.tokens) * pairs * 8;
+    const size_t lds = static_cast<size_t>(p.tokens) * pairs * 8 + a.weight_lds * 4;
     if (norm) hipLaunchKernelGGL((norm_rotary_kernel<dt, v, cpl, true>), grid, block, lds, st, a);
     else hipLaunchKernelGGL((norm_rotary_kernel<dt, v, cpl, false>), grid, block, lds, st, a);
     return check_launch("norm_rotary_kernel");
@@ -562,7 +614,7 @@ extern "C" int si_norm_rotary_bwd(const void* dy, const int64_t* dy_strides, con
   rc = rot_dispatch(dtype, p, [&](auto DT, auto V, auto CPL) {
     constexpr int dt = decltype(DT)::value, v = decltype(V)::value, cpl = decltype(CPL)::value;
     hipLaunchKernelGGL((norm_rotary_bwd_kernel<dt, v, cpl>), dim3(static_cast<unsigned>(p.blocks)), dim3(kRotThreads),
-                       static_cast<size_t>(p.tokens) * pairs * 8, st, a);
+                       static_cast<size_t>(p.tokens) * pairs * 8 + a.weight_lds * 4, st, a);
     return check_launch("norm_rotary_bwd_kernel");
   });
   if (rc || !dweight) return rc;

@@ -108,10 +108,18 @@ def _apply(x, positions, freqs, weight, eps, interleaved, start, magnitude, inve
     return _forward(x, weight, positions, freqs, args)
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """``[T, H, D]`` with a contiguous last dimension: a view where there is one."""
-    x = x.reshape(-1, *x.shape[-2:]) if x.dim() != 3 else x
-    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+def _rows(x: torch.Tensor):
+    """``x [..., H, D]`` as rows of a contiguous last dimension: the tensor to read (x itself where it can be), the strides of its
+    tokens and heads."""
+    H, D = x.shape[-2:]
+    if x.is_contiguous():
+        return x, _lib.stride_array((H * D, D))
+    x = x.reshape(-1, H, D)
+    s = x.stride()
+    if s[2] != 1 and D > 1:
+        x = x.contiguous()
+        s = (H * D, D)
+    return x, _lib.stride_array(s[:2])
 
 
 def _fp32(weight: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -127,15 +135,49 @@ def _forward(x, weight, positions, freqs, args):
     L = _lib.load()
     with _lib.on_device(dev):
         y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        if x.numel() == 0:
+        n = x.numel()
+        if n == 0:
             return y
-        rows, w = _rows(x), _fp32(weight)
-        T, H, D = rows.shape
-        rc = L.si_norm_rotary(rows.data_ptr(), _lib.stride_array(rows.stride()), eps is not None, None if w is None else w.data_ptr(),
-                              eps or 0.0, positions.data_ptr(), positions.dtype is torch.int64, positions.numel(), freqs.data_ptr(),
-                              freqs.shape[0], start, halves, magnitude, inverse, T, H, D, dt, y.data_ptr(), _lib.stream_ptr(dev))
+        H, D = x.shape[-2:]
+        (rows, strides), w = _rows(x), _fp32(weight)
+        rc = L.si_norm_rotary(rows.data_ptr(), strides, eps is not None, None if w is None else w.data_ptr(), eps or 0.0,
+                              positions.data_ptr(), positions.dtype is torch.int64, positions.numel(), freqs.data_ptr(),
+                              freqs.shape[0], start, halves, magnitude, inverse, n // (H * D), H, D, dt, y.data_ptr(),
+                              _lib.stream_ptr(dev))
     _lib.check(rc)
     return y
+
+
+def _backward(ctx, dy):
+    positions, freqs, *saved = ctx.saved_tensors
+    eps, halves, start, magnitude, inverse, dt = ctx.args
+    if not saved:
+        return _forward(dy, None, positions, freqs, (None, halves, start, magnitude, not inverse, dt)), None, None, None, None
+    x, weight = saved[0], saved[1] if len(saved) > 1 else None
+    need_w = weight is not None and ctx.needs_input_grad[1]
+    dev = x.device
+    L = _lib.load()
+    with _lib.on_device(dev):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        n = x.numel()
+        H, D = x.shape[-2:]
+        dw = torch.empty(D, dtype=torch.float32, device=dev) if need_w else None
+        if n == 0:
+            return dx, None if dw is None else dw.zero_().to(weight.dtype), None, None, None
+        (rows, strides), (drows, dstrides), w = _rows(x), _rows(dy), _fp32(weight)
+        T = n // (H * D)
+        size = L.si_norm_rotary_bwd_workspace_bytes(T, H, D, freqs.shape[0]) if need_w else 0
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if need_w else None
+        rc = L.si_norm_rotary_bwd(drows.data_ptr(), dstrides, rows.data_ptr(), strides, None if w is None else w.data_ptr(), eps,
+                                  positions.data_ptr(), positions.dtype is torch.int64, positions.numel(), freqs.data_ptr(),
+                                  freqs.shape[0], start, halves, magnitude, inverse, T, H, D, dt, dx.data_ptr(),
+                                  None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(), size,
+                                  _lib.stream_ptr(dev))
+    _lib.check(rc)
+    return dx, None if dw is None else dw if weight.dtype is torch.float32 else dw.to(weight.dtype), None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 class _RotaryFunc(torch.autograd.Function):
@@ -143,36 +185,16 @@ class _RotaryFunc(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, positions, freqs, args):
-        norm = args[0] is not None
-        ctx.save_for_backward(positions, freqs, *((x, weight) if norm and weight is not None else (x,) if norm else ()))
+        if args[0] is None:
+            ctx.save_for_backward(positions, freqs)
+        elif weight is None:
+            ctx.save_for_backward(positions, freqs, x)
+        else:
+            ctx.save_for_backward(positions, freqs, x, weight)
         ctx.args = args
-        return _forward(x.detach(), None if weight is None else weight.detach(), positions, freqs, args)
+        return _forward(x, weight, positions, freqs, args)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        positions, freqs, *saved = ctx.saved_tensors
-        eps, halves, start, magnitude, inverse, dt = ctx.args
-        if not saved:
-            return _forward(dy, None, positions, freqs, (None, halves, start, magnitude, not inverse, dt)), None, None, None, None
-        x, weight = saved[0], saved[1] if len(saved) > 1 else None
-        need_w = weight is not None and ctx.needs_input_grad[1]
-        dev = x.device
-        L = _lib.load()
-        with _lib.on_device(dev):
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-            D = x.shape[-1]
-            dw = torch.empty(D, dtype=torch.float32, device=dev) if need_w else None
-            if x.numel() == 0:
-                return dx, None if dw is None else dw.zero_().to(weight.dtype), None, None, None
-            rows, drows, w = _rows(x), _rows(dy), _fp32(weight)
-            T, H, _ = rows.shape
-            size = L.si_norm_rotary_bwd_workspace_bytes(T, H, D, freqs.shape[0]) if need_w else 0
-            ws = torch.empty(size, dtype=torch.uint8, device=dev) if need_w else None
-            rc = L.si_norm_rotary_bwd(
-                drows.data_ptr(), _lib.stride_array(drows.stride()), rows.data_ptr(), _lib.stride_array(rows.stride()),
-                None if w is None else w.data_ptr(), eps, positions.data_ptr(), positions.dtype is torch.int64, positions.numel(),
-                freqs.data_ptr(), freqs.shape[0], start, halves, magnitude, inverse, T, H, D, dt, dx.data_ptr(),
-                None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(), size, _lib.stream_ptr(dev))
-        _lib.check(rc)
-        return dx, None if dw is None else dw if weight.dtype is torch.float32 else dw.to(weight.dtype), None, None, None
+        # (a second derivative is an error; without one asked for, nothing has to see to that: 10 us)
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
