@@ -39,7 +39,8 @@ struct WriteQArgs {
 constexpr int kLeastExp = -64;
 constexpr int kRowThreads = 256;    // kernel of one token a scale
 constexpr int kBlockThreads = 512;  // kernel of blocks
-constexpr int kHeld = 9;            // pieces of a thread in registers; those behind are read twice
+constexpr int kHeld = 9;            // pieces of a row that a lane holds in registers; those behind are read twice
+constexpr int kHeldRows = 10;       // rows of a block of which a thread holds a piece: 64 of 72 pieces over 512 threads
 
 template <int DT>
 struct WqElem;
@@ -75,13 +76,54 @@ struct WqPiece<DT, 1> {
   __device__ __forceinline__ float at(int) const { return static_cast<float>(w); }
 };
 
-// The largest finite |x| of a piece and of m.
-template <typename P, int V>
-__device__ __forceinline__ float wq_max(const P& p, float m) {
+// Magnitudes are compared as their bits, 16-bit ones two at a time; a lane's largest is that of both halves.
+template <int DT, int V>
+__device__ __forceinline__ uint32_t wq_max(const WqPiece<DT, V>& p, uint32_t m) {
+  if constexpr (DT == 0) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const uint32_t x = __float_as_uint(p.at(e)) & 0x7fffffffu;
+      m = x > m ? x : m;
+    }
+    return m;
+  } else {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    uint32_t w[V == 1 ? 1 : V / 2];
+    if constexpr (V == 1) w[0] = __builtin_bit_cast(uint16_t, p.w);
+    else __builtin_memcpy(w, &p.w, sizeof(w));
+#pragma unroll
+    for (uint32_t x : w)
+      m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                 __builtin_bit_cast(u16x2, x & 0x7fff7fffu)));
+    return m;
+  }
+}
+// The larger half, and the value of such bits.
+template <int DT>
+__device__ __forceinline__ uint32_t wq_half(uint32_t m) {
+  if constexpr (DT == 0) return m;
+  const uint32_t lo = m & 0xffffu, hi = m >> 16;
+  return lo > hi ? lo : hi;
+}
+template <int DT>
+__device__ __forceinline__ float wq_value(uint32_t bits) {
+  if constexpr (DT == 0) return __uint_as_float(bits);
+  else if constexpr (DT == 1) return __uint_as_float(bits << 16);
+  else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+}
+template <int DT>
+constexpr uint32_t kWqInf = DT == 0 ? 0x7f800000u : DT == 1 ? 0x7f80u : 0x7c00u;
+// The same of the finite values alone: rows that hold others go through this.
+template <int DT, int V>
+__device__ __forceinline__ uint32_t wq_max_finite(const WqPiece<DT, V>& p, uint32_t m) {
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const float x = __builtin_fabsf(p.at(e));
-    m = x < __builtin_inff() && x > m ? x : m;
+    uint32_t x;
+    if constexpr (DT == 0) x = __float_as_uint(p.at(e));
+    else if constexpr (DT == 1) x = __float_as_uint(p.at(e)) >> 16;
+    else x = __builtin_bit_cast(uint16_t, static_cast<_Float16>(p.at(e)));
+    x &= DT == 0 ? 0x7fffffffu : 0x7fffu;
+    m = x < kWqInf<DT> && x > m ? x : m;
   }
   return m;
 }
@@ -141,17 +183,26 @@ __global__ __launch_bounds__(kRowThreads) void paged_write_q_rows_kernel(WriteQA
   const int64_t slot = a.slots[row];
   if (slot < 0 || slot >= a.nslots) return;
   const WqSlot at = wq_slot(a, slot);
-  float m = 0.f;
+  auto largest = [&](auto&& of) {
+    uint32_t m = 0;
 #pragma unroll
-  for (int c = 0; c < kHeld; ++c)
-    if (static_cast<uint32_t>(c * lpr + lane) < a.pieces) m = wq_max<P, V>(held[c], m);
-  for (uint32_t i = kHeld * lpr + lane; i < a.pieces; i += lpr) {
-    P p;
-    p.load(src + static_cast<int64_t>(i) * (V * SIZE));
-    m = wq_max<P, V>(p, m);
-  }
-  for (int k = 1; k < lpr; k *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, k));
-  const int e = wq_exp(m);
+    for (int c = 0; c < kHeld; ++c)
+      if (static_cast<uint32_t>(c * lpr + lane) < a.pieces) m = of(held[c], m);
+    for (uint32_t i = kHeld * lpr + lane; i < a.pieces; i += lpr) {
+      P p;
+      p.load(src + static_cast<int64_t>(i) * (V * SIZE));
+      m = of(p, m);
+    }
+    m = wq_half<DT>(m);
+    for (int k = 1; k < lpr; k *= 2) {
+      const uint32_t x = __shfl_xor(m, k);
+      m = x > m ? x : m;
+    }
+    return m;
+  };
+  uint32_t m = largest([](const P& p, uint32_t x) { return wq_max<DT, V>(p, x); });
+  if (__builtin_expect(m >= kWqInf<DT>, 0)) m = largest([](const P& p, uint32_t x) { return wq_max_finite<DT, V>(p, x); });
+  const int e = wq_exp(wq_value<DT>(m));
   const float inv = wq_pow2(-e);
   uint8_t* dst = a.codes + at.page * a.pstride + at.off * a.cstride;
 #pragma unroll
@@ -169,12 +220,15 @@ __global__ __launch_bounds__(kRowThreads) void paged_write_q_rows_kernel(WriteQA
 
 // A scale for each block.
 template <int DT, int V>
-__global__ __launch_bounds__(kBlockThreads) void paged_write_q_blocks_kernel(WriteQArgs a) {
+__global__ __launch_bounds__(kBlockThreads, DT == 0 ? 2 : 4) void paged_write_q_blocks_kernel(WriteQArgs a) {
   typedef WqPiece<DT, V> P;
   constexpr int SIZE = DT == 0 ? 4 : 2, WAVES = kBlockThreads / kWave;
-  __shared__ float max_lds[WAVES];
+  __shared__ uint32_t max_lds[2][WAVES];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.chunk, r1 = r0 + a.chunk < a.n ? r0 + a.chunk : a.n;
+  // A thread takes one piece of every step-th row of a run (rows of more pieces than threads: every 512th piece of each row).
+  const uint32_t cols = a.pieces < kBlockThreads ? a.pieces : kBlockThreads, step = kBlockThreads / cols;
+  const uint32_t tr = t / cols, tc = t - tr * cols;
   auto slot_at = [&](int64_t r) {
     const int64_t s = r >= 0 && r < a.n ? a.slots[r] : -1;
     return s < a.nslots ? s : -1;
@@ -210,7 +264,7 @@ __global__ __launch_bounds__(kBlockThreads) void paged_write_q_blocks_kernel(Wri
     const uint32_t blk = at.off / a.block, first = at.off - blk * a.block;
     // its rows, up to the last one with a slot
     int run = 1;
-    bool gaps = false;
+    bool gaps = false, apart = false;  // rows without a slot; slots that do not follow each other
     {
       const int64_t end = slot + (a.block - first);
       int64_t last = slot;
@@ -223,6 +277,7 @@ __global__ __launch_bounds__(kBlockThreads) void paged_write_q_blocks_kernel(Wri
         const uint64_t ours = __builtin_amdgcn_ballot_w64(next >= 0) & mask;
         if (ours) {
           const int to = 63 - __builtin_clzll(ours);
+          apart = apart || (__builtin_amdgcn_ballot_w64(next >= 0 && next != prev2 + 1) & mask);
           gaps = gaps || w - (r + run) + to + 1 != __builtin_popcountll(ours);
           run = static_cast<int>(w - r) + to + 1;
           last = __shfl(next, to);
@@ -232,55 +287,81 @@ __global__ __launch_bounds__(kBlockThreads) void paged_write_q_blocks_kernel(Wri
     }
     const float old = first > 0 ? a.scales[at.page * a.spage + blk] : 0.f;
     uint8_t* base = a.codes + at.page * a.pstride + static_cast<int64_t>(blk) * a.block * a.cstride;
-    const uint32_t total = static_cast<uint32_t>(run) * a.pieces;
-    auto source = [&](uint32_t i, uint32_t& row, uint32_t& c) {
-      row = i / a.pieces;
-      c = i - row * a.pieces;
-      return a.rows + ((r + row) * a.rstride + static_cast<int64_t>(c) * V) * SIZE;
+    const uint32_t rows = static_cast<uint32_t>(run);
+    const bool hold = a.pieces <= kBlockThreads && rows <= kHeldRows * step && !gaps && !apart;  // (the same in every thread)
+    auto source = [&](uint32_t row, uint32_t c) { return a.rows + ((r + row) * a.rstride + static_cast<int64_t>(c) * V) * SIZE; };
+    auto has_slot = [&](uint32_t row) { return !gaps || slot_at(r + row) >= 0; };
+    // rows that are not held, piece by piece
+    auto each = [&](auto&& f) {
+      if (tr < step)
+#pragma unroll 1
+        for (uint32_t row = tr; row < rows; row += step) {
+          if (!has_slot(row)) continue;
+          for (uint32_t c = tc; c < a.pieces; c += kBlockThreads) {
+            P p;
+            p.load(source(row, c));
+            f(row, c, p);
+          }
+        }
     };
-    auto has_slot = [&](uint32_t i) { return !gaps || slot_at(r + i / a.pieces) >= 0; };
-    P held[kHeld];
-    float m = 0.f;
+    // (an opaque copy of the first row: what depends on it alone would be kept in registers from run to run)
+    uint32_t row0 = tr < step ? tr : 0x7fffffffu;
+    asm volatile("" : "+v"(row0));
+    P held[kHeldRows];
+    if (hold) {
+      const char* at0 = source(tr, tc);
+      const int64_t rise = step * a.rstride * SIZE;
+      uint32_t row = row0;
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const uint32_t i = k * kBlockThreads + t;
-      uint32_t row, c;
-      if (i < total) held[k].load(source(i, row, c));
+      for (int k = 0; k < kHeldRows; ++k) {
+        if (row < rows) held[k].load(at0);
+        row += step;
+        at0 += rise;
+      }
     }
+    auto joined = [&](uint32_t x, uint32_t* lds) {  // the largest of all threads
+      x = wave_max_u32(x);
+      if (lane == 0) lds[wave] = x;
+      __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k)
-      if (static_cast<uint32_t>(k * kBlockThreads + t) < total && has_slot(k * kBlockThreads + t)) m = wq_max<P, V>(held[k], m);
-    for (uint32_t i = kHeld * kBlockThreads + t; i < total; i += kBlockThreads) {
-      uint32_t row, c;
-      P p;
-      p.load(source(i, row, c));
-      if (has_slot(i)) m = wq_max<P, V>(p, m);
+      for (int w = 0; w < WAVES; ++w) x = lds[w] > x ? lds[w] : x;
+      return x;
+    };
+    uint32_t m = 0;
+    if (hold) {
+      uint32_t row = row0;
+#pragma unroll
+      for (int k = 0; k < kHeldRows; ++k) {
+        if (row < rows) m = wq_max<DT, V>(held[k], m);
+        row += step;
+      }
+    } else {
+      each([&](uint32_t, uint32_t, const P& p) { m = wq_max<DT, V>(p, m); });
     }
-#pragma unroll
-    for (int k = 1; k < kWave; k *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, k));
-    if (lane == 0) max_lds[wave] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) m = __builtin_fmaxf(m, max_lds[w]);
-    const float need = wq_pow2(wq_exp(m));
+    m = joined(wq_half<DT>(m), max_lds[0]);
+    if (__builtin_expect(m >= kWqInf<DT>, 0)) {  // (the same in every thread)
+      m = 0;
+      each([&](uint32_t, uint32_t, const P& p) { m = wq_max_finite<DT, V>(p, m); });
+      m = joined(m, max_lds[1]);
+    }
+    const float need = wq_pow2(wq_exp(wq_value<DT>(m)));
     const bool kept = old > 0.f && old < __builtin_inff();  // (earlier tokens with a scale that is one)
     const float scale = kept && old > need ? old : need, inv = 1.0f / scale;
-    auto put = [&](uint32_t i, const P& p) {
-      const uint32_t row = i / a.pieces, c = i - row * a.pieces;
-      const int64_t s = row ? slot_at(r + row) : slot;
-      if (s < 0) return;
-      wq_store<V>(base + (first + (s - slot)) * a.cstride + static_cast<int64_t>(c) * V, p, inv);
-    };
+    if (hold) {
+      uint8_t* to = base + (first + tr) * a.cstride + static_cast<int64_t>(tc) * V;
+      const int64_t rise = step * a.cstride;
+      uint32_t row = row0;
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const uint32_t i = k * kBlockThreads + t;
-      if (i < total) put(i, held[k]);
-    }
-    for (uint32_t i = kHeld * kBlockThreads + t; i < total; i += kBlockThreads) {
-      uint32_t row, c;
-      P p;
-      p.load(source(i, row, c));
-      put(i, p);
+      for (int k = 0; k < kHeldRows; ++k) {
+        if (row < rows) wq_store<V>(to, held[k], inv);
+        row += step;
+        to += rise;
+      }
+    } else {
+      each([&](uint32_t row, uint32_t c, const P& p) {
+        const int64_t s = row ? slot_at(r + row) : slot;
+        wq_store<V>(base + (first + (s - slot)) * a.cstride + static_cast<int64_t>(c) * V, p, inv);
+      });
     }
     if (kept && scale > old) {  // earlier tokens to the new scale
       const float ratio = old / scale;
@@ -336,8 +417,8 @@ extern "C" int si_paged_write_q(const void* rows, int64_t row_stride, int dtype,
       break;
     }
   }
-  // (a run has at most 64 rows for each of its slots: its pieces are counted in 32 bits)
-  if (block * (D / vec) > 1 << 25) return set_error(SI_ERR_UNSUPPORTED, "blocks of more than 2^25 pieces");
+  // (a run has at most 64 rows for each of its slots, counted in 31 bits, and a block's pieces are counted in 32)
+  if (block > 1 << 24 || block * (D / vec) > 0x7fffffff) return set_error(SI_ERR_UNSUPPORTED, "blocks of more than 2^24 tokens");
   WriteQArgs a{};
   a.rows = static_cast<const char*>(rows);
   a.rstride = row_stride;
