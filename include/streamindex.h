@@ -523,7 +523,7 @@ int si_paged_write_q(const void* rows, int64_t row_stride, int dtype, const int6
  * no others; scales of seen keys are finite.
  */
 int64_t si_paged_attn_q_fwd_scratch_bytes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys,
-                                          int64_t keys2, int qkv_dtype);
+                                          int64_t keys2);
 int si_paged_attn_q_fwd(const void* q, const int64_t* q_strides, const void* kv, const int64_t* kv_strides,
                         const float* scales, int64_t scale_stride, int64_t block, int64_t pages, int64_t page_size,
                         const int32_t* block_table, int64_t table_stride, int64_t P, const void* kv2,

@@ -92,7 +92,7 @@ SIGNATURES = {
                                  _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, ctypes.c_float, _I32,
                                  _P, _P, _P, _I64, _P]),
     "si_paged_write_q": (_I32, [_P, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P]),
-    "si_paged_attn_q_fwd_scratch_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32]),
+    "si_paged_attn_q_fwd_scratch_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "si_paged_attn_q_fwd": (_I32, [_P, _I64P, _P, _I64P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64P, _P, _I64, _I64,
                                    _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, ctypes.c_float,
                                    _I32, _P, _P, _P, _I64, _P]),

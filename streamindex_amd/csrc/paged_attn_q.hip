@@ -10,8 +10,13 @@
 //     they are, with Q as a sum of e4m3 pieces, but sum eight products at a time to 2^-13 of the largest.  Measured: one of
 //     900 beside one of 65,536 comes back as 896.)
 //   * A score is (accumulator) x (s_k x the softmax scale), in fp32.
-//   * O^T += V^T P^T with V's codes converted to bf16 on their way from LDS, where each is read by one wave, and P s_k
-//     rounded to bf16 (fp16 outputs: the sum of two bf16, 16 bits), so that the scales cost no pass over V.
+//   * O^T += V^T P^T with V's codes converted on their way from LDS, where each is read by one wave, and P s_k rounded to q's
+//     type, so that the scales cost no pass over V.
+//
+// Bound, long keys: issue.  Two vector instructions beside a matrix instruction cost it a third of its time, and four waves convert
+// each code for S^T.  (Converting each code once, into a second ring of tiles in LDS from which S^T and P V read elements,
+// was slower all the same: 742 TFLOP/s at D = 512 and 688 at 256, against 888 and 940, one request of 8,192 earlier tokens,
+// 64 heads, 1,024 and 2,048 new ones.)
 //
 // A masked key's code NaN is zeroed in LDS before P V (0 x NaN is NaN); every row that sees it has a score of NaN.
 #include <cstdint>
@@ -39,7 +44,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 // PAIR: tiles of 32 keys, a tile's steps one after the other, and one workgroup more a CU, which fills the gaps.
-template <int D, bool F16, bool PAIR>
+template <int D, bool PAIR>
 struct QShape {
   static constexpr int TK = PAIR ? 32 : 64;      // keys of a tile
   static constexpr int CPR = D / 16;             // 16-byte chunks of a key row
@@ -49,15 +54,12 @@ struct QShape {
   static constexpr int LPT = (CH + kPagedThreads - 1) / kPagedThreads;  // copies of a thread
   static constexpr int LANDED = CH / kPagedThreads;                     // of every thread
   static constexpr int NG = D / 64;              // whole groups of 64 dimensions
-  static constexpr int PP = F16 ? 2 : 1;         // pieces of P
   static constexpr int MBT = D / 16;             // 16-dim output blocks
   static constexpr int MBW = (MBT + 3) / 4;      // per wave
-  static constexpr int NS = D == 512 && !F16 && !PAIR ? 4 : 3;  // tiles in LDS
+  static constexpr int NS = D == 512 && !PAIR ? 4 : 3;  // tiles in LDS
 };
 // Workgroups of a CU: LDS and registers set them.
-constexpr int q_per_cu(int D, bool F16, bool PAIR) {
-  return PAIR ? 2 : D >= 512 ? 1 : D == 256 ? (F16 ? 1 : 2) : D == 128 ? (F16 ? 2 : 3) : F16 ? 3 : 4;
-}
+constexpr int q_per_cu(int D, bool PAIR) { return PAIR ? 2 : D >= 512 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
 
 // Chunk c of key k is stored at c ^ q_swz(k), so that both reads of a tile spread over the banks: 16 keys 16 mb + 0 .. 15 at one
 // chunk (S^T), and keys 4 g + 0 .. 3 and 16 + 4 g + 0 .. 3 at one chunk (V^T).
@@ -112,18 +114,18 @@ struct QScaleView {
 };
 
 template <int D, bool F16, bool PAIR>
-__global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_attn_q_kernel(PagedAttnQArgs args) {
-  using SH = QShape<D, F16, PAIR>;
+__global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q_kernel(PagedAttnQArgs args) {
+  using SH = QShape<D, PAIR>;
   const PagedAttnArgs& a = args.a;
   constexpr int TK = SH::TK, MB = TK / 16, KSTEPS = TK / 32;
-  constexpr int MBW = SH::MBW, ROW = SH::ROW, NG = SH::NG, PP = SH::PP;
+  constexpr int MBW = SH::MBW, ROW = SH::ROW, NG = SH::NG;
   constexpr int M = kRows, NB = M / 16;
   constexpr int NS = SH::NS, AHEAD = NS - 1, PAGES = 4, NP = PAIR ? 1 : 2;
   constexpr float kLn2 = 0.6931471805599453f;
   constexpr int PARTS = NS * SH::TILE >= M * D * 2 ? 1 : 2;  // of the output, staged in the tiles' LDS
   static_assert(NS * SH::TILE >= M * D * 2 / PARTS, "the output is staged in the tiles' LDS");
   __shared__ __attribute__((aligned(16))) char kv_lds[NS * SH::TILE];
-  __shared__ __attribute__((aligned(16))) char p_lds[NP][PP][KSTEPS][NB * 64 * 16];
+  __shared__ __attribute__((aligned(16))) char p_lds[NP][KSTEPS][NB * 64 * 16];
   __shared__ __attribute__((aligned(16))) float alpha_lds[NP][M];
   __shared__ float sink_lds[M];
   __shared__ __attribute__((aligned(16))) int flag_lds[NP][4];
@@ -402,9 +404,14 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_a
   scalar_tie(all2hi);
 
   // ---- softmax -----------------------------------------------------------------
-  // Weights are 2^(score - m_ref), from 2^-32 on where the reference is set, up to 1, where it moves: see the 16-bit kernel.
-  // Both types' weights travel as bf16, with fp32's range, so P times a scale loses bits only below 2^-126.
-  constexpr float kHead = -32.0f, kLazy = 32.0f;
+  // Weights are 2^(score - m_ref), and their products with the scales go to P V.  bf16: the 16-bit kernel's references, from 2^-32
+  // to 1, the products having fp32's range.  fp16: 2^11 to 2^15 is where the largest product with a scale lies, so that 2^-25
+  // of it keeps its 11 bits; the reference is that of the scores plus the exponents of their scales (from 2^-80 on: the weights'
+  // sum stays in range).
+  constexpr float kHead = F16 ? 11.0f : -32.0f, kLazy = F16 ? 4.0f : 32.0f;
+  auto above = [&](float x, float scale) __attribute__((always_inline)) {  // what the reference counts of a score
+    return F16 ? x + static_cast<float>(max(__builtin_amdgcn_frexp_expf(scale), -80)) : x;
+  };
   float m_ref = kNever, l_run = 0.f;
   int skey = 0;
   auto softmax_begin = [&](int t, uint64_t okmask, f32x4 (&st)[MB], f32x4 (&sc)[MB], float& ref, int pbuf) __attribute__((always_inline)) {
@@ -428,9 +435,9 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_a
         for (int r = 0; r < 4; ++r) {
           const bool ok = static_cast<uint32_t>(16 * mb + g4 + r + lo) < static_cast<uint32_t>(cnt) && ((mine >> (16 * mb + r)) & 1);
           odd = odd || (!ok && !(__builtin_fabsf(st[mb][r]) < __builtin_inff()));
-          st[mb][r] = ok ? st[mb][r] * (sc[mb][r] * rscale) : kNever;
           sc[mb][r] = ok ? sc[mb][r] : 0.f;  // (a masked key's scale may be anything)
-          lmax = __builtin_fmaxf(lmax, st[mb][r]);
+          st[mb][r] = ok ? st[mb][r] * (sc[mb][r] * rscale) : kNever;
+          lmax = __builtin_fmaxf(lmax, above(st[mb][r], sc[mb][r]));
         }
       flags = __builtin_amdgcn_ballot_w64(odd) ? kOdd : 0;
     } else {
@@ -439,7 +446,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_a
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           st[mb][r] = st[mb][r] * (sc[mb][r] * rscale);
-          lmax = __builtin_fmaxf(lmax, st[mb][r]);
+          lmax = __builtin_fmaxf(lmax, above(st[mb][r], sc[mb][r]));
         }
     }
     skey = static_cast<int>(static_cast<uint32_t>(skey) + static_cast<uint32_t>(TK));
@@ -471,18 +478,8 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_a
 #pragma unroll
     for (int s = 0; s < KSTEPS; ++s) {
       const f32x4 x = p[2 * s] * sc[2 * s], y = p[2 * s + 1] * sc[2 * s + 1];
-      const u32x4 w = u32x4{f32x2_to_bf16x2(x[0], x[1]), f32x2_to_bf16x2(x[2], x[3]), f32x2_to_bf16x2(y[0], y[1]),
-                            f32x2_to_bf16x2(y[2], y[3])};
-      asm volatile("ds_write_b128 %0, %1" ::"v"(lds_addr(&p_lds[pbuf][0][s][ln16])), "v"(w) : "memory");
-      if constexpr (PP == 2) {
-        u32x4 v;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const f32x4& z = c < 2 ? x : y;
-          v[c] = f32x2_to_bf16x2(z[2 * (c & 1)] - elem_lo<false>(w[c]), z[2 * (c & 1) + 1] - elem_hi<false>(w[c]));
-        }
-        asm volatile("ds_write_b128 %0, %1" ::"v"(lds_addr(&p_lds[pbuf][PP - 1][s][ln16])), "v"(v) : "memory");
-      }
+      const u32x4 w = u32x4{pack2<F16>(x[0], x[1]), pack2<F16>(x[2], x[3]), pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3])};
+      asm volatile("ds_write_b128 %0, %1" ::"v"(lds_addr(&p_lds[pbuf][s][ln16])), "v"(w) : "memory");
     }
   };
 
@@ -503,11 +500,11 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_a
       vbase[0] = at + 64 * (f >> 2);
       vbase[1] = at - 64 * (f >> 2);
     }
-    bf16x8 pf[PP][KSTEPS][NB];
-    const uint32_t psrc = lds_addr(&p_lds[pbuf][0][0][0]) + ln * 16;
-    attn_static_for<0, PP * KSTEPS * NB>([&](auto NC) {
+    bf16x8 pf[KSTEPS][NB];
+    const uint32_t psrc = lds_addr(&p_lds[pbuf][0][0]) + ln * 16;
+    attn_static_for<0, KSTEPS * NB>([&](auto NC) {
       constexpr int n = decltype(NC)::value;
-      pf[n / (KSTEPS * NB)][n / NB % KSTEPS][n % NB] = ld128<1024 * n>(psrc);
+      pf[n / NB][n % NB] = ld128<1024 * n>(psrc);
     });
     i32x2 v[VQ][KSTEPS];
     auto issue = [&](auto JC) __attribute__((always_inline)) {
@@ -525,20 +522,16 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_a
       if constexpr (KSTEPS == 2) reg_tie(v[j % VQ][KSTEPS - 1]);
       if constexpr (j == 0) {
 #pragma unroll
-        for (int p = 0; p < PP; ++p)
+        for (int s = 0; s < KSTEPS; ++s)
 #pragma unroll
-          for (int s = 0; s < KSTEPS; ++s)
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) reg_tie(pf[p][s][nb]);
+          for (int nb = 0; nb < NB; ++nb) reg_tie(pf[s][nb]);
       }
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
         const i32x2 c = v[j % VQ][s];
-        const bf16x8 vf = codes8<false>(c[0], c[1]);
+        const bf16x8 vf = codes8<F16>(c[0], c[1]);
 #pragma unroll
-        for (int p = 0; p < PP; ++p)
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) oacc[j][nb] = mfma16x16x32<false>(vf, pf[p][s][nb], oacc[j][nb]);
+        for (int nb = 0; nb < NB; ++nb) oacc[j][nb] = mfma16x16x32<F16>(vf, pf[s][nb], oacc[j][nb]);
       }
       if constexpr (j + VQ < MBW) issue(std::integral_constant<int, j + VQ>{});
       between(JC);
@@ -775,7 +768,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, F16, PAIR)) void paged_a
 }
 
 // Row blocks from which PAIR is taken.
-constexpr int64_t q_pair_from(int64_t D, bool f16) { return D >= 512 ? 257 : INT64_MAX; }
+constexpr int64_t q_pair_from(int64_t D) { return D >= 512 ? 257 : INT64_MAX; }
 
 // Sizes of a call, from what the host knows.
 struct PagedQSizes {
@@ -788,15 +781,15 @@ struct PagedQSizes {
   int64_t bytes;         // scratch
   int behind;            // tokens of a row block before its last one at most
 };
-static PagedQSizes q_sizes(int64_t N, int64_t H, int64_t D, bool f16, int64_t R, int64_t window, int64_t keys1, int64_t keys2) {
+static PagedQSizes q_sizes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys1, int64_t keys2) {
   PagedQSizes p{};
   const int64_t M = kRows;
   // a request's last row block is part empty unless M divides n H
   int64_t g = M;
   while (H % g) g /= 2;
   p.blocks = (N * H + (R < N ? R : N) * (M - g)) / M;
-  p.pair = p.blocks >= q_pair_from(D, f16);
-  const int64_t want = p.want = 256 * q_per_cu(static_cast<int>(D), f16, p.pair), tile = p.pair ? 32 : 64;
+  p.pair = p.blocks >= q_pair_from(D);
+  const int64_t want = p.want = 256 * q_per_cu(static_cast<int>(D), p.pair), tile = p.pair ? 32 : 64;
   p.grid = 2 * p.blocks <= want ? want : p.blocks + want;
   const int64_t span = M / H + 1 + window;
   p.behind = static_cast<int>((M - 1 + H - g) / H);  // (a row block begins at any multiple of g heads of a token)
@@ -824,7 +817,7 @@ static int launch_paged_attn_q(bool f16, const PagedAttnQArgs& a, const PagedQSi
   const dim3 grid(static_cast<unsigned>(((p.grid < 1 ? 1 : p.grid) + 7) & ~int64_t{7})), block(kPagedThreads);
   auto launch = [&](auto F16) {
     constexpr bool half = decltype(F16)::value;
-    if constexpr (q_pair_from(D, half) < INT64_MAX) {
+    if constexpr (q_pair_from(D) < INT64_MAX) {
       if (p.pair) {
         hipLaunchKernelGGL((paged_attn_q_kernel<D, half, true>), grid, block, 0, st, a);
         return;
@@ -865,12 +858,12 @@ static int set_scales(QScales& s, const float* scales, int64_t stride, int64_t b
 using namespace si;
 
 extern "C" int64_t si_paged_attn_q_fwd_scratch_bytes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys,
-                                                     int64_t keys2, int qkv_dtype) {
+                                                     int64_t keys2) {
   const int64_t lim = 0x7fffffff;
   if (N <= 0 || H <= 0 || R <= 0 || window < 0 || keys < 0 || keys2 < 0 || !paged_attn_served(D) || N > lim || H > lim ||
       N * H > lim || R > lim)
     return 0;
-  return q_sizes(N, H, D, qkv_dtype == SI_DTYPE_F16, R, window == 0 || window > lim ? lim : window, keys < lim ? keys : lim,
+  return q_sizes(N, H, D, R, window == 0 || window > lim ? lim : window, keys < lim ? keys : lim,
                  keys2 < lim ? keys2 : lim).bytes;
 }
 
@@ -923,7 +916,7 @@ extern "C" int si_paged_attn_q_fwd(const void* q, const int64_t* q_strides, cons
   a.R = static_cast<int>(R);
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   const bool f16 = qkv_dtype == SI_DTYPE_F16;
-  PagedQSizes p = q_sizes(N, H, D, f16, R > 0 ? R : 1, a.window, paged_cache_keys(pages, P, page_size),
+  PagedQSizes p = q_sizes(N, H, D, R > 0 ? R : 1, a.window, paged_cache_keys(pages, P, page_size),
                           ratio > 0 ? paged_cache_keys(pages2, P2, page_size2) : 0);
   a.want = static_cast<int>(p.want);
   a.behind = p.behind;

@@ -98,7 +98,7 @@ def paged_attn_q_fwd(q: torch.Tensor, kv_cache: torch.Tensor, kv_scales: torch.T
       kv_scales, kv2_scales: ``[pages, blocks]`` fp32, ``blocks`` a divisor of the page size, any finite values.
       The others: as there.
     Returns:
-      ``(o [N, H, D] in q's type, lse [N, H] fp32)``.  Weights times scales are rounded to bf16 (with fp16 queries to 16 bits).
+      ``(o [N, H, D] in q's type, lse [N, H] fp32)``.  Weights times scales are rounded to q's type.
       A row without a key gets ``o = 0`` and ``lse = sink`` (or ``-1e30`` if the sink is ``-inf``).  A code of NaN reaches the
       rows that see its key and no others; so does a scale that is not finite.  Scores are fp32: one below its range weighs
       nothing, one above it makes its row NaN.
@@ -148,7 +148,7 @@ def paged_attn_q_fwd(q: torch.Tensor, kv_cache: torch.Tensor, kv_scales: torch.T
     with _lib.on_device(dev):
         o = torch.empty((N, H, D), dtype=dtype, device=dev)
         lse = torch.empty((N, H), dtype=torch.float32, device=dev)
-        scratch, nscratch = _lib.scratch(_attn_scratch(N, H, D, R, window, c1[6] * c1[9], c2[6] * c2[9], dt), dev)
+        scratch, nscratch = _lib.scratch(_attn_scratch(N, H, D, R, window, c1[6] * c1[9], c2[6] * c2[9]), dev)
         rc = L.si_paged_attn_q_fwd(q.data_ptr(), _lib.strides(q), *c1, *c2, window, ratio, cu.data_ptr(), lens.data_ptr(),
                                    attn_sink.data_ptr(), N, H, D, R, D ** -0.5 if softmax_scale is None else float(softmax_scale),
                                    dt, o.data_ptr(), lse.data_ptr(), None if scratch is None else scratch.data_ptr(), nscratch,

@@ -80,8 +80,8 @@ def test_attn_refusals(lib, kw, word, rc):
 
 def test_attn_scratch(lib):
     need = lib.si_paged_attn_q_fwd_scratch_bytes
-    assert need(1, 64, 576, 1, 128, 64 * 64, 64 * 64, 0) > 0
-    assert need(1, 64, 576, 1, 0, 128, 0, 0) == 0  # two tiles: never split
-    assert need(0, 64, 576, 1, 0, 4096, 0, 0) == 0 and need(4, 64, 96, 1, 0, 4096, 0, 0) == 0
-    for dtype in (0, 1):  # bounded whatever the lengths
-        assert 0 < need(1 << 20, 64, 576, 64, 0, 1 << 40, 1 << 40, dtype) < 1 << 28
+    assert need(1, 64, 576, 1, 128, 64 * 64, 64 * 64) > 0
+    assert need(1, 64, 576, 1, 0, 128, 0) == 0  # two tiles: never split
+    assert need(0, 64, 576, 1, 0, 4096, 0) == 0 and need(4, 64, 96, 1, 0, 4096, 0) == 0
+    # bounded whatever the lengths
+    assert 0 < need(1 << 20, 64, 576, 64, 0, 1 << 40, 1 << 40) < 1 << 28
