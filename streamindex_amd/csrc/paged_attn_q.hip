@@ -90,21 +90,30 @@ __device__ __forceinline__ i32x2 ldq64(uint32_t addr) {
   asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(OFF));
   return r;
 }
-// Eight codes as elements of the type (exact).
+// lds_wait for any registers.
+template <int N, typename T>
+__device__ __forceinline__ void lds_wait_for(T& x, T& y) {
+  asm volatile("s_waitcnt lgkmcnt(%2)" : "+v"(x), "+v"(y) : "n"(N));
+}
+template <int N, typename T>
+__device__ __forceinline__ void lds_wait_one(T& x) {
+  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(x) : "n"(N));
+}
+// Two of four codes as elements of the type (exact).
+template <bool F16>
+__device__ __forceinline__ uint32_t codes2(int codes, bool high) {
+  const uint32_t x = static_cast<uint32_t>(codes);
+  if constexpr (F16) {
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
+  } else {
+    return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true)
+                                             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false));
+  }
+}
 template <bool F16>
 __device__ __forceinline__ bf16x8 codes8(int lo, int hi) {
-  const uint32_t x = static_cast<uint32_t>(lo), y = static_cast<uint32_t>(hi);
-  if constexpr (F16) {
-    return __builtin_bit_cast(bf16x8, u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false)),
-                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true)),
-                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.0f, false)),
-                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.0f, true))});
-  } else {
-    return __builtin_bit_cast(bf16x8, u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false)),
-                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true)),
-                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.0f, false)),
-                                            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.0f, true))});
-  }
+  return __builtin_bit_cast(bf16x8, u32x4{codes2<F16>(lo, false), codes2<F16>(lo, true), codes2<F16>(hi, false), codes2<F16>(hi, true)});
 }
 
 struct QScaleView {
@@ -340,9 +349,10 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q
   };
 
   // ---- S^T -------------------------------------------------------------------
-  // Unit u: 16 keys of one group of 64 dimensions, groups outermost.  A-fragments: key 16 mb + i16, chunk 4 j + g (D = 32: half a
-  // chunk).
-  constexpr int UNITS = QG * MB, QD = PAIR || UNITS < 4 ? 2 : 4;
+  // Pair n: 32 keys, 16 mb and 16 (mb + 1) on, of one group j of 64 dimensions, groups outermost.  A-fragments: key 16 mb + i16,
+  // chunk 4 j + g (D = 32: half a chunk).  The codes of pair n + 1 are converted between the MFMAs of pair n, whose accumulators
+  // alternate; with PAIR, where registers are short and the other workgroup fills the gaps, 16 keys' in front of their own.
+  constexpr int PAIRS = QG * MB / 2, QP = PAIRS < 2 ? PAIRS : 2;
   auto qk = [&](int slot, f32x4 (&st)[MB], f32x4 (&sc)[MB], auto&& start, auto&& beside) __attribute__((always_inline)) {
     const uint32_t tile = lds_addr(ring(slot));
     const int ln = lane_now(), lg = ln >> 4, lk = ln & 15;
@@ -355,34 +365,89 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q
       kbase[b][1] = at - 64 * (f >> 2);
     }
     const uint32_t sat = lds_addr(reinterpret_cast<const char*>(&scale_lds[wave][slot][0])) + 16 * lg;
-    i32x4 s4[MB];
-    typename std::conditional<D == 32, i32x2, i32x4>::type k[QD];
-    auto issue = [&](auto UC) __attribute__((always_inline)) {
-      constexpr int u = decltype(UC)::value, j = u / MB, mb = u % MB;
-      const uint32_t at = kbase[mb & 1][j & 1];
-      if constexpr (D == 32) k[u % QD] = ldq64<16 * ROW * mb>(at);
-      else k[u % QD] = ldq<64 * j + 16 * ROW * mb>(at);
+    typedef typename std::conditional<D == 32, i32x2, i32x4>::type Codes;
+    auto ask = [&](auto JC, auto BC) __attribute__((always_inline)) {  // 16 keys of a group
+      constexpr int j = decltype(JC)::value, mb = decltype(BC)::value;
+      if constexpr (D == 32) return ldq64<16 * ROW * mb>(kbase[mb & 1][0]);
+      else return ldq<64 * j + 16 * ROW * mb>(kbase[mb & 1][j & 1]);
     };
-    attn_static_for<0, QD>(issue);
+    i32x4 s4[MB];
+    auto ask_scales = [&]() __attribute__((always_inline)) {  // behind the last codes
+      attn_static_for<0, MB>([&](auto BC) {
+        constexpr int mb = decltype(BC)::value;
+        s4[mb] = ldq<64 * mb>(sat);
+      });
+    };
+    if constexpr (PAIR) {
+      Codes k[2];
+      k[0] = ask(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+      k[1] = ask(std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{});
+      start();
+      static_assert(!PAIR || MB == 2, "tiles of 32 keys");
+      st[0] = st[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      attn_static_for<0, 2 * QG>([&](auto UC) {
+        constexpr int u = decltype(UC)::value, j = u / 2, b = u % 2;
+        constexpr int later = u + 1 < 2 * QG ? 1 : MB;
+        lds_wait_one<later>(k[b]);
+#pragma unroll
+        for (int h = 0; h < QH; ++h) st[b] = mfma16x16x32<F16>(codes8<F16>(k[b][2 * h], k[b][2 * h + 1]), qf[j][h], st[b]);
+        if constexpr (j + 1 < QG) k[b] = ask(std::integral_constant<int, j + 1>{}, std::integral_constant<int, b>{});
+        else if constexpr (b == 0) ask_scales();
+        beside(UC);
+      });
+    } else {
+    Codes k[QP][2];
+    auto issue = [&](auto NC) __attribute__((always_inline)) {  // pair n; behind the last one the scales
+      constexpr int n = decltype(NC)::value, j = n / (MB / 2), b = 2 * (n % (MB / 2));
+      if constexpr (n < PAIRS) {
+        k[n % QP][0] = ask(std::integral_constant<int, j>{}, std::integral_constant<int, b>{});
+        k[n % QP][1] = ask(std::integral_constant<int, j>{}, std::integral_constant<int, b + 1>{});
+      } else if constexpr (n == PAIRS) {
+        ask_scales();
+      }
+    };
+    auto wait = [&](auto NC) __attribute__((always_inline)) {  // for pair n, where those up to n - 1 + QP have been asked for
+      constexpr int n = decltype(NC)::value, last = n == 0 ? QP - 1 : n - 1 + QP;
+      constexpr int later = 2 * ((last < PAIRS - 1 ? last : PAIRS - 1) - n) + (last >= PAIRS ? MB : 0);
+      lds_wait_for<later>(k[n % QP][0], k[n % QP][1]);
+    };
+    attn_static_for<0, QP>(issue);
     start();
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) st[mb] = f32x4{0.f, 0.f, 0.f, 0.f};
-    attn_static_for<0, UNITS>([&](auto UC) {
-      constexpr int u = decltype(UC)::value, j = u / MB, mb = u % MB;
-      constexpr int later = (UNITS - 1 - u < QD - 1 ? UNITS - 1 - u : QD - 1) + (u > UNITS - QD ? MB : 0);
-      asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(k[u % QD]) : "n"(later));
+    bf16x8 f[QH][2];
+    auto convert = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < QH; ++h)
-        st[mb] = mfma16x16x32<F16>(codes8<F16>(k[u % QD][2 * h], k[u % QD][2 * h + 1]), qf[j][h], st[mb]);
-      if constexpr (u + QD < UNITS) issue(std::integral_constant<int, u + QD>{});
-      if constexpr (u == UNITS - QD) {  // the scales, behind the last codes
-        attn_static_for<0, MB>([&](auto BC) {
-          constexpr int b = decltype(BC)::value;
-          s4[b] = ldq<64 * b>(sat);
-        });
+#pragma unroll
+        for (int b = 0; b < 2; ++b) f[h][b] = codes8<F16>(k[slot][b][2 * h], k[slot][b][2 * h + 1]);
+    };
+    wait(std::integral_constant<int, 0>{});
+    convert(0);
+    issue(std::integral_constant<int, QP>{});
+    attn_static_for<0, PAIRS>([&](auto NC) {
+      constexpr int n = decltype(NC)::value, j = n / (MB / 2), b0 = 2 * (n % (MB / 2));
+      bf16x8 next[QH][2];
+      if constexpr (n + 1 < PAIRS) wait(std::integral_constant<int, n + 1>{});
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < QH; ++h)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          st[b0 + b] = mfma16x16x32<F16>(f[h][b], qf[j][h], st[b0 + b]);
+          if constexpr (n + 1 < PAIRS) next[h][b] = codes8<F16>(k[(n + 1) % QP][b][2 * h], k[(n + 1) % QP][b][2 * h + 1]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      if constexpr (n + 1 < PAIRS) {
+        issue(std::integral_constant<int, n + 1 + QP>{});
+#pragma unroll
+        for (int h = 0; h < QH; ++h)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) f[h][b] = next[h][b];
       }
-      beside(UC);
+      beside(NC);
     });
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s4[0]), "+v"(s4[1]));
     if constexpr (MB == 4) asm volatile("" : "+v"(s4[MB - 2]), "+v"(s4[MB - 1]));
 #pragma unroll
@@ -514,27 +579,57 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q
         v[j % VQ][s] = tr_read8<64 * j + 32 * ROW * s>(vbase[j & 1]);
       });
     };
+    auto wait = [&](auto JC) __attribute__((always_inline)) {  // for block j, where those up to j - 1 + VQ have been asked for
+      constexpr int j = decltype(JC)::value, last = j == 0 ? VQ - 1 : j - 1 + VQ;
+      constexpr int later = KSTEPS * ((last < MBW - 1 ? last : MBW - 1) - j);
+      if constexpr (KSTEPS == 2) lds_wait_for<later>(v[j % VQ][0], v[j % VQ][KSTEPS - 1]);
+      else lds_wait_one<later>(v[j % VQ][0]);
+    };
     attn_static_for<0, VQ>(issue);
+    wait(std::integral_constant<int, 0>{});
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) reg_tie(pf[s][nb]);
+    bf16x8 vf[KSTEPS];
+    auto convert = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s) vf[s] = codes8<F16>(v[slot][s][0], v[slot][s][1]);
+    };
+    constexpr bool AHEAD_OF = !PAIR;  // the codes of block j + 1 are converted among the MFMAs of block j
+    if constexpr (AHEAD_OF) {
+      convert(0);
+      if constexpr (VQ < MBW) issue(std::integral_constant<int, VQ>{});
+    }
     attn_static_for<0, MBW>([&](auto JC) {
       constexpr int j = decltype(JC)::value;
-      constexpr int later = (MBW - 1 - j) < (VQ - 1) ? (MBW - 1 - j) : (VQ - 1);
-      asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(v[j % VQ][0]) : "n"(KSTEPS * later));
-      if constexpr (KSTEPS == 2) reg_tie(v[j % VQ][KSTEPS - 1]);
-      if constexpr (j == 0) {
-#pragma unroll
-        for (int s = 0; s < KSTEPS; ++s)
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) reg_tie(pf[s][nb]);
+      if constexpr (!AHEAD_OF) {
+        if constexpr (j > 0) wait(JC);
+        convert(j % VQ);
+        if constexpr (j + VQ < MBW) issue(std::integral_constant<int, j + VQ>{});
+      } else if constexpr (j + 1 < MBW) {
+        wait(std::integral_constant<int, j + 1>{});
       }
+      u32x4 next[KSTEPS];
 #pragma unroll
-      for (int s = 0; s < KSTEPS; ++s) {
-        const i32x2 c = v[j % VQ][s];
-        const bf16x8 vf = codes8<F16>(c[0], c[1]);
+      for (int s = 0; s < KSTEPS; ++s)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) oacc[j][nb] = mfma16x16x32<F16>(vf, pf[s][nb], oacc[j][nb]);
-      }
-      if constexpr (j + VQ < MBW) issue(std::integral_constant<int, j + VQ>{});
+        for (int nb = 0; nb < NB; ++nb) {
+          oacc[j][nb] = mfma16x16x32<F16>(vf[s], pf[s][nb], oacc[j][nb]);
+          if constexpr (AHEAD_OF && j + 1 < MBW) next[s][nb] = codes2<F16>(v[(j + 1) % VQ][s][nb >> 1], nb & 1);
+        }
+      static_assert(NB == 4, "a conversion beside each MFMA");
+      if constexpr (AHEAD_OF && j + 1 + VQ < MBW) issue(std::integral_constant<int, j + 1 + VQ>{});
       between(JC);
+#pragma unroll
+      for (int i = 0; i < (AHEAD_OF ? KSTEPS * NB : 0); ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // an MFMA, then
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);  // vector instructions
+      }
+      if constexpr (AHEAD_OF && j + 1 < MBW) {
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s) vf[s] = __builtin_bit_cast(bf16x8, next[s]);
+      }
     });
   };
   // A masked key has a score that is not finite: the tile's NaN codes become zero, in LDS, where every wave has done with its
@@ -619,7 +714,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q
       if constexpr (more) {
         qk(next, st, sc, start, [&](auto UC) {
           constexpr int u = decltype(UC)::value;
-          if constexpr (ahead) attn_static_for<u * SH::LPT / UNITS, (u + 1) * SH::LPT / UNITS>([&](auto IC) { copy(src, dst, IC); });
+          if constexpr (ahead) attn_static_for<u * SH::LPT / PAIRS, (u + 1) * SH::LPT / PAIRS>([&](auto IC) { copy(src, dst, IC); });
         });
       } else {
         start();
