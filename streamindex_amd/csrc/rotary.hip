@@ -428,9 +428,9 @@ static RotPlan rot_plan(int64_t rows, int64_t H, int64_t D, int64_t pairs, int v
   RotPlan p{};
   p.vec = vec;
   const int64_t n = (D + vec - 1) / vec;  // pieces of a row
-  // the fewest lanes of a row that 9 pieces each reach (16 from 64 lanes on): longer runs of independent loads a lane
+  // the fewest lanes of a row that 9 pieces each reach, 5 in the backward (16 from 64 lanes on): longer runs of independent loads
   p.log_lpr = 0;
-  while ((int64_t{9} << p.log_lpr) < n && p.log_lpr < 6) ++p.log_lpr;
+  while ((int64_t{bwd ? 5 : 9} << p.log_lpr) < n && p.log_lpr < 6) ++p.log_lpr;
   while (p.log_lpr < 3 && (int64_t{1} << p.log_lpr) < n) ++p.log_lpr;  // (128 bytes of a row at once)
   // few rows: shorter chains, more workgroups
   while (p.log_lpr < 6 && (int64_t{1} << p.log_lpr) < n && rows <= int64_t{512} * (kRotThreads >> p.log_lpr) / 2) ++p.log_lpr;
@@ -439,7 +439,7 @@ static RotPlan rot_plan(int64_t rows, int64_t H, int64_t D, int64_t pairs, int v
   while (p.log_lpr < 6 && tokens(kRotThreads >> p.log_lpr) * pairs * 8 > kRotTable) ++p.log_lpr;  // (4 rows of 512 pairs fit)
   p.lpr = 1 << p.log_lpr;
   const int64_t cpl = (n + p.lpr - 1) / p.lpr;
-  p.cpl = cpl <= 1 ? 1 : cpl <= 2 ? 2 : cpl <= 4 ? 4 : cpl <= 9 ? 9 : 16;
+  p.cpl = cpl <= 1 ? 1 : cpl <= 2 ? 2 : cpl <= 4 ? 4 : cpl <= 5 ? 5 : cpl <= 9 ? 9 : 16;
   const int64_t groups = kRotThreads / p.lpr, all = (rows + groups - 1) / groups;
   // backward: at most 512 workgroups, two a CU, whose sums of dw are joined; forward: up to 8 groups of rows
   int64_t iters = bwd ? (all + 511) / 512 : all / 4096, per;
@@ -491,6 +491,7 @@ static int rot_dispatch(int dtype, const RotPlan& p, F&& f) {
       case 1: return f(DT, V, integral_constant<int, 1>{});
       case 2: return f(DT, V, integral_constant<int, 2>{});
       case 4: return f(DT, V, integral_constant<int, 4>{});
+      case 5: return f(DT, V, integral_constant<int, 5>{});
       case 9: return f(DT, V, integral_constant<int, 9>{});
     }
     // (more than 9 pieces only where each is one value: 64 lanes hold 576 pieces)
