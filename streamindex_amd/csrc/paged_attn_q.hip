@@ -335,14 +335,7 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q
   Within in_next = within[AHEAD];
   from = froms[AHEAD];
 
-  const float rscale = __builtin_fabsf(a.scale_log2);  // of the scores, in log2 units: a negative one changes the sign of Q
-  if (__builtin_expect(a.scale_log2 <= 0.f, 0)) {
-    const uint32_t keep = a.scale_log2 == 0.f ? 0u : ~0u, flip = a.scale_log2 == 0.f ? 0u : 0x80008000u;
-#pragma unroll
-    for (int j = 0; j < QG; ++j)
-#pragma unroll
-      for (int h = 0; h < QH; ++h) qf[j][h] = __builtin_bit_cast(bf16x8, (__builtin_bit_cast(u32x4, qf[j][h]) & keep) ^ flip);
-  }
+  const float rscale = a.scale_log2;  // of the scores, in log2 units
   auto sink_to_lds = [&]() __attribute__((always_inline)) {
     const uint32_t dst = lds_addr(reinterpret_cast<const char*>(&sink_lds[wave * 16 + i16]));
     asm volatile("ds_write_b32 %0, %1" ::"v"(dst), "v"(sink_v) : "memory");  // (the four lanes of a row write the same)
