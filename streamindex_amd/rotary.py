@@ -12,13 +12,14 @@ no counterpart.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .quant import _dtype_code
+from .quant import _DT, _dtype_code
 from .sparse_attn import _check_device
 
 __all__ = ["rotary", "norm_rotary", "rotary_freqs"]
@@ -82,28 +83,38 @@ def norm_rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, w
 
 def _apply(x, positions, freqs, weight, eps, interleaved, start, magnitude, inverse):
     assert x.is_cuda, "x must be on the GPU"
-    _check_device(x.device, positions=positions, freqs=freqs, weight=weight)
-    dt = _dtype_code(x)
-    lead, D = x.dim() - 2, x.shape[-1] if x.dim() else 0
+    at_device = x.get_device()
+    if not (positions.get_device() == freqs.get_device() == at_device and (weight is None or weight.get_device() == at_device)):
+        _check_device(x.device, positions=positions, freqs=freqs, weight=weight)
+    dt = _DT.get(x.dtype)
+    if dt is None:
+        dt = _dtype_code(x)
+    shape = x.shape
+    lead = len(shape) - 2
     if lead < 0:
-        raise ValueError(f"x must be [..., H, D], got {list(x.shape)}")
-    if freqs.dim() != 1 or not freqs.dtype.is_floating_point or freqs.requires_grad:
+        raise ValueError(f"x must be [..., H, D], got {list(shape)}")
+    D = shape[-1]
+    ft = freqs.dtype
+    if freqs.dim() != 1 or not (ft is torch.float64 or ft.is_floating_point) or freqs.requires_grad:
         raise ValueError("freqs must be [dims / 2] floating point without gradient")
-    pairs = freqs.shape[0]
-    at = D - 2 * pairs if start is None else start
-    if D < 1 or D > MOST_D or at < 0 or at + 2 * pairs > D:
-        raise ValueError(f"the head needs 1 to {MOST_D} dimensions and the rotary ones within it, got {D} and {at} to {at + 2 * pairs}")
+    dims = 2 * freqs.shape[0]
+    at = D - dims if start is None else start
+    if D < 1 or D > MOST_D or at < 0 or at + dims > D:
+        raise ValueError(f"the head needs 1 to {MOST_D} dimensions and the rotary ones within it, got {D} and {at} to {at + dims}")
     n = positions.dim()
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-    if n > lead or positions.shape != x.shape[lead - n:lead]:
-        raise ValueError(f"positions must be {list(x.shape[:lead])} or its last sizes, got {list(positions.shape)}")
-    if weight is not None and weight.shape != (D,):
+    pt = positions.dtype
+    if pt is not torch.int64 and pt is not torch.int32:
+        raise ValueError(f"positions must be int32 or int64, got {pt}")
+    if n > lead or positions.shape != shape[lead - n:lead]:
+        raise ValueError(f"positions must be {list(shape[:lead])} or its last sizes, got {list(positions.shape)}")
+    if weight is not None and (weight.dim() != 1 or weight.shape[0] != D):
         raise ValueError(f"weight must be [{D}], got {list(weight.shape)}")
-    positions = positions if positions.is_contiguous() else positions.contiguous()
-    freqs = freqs if freqs.dtype is torch.float64 and freqs.is_contiguous() else freqs.double().contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if ft is not torch.float64 or not freqs.is_contiguous():
+        freqs = freqs.double().contiguous()
     args = (eps, not interleaved, at, float(magnitude), bool(inverse), dt)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)):
+    if (x.requires_grad or (weight is not None and weight.requires_grad)) and torch.is_grad_enabled():
         return _RotaryFunc.apply(x, weight, positions, freqs, args)
     return _forward(x, weight, positions, freqs, args)
 
@@ -132,20 +143,30 @@ def _fp32(weight: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 def _forward(x, weight, positions, freqs, args):
     eps, halves, start, magnitude, inverse, dt = args
     dev = x.device
+    H, D = x.shape[-2:]
+    n = x.numel()
     L = _lib.load()
     with _lib.on_device(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        n = x.numel()
+        if x.is_contiguous():
+            y, rows, strides = torch.empty_like(x), x, _lib.stride_array((H * D, D))
+        else:
+            y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            rows, strides = _rows(x) if n else (x, None)
         if n == 0:
             return y
-        H, D = x.shape[-2:]
-        (rows, strides), w = _rows(x), _fp32(weight)
+        w = _fp32(weight)
         rc = L.si_norm_rotary(rows.data_ptr(), strides, eps is not None, None if w is None else w.data_ptr(), eps or 0.0,
                               positions.data_ptr(), positions.dtype is torch.int64, positions.numel(), freqs.data_ptr(),
                               freqs.shape[0], start, halves, magnitude, inverse, n // (H * D), H, D, dt, y.data_ptr(),
                               _lib.stream_ptr(dev))
-    _lib.check(rc)
+    if rc:
+        _lib.check(rc)
     return y
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(*sizes) -> int:
+    return _lib.load().si_norm_rotary_bwd_workspace_bytes(*sizes)
 
 
 def _backward(ctx, dy):
@@ -166,7 +187,7 @@ def _backward(ctx, dy):
             return dx, None if dw is None else dw.zero_().to(weight.dtype), None, None, None
         (rows, strides), (drows, dstrides), w = _rows(x), _rows(dy), _fp32(weight)
         T = n // (H * D)
-        size = L.si_norm_rotary_bwd_workspace_bytes(T, H, D, freqs.shape[0]) if need_w else 0
+        size = _workspace(T, H, D, freqs.shape[0]) if need_w else 0
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if need_w else None
         rc = L.si_norm_rotary_bwd(drows.data_ptr(), dstrides, rows.data_ptr(), strides, None if w is None else w.data_ptr(), eps,
                                   positions.data_ptr(), positions.dtype is torch.int64, positions.numel(), freqs.data_ptr(),
