@@ -15,7 +15,8 @@ import random
 import pytest
 import torch
 
-from streamindex_amd import (_lib, norm_rotary, paged_attn_fwd, paged_attn_q_fwd, paged_plan, paged_write_q, rotary, rotary_freqs)
+from streamindex_amd import (_lib, norm_rotary, paged_attn_fwd, paged_attn_q_fwd, paged_compress, paged_plan, paged_write,
+                             paged_write_q, rotary, rotary_freqs)
 
 from tests.test_gpu_paged import EVERY, half_step, i32, make_table
 
@@ -634,6 +635,52 @@ def test_serving_together(H, D, page, block, dtype):
                     assert ((got - want).abs() <= 2.0**-4 * want.abs() + sc * 2.0**-10).all()
                 t += 1
             done[r] += new[r]
+
+
+@pytest.mark.parametrize("H,d,m,n_win,page,block", [(64, 576, 16, 24, 64, 16), (8, 64, 8, 20, 6, 1)])
+def test_hca_serving_together(H, d, m, n_win, page, block):
+    """An HCA layer over caches in 8 bits, in chunks and single tokens: rows and compressed entries quantised as they come, every output
+    against 64-bit arithmetic over the caches as they stand, and each new entry against the compressor's, half an e4m3 step."""
+    R, total, pages = 3, [5 * m + 3, 2, 4 * m], 60
+    g = torch.Generator().manual_seed(m)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(BF).to(DEV)  # noqa: E731
+    q, x = [rnd(t, H, d) for t in total], [rnd(t, 3 * d) for t in total]
+    bias, sink = torch.randn(m, d, generator=g).to(DEV), torch.randn(H, generator=g).to(DEV)
+    kv, ents = (torch.full((pages, page, d), 0x7f, dtype=torch.uint8, device=DEV).view(F8) for _ in range(2))
+    sc, esc = (torch.full((pages, page // block), math.nan, device=DEV) for _ in range(2))
+    streams = torch.full((pages, page, 2 * d), math.nan, dtype=BF, device=DEV)  # compressor content and gate
+    free, efree = (torch.randperm(pages, generator=g).to(torch.int32).to(DEV) for _ in range(2))
+    table, etable = (torch.full((R, max(total) // page + 1), -1, dtype=torch.int32, device=DEV) for _ in range(2))
+    ctx, at, eat = i32([0] * R), i32([0]), i32([0])
+    done, rng = [0] * R, random.Random(m)
+    while any(done[r] < total[r] for r in range(R)):
+        new = [min(total[r] - done[r], rng.choice([0, 1, 1, m + 2])) for r in range(R)]
+        if not any(new):
+            continue
+        cut = lambda t: torch.cat([t[r][done[r]:done[r] + new[r]] for r in range(R)] + [rnd(1, *t[0].shape[1:])])  # noqa: E731
+        qs, xs = cut(q), cut(x)
+        N = len(qs)
+        tok = paged_plan(ctx, i32(new), table, free, page, N, free_start=at)
+        ent = paged_plan(ctx, i32(new), etable, efree, page, N // m + R, ratio=m, free_start=eat)
+        ctx, at, eat = tok.seq_lens, tok.free_next, ent.free_next
+        paged_write_q(xs[:, :d], kv, sc, tok.slots)
+        paged_write(xs[:, d:], streams, tok.slots)
+        E = len(ent.slots)
+        made = torch.zeros(1, E, d, dtype=BF, device=DEV)
+        paged_compress(streams[..., :d], streams[..., d:], bias, table, ent.request, ent.positions, made,
+                       torch.where(ent.slots >= 0, torch.arange(E, device=DEV), -1))
+        paged_write_q(made[0], ents, esc, ent.slots)
+        got = paged_attn_q_fwd(qs, kv, sc, table, tok.cu, tok.seq_lens, sink, window=n_win, kv2_cache=ents, kv2_scales=esc, block_table2=etable,
+                               ratio=m)
+        s = Step([(done[r], new[r]) for r in range(R)], H, d, window=n_win, ratio=m, page=page, pad=1)
+        s.q, s.kv, s.sc, s.table, s.kv2, s.sc2, s.table2, s.sink = qs, kv, sc, table, ents, esc, etable, sink
+        s.check(got)
+        for i, slot in enumerate(ent.slots.tolist()):
+            if slot >= 0:
+                scale = esc.view(-1)[slot // block].double()
+                want, have = made[0, i].double(), ents.view(-1, d)[slot].double() * scale
+                assert ((have - want).abs() <= 2.0**-4 * want.abs() + scale * 2.0**-10).all()
+        done = [done[r] + new[r] for r in range(R)]
 
 
 def test_close_to_16_bits():
