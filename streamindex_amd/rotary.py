@@ -73,6 +73,7 @@ def norm_rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, w
                 inverse: bool = False) -> torch.Tensor:
     """``rotary(x * (mean(x ** 2) + eps) ** -0.5 * weight, ...)``, the mean over each head's D, in one pass.
 
+    Squares are summed in fp32: values beyond about 2^60 overflow them and their row becomes 0.
     ``weight``: ``[D]``, None for ones; the other arguments are :func:`rotary`'s.  Gradients in x and the weight (the same
     bits every time).
     """
