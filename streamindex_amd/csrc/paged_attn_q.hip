@@ -18,6 +18,10 @@
 // was slower all the same: 742 TFLOP/s at D = 512 and 688 at 256, against 888 and 940, one request of 8,192 earlier tokens,
 // 64 heads, 1,024 and 2,048 new ones.)
 //
+// bf16, one request of 1,024 new tokens (2,048 at D = 256 and below) behind 8,192, 64 heads: 576 835 - 847 TFLOP/s, 512 888 - 901,
+// 256 931 - 950, 128 785 - 792, 64 541, 32 297 (16-bit caches: 1,190, 1,117, 990, 735, 590, 305).  Decode, 64 heads, D = 576,
+// 32 requests of 20,000 keys: 133 us, 2.8 TB/s of codes (16-bit caches 155).
+//
 // A masked key's code NaN is zeroed in LDS before P V (0 x NaN is NaN); every row that sees it has a score of NaN.
 #include <cstdint>
 #include <string>
@@ -855,7 +859,10 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q
   }
 }
 
-// Row blocks from which PAIR is taken.
+// Row blocks from which PAIR is taken: where two workgroups a CU have work.  PAIR / not, D = 576: 64 heads, five chunks of 300 to 4,096
+// tokens, window 128 and compressed entries (5 to 17 tiles a row block) 495 / 603 us; 1,024 new tokens behind 8,192 (1,024 row blocks,
+// 144 tiles) 1,560 / 1,561; D = 512 the same 1,308 / 1,425.  Fewer dimensions have two workgroups a CU and more without it: D = 256
+// (2,048 row blocks) 1,607 / 1,290, 128 1,017 / 785.
 constexpr int64_t q_pair_from(int64_t D) { return D >= 512 ? 257 : INT64_MAX; }
 
 // Sizes of a call, from what the host knows.

@@ -12,6 +12,10 @@
 // Rows are read once and stay in registers between the maximum and the codes.  With a scale for each token 8 to 64 lanes
 // share a row.  With a scale for each block a workgroup takes the blocks that begin in its share of the rows, one after the
 // other, whole: a block's rows stand next to each other, as a plan's do.
+//
+// Bound, many rows: memory, with vector instructions in 52 % of the CUs' busy cycles.  Nine requests' bf16 rows of 576 values, 64
+// tokens a page and a scale, 133 MB read and written: 27.4 us, 4.8 TB/s.  (Divisions for every piece, rows read a second time: 50;
+// 180 registers a lane and half the waves: 38.)  Few rows: latency.  256 rows with a scale each, 4.3 to 5.3 us.
 #include <hip/hip_fp16.h>
 
 #include <string>
