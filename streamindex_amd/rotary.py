@@ -75,7 +75,8 @@ def norm_rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, w
 
     Squares are summed in fp32: values beyond about 2^60 overflow them and their row becomes 0.
     ``weight``: ``[D]``, None for ones; the other arguments are :func:`rotary`'s.  Gradients in x and the weight (the same
-    bits every time).
+    bits every time).  A step with its backward can be captured into a graph; results of eager calls on the same leaves have to be
+    gone by then, since autograd ties the leaves to the stream of the first.
     """
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")

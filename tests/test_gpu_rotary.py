@@ -282,6 +282,14 @@ def test_many_rows_and_the_same_bits_twice():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("lead,H,D,dims,halves", [
+    ((43711,), 3, 64, 64, True), ((131079,), 1, 64, 64, False), ((8209,), 16, 100, 50, False), ((16387,), 8, 36, 12, True)])
+def test_two_groups_of_rows(lead, H, D, dims, halves):
+    """Enough rows that a workgroup takes two groups of them: with one table, with one for each group, past the last row."""
+    Problem(lead, H, D, dims, BF, halves).check()
+    Problem(lead, H, D, dims, HF, halves, norm=False).check()
+
+
 def test_inverse_undoes():
     p = Problem((50,), 4, 576, 64, F32, norm=False, m=1.0)
     back = rotary(p.call(), p.pos, p.freqs, inverse=True)
