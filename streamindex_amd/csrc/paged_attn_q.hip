@@ -861,7 +861,8 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q
 
 // Row blocks from which PAIR is taken: where two workgroups a CU have work.  PAIR / not, D = 576: 64 heads, five chunks of 300 to 4,096
 // tokens, window 128 and compressed entries (5 to 17 tiles a row block) 495 / 603 us; 1,024 new tokens behind 8,192 (1,024 row blocks,
-// 144 tiles) 1,560 / 1,561; D = 512 the same 1,308 / 1,425.  Fewer dimensions have two workgroups a CU and more without it: D = 256
+// 144 tiles) 1,560 / 1,561; D = 512 the same 1,308 / 1,425; of few row blocks, 32 single tokens behind 20,000 keys 168 / 144, 64 behind
+// 40,000 with a window and compressed entries 41 / 30.  Fewer dimensions have two workgroups a CU and more without it: D = 256
 // (2,048 row blocks) 1,607 / 1,290, 128 1,017 / 785.
 constexpr int64_t q_pair_from(int64_t D) { return D >= 512 ? 257 : INT64_MAX; }
 
