@@ -450,8 +450,9 @@ static RotPlan rot_plan(int64_t rows, int64_t H, int64_t D, int64_t pairs, int v
   // Backward: at most 512 workgroups, two a CU, whose sums of dw are joined (training step of 4,096 tokens, 64 heads, D = 576: 311 us,
   // 384 workgroups 337, 256 363).  Forward: two groups of rows, so that a weight and a table serve both; 1 / 2 / 4 groups: 137 / 117 /
   // 120 us with a weight at those sizes, 490 / 427 / 454 at 16,384 tokens; without one 108.5 / 112.8 / 119 and 419 / 424 / 456;
-  // rotation alone, 24 heads of 128, 100,003 tokens, 229 / 227 / 231 (8: 249), 64 heads of 64 365 / 334 / 333.
-  int64_t iters = bwd ? (all + 511) / 512 : all < 4096 ? 1 : 2, per;
+  // rotation alone, 24 heads of 128, 100,003 tokens, 229 / 227 / 231 (8: 249), 64 heads of 64 365 / 334 / 333.  (A launch has fewer
+  // than 2^24 workgroups.)
+  int64_t iters = bwd ? (all + 511) / 512 : all < 4096 ? 1 : 2 + (all >> 24), per;
   per = iters = iters < 1 ? 1 : iters;
   while (per > 1 && tokens(per * groups) * pairs * 8 > kRotTable / 3) per = (per + 1) / 2;
   p.per = static_cast<int>(per);

@@ -222,6 +222,23 @@ def test_strides(dtype):
                 assert c.codes.stride() == other.stride() and want.isfinite().all()
 
 
+@pytest.mark.parametrize("block", [1, 16])
+def test_far_offsets(block):
+    """Cache rows past 2^32 bytes, scales past 2^31, rows past 2^31 values: as near ones."""
+    slots = plan_slots([(3, 40), (70, 9)], 16, 10, seed=2)
+    rows = make_rows(len(slots), 64, BF)
+    c = Cache(10, 16, block, 64)
+    far = torch.empty(6 << 30, dtype=torch.uint8, device=DEV).view(F8).as_strided((10, 16, 64), ((6 << 30) // 10 // 16 * 16, 64, 1))
+    far.view(torch.uint8).copy_(c.codes.view(torch.uint8))
+    scales = torch.empty((10 << 30) // 4, device=DEV).as_strided((10, 16 // block), ((10 << 30) // 40, 1))
+    scales.copy_(c.scales)
+    wide = torch.empty((len(slots) + 1) * (1 << 26), dtype=BF, device=DEV).as_strided((len(slots), 64), (1 << 26, 1))
+    wide.copy_(rows)
+    paged_write_q(wide, far, scales, slots)
+    c.check(rows, slots)
+    assert torch.equal(far.contiguous().view(torch.uint8), c.codes.view(torch.uint8)) and torch.equal(scales.contiguous(), c.scales)
+
+
 def test_nothing_between_rows_is_written():
     wide = torch.full((4, 8, 100), 7, dtype=torch.uint8, device=DEV)
     cache = wide.view(F8)[..., 20:84]

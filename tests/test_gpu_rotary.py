@@ -290,6 +290,42 @@ def test_two_groups_of_rows(lead, H, D, dims, halves):
     Problem(lead, H, D, dims, HF, halves, norm=False).check()
 
 
+def test_far_offsets():
+    """Values past 2^31 of x and of the gradient, rows past 2^31, strides past 2^32 bytes: as the same rows near the front."""
+    freqs = rotary_freqs(64)
+
+    def last_as_alone(x, pos, f, tokens, norm, gradient):
+        with torch.no_grad():
+            call = (lambda a, b: norm_rotary(a, b, f)) if norm else (lambda a, b: rotary(a, b, f))
+            y = call(x, pos)
+            for at in (slice(0, tokens), slice(x.shape[0] - tokens, None)):
+                want = call(x[at].clone(), pos[at])
+                # (few rows have more lanes each: sums in another order, two roundings, each value else within 2^-18 of its terms,
+                # below 4)
+                assert norm or torch.equal(y[at], want)
+                assert ((y[at].float() - want.float()).abs() <= 1.01 * 2.0 ** -7 * want.float().abs() + 2.0 ** -15).all()
+            del y
+        if not gradient:
+            return
+        dy = torch.empty_like(x).uniform_(-1, 1)
+        x.requires_grad_()
+        dx, = torch.autograd.grad(call(x, pos), [x], dy)
+        for at in (slice(0, tokens), slice(x.shape[0] - tokens, None)):
+            near = x[at].detach().clone().requires_grad_()
+            want, = torch.autograd.grad(call(near, pos[at]), [near], dy[at].clone())
+            # (as above: each within 2^-17 of its terms, r (|a| + |b|) (1 + |n| mean |n|) <= sqrt(3) 2 (1 + 1.74 * 0.87) < 9)
+            assert ((dx[at].float() - want.float()).abs() <= 1.01 * 2.0 ** -7 * want.float().abs() + 2.0 ** -12).all()
+
+    T = 2 ** 31 // (64 * 512) + 5
+    last_as_alone(torch.empty(T, 64, 512, dtype=BF, device=DEV).uniform_(-1, 1), torch.arange(T, device=DEV), freqs, 3, True, True)
+    T = 2 ** 31 + 300
+    last_as_alone(torch.empty(T, 1, 2, dtype=BF, device=DEV).uniform_(-1, 1), (torch.arange(T, device=DEV) // 1000).int(),
+                  rotary_freqs(2), 70, False, False)
+    x = torch.empty(3 << 31, dtype=BF, device=DEV).as_strided((3, 2, 128), (1 << 31, 1 << 30, 1)).uniform_(-1, 1)
+    pos = torch.arange(3, device=DEV)
+    assert torch.equal(norm_rotary(x, pos, freqs), norm_rotary(x.contiguous(), pos, freqs))
+
+
 def test_inverse_undoes():
     p = Problem((50,), 4, 576, 64, F32, norm=False, m=1.0)
     back = rotary(p.call(), p.pos, p.freqs, inverse=True)
