@@ -6,7 +6,7 @@ Queries and keys come to the attention "RoPE-rotated" (``flash_sparse/csa.py:184
 * :func:`norm_rotary` — each head's row over its root mean square, by a weight, then the rotation, in one pass;
 * :func:`rotary_freqs` — the frequencies, stretched for long contexts or not.
 
-Both have gradients, in x and the weight.  Angles are 64-bit, everything else fp32, rounded once to x's type.  The reference has
+Both have gradients, in x and the weight, of the first order and backward; forward-mode derivatives raise.  Angles are 64-bit, everything else fp32, rounded once to x's type.  The reference has
 no counterpart.
 """
 
@@ -17,6 +17,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .quant import _DT, _dtype_code
@@ -116,9 +117,14 @@ def _apply(x, positions, freqs, weight, eps, interleaved, start, magnitude, inve
     if ft is not torch.float64 or not freqs.is_contiguous():
         freqs = freqs.double().contiguous()
     args = (eps, not interleaved, at, float(magnitude), bool(inverse), dt)
-    if (x.requires_grad or (weight is not None and weight.requires_grad)) and torch.is_grad_enabled():
+    if ((x.requires_grad or (weight is not None and weight.requires_grad)) and torch.is_grad_enabled()) or _forward_mode():
         return _RotaryFunc.apply(x, weight, positions, freqs, args)
     return _forward(x, weight, positions, freqs, args)
+
+
+def _forward_mode() -> bool:
+    """Whether tensors may carry tangents, which autograd's function refuses and a kernel would drop."""
+    return forward_ad._current_level >= 0
 
 
 def _rows(x: torch.Tensor):
@@ -172,6 +178,8 @@ def _workspace(*sizes) -> int:
 
 
 def _backward(ctx, dy):
+    if _forward_mode() and forward_ad.unpack_dual(dy).tangent is not None:
+        raise NotImplementedError("the gradients of rotary and norm_rotary have no forward-mode derivative")
     positions, freqs, *saved = ctx.saved_tensors
     eps, halves, start, magnitude, inverse, dt = ctx.args
     if not saved:
