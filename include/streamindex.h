@@ -506,8 +506,9 @@ int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* kv, c
  * slot_stride in bytes) and fp32 scales [pages, page_size / block] (scale_stride
  * elements a page), one for `block` tokens.  The scale becomes the smallest power
  * of two, from 2^-64 on, with 448 scale >= |x| for the finite x of the block's new
- * rows, and no smaller than the one of the block's earlier tokens, those before its
- * first new row, whose codes are rescaled where it grows.  Slots outside the
+ * rows, unless the one of the block's earlier tokens, those before its first new
+ * row, is larger and stays (a power of two or not); where it grows, their codes are
+ * rounded to it.  Slots outside the
  * cache write nothing; slots are distinct, and a block's rows follow each other
  * in rising order, as a plan's do (fewer than 64 rows without a slot between).
  */

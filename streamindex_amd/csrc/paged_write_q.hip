@@ -6,6 +6,9 @@
 // code * s_old / s, which loses what falls below 2^-9 of the new scale and nothing else.  Infinities and NaN become NaN and count
 // for no scale.
 //
+// An earlier scale that another program set need not be a power of two; where it is large enough, it stays.  Quotients by it, and
+// products of codes with it, take fp32's last bit as a sign that something is left, so that e4m3 is their only rounding too.
+//
 // A power of two costs e4m3 at most the lowest bit of its subnormal values, makes every code and its reading exact, and
 // lets a block's scale grow without a second rounding of its normal values.
 //
@@ -140,6 +143,23 @@ __device__ __forceinline__ int wq_exp(float m) {
   return e > kLeastExp ? e : kLeastExp;
 }
 __device__ __forceinline__ float wq_pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// q, the fp32 value nearest to q + rest, with its last bit set where that is not zero: rounded to fewer bits, this is as q + rest
+// rounded once.
+__device__ __forceinline__ float wq_odd(float q, float rest) {
+  const uint32_t b = __float_as_uint(q);
+  const bool more = rest > 0.f || rest < 0.f;
+  return more && q != 0.f && !(b & 1) ? __uint_as_float((rest > 0.f) == (q > 0.f) ? b + 1 : b - 1) : q;
+}
+// x / s and x s for a rounding to e4m3, whatever s > 0.  (Where fma's result falls below fp32's range the code is zero anyway.)
+__device__ __forceinline__ float wq_quotient(float x, float s) {
+  const float q = x / s;
+  return wq_odd(q, __builtin_fmaf(-q, s, x));
+}
+__device__ __forceinline__ float wq_product(float x, float s) {
+  const float q = x * s;
+  return wq_odd(q, __builtin_fmaf(x, s, -q));
+}
 
 template <int V, typename P>
 __device__ __forceinline__ void wq_store(uint8_t* dst, const P& p, float inv) {
@@ -351,7 +371,29 @@ __global__ __launch_bounds__(kBlockThreads, DT == 0 ? 2 : 4) void paged_write_q_
     const float need = wq_pow2(wq_exp(wq_value<DT>(m)));
     const bool kept = old > 0.f && old < __builtin_inff();  // (earlier tokens with a scale that is one)
     const float scale = kept && old > need ? old : need, inv = 1.0f / scale;
-    if (hold) {
+    auto place = [&](uint32_t row, uint32_t c) {
+      const int64_t s = row ? slot_at(r + row) : slot;
+      return base + (first + (s - slot)) * a.cstride + static_cast<int64_t>(c) * V;
+    };
+    if (__builtin_expect(__float_as_uint(scale) & 0x7fffffu, 0)) {
+      // an earlier scale that is no power of two (the same in every thread): value by value, a rare path that takes no registers
+      if (tr < step)
+#pragma unroll 1
+        for (uint32_t row = tr; row < rows; row += step) {
+          if (!has_slot(row)) continue;
+#pragma unroll 1
+          for (uint32_t c = tc; c < a.pieces; c += kBlockThreads) {
+            const char* from = source(row, c);
+            uint8_t* to = place(row, c);
+#pragma unroll 1
+            for (int e = 0; e < V; ++e) {
+              WqPiece<DT, 1> x;
+              x.load(from + e * SIZE);
+              to[e] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(wq_quotient(x.at(0), scale), 0.f, 0, false));
+            }
+          }
+        }
+    } else if (hold) {
       uint8_t* to = base + (first + tr) * a.cstride + static_cast<int64_t>(tc) * V;
       const int64_t rise = step * a.cstride;
       uint32_t row = row0;
@@ -362,10 +404,7 @@ __global__ __launch_bounds__(kBlockThreads, DT == 0 ? 2 : 4) void paged_write_q_
         to += rise;
       }
     } else {
-      each([&](uint32_t row, uint32_t c, const P& p) {
-        const int64_t s = row ? slot_at(r + row) : slot;
-        wq_store<V>(base + (first + (s - slot)) * a.cstride + static_cast<int64_t>(c) * V, p, inv);
-      });
+      each([&](uint32_t row, uint32_t c, const P& p) { wq_store<V>(place(row, c), p, inv); });
     }
     if (kept && scale > old) {  // earlier tokens to the new scale
       const float ratio = old / scale;
@@ -375,13 +414,13 @@ __global__ __launch_bounds__(kBlockThreads, DT == 0 ? 2 : 4) void paged_write_q_
 #pragma unroll
         for (int e = 0; e < V; e += V < 4 ? 1 : 4) {
           if constexpr (V == 1) {
-            const float x = __builtin_amdgcn_cvt_f32_fp8(*p, 0) * ratio;
+            const float x = wq_product(__builtin_amdgcn_cvt_f32_fp8(*p, 0), ratio);
             *p = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x, 0.f, 0, false));
           } else {
             const int w = *reinterpret_cast<const int*>(p + e);
             const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-            int x = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * ratio, lo[1] * ratio, 0, false);
-            x = __builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * ratio, hi[1] * ratio, x, true);
+            int x = __builtin_amdgcn_cvt_pk_fp8_f32(wq_product(lo[0], ratio), wq_product(lo[1], ratio), 0, false);
+            x = __builtin_amdgcn_cvt_pk_fp8_f32(wq_product(hi[0], ratio), wq_product(hi[1], ratio), x, true);
             *reinterpret_cast<int*>(p + e) = x;
           }
         }

@@ -53,9 +53,9 @@ def paged_write_q(rows: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor,
       slots: ``[N]`` int64; one outside the cache (-1) writes nothing.  Slots are distinct and the rows of one block follow each
         other in rising order, as a plan's do, with fewer than 64 rows without a slot between two of them; otherwise what that
         block holds is undefined.
-    A block's scale becomes the smallest power of two (at least 2^-64) that holds its new rows within e4m3's 448, and no smaller
-    than the scale of its earlier tokens, those before the first new one: a block written from its first token on starts anew, and an
-    earlier scale that is not positive and finite counts as none (the codes stay).
+    A block's scale becomes the smallest power of two (at least 2^-64) that holds its new rows within e4m3's 448, unless that of its
+    earlier tokens, those before the first new one, is larger and stays, a power of two or not.  A block written from its first token on
+    starts anew, and an earlier scale that is not positive and finite counts as none (the codes stay).
     Where the scale grows, the earlier codes are rounded to it.  New codes are the nearest (ties to even) to ``x / scale``.
     Infinities and NaN become NaN and do not count for the scale.
     """
