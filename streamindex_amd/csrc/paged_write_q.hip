@@ -309,7 +309,7 @@ __global__ __launch_bounds__(kBlockThreads, DT == 0 ? 2 : 4) void paged_write_q_
         if (stop || !ours) break;
       }
     }
-    const float old = first > 0 ? a.scales[at.page * a.spage + blk] : 0.f;
+    const float old = first > 0 ? a.scales[at.page * a.spage + blk] : 0.f;  // (in front of joined()'s barrier: it is overwritten behind)
     uint8_t* base = a.codes + at.page * a.pstride + static_cast<int64_t>(blk) * a.block * a.cstride;
     const uint32_t rows = static_cast<uint32_t>(run);
     const bool hold = a.pieces <= kBlockThreads && rows <= kHeldRows * step && !gaps && !apart;  // (the same in every thread)
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(kBlockThreads, DT == 0 ? 2 : 4) void paged_write_q_
         }
       }
     }
-    // (every thread has the old scale: it went into the maximum behind the barrier)
+    // (every thread asked for the old scale before joined()'s barrier, which this store stands behind)
     if (t == 0) a.scales[at.page * a.spage + blk] = scale;
     __syncthreads();  // max_lds is free, and a later run of this workgroup sees this one's codes and scale
     r += run;
