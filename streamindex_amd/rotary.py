@@ -32,20 +32,21 @@ def rotary_freqs(dims: int, base: float = 10000.0, *, factor: float = 1.0, origi
                  slow: float = 1.0, device="cuda") -> torch.Tensor:
     """Radians a position of each pair, ``base ** (-2 i / dims)``, ``[dims / 2]`` fp64.
 
-    ``factor > 1`` stretches a context of ``original_length`` tokens: pairs that turn fewer than ``slow`` times in it are
-    divided by ``factor``, those that turn more than ``fast`` times stay, and between them the share goes in a straight line
-    over the pairs.
+    ``factor > 1`` stretches a context of ``original_length`` tokens, as the interpolation by parts of YaRN does (Peng, Quesnelle,
+    Fan and Shippole, 2023): pairs that turn fewer than ``slow`` times in it are divided by ``factor``, those that turn more than
+    ``fast`` times stay, and between them the share goes in a straight line over the pairs.  ``base`` is above 1 then.
     """
-    if dims < 0 or dims % 2 or base <= 0 or factor < 1 or original_length < 1 or not fast > slow > 0:
+    if (dims < 0 or dims % 2 or not 0 < base < math.inf or not 1 <= factor < math.inf or original_length < 1 or not fast > slow > 0
+            or (factor > 1 and base <= 1)):
         raise ValueError(f"bad frequencies: dims={dims}, base={base}, factor={factor}, original_length={original_length}, "
                          f"fast={fast}, slow={slow}")
     f = [base ** (-2.0 * i / dims) for i in range(dims // 2)]
-    if factor > 1 and base > 1:
+    if factor > 1:
         def pair(turns):  # that turns so often in original_length
             return dims * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dims - 1)
-        share = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(dims // 2)]
+        lo, hi, last = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dims - 1), pair(slow)
+        share = [1.0 if i >= last else min(1.0, max(0.0, (i - lo) / max(hi - lo, 1))) for i in range(dims // 2)]
         f = [x * (1 - s) + x / factor * s for x, s in zip(f, share)]
     return torch.tensor(f, dtype=torch.float64, device=device)
 
