@@ -508,7 +508,8 @@ int si_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* kv, c
  * of two, from 2^-64 on, with 448 scale >= |x| for the finite x of the block's new
  * rows, unless the one of the block's earlier tokens, those before its first new
  * row, is larger and stays (a power of two or not); where it grows, their codes are
- * rounded to it.  Slots outside the
+ * rounded to it.  Tokens behind the first new row that are not written lose their
+ * meaning.  Slots outside the
  * cache write nothing; slots are distinct, and a block's rows follow each other
  * in rising order, as a plan's do (fewer than 64 rows without a slot between).
  */
@@ -521,7 +522,7 @@ int si_paged_write_q(const void* rows, int64_t row_stride, int dtype, const int6
  * D] (strides in bytes, multiples of 16) with fp32 scales [pages, page_size /
  * block] (scale_stride elements a page); an entry is its code times its scale.
  * q and o are of qkv_dtype.  A code of NaN reaches the rows that see its key and
- * no others; scales of seen keys are finite.
+ * no others; scales of seen keys are zero or of a magnitude from 2^-64 to 2^100.
  */
 int64_t si_paged_attn_q_fwd_scratch_bytes(int64_t N, int64_t H, int64_t D, int64_t R, int64_t window, int64_t keys,
                                           int64_t keys2);

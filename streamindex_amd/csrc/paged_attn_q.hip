@@ -467,7 +467,8 @@ __global__ __launch_bounds__(kPagedThreads, q_per_cu(D, PAIR)) void paged_attn_q
 
   // ---- softmax -----------------------------------------------------------------
   // Weights are 2^(score - m_ref), and their products with the scales go to P V.  bf16: the 16-bit kernel's references, from 2^-32
-  // to 1, the products having fp32's range.  fp16: 2^11 to 2^15 is where the largest product with a scale lies, so that 2^-25
+  // to 1, the products having fp32's range: scales from 2^-64 on keep those of weights down to 2^-30 of the largest, and up to 2^100
+  // their sums over 2^19 keys stay finite.  fp16: 2^11 to 2^15 is where the largest product with a scale lies, so that 2^-25
   // of it keeps its 11 bits; the reference is that of the scores plus the exponents of their scales (from 2^-80 on: the weights'
   // sum stays in range).
   constexpr float kHead = F16 ? 11.0f : -32.0f, kLazy = F16 ? 4.0f : 32.0f;

@@ -57,7 +57,8 @@ def paged_write_q(rows: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor,
     earlier tokens, those before the first new one, is larger and stays, a power of two or not.  A block written from its first token on
     starts anew, and an earlier scale that is not positive and finite counts as none (the codes stay).
     Where the scale grows, the earlier codes are rounded to it.  New codes are the nearest (ties to even) to ``x / scale``.
-    Infinities and NaN become NaN and do not count for the scale.
+    Infinities and NaN become NaN and do not count for the scale.  Tokens of the block behind its first new row that are not written
+    again lose their meaning: their codes stay and their scale is the new one.
     """
     assert rows.is_cuda
     dev = rows.device
@@ -96,13 +97,15 @@ def paged_attn_q_fwd(q: torch.Tensor, kv_cache: torch.Tensor, kv_scales: torch.T
     Args:
       q: ``[N, H, D]`` bf16 or fp16.
       kv_cache, kv2_cache: ``[pages, page_size, D]`` float8_e4m3fn, rows 16-byte aligned, within 64 GiB of the first.
-      kv_scales, kv2_scales: ``[pages, blocks]`` fp32, ``blocks`` a divisor of the page size, any finite values.
+      kv_scales, kv2_scales: ``[pages, blocks]`` fp32, ``blocks`` a divisor of the page size; of either sign, zero or from 2^-64 (the
+        least that :func:`paged_write_q` sets) to 2^100.
       The others: as there.
     Returns:
-      ``(o [N, H, D] in q's type, lse [N, H] fp32)``.  Weights times scales are rounded to q's type.
+      ``(o [N, H, D] in q's type, lse [N, H] fp32)``.  Weights times scales are rounded to q's type: in fp16 those below 2^-25 of a
+      row's largest lose bits, and below 2^-36 they are lost; in bf16 those of scales outside the range above leave fp32's.
       A row without a key gets ``o = 0`` and ``lse = sink`` (or ``-1e30`` if the sink is ``-inf``).  A code of NaN reaches the
-      rows that see its key and no others; so does a scale that is not finite.  Scores are fp32: one below its range weighs
-      nothing, one above it makes its row NaN.
+      rows that see its key and no others; so does a scale that is not finite.  Scores are fp32, as are q's products with the codes
+      before their scale: one below its range weighs nothing, one above it makes its row NaN.
     """
     assert q.is_cuda
     dev = q.device

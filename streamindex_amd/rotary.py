@@ -75,7 +75,8 @@ def norm_rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, w
                 inverse: bool = False) -> torch.Tensor:
     """``rotary(x * (mean(x ** 2) + eps) ** -0.5 * weight, ...)``, the mean over each head's D, in one pass.
 
-    Squares are summed in fp32: values beyond about 2^60 overflow them and their row becomes 0.
+    Squares are summed in fp32: values beyond about 2^60 overflow them and their row becomes 0; with an ``eps`` below 2^-120, rows of
+    values below about 2^-60 lose bits, and then everything.
     ``weight``: ``[D]``, None for ones; the other arguments are :func:`rotary`'s.  Gradients in x and the weight (the same
     bits every time).  A step with its backward can be captured into a graph; results of eager calls on the same leaves have to be
     gone by then, since autograd ties the leaves to the stream of the first.
