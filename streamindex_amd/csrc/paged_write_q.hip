@@ -17,8 +17,8 @@
 // other, whole: a block's rows stand next to each other, as a plan's do.
 //
 // Bound, many rows: memory, with vector instructions in 52 % of the CUs' busy cycles.  Nine requests' bf16 rows of 576 values, 64
-// tokens a page and a scale, 133 MB read and written: 27.4 us, 4.8 TB/s.  (Divisions for every piece, rows read a second time: 50;
-// 180 registers a lane and half the waves: 38.)  Few rows: latency.  256 rows with a scale each, 4.3 to 5.3 us.
+// tokens a page and a scale, 133 MB read and written: 27.6 us, 4.8 TB/s; with a scale for each token 21.4 us.  (Divisions for every piece, rows read a second time: 50;
+// 180 registers a lane and half the waves: 38.)  Few rows: latency.  256 single rows into blocks of 16: 5.3 us.
 #include <hip/hip_fp16.h>
 
 #include <string>

@@ -17,7 +17,7 @@
 // result.  The partner piece of a pair of halves is read again, from the cache.
 //
 // Bound: memory.  bf16, 4,096 tokens, 64 heads, D = 576 (302 MB in, 302 out): 113 us, 5.3 TB/s, what a large copy reaches; backward
-// with dw 196 + 5 us (604 MB in, 302 out, 4.5 TB/s).  fp16, 16,001 tokens, 24 heads of 128, rotated in halves (98 MB each way):
+// with dw 195 + 5 us (604 MB in, 302 out, 4.5 TB/s; 27,405 tokens 1,248 + 6 us, 4.8 TB/s).  fp16, 16,001 tokens, 24 heads of 128, rotated in halves (98 MB each way):
 // 32.6 us, 6.0 TB/s, some of it from the last-level cache (42 us with cold caches); vector instructions and the LDS fill 70 % of the busy cycles
 // there, the latter mostly with bank conflicts, but a table read without them was no faster (32.8 against 33.4).
 #include <hip/hip_fp16.h>

@@ -37,8 +37,8 @@ inline RotPlan rot_plan(int64_t rows, int64_t H, int64_t D, int64_t pairs, int v
   // Backward: at most 512 workgroups, two a CU, whose sums of dw are joined (training step of 4,096 tokens, 64 heads, D = 576: 311 us,
   // 384 workgroups 337, 256 363).  Forward: two groups of rows, so that a weight and a table serve both; 1 / 2 / 4 groups: 137 / 117 /
   // 120 us with a weight at those sizes, 490 / 427 / 454 at 16,384 tokens; without one 108.5 / 112.8 / 119 and 419 / 424 / 456;
-  // rotation alone, 24 heads of 128, 100,003 tokens, 229 / 227 / 231 (8: 249), 64 heads of 64 365 / 334 / 333.  (A launch has fewer
-  // than 2^24 workgroups.)
+  // rotation alone, 24 heads of 128, 100,003 tokens, 229 / 227 / 231 (8: 249), 64 heads of 64 365 / 334 / 333.  One rule for all: it
+  // costs wide rows without a weight 1 to 4 %.  (A launch has fewer than 2^24 workgroups.)
   int64_t iters = bwd ? (all + 511) / 512 : all < 4096 ? 1 : 2 + (all >> 24), per;
   per = iters = iters < 1 ? 1 : iters;
   // A filling begins at a multiple of `groups` rows, and of `per` times as many only where `per` divides `iters`.
