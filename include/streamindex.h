@@ -543,7 +543,8 @@ int si_paged_attn_q_fwd(const void* q, const int64_t* q_strides, const void* kv,
  * neighbours or, with halves, (i, i + pairs), are turned by the angle
  * t = p freqs[i]: m (a cos t - b sin t, a sin t + b cos t), m = magnitude,
  * -t with inverse.  p of token t is positions[t % npos] (int32, or int64 with
- * pos64), freqs [pairs] fp64 in radians; pairs 0: none.  y [T, H, D] contiguous.
+ * pos64), freqs [pairs] fp64 in radians; pairs 0: none.  y [T, H, D] contiguous and
+ * apart from x, whose halves are read again.
  * dtype 0 = fp32, 1 = bf16, 2 = fp16; D <= 1024.
  */
 int si_norm_rotary(const void* x, const int64_t* x_strides, int norm, const float* weight, float eps,
@@ -552,8 +553,8 @@ int si_norm_rotary(const void* x, const int64_t* x_strides, int norm, const floa
                    void* stream);
 
 /*
- * Gradients of si_norm_rotary with norm: dx [T, H, D] contiguous and, unless
- * NULL, dweight [D] fp32 (with or without a weight), for which workspace holds
+ * Gradients of si_norm_rotary with norm: dx [T, H, D] contiguous, apart from dy
+ * and x, and, unless NULL, dweight [D] fp32 (with or without a weight), for which workspace holds
  * at least si_norm_rotary_bwd_workspace_bytes(...) bytes; the same bits every
  * time.  The gradient of the rotation alone is si_norm_rotary without norm and
  * with inverse the other way round.

@@ -91,3 +91,15 @@ def test_steps(page, block, D, dtype):
     c.scales *= 1.37 * torch.rand(c.scales.shape, generator=torch.Generator().manual_seed(3)).to(DEV) + 0.01
     for k in range(2):
         c.check(make_rows(len(slots), D, dtype, seed=k), slots)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_the_largest_scales(dtype):
+    """Earlier scales next to fp32's largest value, whose reciprocal is below its normal range."""
+    g = torch.Generator().manual_seed(4)
+    top = torch.tensor([2.0 ** 126, 2.0 ** 127, 1.5 * 2.0 ** 126, 1.3 * 2.0 ** 127, torch.finfo(torch.float32).max])
+    c = Cache(len(top), 2, 2, 64, seed=1)
+    c.scales[:, 0] = top.to(DEV)
+    x = (torch.rand(len(top), 64, generator=g) * 2 - 1) * torch.exp2(torch.randint(90, 128, (len(top), 64), generator=g).float())
+    c.check(x.to(dtype).to(DEV), torch.arange(len(top), device=DEV) * 2 + 1)
+    assert torch.equal(c.scales[:, 0].cpu(), top)
